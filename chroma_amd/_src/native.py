@@ -19,9 +19,7 @@ PACKAGE = Path(__file__).resolve().parents[1]
 REPO = PACKAGE.parent
 LIBRARY = PACKAGE / "lib" / "libchroma_hip.so"
 RUNTIME_SOURCE = PACKAGE / "csrc" / "runtime.cpp"
-SELECT_SOURCE = PACKAGE / "csrc" / "select.hip"
-COPY_SOURCE = PACKAGE / "csrc" / "copy.hip"
-MASKS_SOURCE = PACKAGE / "csrc" / "masks.hip"
+DEVICE_SOURCES = [PACKAGE / "csrc" / f"{name}.hip" for name in ("select", "copy", "masks", "paged", "cache", "adjust")]
 DEVICE_INCLUDE = PACKAGE / "csrc" / "include"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
@@ -33,8 +31,8 @@ _library = None
 
 
 def build_runtime(output: Path = LIBRARY) -> Path:
-    """Build the runtime library: the host runtime (``runtime.cpp``, g++) and the row selection kernels
-    (``select.hip``, hipcc for gfx950 with the same device flags as generated programs), linked by hipcc
+    """Build the runtime library: the host runtime (``runtime.cpp``, g++) and the kernels it offers on their own
+    (``DEVICE_SOURCES``, hipcc for gfx950 with the same device flags as generated programs), linked by hipcc
     against the HIP runtime."""
     from chroma_amd._src.build import DEVICE_FLAGS, architecture
 
@@ -43,19 +41,14 @@ def build_runtime(output: Path = LIBRARY) -> Path:
     hipcc = shlex.split(os.environ.get("HIPCC", str(ROCM / "bin" / "hipcc")))
     device_flags = [flag for flag in DEVICE_FLAGS if flag != "--genco"]
     with tempfile.TemporaryDirectory(prefix="chroma-runtime-") as work:
-        host_object, device_object, copy_object = Path(work) / "runtime.o", Path(work) / "select.o", Path(work) / "copy.o"
-        masks_object = Path(work) / "masks.o"
+        host_object = Path(work) / "runtime.o"
+        device_objects = [Path(work) / f"{source.stem}.o" for source in DEVICE_SOURCES]
         commands = [
             [*shlex.split(os.environ.get("CXX", "g++")), "-std=c++17", "-O2", "-c", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__",
              f"-I{ROCM / 'include'}", str(RUNTIME_SOURCE), "-o", str(host_object)],
-            [*hipcc, f"--offload-arch={architecture()}", *device_flags, "-c", "-fPIC", "-fvisibility=hidden", f"-I{DEVICE_INCLUDE}",
-             str(SELECT_SOURCE), "-o", str(device_object)],
-            [*hipcc, f"--offload-arch={architecture()}", *device_flags, "-c", "-fPIC", "-fvisibility=hidden", f"-I{DEVICE_INCLUDE}",
-             str(COPY_SOURCE), "-o", str(copy_object)],
-            [*hipcc, f"--offload-arch={architecture()}", *device_flags, "-c", "-fPIC", "-fvisibility=hidden", f"-I{DEVICE_INCLUDE}",
-             str(MASKS_SOURCE), "-o", str(masks_object)],
-            [*hipcc, f"--offload-arch={architecture()}", "-shared", "-fPIC", str(host_object), str(device_object), str(copy_object),
-             str(masks_object), "-o", str(temporary),
+            *([*hipcc, f"--offload-arch={architecture()}", *device_flags, "-c", "-fPIC", "-fvisibility=hidden", f"-I{DEVICE_INCLUDE}",
+               str(source), "-o", str(target)] for source, target in zip(DEVICE_SOURCES, device_objects)),
+            [*hipcc, f"--offload-arch={architecture()}", "-shared", "-fPIC", str(host_object), *map(str, device_objects), "-o", str(temporary),
              f"-L{ROCM / 'lib'}", f"-Wl,-rpath,{ROCM / 'lib'}", "-lamdhip64"],
         ]
         for command in commands:
@@ -71,6 +64,36 @@ class Rect(ctypes.Structure):
 
     _fields_ = [("dst", ctypes.c_void_p), ("dst_pitch", ctypes.c_size_t), ("src", ctypes.c_void_p), ("src_pitch", ctypes.c_size_t),
                 ("width", ctypes.c_size_t), ("height", ctypes.c_size_t)]
+
+
+class PagedAttention(ctypes.Structure):
+    """``chroma_hip_paged_attention_call``: attention of one new token per sequence over a paged cache."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("q", "k_pages", "v_pages", "k_new", "v_new", "sinks", "table", "lengths", "out")),
+        *((name, ctypes.c_int64) for name in ("sequences", "kv_heads", "group", "dim", "pages", "page_rows", "page_stride", "row_stride",
+                                              "head_stride", "q_stride", "new_stride", "out_stride", "table_stride", "longest", "window", "first")),
+        ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class CacheRows(ctypes.Structure):
+    """``chroma_hip_cache_rows``: the rows of a key-value cache."""
+
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("rows", ctypes.c_int64), ("layer_pitch", ctypes.c_int64)]
+
+
+class Adjust(ctypes.Structure):
+    """``chroma_hip_adjust_call``: penalties, biases and a mask on rows of logits."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        *((name, ctypes.c_int64) for name in ("rows", "width", "x_stride", "y_stride")),
+        ("history", ctypes.c_void_p), ("history_lengths", ctypes.c_void_p), ("history_stride", ctypes.c_int64), ("history_width", ctypes.c_int64),
+        ("repetition", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("bias_stride", ctypes.c_int64), ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
 
 
 def library() -> ctypes.CDLL:
@@ -122,6 +145,12 @@ def library() -> ctypes.CDLL:
                                                     c.c_void_p, c.c_char_p, c.c_size_t]
         lib.chroma_hip_run_top.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_int, c.c_int, c.c_size_t, c.c_size_t, c.c_int,
                                            c.c_void_p, c.c_void_p, c.c_char_p, c.c_size_t]
+        lib.chroma_hip_paged_attention_workspace.argtypes = [c.POINTER(PagedAttention)]
+        lib.chroma_hip_paged_attention_workspace.restype = c.c_size_t
+        lib.chroma_hip_paged_attention.argtypes = [c.POINTER(PagedAttention), c.c_void_p, c.c_size_t, c.c_void_p, c.c_char_p, c.c_size_t]
+        lib.chroma_hip_cache_move.argtypes = [c.POINTER(CacheRows), c.POINTER(CacheRows), c.c_int64, c.c_int64, c.c_void_p, c.c_int64, c.c_void_p,
+                                              c.c_char_p, c.c_size_t]
+        lib.chroma_hip_rows_adjust.argtypes = [c.POINTER(Adjust), c.c_void_p, c.c_char_p, c.c_size_t]
         _library = lib
         return lib
 
@@ -153,6 +182,10 @@ EXPORTED = (
     "chroma_hip_rows_topk",
     "chroma_hip_rows_topk_static",
     "chroma_hip_run_top",
+    "chroma_hip_paged_attention_workspace",
+    "chroma_hip_paged_attention",
+    "chroma_hip_cache_move",
+    "chroma_hip_rows_adjust",
 )
 
 

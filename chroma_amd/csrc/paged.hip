@@ -1,0 +1,133 @@
+// ``chroma_hip_paged_attention``: attention of one new token per sequence over a paged cache (attention_paged.h) on
+// device memory that a caller owns.
+#include "../../include/chroma_hip.h"
+
+#include <hip/hip_runtime.h>
+
+#include <chroma_hip/attention_paged.h>
+
+#include <cstdio>
+
+namespace {
+
+using Call = chroma_hip_paged_attention_call;
+
+template <class T> __global__ void __launch_bounds__(64) paged_attention(chroma::PagedOperands<T> a) { chroma::attention_paged<T>(a); }
+
+constexpr int64_t kMost = int64_t(1) << 31;  // extents that the kernels count in 32 bits stay below this
+
+int refuse(const char* message, char* error, size_t size) {
+    if (error && size) {
+        std::snprintf(error, size, "paged_attention: %s", message);
+    }
+    return CHROMA_HIP_RUNTIME_ERROR;
+}
+
+// What is wrong with the call, or null.
+const char* mistake(const Call& c) {
+    if (c.dtype != CHROMA_HIP_FLOAT32 && c.dtype != CHROMA_HIP_BFLOAT16) {
+        return "dtype must be CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16";
+    }
+    if (c.sequences < 1 || c.sequences > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.group < 1 || c.group > 65535) {
+        return "want 1 to 65535 sequences, KV heads and query heads of a KV head";
+    }
+    if (c.dim < 8 || c.dim > 256 || c.dim % 8) {
+        return "the head dimension must be a multiple of 8 from 8 to 256";
+    }
+    if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest >= kMost - 4096) {
+        return "pages, page_rows or longest out of range";
+    }
+    if (c.window < 0 || c.first < 0) {
+        return "window and first must not be negative";
+    }
+    if ((c.k_new == nullptr) != (c.v_new == nullptr)) {
+        return "k_new and v_new come together";
+    }
+    if (c.table_stride < (c.longest + c.page_rows - 1) / c.page_rows) {
+        return "a table row is shorter than the longest sequence's pages";
+    }
+    const int64_t chunk = c.dtype == CHROMA_HIP_BFLOAT16 ? 8 : 4, heads = c.kv_heads * c.group * c.dim;
+    if (c.q_stride < heads || c.out_stride < heads || (c.k_new && c.new_stride < c.kv_heads * c.dim) || c.page_stride < 0 ||
+        c.row_stride < c.dim || c.head_stride < 0 || (c.kv_heads > 1 && c.head_stride < c.dim)) {
+        return "a stride is smaller than what lies in it";
+    }
+    if ((c.q_stride | c.out_stride | c.page_stride | c.row_stride | c.head_stride | (c.k_new ? c.new_stride : 0)) % chunk) {
+        return "strides must be whole 16-byte chunks";
+    }
+    return nullptr;
+}
+
+template <class T> chroma::PagedOperands<T> operands(const Call& c) {
+    chroma::PagedOperands<T> a;
+    a.q = static_cast<const T*>(c.q);
+    a.k = static_cast<const T*>(c.k_pages);
+    a.v = static_cast<const T*>(c.v_pages);
+    a.k_new = static_cast<const T*>(c.k_new);
+    a.v_new = static_cast<const T*>(c.v_new);
+    a.sinks = static_cast<const T*>(c.sinks);
+    a.table = c.table;
+    a.lengths = c.lengths;
+    a.out = static_cast<T*>(c.out);
+    a.page_stride = uint64_t(c.page_stride);
+    a.row_stride = uint64_t(c.row_stride);
+    a.head_stride = uint64_t(c.head_stride);
+    a.q_stride = uint64_t(c.q_stride);
+    a.new_stride = uint64_t(c.new_stride);
+    a.out_stride = uint64_t(c.out_stride);
+    a.table_stride = uint64_t(c.table_stride);
+    a.pages = uint64_t(c.pages);
+    a.page_rows = uint32_t(c.page_rows);
+    a.longest = uint32_t(c.longest);
+    // a window or first rows past the longest sequence are all of it
+    a.window = uint32_t(c.window < kMost ? c.window : kMost - 1);
+    a.first = uint32_t(c.first < kMost ? c.first : kMost - 1);
+    a.kv_heads = uint32_t(c.kv_heads);
+    a.group = uint32_t(c.group);
+    a.dim = uint32_t(c.dim);
+    a.scale = c.scale;
+    return a;
+}
+
+template <class T> void launch(const Call& c, hipStream_t stream) {
+    paged_attention<T><<<dim3(unsigned(c.group), unsigned(c.kv_heads), unsigned(c.sequences)), 64, 0, stream>>>(operands<T>(c));
+}
+
+}  // namespace
+
+extern "C" {
+
+__attribute__((visibility("default"))) size_t chroma_hip_paged_attention_workspace(const Call* call) {
+    (void)call;
+    return 0;
+}
+
+__attribute__((visibility("default"))) int chroma_hip_paged_attention(const Call* call, void* workspace, size_t workspace_bytes, void* stream,
+                                                                      char* error, size_t error_size) {
+    if (!call) {
+        return refuse("null call", error, error_size);
+    }
+    const Call& c = *call;
+    if (const char* wrong = mistake(c)) {
+        return refuse(wrong, error, error_size);
+    }
+    if (!c.q || !c.k_pages || !c.v_pages || !c.lengths || !c.out || (!c.table && c.longest)) {
+        return refuse("null device pointer", error, error_size);
+    }
+    if ((reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages) |
+         reinterpret_cast<uintptr_t>(c.k_new) | reinterpret_cast<uintptr_t>(c.v_new) | reinterpret_cast<uintptr_t>(c.out)) & 15u) {
+        return refuse("q, pages, new rows and out must start on 16 bytes", error, error_size);
+    }
+    const size_t need = chroma_hip_paged_attention_workspace(call);
+    if (need && (!workspace || workspace_bytes < need)) {
+        return refuse("workspace smaller than chroma_hip_paged_attention_workspace", error, error_size);
+    }
+    if (c.dtype == CHROMA_HIP_FLOAT32) {
+        launch<float>(c, static_cast<hipStream_t>(stream));
+    } else {
+        launch<uint16_t>(c, static_cast<hipStream_t>(stream));
+    }
+    const hipError_t status = hipGetLastError();
+    return status == hipSuccess ? CHROMA_HIP_OK : refuse(hipGetErrorString(status), error, error_size);
+}
+
+}  // extern "C"

@@ -176,6 +176,101 @@ int chroma_hip_rows_topk_static(const void* x, int dtype, size_t rows, size_t wi
 int chroma_hip_run_top(void* handle, const void* const* inputs, void* const* outputs, int output_index, int dtype, size_t rows,
                        size_t width, int k, void* values, int64_t* ids, char* error, size_t error_size);
 
+/* --- many sequences over one paged key-value cache ---
+ * Operators of batched decoding on device memory, beside the single-sequence decoder above (no counterpart in the
+ * reference, whose decoder keeps one sequence in a contiguous host cache, chroma/_src/decoder.py:57-152). All pointers
+ * except ``moves`` are device memory of the current device; each call queues its kernels on ``stream`` (a hipStream_t;
+ * null for the null stream), allocates nothing and can be captured into a graph. */
+
+/* Attention of one new token per sequence over its cached keys and values, which lie in pages.
+ *
+ *   o = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)),  s_j = scale * (q . k_j)
+ *
+ * over the rows j the token sees: row j < lengths[b] of sequence b, held by row j % page_rows of page
+ * table[b][j / page_rows], and, when ``k_new`` / ``v_new`` are given, one new row at position lengths[b]. The token's
+ * position t is lengths[b] with a new row and lengths[b] - 1 without. ``window`` > 0 leaves out the cached rows
+ * j <= t - window except the ``first`` first ones. The sink term (a learned logit per query head) is left out when ``sinks`` is null.
+ * A token that sees no row gets zeros. Scores, sums and products are kept in float and rounded once, at the end.
+ *
+ * Lengths are read on the device: one below 0 counts as 0 and one above ``longest`` as ``longest``, and only the first
+ * ceil(longest / page_rows) entries of a table row are read. A row on a page outside [0, pages) is not seen.
+ *
+ * The head dimension is innermost and contiguous; strides count elements. Each query head of KV head h, h * group + g,
+ * lies at (h * group + g) * dim of its sequence's q and out. q, out, k_pages, v_pages, k_new and v_new start on 16 bytes
+ * and their strides are whole 16-byte chunks. out must not overlap an input. */
+typedef struct chroma_hip_paged_attention_call {
+    const void* q;          /* [sequences, kv_heads, group, dim] */
+    const void* k_pages;    /* [pages, page_rows, kv_heads, dim] at page_stride, row_stride, head_stride */
+    const void* v_pages;    /* laid out as k_pages */
+    const void* k_new;      /* [sequences, kv_heads, dim], or null (then v_new is null too) */
+    const void* v_new;
+    const void* sinks;      /* [kv_heads * group] or null */
+    const int64_t* table;   /* [sequences, table_stride] */
+    const int64_t* lengths; /* [sequences] */
+    void* out;              /* [sequences, kv_heads, group, dim] */
+    int64_t sequences, kv_heads, group;
+    int64_t dim; /* a multiple of 8, at most 256 */
+    int64_t pages, page_rows;
+    int64_t page_stride, row_stride, head_stride;
+    int64_t q_stride, new_stride, out_stride; /* between sequences */
+    int64_t table_stride;
+    int64_t longest;
+    int64_t window, first; /* 0: no window, no first rows */
+    float scale;
+    int32_t dtype; /* of every value: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
+} chroma_hip_paged_attention_call;
+
+/* Scratch bytes the call needs (it depends on the extents only; 0 when none is needed or the call would be refused).
+ * Calls that may run at the same time need workspaces of their own. */
+size_t chroma_hip_paged_attention_workspace(const chroma_hip_paged_attention_call* call);
+int chroma_hip_paged_attention(const chroma_hip_paged_attention_call* call, void* workspace, size_t workspace_bytes, void* stream,
+                               char* error, size_t error_size);
+
+/* Rows of a cache: ``keys`` and ``values`` hold [layers, rows, row bytes], layers ``layer_pitch`` bytes apart. The pages of a
+ * paged cache are runs of page_rows rows. */
+typedef struct chroma_hip_cache_rows {
+    void* keys;
+    void* values;
+    int64_t rows;
+    int64_t layer_pitch;
+} chroma_hip_cache_rows;
+
+/* Copies rows of keys and values, in every layer: move i takes moves[3 i + 2] rows from row moves[3 i] of ``from`` to row
+ * moves[3 i + 1] of ``to``. It stores new rows into pages, copies pages for a forked sequence and brings the live pages
+ * of a cache together. ``moves`` is host memory, read before the call returns. All ranges must lie inside their caches,
+ * no row may be written twice, and where ``to`` and ``from`` are the same cache no row may be both written and read
+ * (then no order of the moves matters); caches that overlap in memory must be the same. Rows that no move names keep
+ * their bytes. */
+int chroma_hip_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes,
+                          const int64_t* moves, int64_t count, void* stream, char* error, size_t error_size);
+
+/* Logits made ready for the choice of a token, row by row, y = x with, in this order:
+ *   - tokens that occur c > 0 times among the row's history: x > 0 ? x / repetition : x * repetition, then
+ *     minus (presence + frequency * c);
+ *   - plus ``bias``;
+ *   - -inf where the token's bit of ``mask`` (bit i % 32 of word i / 32) is 0.
+ * The arithmetic is float's, one rounding per operation, and the result is rounded to y's type once. ``history`` holds
+ * token ids; of row r the first history_lengths[r] count (all history_width when null; less than 0 counts as 0, more
+ * than history_width as history_width), and ids outside [0, width) count for nothing. A null parameter array changes
+ * nothing. y may be x itself with the same stride (then only what changes is written); otherwise it must not overlap x. */
+typedef struct chroma_hip_adjust_call {
+    const void* x; /* [rows, width] at x_stride elements */
+    void* y;       /* [rows, width] at y_stride elements */
+    int64_t rows, width, x_stride, y_stride;
+    const int64_t* history; /* [rows, history_width] at history_stride, or null */
+    const int64_t* history_lengths;
+    int64_t history_stride, history_width;
+    const float* repetition; /* [rows] each, or null: 1 */
+    const float* presence;   /* or null: 0 */
+    const float* frequency;
+    const float* bias; /* [rows, width] at bias_stride elements (0: one row for all), or null */
+    int64_t bias_stride;
+    const uint32_t* mask; /* [rows, ceil(width / 32)] at mask_stride words (0: one row for all), or null */
+    int64_t mask_stride;
+    int32_t dtype; /* of x and y: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
+} chroma_hip_adjust_call;
+int chroma_hip_rows_adjust(const chroma_hip_adjust_call* call, void* stream, char* error, size_t error_size);
+
 #ifdef __cplusplus
 }
 #endif
