@@ -6,13 +6,23 @@
 
 #include <chroma_hip/attention_paged.h>
 
+#include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 namespace {
 
 using Call = chroma_hip_paged_attention_call;
 
-template <class T> __global__ void __launch_bounds__(64) paged_attention(chroma::PagedOperands<T> a) { chroma::attention_paged<T>(a); }
+template <class T, int DP>
+__global__ void __launch_bounds__(256) paged_attention(chroma::PagedOperands<T> a, uint32_t splits, float* partial) {
+    chroma::attention_paged<T, DP>(a, splits, partial);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(256) paged_attention_combine(chroma::PagedOperands<T> a, uint32_t splits, const float* partial) {
+    chroma::attention_paged_combine<T, DP>(a, splits, partial);
+}
 
 constexpr int64_t kMost = int64_t(1) << 31;  // extents that the kernels count in 32 bits stay below this
 
@@ -28,8 +38,8 @@ const char* mistake(const Call& c) {
     if (c.dtype != CHROMA_HIP_FLOAT32 && c.dtype != CHROMA_HIP_BFLOAT16) {
         return "dtype must be CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16";
     }
-    if (c.sequences < 1 || c.sequences > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.group < 1 || c.group > 65535) {
-        return "want 1 to 65535 sequences, KV heads and query heads of a KV head";
+    if (c.sequences < 1 || c.sequences > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.group < 1 || c.group > 1024) {
+        return "want 1 to 65535 sequences and KV heads and 1 to 1024 query heads of a KV head";
     }
     if (c.dim < 8 || c.dim > 256 || c.dim % 8) {
         return "the head dimension must be a multiple of 8 from 8 to 256";
@@ -88,8 +98,47 @@ template <class T> chroma::PagedOperands<T> operands(const Call& c) {
     return a;
 }
 
-template <class T> void launch(const Call& c, hipStream_t stream) {
-    paged_attention<T><<<dim3(unsigned(c.group), unsigned(c.kv_heads), unsigned(c.sequences)), 64, 0, stream>>>(operands<T>(c));
+// Whether a call of these types and head dimension runs on the kernels of padded dimension DP.
+template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP == (sizeof(T) == 2 ? 32 : 16) || c.dim > DP / 2); }
+
+// Workgroups that share a sequence's keys: as many as bring the launch to kWorkgroups, and no more than leave a key
+// block for every wave of the longest sequence that the window allows.
+constexpr int64_t kWorkgroups = 512;
+template <class T, int DP> int64_t splits_of(const Call& c) {
+    int64_t rows = c.longest + 1;
+    if (c.window) {
+        rows = std::min(rows, std::min(c.window, c.longest) + std::min(c.first, c.longest) + 1);
+    }
+    const int64_t keys = chroma::paged_keys<T, DP>(), most = (rows + keys * chroma::kPagedWaves - 1) / (keys * chroma::kPagedWaves);
+    const int64_t units = c.sequences * c.kv_heads * ((c.group + 15) / 16);
+    return std::max<int64_t>(1, std::min(most, (kWorkgroups + units - 1) / units));
+}
+
+template <class T, int DP> size_t scratch_bytes(const Call& c) {
+    const int64_t splits = splits_of<T, DP>(c);
+    return splits == 1 ? 0 : size_t(c.sequences * c.kv_heads * ((c.group + 15) / 16) * splits) * chroma::paged_partial_floats<DP>() * sizeof(float);
+}
+
+template <class T, int DP> void launch(const Call& c, float* partial, hipStream_t stream) {
+    const uint32_t splits = uint32_t(splits_of<T, DP>(c)), tiles = uint32_t((c.group + 15) / 16);
+    const chroma::PagedOperands<T> a = operands<T>(c);
+    paged_attention<T, DP><<<dim3(unsigned(c.kv_heads), tiles * splits, unsigned(c.sequences)), 256, 0, stream>>>(a, splits, partial);
+    if (splits > 1) {
+        paged_attention_combine<T, DP><<<dim3(unsigned(c.kv_heads), tiles, unsigned(c.sequences)), 256, 0, stream>>>(a, splits, partial);
+    }
+}
+
+// f(type, padded dimension) of the call's kernels.
+template <class F> auto with_kernels(const Call& c, F f) {
+    if (c.dtype == CHROMA_HIP_BFLOAT16) {
+        using T = uint16_t;
+        return fits<T, 32>(c) ? f(T(), std::integral_constant<int, 32>()) : fits<T, 64>(c) ? f(T(), std::integral_constant<int, 64>())
+             : fits<T, 128>(c) ? f(T(), std::integral_constant<int, 128>()) : f(T(), std::integral_constant<int, 256>());
+    }
+    using T = float;
+    return fits<T, 16>(c) ? f(T(), std::integral_constant<int, 16>()) : fits<T, 32>(c) ? f(T(), std::integral_constant<int, 32>())
+         : fits<T, 64>(c) ? f(T(), std::integral_constant<int, 64>()) : fits<T, 128>(c) ? f(T(), std::integral_constant<int, 128>())
+                                                                                      : f(T(), std::integral_constant<int, 256>());
 }
 
 }  // namespace
@@ -97,8 +146,10 @@ template <class T> void launch(const Call& c, hipStream_t stream) {
 extern "C" {
 
 __attribute__((visibility("default"))) size_t chroma_hip_paged_attention_workspace(const Call* call) {
-    (void)call;
-    return 0;
+    if (!call || mistake(*call)) {
+        return 0;
+    }
+    return with_kernels(*call, [&](auto type, auto dim) { return scratch_bytes<decltype(type), decltype(dim)::value>(*call); });
 }
 
 __attribute__((visibility("default"))) int chroma_hip_paged_attention(const Call* call, void* workspace, size_t workspace_bytes, void* stream,
@@ -121,11 +172,13 @@ __attribute__((visibility("default"))) int chroma_hip_paged_attention(const Call
     if (need && (!workspace || workspace_bytes < need)) {
         return refuse("workspace smaller than chroma_hip_paged_attention_workspace", error, error_size);
     }
-    if (c.dtype == CHROMA_HIP_FLOAT32) {
-        launch<float>(c, static_cast<hipStream_t>(stream));
-    } else {
-        launch<uint16_t>(c, static_cast<hipStream_t>(stream));
+    if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) {
+        return refuse("the workspace must start on 16 bytes", error, error_size);
     }
+    with_kernels(c, [&](auto type, auto dim) {
+        launch<decltype(type), decltype(dim)::value>(c, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
+        return 0;
+    });
     const hipError_t status = hipGetLastError();
     return status == hipSuccess ? CHROMA_HIP_OK : refuse(hipGetErrorString(status), error, error_size);
 }
