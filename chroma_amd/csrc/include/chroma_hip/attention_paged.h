@@ -25,7 +25,7 @@ template <class T> struct PagedOperands {
     uint64_t page_stride, row_stride, head_stride, q_stride, new_stride, out_stride, table_stride;
     uint64_t pages;
     uint32_t page_rows, longest, window, first;
-    uint32_t kv_heads, group, dim;
+    uint32_t sequences, kv_heads, group, dim;
     float scale;
 };
 
@@ -54,24 +54,56 @@ template <class T> __device__ __forceinline__ float paged_widen(T v) {
     }
 }
 
-// The kernel is the few-query one of attention_flash.h for one query and rows found through the table: a tile is 16 query
-// heads of a KV head, a workgroup's 4 waves take key blocks in turn, and ``splits`` workgroups share a sequence's blocks,
-// joined by ``attention_paged_combine``. A wave copies its block of K and V global -> LDS into buffers of its own (no
-// barrier in the loop); lane l finds row l of the block once, and the lanes that copy it receive its place by a shuffle.
-// DP is the head dimension in whole matrix-core operands; what lies past ``dim`` in a row is zero.
+// The keys of every sequence are cut into blocks, and the blocks of all sequences, in order, into ``ranges`` equal shares:
+// one wave per (share, KV head, 16 query heads of it), so that long and short sequences load the chip alike. A wave copies a
+// block of K and of V global -> LDS into buffers of its own (there is no barrier); lane l finds row l of the block through
+// the table, and the lanes that copy it receive its place by a shuffle. The products are those of attention_flash.h, a
+// tile's 16 rows the query heads. Where a share ends inside a sequence its (maximum, sum, p . v) go to scratch and
+// ``attention_paged_combine`` adds the sequence's parts. DP is the head dimension in whole matrix-core operands; what lies
+// past ``dim`` in a row is zero.
 //
 // Rows that are not seen keep their probability at exactly 0 and their values out of the products, so that they may hold
 // anything. A bfloat16 probability meets V as two bfloat16 halves (2^-16 of it is lost): the products are a small part of
 // the time, and one half alone (2^-9) would add as much error as the result's own rounding.
-constexpr uint32_t kPagedWaves = 4;
+constexpr uint32_t kPagedWaves = 4;  // of a workgroup: on adjacent KV heads, whose rows adjoin in memory
 
 template <class T, int DP> constexpr uint32_t paged_keys() {  // keys of a block: 16 KiB of K and V, a multiple of an operand
     constexpr uint32_t fits = 16384u / (2u * DP * sizeof(T)), least = sizeof(T) == 2 ? 32u : 16u;
     return fits > 64u ? 64u : fits < least ? least : fits;
 }
 
-// Floats of one (sequence, KV head, 16 query heads, split): per row the maximum and the sum, then the DP sums of p . v.
-template <int DP> constexpr uint32_t paged_partial_floats() { return 16u * (DP + 2u); }
+// Key blocks of a sequence: the first rows', then those from range.low on; one (of nothing) where nothing is seen.
+template <uint32_t KEYS> __device__ __forceinline__ uint32_t paged_blocks(const PagedRange& r) {
+    const uint32_t n = (r.head + KEYS - 1u) / KEYS + (r.end - r.low + KEYS - 1u) / KEYS;
+    return n ? n : 1u;
+}
+
+__device__ __forceinline__ uint32_t paged_scan(uint32_t v) {  // inclusive sums over the wave
+    const uint32_t lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) {
+        const uint32_t before = __shfl_up(v, step, kWave);
+        v += lane >= uint32_t(step) ? before : 0u;
+    }
+    return v;
+}
+
+// The number of blocks of all sequences.
+template <uint32_t KEYS, class T> __device__ __forceinline__ uint32_t paged_total(const PagedOperands<T>& a) {
+    uint32_t mine = 0;
+    for (uint32_t b = threadIdx.x % kWave; b < a.sequences; b += kWave) {
+        mine += paged_blocks<KEYS>(paged_range(a, b));
+    }
+    return __builtin_amdgcn_readlane(paged_scan(mine), kWave - 1);
+}
+
+// Scratch: per (slot, query head) the maximum and the sum, then the DP sums of p . v. The part of sequence b in share w has
+// slot w + b (one of the two grows from a part to the next).
+template <int DP> struct PagedScratch {
+    float* stats;
+    float* sums;
+    __device__ __forceinline__ PagedScratch(float* base, uint64_t slots, uint64_t heads) : stats(base + slots * heads * DP), sums(base) {}
+};
 
 template <class T> __device__ __forceinline__ void paged_store4(T* to, const f32x4_t& v) {
     if constexpr (sizeof(T) == 2) {
@@ -82,37 +114,43 @@ template <class T> __device__ __forceinline__ void paged_store4(T* to, const f32
     }
 }
 
-// grid: (KV heads, row tiles x splits, sequences), 256 threads
-template <class T, int DP>
-__device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint32_t splits, float* __restrict__ partial) {
+// grid: ceil(ranges x KV heads x row tiles / kPagedWaves), 256 threads
+template <class T, int DP, uint32_t KEYS>
+__device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint32_t ranges, float* __restrict__ scratch) {
     constexpr bool BF16 = sizeof(T) == 2;
-    constexpr uint32_t KEYS = paged_keys<T, DP>(), CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
-    constexpr uint32_t WAVE = 2u * KEYS * DP, OPAD = DP + 4u;
+    constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
+    constexpr uint32_t WAVE = 2u * KEYS * DP;
     constexpr int COPIES = KEYS * DP * sizeof(T) / 1024, PARTS = PER_ROW / 4u, TILES = KEYS / 16;
     constexpr uint32_t SWZ = PER_ROW % 8u == 0 ? 7u : 3u;  // chunk c of row r lies at c ^ ((r / 2) & SWZ)
-    static_assert(PER_ROW % 4u == 0 && 64u % PER_ROW == 0 && 16u * (OPAD + 2u) * 4u <= WAVE * sizeof(T), "head dimension");
+    static_assert(PER_ROW % 4u == 0 && 64u % PER_ROW == 0 && KEYS <= 64u && KEYS % (BF16 ? 32u : 16u) == 0, "block");
     __shared__ __attribute__((aligned(1024))) T lds[kPagedWaves * WAVE];
     const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
-    const uint32_t kv = blockIdx.x, tile = blockIdx.y / splits, split = blockIdx.y % splits, b = blockIdx.z;
-    const uint32_t row0 = tile * 16u, chunks = a.dim / CHUNK;
+    const uint32_t tiles = (a.group + 15u) / 16u, heads = a.kv_heads * tiles, worker = blockIdx.x * kPagedWaves + wave;
+    const uint32_t w = worker / heads, kv = worker % heads / tiles, row0 = worker % heads % tiles * 16u, chunks = a.dim / CHUNK;
     const float neg_inf = -__builtin_inff();
     T* ks = lds + wave * WAVE;
     T* vs = ks + KEYS * DP;
-    const PagedRange range = paged_range(a, b);
-    const T* q = a.q + b * a.q_stride + uint64_t(kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u)) * a.dim;
-    const T* k_new = a.k_new + b * a.new_stride + uint64_t(kv) * a.dim;
-    const T* v_new = a.v_new + b * a.new_stride + uint64_t(kv) * a.dim;
-    const T* k_pages = a.k + kv * a.head_stride;
-    const T* v_pages = a.v + kv * a.head_stride;
-    const int64_t* table = a.table + b * a.table_stride;
-    uint4 qf[PARTS];
-#pragma unroll
-    for (int c = 0; c < PARTS; ++c) {
-        qf[c] = uint4{0u, 0u, 0u, 0u};
-        if (c * 4u + quad < chunks) {
-            qf[c] = *reinterpret_cast<const uint4*>(q + (c * 4u + quad) * CHUNK);
+    const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, a.kv_heads * a.group);
+
+    // This wave's share of the blocks, and the sequence b and its block n at which it begins.
+    const uint32_t total_blocks = paged_total<KEYS>(a), share = (total_blocks + ranges - 1u) / ranges;
+    if (uint64_t(w) * share >= total_blocks) {
+        return;
+    }
+    const uint32_t begin = w * share;
+    uint32_t left = total_blocks - begin < share ? total_blocks - begin : share, b = 0, n = 0;
+    for (uint32_t before = 0, b0 = 0; b0 < a.sequences; b0 += kWave) {
+        const uint32_t own = b0 + lane < a.sequences ? paged_blocks<KEYS>(paged_range(a, b0 + lane)) : 0u;
+        const uint32_t upto = before + paged_scan(own);
+        const unsigned long long past = __ballot(upto > begin);
+        if (past) {
+            const uint32_t at = __builtin_ctzll(past);
+            b = b0 + at;
+            n = begin - __builtin_amdgcn_readlane(upto - own, at);
+            break;
         }
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     if (chunks < PER_ROW) {
         for (uint32_t c = lane; c < 2u * KEYS * PER_ROW; c += 64u) {
@@ -120,233 +158,269 @@ __device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint3
         }
         __builtin_amdgcn_s_waitcnt(0);  // before copies into the same places
     }
+    const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
+    const T* k_pages = a.k + kv * a.head_stride;
+    const T* v_pages = a.v + kv * a.head_stride;
 
-    // Blocks: the first rows', then those from range.low on; this wave's are first, first + stride, ...
-    const uint32_t head_blocks = (range.head + KEYS - 1u) / KEYS, blocks = head_blocks + (range.end - range.low + KEYS - 1u) / KEYS;
-    const uint32_t stride = kPagedWaves * splits;
-    auto block_begin = [&](uint32_t n) { return n < head_blocks ? n * KEYS : range.low + (n - head_blocks) * KEYS; };
-    auto block_end = [&](uint32_t n) { return n < head_blocks ? range.head : range.end; };
-    // The page of this lane's row of block n (-1: none).
-    auto page_of = [&](uint32_t n) -> int64_t {
-        const uint32_t j = block_begin(n) + lane;
-        return lane < KEYS && j < block_end(n) && j < range.length ? table[j / a.page_rows] : -1;
-    };
-    unsigned long long seen = 0;
-    auto copy = [&](uint32_t n, int64_t page) {
-        const uint32_t begin = block_begin(n), j = begin + lane;
-        const bool held = page >= 0 && uint64_t(page) < a.pages;
-        const uint64_t place = held ? uint64_t(page) * a.page_stride + uint64_t(j % a.page_rows) * a.row_stride : 0u;
-        seen = __ballot(held || (lane < KEYS && j >= range.length && j < block_end(n)));
+    for (; left; ++b, n = 0) {
+        const PagedRange range = paged_range(a, b);
+        const T* q = a.q + b * a.q_stride + uint64_t(head) * a.dim;
+        const T* k_new = a.k_new + b * a.new_stride + uint64_t(kv) * a.dim;
+        const T* v_new = a.v_new + b * a.new_stride + uint64_t(kv) * a.dim;
+        const int64_t* table = a.table + b * a.table_stride;
+        const uint32_t head_blocks = (range.head + KEYS - 1u) / KEYS, blocks = paged_blocks<KEYS>(range);
+        const uint32_t count = blocks - n < left ? blocks - n : left, stop = n + count;
+        left -= count;
+        auto block_begin = [&](uint32_t x) { return x < head_blocks ? x * KEYS : range.low + (x - head_blocks) * KEYS; };
+        auto block_end = [&](uint32_t x) { return x < head_blocks ? range.head : range.end; };
+        // The page of this lane's row of block x (-1: none).
+        auto page_of = [&](uint32_t x) -> int64_t {
+            const uint32_t j = block_begin(x) + lane;
+            return lane < KEYS && j < block_end(x) && j < range.length ? table[j / a.page_rows] : -1;
+        };
+        unsigned long long seen = 0;
+        auto copy = [&](uint32_t x, int64_t page) {
+            const uint32_t first = block_begin(x), j = first + lane;
+            const bool held = page >= 0 && uint64_t(page) < a.pages;
+            const uint64_t place = held ? uint64_t(page) * a.page_stride + uint64_t(j % a.page_rows) * a.row_stride : 0u;
+            seen = __ballot(held || (lane < KEYS && j >= range.length && j < block_end(x)));
 #pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-            const uint32_t r = i * (64u / PER_ROW) + lane / PER_ROW, chunk = (lane % PER_ROW) ^ ((r / 2u) & SWZ);
-            const uint64_t from = __shfl(place, r, kWave);
-            const bool fresh = begin + r == range.length && range.end > range.length;
-            const T* k = (fresh ? k_new : k_pages + from) + chunk * CHUNK;
-            const T* v = (fresh ? v_new : v_pages + from) + chunk * CHUNK;
-            if (chunk < chunks) {
-                __builtin_amdgcn_global_load_lds((global_void*)k, (lds_void*)(ks + i * (1024u / sizeof(T))), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_void*)v, (lds_void*)(vs + i * (1024u / sizeof(T))), 16, 0, 0);
+            for (int i = 0; i < COPIES; ++i) {
+                const uint32_t r = i * (64u / PER_ROW) + lane / PER_ROW, chunk = (lane % PER_ROW) ^ ((r / 2u) & SWZ);
+                const uint64_t from = __shfl(place, r, kWave);
+                const bool fresh = first + r == range.length && range.end > range.length;
+                const T* k = (fresh ? k_new : k_pages + from) + chunk * CHUNK;
+                const T* v = (fresh ? v_new : v_pages + from) + chunk * CHUNK;
+                if (chunk < chunks) {
+                    __builtin_amdgcn_global_load_lds((global_void*)k, (lds_void*)(ks + i * (1024u / sizeof(T))), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((global_void*)v, (lds_void*)(vs + i * (1024u / sizeof(T))), 16, 0, 0);
+                }
             }
-        }
-    };
-
-    float peak = neg_inf, total = 0.0f;
-    f32x4_t o[DP / 16];
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) {
-        o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    uint32_t n = split * kPagedWaves + wave;
-    if (n < blocks) {
+        };
         copy(n, page_of(n));
-    }
-    while (n < blocks) {
-        const uint32_t next = n + stride;
-        int64_t next_page = -1;
-        if (next < blocks) {
-            next_page = page_of(next);
+        uint4 qf[PARTS];
+#pragma unroll
+        for (int c = 0; c < PARTS; ++c) {
+            qf[c] = uint4{0u, 0u, 0u, 0u};
+            if (c * 4u + quad < chunks) {
+                qf[c] = *reinterpret_cast<const uint4*>(q + (c * 4u + quad) * CHUNK);
+            }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
-        __builtin_amdgcn_sched_barrier(0);
-        if (seen != (KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull)) {  // 0 times an infinite value would be NaN
-            for (uint32_t c = lane; c < KEYS * PER_ROW; c += 64u) {
-                if (!((seen >> (c / PER_ROW)) & 1ull)) {
-                    *reinterpret_cast<uint4*>(vs + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
+        float peak = neg_inf, total = 0.0f;
+        f32x4_t o[DP / 16];
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; ++dt) {
+            o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        while (n < stop) {
+            const uint32_t next = n + 1u;
+            int64_t next_page = -1;
+            if (next < stop) {
+                next_page = page_of(next);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+            __builtin_amdgcn_sched_barrier(0);
+            if (seen != (KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull)) {  // 0 times an infinite value would be NaN
+                for (uint32_t c = lane; c < KEYS * PER_ROW; c += 64u) {
+                    if (!((seen >> (c / PER_ROW)) & 1ull)) {
+                        *reinterpret_cast<uint4*>(vs + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
+                    }
                 }
             }
-        }
-        // scores of keys 16 t + 4 quad + r for this lane's query head
-        float u[TILES][4], top = neg_inf;
+            // scores of keys 16 t + 4 quad + r for this lane's query head
+            float u[TILES][4], top = neg_inf;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < TILES; ++t) {
+                f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int c = 0; c < PARTS; ++c) {
-                const uint32_t r = t * 16u + col;
-                const uint4 kf = *reinterpret_cast<const uint4*>(ks + r * DP + ((c * 4u + quad) ^ ((r / 2u) & SWZ)) * CHUNK);
-                if constexpr (BF16) {
-                    kwave_mfma<T>(kf, qf[c], s);
-                } else {
-                    s += kwave_unit(kf, qf[c]);
+                for (int c = 0; c < PARTS; ++c) {
+                    const uint32_t r = t * 16u + col;
+                    const uint4 kf = *reinterpret_cast<const uint4*>(ks + r * DP + ((c * 4u + quad) ^ ((r / 2u) & SWZ)) * CHUNK);
+                    if constexpr (BF16) {
+                        kwave_mfma<T>(kf, qf[c], s);
+                    } else {
+                        s += kwave_unit(kf, qf[c]);
+                    }
+                }
+                const uint32_t bits = uint32_t(seen >> (t * 16u + quad * 4u)) & 15u;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    u[t][r] = (bits >> r) & 1u ? s[r] * a.scale : neg_inf;
+                    top = __builtin_fmaxf(top, u[t][r]);
                 }
             }
-            const uint32_t bits = uint32_t(seen >> (t * 16u + quad * 4u)) & 15u;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                u[t][r] = (bits >> r) & 1u ? s[r] * a.scale : neg_inf;
-                top = __builtin_fmaxf(top, u[t][r]);
-            }
-        }
-        if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
-            top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = __builtin_fmaxf(top, __shfl_xor(top, 32, kWave));
-            top = __builtin_fmaxf(top, peak);
-            const float shrink = peak == neg_inf ? 0.0f : fast_exp(peak - top);
-            total *= shrink;
-#pragma unroll
-            for (int dt = 0; dt < DP / 16; ++dt) {
-                o[dt] *= shrink;
-            }
-            peak = top;
-        }
-        const float base = peak == neg_inf ? 0.0f : peak;
-        float part = 0.0f;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                u[t][r] = fast_exp(u[t][r] - base);
-                part += u[t][r];
-            }
-        }
-        total += part;
-        if constexpr (BF16) {
-            // slots 0-3 and 4-7 of lane (d, quad) hold keys 32 h + 4 quad + r and 32 h + 16 + 4 quad + r (attention_flash.h)
-#pragma unroll
-            for (int h = 0; h < TILES / 2; ++h) {
-                bf16x8_t high, low;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const float p = u[2 * h + x / 4][x % 4];
-                    high[x] = __bf16(p);
-                    low[x] = __bf16(p - float(high[x]));
-                }
+            if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
+                top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
+                top = __builtin_fmaxf(top, __shfl_xor(top, 32, kWave));
+                top = __builtin_fmaxf(top, peak);
+                const float shrink = peak == neg_inf ? 0.0f : fast_exp(peak - top);
+                total *= shrink;
 #pragma unroll
                 for (int dt = 0; dt < DP / 16; ++dt) {
-                    s16x4_t half[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t r = h * 32u + x * 16u + quad * 4u + col / 4u;
-                        const uint32_t chunk = (dt * 2u + (col % 4u) / 2u) ^ ((r / 2u) & SWZ);
-                        half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + r * DP + chunk * 8u + (col % 2u) * 4u));
-                    }
-                    const uint2 lo = __builtin_bit_cast(uint2, half[0]), hi = __builtin_bit_cast(uint2, half[1]);
-                    const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, uint4{lo.x, lo.y, hi.x, hi.y});
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, high, o[dt], 0, 0, 0);
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, low, o[dt], 0, 0, 0);
+                    o[dt] *= shrink;
                 }
+                peak = top;
             }
-        } else {
-            // product (t, r) takes keys 16 t + 4 quad + r; 16 keys are summed before they join the row's
+            const float base = peak == neg_inf ? 0.0f : peak;
+            float part = 0.0f;
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
 #pragma unroll
-                for (int dt = 0; dt < DP / 16; ++dt) {
-                    f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t key = t * 16u + quad * 4u + r;
-                        const float v = vs[key * DP + ((dt * 4u + col / 4u) ^ ((key / 2u) & SWZ)) * 4u + col % 4u];
-                        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(v, u[t][r], sum, 0, 0, 0);
-                    }
-                    o[dt] += sum;
+                for (int r = 0; r < 4; ++r) {
+                    u[t][r] = fast_exp(u[t][r] - base);
+                    part += u[t][r];
                 }
             }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (next < blocks) {  // both buffers have been read
-            copy(next, next_page);
-        }
-        n = next;
-    }
-
-    // The waves' parts: rows of (DP + 4) floats in each wave's own buffers, then [row][max, sum].
-    total += __shfl_xor(total, 16, kWave);
-    total += __shfl_xor(total, 32, kWave);
-    float* mine = reinterpret_cast<float*>(ks);
+            total += part;
+            if constexpr (BF16) {
+                // slots 0-3 and 4-7 of lane (d, quad) hold keys 32 h + 4 quad + r and 32 h + 16 + 4 quad + r (attention_flash.h)
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) {
-        *reinterpret_cast<f32x4_t*>(mine + col * OPAD + dt * 16u + quad * 4u) = o[dt];
-    }
-    if (quad == 0) {
-        mine[16u * OPAD + 2u * col] = peak;
-        mine[16u * OPAD + 2u * col + 1u] = total;
-    }
-    __syncthreads();
-    const float* parts = reinterpret_cast<const float*>(lds);
-    constexpr uint32_t PART = WAVE * sizeof(T) / 4u;
-    for (uint32_t i = threadIdx.x; i < 16u * (DP / 4u); i += 64u * kPagedWaves) {
-        const uint32_t r = i / (DP / 4u), d = i % (DP / 4u) * 4u;
-        if (row0 + r >= a.group || d >= a.dim) {
-            continue;
-        }
-        const uint32_t head = kv * a.group + row0 + r;
-        const float sink = splits == 1u && a.sinks ? paged_widen<T>(a.sinks[head]) : neg_inf;
-        FlashMerge merge{sink, 0.0f};
+                for (int h = 0; h < TILES / 2; ++h) {
+                    bf16x8_t high, low;
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedWaves; ++w) {
-            merge.top = __builtin_fmaxf(merge.top, parts[w * PART + 16u * OPAD + 2u * r]);
-        }
-        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int x = 0; x < 8; ++x) {
+                        const float p = u[2 * h + x / 4][x % 4];
+                        high[x] = __bf16(p);
+                        low[x] = __bf16(p - float(high[x]));
+                    }
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedWaves; ++w) {
-            const float scale = merge.weight(parts[w * PART + 16u * OPAD + 2u * r]);
-            merge.total += scale * parts[w * PART + 16u * OPAD + 2u * r + 1u];
-            sum += scale * *reinterpret_cast<const f32x4_t*>(parts + w * PART + r * OPAD + d);
+                    for (int dt = 0; dt < DP / 16; ++dt) {
+                        s16x4_t half[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t r = h * 32u + x * 16u + quad * 4u + col / 4u;
+                            const uint32_t chunk = (dt * 2u + (col % 4u) / 2u) ^ ((r / 2u) & SWZ);
+                            half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + r * DP + chunk * 8u + (col % 2u) * 4u));
+                        }
+                        const uint2 lo = __builtin_bit_cast(uint2, half[0]), hi = __builtin_bit_cast(uint2, half[1]);
+                        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, uint4{lo.x, lo.y, hi.x, hi.y});
+                        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, high, o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, low, o[dt], 0, 0, 0);
+                    }
+                }
+            } else {
+                // product (t, r) takes keys 16 t + 4 quad + r; 16 keys are summed before they join the row's
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                    for (int dt = 0; dt < DP / 16; ++dt) {
+                        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t key = t * 16u + quad * 4u + r;
+                            const float v = vs[key * DP + ((dt * 4u + col / 4u) ^ ((key / 2u) & SWZ)) * 4u + col % 4u];
+                            sum = __builtin_amdgcn_mfma_f32_16x16x4f32(v, u[t][r], sum, 0, 0, 0);
+                        }
+                        o[dt] += sum;
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (next < stop) {  // both buffers have been read
+                copy(next, next_page);
+            }
+            n = next;
         }
-        if (splits == 1u) {
-            merge.total += merge.weight(sink);
-            sum *= merge.total == 0.0f ? 0.0f : 1.0f / merge.total;
-            paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + d, sum);
+        total += __shfl_xor(total, 16, kWave);
+        total += __shfl_xor(total, 32, kWave);
+        const bool mine = row0 + col < a.group;
+        if (count == blocks) {
+            const FlashMerge merge{__builtin_fmaxf(peak, a.sinks ? paged_widen<T>(a.sinks[head]) : neg_inf), 0.0f};
+            const float weight = merge.weight(peak), sum = weight * total + (a.sinks ? merge.weight(paged_widen<T>(a.sinks[head])) : 0.0f);
+            const float factor = sum == 0.0f ? 0.0f : weight / sum;
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                if (mine && dt * 16u + quad * 4u < a.dim) {
+                    paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + dt * 16u + quad * 4u, o[dt] * factor);
+                }
+            }
         } else {
-            float* to = partial + (uint64_t(b * gridDim.x + kv) * gridDim.y + blockIdx.y) * paged_partial_floats<DP>();
-            *reinterpret_cast<f32x4_t*>(to + 32u + r * DP + d) = sum;
-            if (d == 0) {
-                to[2u * r] = merge.top;
-                to[2u * r + 1u] = merge.total;
+            const uint64_t at = uint64_t(w + b) * a.kv_heads * a.group + head;
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                if (mine && dt * 16u + quad * 4u < a.dim) {
+                    *reinterpret_cast<f32x4_t*>(parts.sums + at * DP + dt * 16u + quad * 4u) = o[dt];
+                }
+            }
+            if (mine && quad == 0) {
+                *reinterpret_cast<float2*>(parts.stats + 2u * at) = float2{peak, total};
             }
         }
     }
 }
 
-// The splits of every row, in order, and the sink (grid: KV heads x row tiles x sequences, 256 threads).
-template <class T, int DP>
-__device__ __forceinline__ void attention_paged_combine(const PagedOperands<T>& a, uint32_t splits, const float* __restrict__ partial) {
-    constexpr uint32_t PART = paged_partial_floats<DP>();
-    const uint32_t kv = blockIdx.x, row0 = blockIdx.y * 16u, b = blockIdx.z;
-    const float* parts = partial + (uint64_t(b * gridDim.x + kv) * gridDim.y + blockIdx.y) * splits * PART;
-    for (uint32_t i = threadIdx.x; i < 16u * (DP / 4u); i += 256u) {
-        const uint32_t r = i / (DP / 4u), d = i % (DP / 4u) * 4u;
-        if (row0 + r >= a.group || d >= a.dim) {
-            continue;
+// The parts of every sequence that lies in more than one share, and the sink. WAVES waves take a query head (grid:
+// ceil(sequences x query heads x WAVES / 4), 256 threads): a lane holds 4 dimensions of every 64 / (DP / 4)-th part.
+template <class T, int DP, uint32_t KEYS, uint32_t WAVES>
+__device__ __forceinline__ void attention_paged_combine(const PagedOperands<T>& a, uint32_t ranges, float* __restrict__ scratch) {
+    constexpr uint32_t ACROSS = DP / 4u, STEP = 64u / ACROSS * WAVES;
+    __shared__ float sums[WAVES > 1 ? WAVES : 1][WAVES > 1 ? DP : 1], totals[WAVES > 1 ? WAVES : 1];
+    const uint32_t lane = threadIdx.x % 64u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), heads = a.kv_heads * a.group;
+    const uint32_t unit = WAVES > 1 ? blockIdx.x : blockIdx.x * 4u + wave, b = unit / heads, head = unit % heads;
+    if (b >= a.sequences) {
+        return;
+    }
+    const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, heads);
+    uint32_t all = 0, before = 0;
+    for (uint32_t x = lane; x < a.sequences; x += kWave) {
+        const uint32_t own = paged_blocks<KEYS>(paged_range(a, x));
+        all += own;
+        before += x < b ? own : 0u;
+    }
+    all = __builtin_amdgcn_readlane(paged_scan(all), kWave - 1);
+    before = __builtin_amdgcn_readlane(paged_scan(before), kWave - 1);
+    const uint32_t share = (all + ranges - 1u) / ranges, own = paged_blocks<KEYS>(paged_range(a, b));
+    const uint32_t first = before / share, count = (before + own - 1u) / share - first + 1u;
+    if (count == 1u) {
+        return;  // written by its wave
+    }
+    const uint64_t at0 = uint64_t(first + b) * heads + head;
+    const float sink = a.sinks ? paged_widen<T>(a.sinks[head]) : -__builtin_inff();
+    float top = sink;
+    for (uint32_t s = lane; s < count; s += kWave) {
+        top = __builtin_fmaxf(top, parts.stats[2u * (at0 + uint64_t(s) * heads)]);
+    }
+    top = wave_max(top);
+    const FlashMerge merge{top, 0.0f};
+    const uint32_t d = lane % ACROSS * 4u, group = lane / ACROSS + (WAVES > 1 ? wave * (64u / ACROSS) : 0u);
+    f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    float total = 0.0f;
+#pragma unroll 4
+    for (uint32_t s = group; s < count; s += STEP) {
+        const uint64_t at = at0 + uint64_t(s) * heads;
+        const float2 stat = *reinterpret_cast<const float2*>(parts.stats + 2u * at);
+        const f32x4_t o = *reinterpret_cast<const f32x4_t*>(parts.sums + at * DP + d);  // (past dim: what lies there, never stored)
+        const float weight = merge.weight(stat.x);
+        total += weight * stat.y;
+        sum += weight * o;
+    }
+#pragma unroll
+    for (uint32_t step = ACROSS; step < 64u; step *= 2u) {
+        total += __shfl_xor(total, step, kWave);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] += __shfl_xor(sum[i], step, kWave);
         }
-        const uint32_t head = kv * a.group + row0 + r;
-        const float sink = a.sinks ? paged_widen<T>(a.sinks[head]) : -__builtin_inff();
-        FlashMerge merge{sink, 0.0f};
-        for (uint32_t s = 0; s < splits; ++s) {
-            merge.top = __builtin_fmaxf(merge.top, parts[s * PART + 2u * r]);
+    }
+    if constexpr (WAVES > 1) {
+        if (lane < ACROSS) {
+            *reinterpret_cast<f32x4_t*>(&sums[wave][d]) = sum;
+            totals[wave] = total;
         }
-        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t s = 0; s < splits; ++s) {
-            const float scale = merge.weight(parts[s * PART + 2u * r]);
-            merge.total += scale * parts[s * PART + 2u * r + 1u];
-            sum += scale * *reinterpret_cast<const f32x4_t*>(parts + s * PART + 32u + r * DP + d);
+        __syncthreads();
+        if (wave) {
+            return;
         }
-        merge.total += merge.weight(sink);
-        sum *= merge.total == 0.0f ? 0.0f : 1.0f / merge.total;
-        paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + d, sum);
+#pragma unroll
+        for (uint32_t x = 1; x < WAVES; ++x) {
+            sum += *reinterpret_cast<const f32x4_t*>(&sums[x][d]);
+            total += totals[x];
+        }
+    }
+    total += a.sinks ? merge.weight(sink) : 0.0f;
+    if (lane < ACROSS && d < a.dim) {
+        paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + d, sum * (total == 0.0f ? 0.0f : 1.0f / total));
     }
 }
 

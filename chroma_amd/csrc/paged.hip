@@ -15,13 +15,13 @@ namespace {
 using Call = chroma_hip_paged_attention_call;
 
 template <class T, int DP>
-__global__ void __launch_bounds__(256) paged_attention(chroma::PagedOperands<T> a, uint32_t splits, float* partial) {
-    chroma::attention_paged<T, DP>(a, splits, partial);
+__global__ void __launch_bounds__(256) paged_attention(chroma::PagedOperands<T> a, uint32_t ranges, float* scratch) {
+    chroma::attention_paged<T, DP, chroma::paged_keys<T, DP>()>(a, ranges, scratch);
 }
 
-template <class T, int DP>
-__global__ void __launch_bounds__(256) paged_attention_combine(chroma::PagedOperands<T> a, uint32_t splits, const float* partial) {
-    chroma::attention_paged_combine<T, DP>(a, splits, partial);
+template <class T, int DP, uint32_t WAVES>
+__global__ void __launch_bounds__(256) paged_attention_combine(chroma::PagedOperands<T> a, uint32_t ranges, float* scratch) {
+    chroma::attention_paged_combine<T, DP, chroma::paged_keys<T, DP>(), WAVES>(a, ranges, scratch);
 }
 
 constexpr int64_t kMost = int64_t(1) << 31;  // extents that the kernels count in 32 bits stay below this
@@ -46,6 +46,9 @@ const char* mistake(const Call& c) {
     }
     if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest >= kMost - 4096) {
         return "pages, page_rows or longest out of range";
+    }
+    if (c.sequences * (c.longest / 16 + 2) >= kMost || c.sequences * c.kv_heads * c.group >= kMost) {
+        return "more sequences of this length, or more query heads, than the kernels count";
     }
     if (c.window < 0 || c.first < 0) {
         return "window and first must not be negative";
@@ -91,6 +94,7 @@ template <class T> chroma::PagedOperands<T> operands(const Call& c) {
     // a window or first rows past the longest sequence are all of it
     a.window = uint32_t(c.window < kMost ? c.window : kMost - 1);
     a.first = uint32_t(c.first < kMost ? c.first : kMost - 1);
+    a.sequences = uint32_t(c.sequences);
     a.kv_heads = uint32_t(c.kv_heads);
     a.group = uint32_t(c.group);
     a.dim = uint32_t(c.dim);
@@ -101,30 +105,48 @@ template <class T> chroma::PagedOperands<T> operands(const Call& c) {
 // Whether a call of these types and head dimension runs on the kernels of padded dimension DP.
 template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP == (sizeof(T) == 2 ? 32 : 16) || c.dim > DP / 2); }
 
-// Workgroups that share a sequence's keys: as many as bring the launch to kWorkgroups, and no more than leave a key
-// block for every wave of the longest sequence that the window allows.
-constexpr int64_t kWorkgroups = 512;
-template <class T, int DP> int64_t splits_of(const Call& c) {
-    int64_t rows = c.longest + 1;
+// How a call is cut: the most blocks a sequence can have, and the shares that all of them are cut into, as many as bring
+// kWaves waves.
+constexpr int64_t kWaves = 2048;
+struct Cut {
+    int64_t blocks, ranges, heads, tiles;
+    bool joined() const { return blocks > 1; }  // whether a sequence can lie in more than one share
+};
+template <class T, int DP> Cut cut_of(const Call& c) {
+    const int64_t keys = chroma::paged_keys<T, DP>();
+    Cut cut;
+    cut.tiles = (c.group + 15) / 16;
+    cut.heads = c.kv_heads * c.group;
+    const int64_t rows = c.longest + 1;
+    cut.blocks = (rows + keys - 1) / keys;
     if (c.window) {
-        rows = std::min(rows, std::min(c.window, c.longest) + std::min(c.first, c.longest) + 1);
+        const int64_t head = std::min(c.first, c.longest), seen = std::min(c.window, rows);
+        cut.blocks = std::min(cut.blocks + 1, (head + keys - 1) / keys + (seen + keys - 1) / keys);
     }
-    const int64_t keys = chroma::paged_keys<T, DP>(), most = (rows + keys * chroma::kPagedWaves - 1) / (keys * chroma::kPagedWaves);
-    const int64_t units = c.sequences * c.kv_heads * ((c.group + 15) / 16);
-    return std::max<int64_t>(1, std::min(most, (kWorkgroups + units - 1) / units));
+    const int64_t wanted = (kWaves + c.kv_heads * cut.tiles - 1) / (c.kv_heads * cut.tiles);
+    cut.ranges = std::min(wanted, c.sequences * cut.blocks);
+    return cut;
 }
 
 template <class T, int DP> size_t scratch_bytes(const Call& c) {
-    const int64_t splits = splits_of<T, DP>(c);
-    return splits == 1 ? 0 : size_t(c.sequences * c.kv_heads * ((c.group + 15) / 16) * splits) * chroma::paged_partial_floats<DP>() * sizeof(float);
+    const Cut cut = cut_of<T, DP>(c);
+    return cut.joined() ? size_t((cut.ranges + c.sequences) * cut.heads) * (DP + 2) * sizeof(float) : 0;
 }
 
-template <class T, int DP> void launch(const Call& c, float* partial, hipStream_t stream) {
-    const uint32_t splits = uint32_t(splits_of<T, DP>(c)), tiles = uint32_t((c.group + 15) / 16);
+template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_t stream) {
+    const Cut cut = cut_of<T, DP>(c);
     const chroma::PagedOperands<T> a = operands<T>(c);
-    paged_attention<T, DP><<<dim3(unsigned(c.kv_heads), tiles * splits, unsigned(c.sequences)), 256, 0, stream>>>(a, splits, partial);
-    if (splits > 1) {
-        paged_attention_combine<T, DP><<<dim3(unsigned(c.kv_heads), tiles, unsigned(c.sequences)), 256, 0, stream>>>(a, splits, partial);
+    const uint32_t ranges = uint32_t(cut.ranges);
+    const int64_t waves = cut.ranges * c.kv_heads * cut.tiles;
+    paged_attention<T, DP><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
+    if (!cut.joined()) {
+        return;
+    }
+    const int64_t units = c.sequences * cut.heads;
+    if (cut.blocks > 64 && units < 2048) {
+        paged_attention_combine<T, DP, 4><<<unsigned(units), 256, 0, stream>>>(a, ranges, scratch);
+    } else {
+        paged_attention_combine<T, DP, 1><<<unsigned((units + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
     }
 }
 
