@@ -54,23 +54,34 @@ template <class T> __device__ __forceinline__ float paged_widen(T v) {
     }
 }
 
-// The keys of every sequence are cut into blocks, and the blocks of all sequences, in order, into ``ranges`` equal shares:
-// one wave per (share, KV head, 16 query heads of it), so that long and short sequences load the chip alike. A wave copies a
-// block of K and of V global -> LDS into buffers of its own (there is no barrier); lane l finds row l of the block through
-// the table, and the lanes that copy it receive its place by a shuffle. The products are those of attention_flash.h, a
-// tile's 16 rows the query heads. Where a share ends inside a sequence its (maximum, sum, p . v) go to scratch and
-// ``attention_paged_combine`` adds the sequence's parts. DP is the head dimension in whole matrix-core operands; what lies
-// past ``dim`` in a row is zero.
+// A wave takes blocks of a sequence's keys for 16 query heads of a KV head. It copies a block of K and of V global -> LDS into
+// buffers of its own (no barrier); lane l finds row l of the block through the table, and the lanes that copy it receive its
+// place by a shuffle. The products are those of attention_flash.h, a tile's 16 rows the query heads. Short sequences have a
+// workgroup whose waves take the blocks in turn (``attention_paged_whole``, one launch). Otherwise the blocks of all
+// sequences, in order, are cut into equal shares, so that long and short sequences load the chip alike
+// (``attention_paged_shares``); where a share ends inside a sequence its (maximum, sum, p . v) go to scratch, and
+// ``attention_paged_combine`` adds the sequence's parts in order. (Adding them in the wave that comes last, behind
+// device-scope stores and flags, was slower: one sequence of 900 rows 19.6 us against 14.2 with the second launch, 32 up to 4096
+// 50 against 38.) DP is the head dimension in whole matrix-core operands; what lies past ``dim`` in a row is zero.
 //
 // Rows that are not seen keep their probability at exactly 0 and their values out of the products, so that they may hold
 // anything. A bfloat16 probability meets V as two bfloat16 halves (2^-16 of it is lost): the products are a small part of
 // the time, and one half alone (2^-9) would add as much error as the result's own rounding.
-constexpr uint32_t kPagedWaves = 4;  // of a workgroup: on adjacent KV heads, whose rows adjoin in memory
+constexpr uint32_t kPagedWaves = 4;  // of a workgroup on shares: they take adjacent KV heads, whose rows adjoin in memory
 
 template <class T, int DP> constexpr uint32_t paged_keys() {  // keys of a block: 16 KiB of K and V, a multiple of an operand
     constexpr uint32_t fits = 16384u / (2u * DP * sizeof(T)), least = sizeof(T) == 2 ? 32u : 16u;
     return fits > 64u ? 64u : fits < least ? least : fits;
 }
+
+// In a workgroup that takes a whole sequence: blocks of half the size and 8 waves (two workgroups a compute unit; 4 waves
+// of whole blocks take 8 mixed sequences up to 2000 rows in 19.5 us, these in 15.8, 8 of whole blocks in 14.3 but 128 up to 1000 in
+// 38 against 31).
+template <class T, int DP> constexpr uint32_t paged_whole_keys() {
+    constexpr uint32_t keys = paged_keys<T, DP>(), least = sizeof(T) == 2 ? 32u : 16u;
+    return keys / 2u < least ? least : keys / 2u;
+}
+template <class T, int DP> constexpr uint32_t paged_whole_waves() { return paged_whole_keys<T, DP>() * DP * sizeof(T) > 8192u ? 4u : 8u; }
 
 // Key blocks of a sequence: the first rows', then those from range.low on; one (of nothing) where nothing is seen.
 template <uint32_t KEYS> __device__ __forceinline__ uint32_t paged_blocks(const PagedRange& r) {
@@ -97,7 +108,15 @@ template <uint32_t KEYS, class T> __device__ __forceinline__ uint32_t paged_tota
     return __builtin_amdgcn_readlane(paged_scan(mine), kWave - 1);
 }
 
-// Scratch: per (slot, query head) the maximum and the sum, then the DP sums of p . v. The part of sequence b in share w has
+// Share w < ranges holds blocks [begin(w), begin(w + 1)) of ``total``, one at least; ``of`` gives the share that holds a block.
+struct PagedShares {
+    uint64_t total, ranges;
+    __device__ __forceinline__ PagedShares(uint32_t blocks, uint32_t most) : total(blocks), ranges(most < blocks ? most : blocks) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return uint32_t(w * total / ranges); }
+    __device__ __forceinline__ uint32_t of(uint32_t block) const { return uint32_t(((block + 1ull) * ranges - 1ull) / total); }
+};
+
+// Scratch: per (slot, query head) the DP sums of p . v, then the maximum and the sum. The part of sequence b in share w has
 // slot w + b (one of the two grows from a part to the next).
 template <int DP> struct PagedScratch {
     float* stats;
@@ -114,63 +133,42 @@ template <class T> __device__ __forceinline__ void paged_store4(T* to, const f32
     }
 }
 
-// grid: ceil(ranges x KV heads x row tiles / kPagedWaves), 256 threads
-template <class T, int DP, uint32_t KEYS>
-__device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint32_t ranges, float* __restrict__ scratch) {
-    constexpr bool BF16 = sizeof(T) == 2;
-    constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
-    constexpr uint32_t WAVE = 2u * KEYS * DP;
-    constexpr int COPIES = KEYS * DP * sizeof(T) / 1024, PARTS = PER_ROW / 4u, TILES = KEYS / 16;
-    constexpr uint32_t SWZ = PER_ROW % 8u == 0 ? 7u : 3u;  // chunk c of row r lies at c ^ ((r / 2) & SWZ)
+// One wave's pass over key blocks of one sequence, 16 query heads of a KV head: (maximum, sum, p . v) of what they hold.
+// ``ks`` and ``vs``: LDS of KEYS rows of DP values each. Lane (quad, col) ends up with values 16 dt + 4 quad .. + 3 of head
+// ``col`` in o[dt], and that head's maximum and sum.
+template <class T, int DP, uint32_t KEYS> struct PagedWave {
+    static constexpr bool BF16 = sizeof(T) == 2;
+    static constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
+    static constexpr int COPIES = KEYS * DP * sizeof(T) / 1024, PARTS = PER_ROW / 4u, TILES = KEYS / 16;
+    static constexpr uint32_t SWZ = PER_ROW % 8u == 0 ? 7u : 3u;  // chunk c of row r lies at c ^ ((r / 2) & SWZ)
+    static constexpr uint32_t ELEMENTS = 2u * KEYS * DP;          // of LDS
     static_assert(PER_ROW % 4u == 0 && 64u % PER_ROW == 0 && KEYS <= 64u && KEYS % (BF16 ? 32u : 16u) == 0, "block");
-    __shared__ __attribute__((aligned(1024))) T lds[kPagedWaves * WAVE];
-    const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
-    const uint32_t tiles = (a.group + 15u) / 16u, heads = a.kv_heads * tiles, worker = blockIdx.x * kPagedWaves + wave;
-    const uint32_t w = worker / heads, kv = worker % heads / tiles, row0 = worker % heads % tiles * 16u, chunks = a.dim / CHUNK;
-    const float neg_inf = -__builtin_inff();
-    T* ks = lds + wave * WAVE;
-    T* vs = ks + KEYS * DP;
-    const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, a.kv_heads * a.group);
 
-    // This wave's share of the blocks, and the sequence b and its block n at which it begins.
-    const uint32_t total_blocks = paged_total<KEYS>(a), share = (total_blocks + ranges - 1u) / ranges;
-    if (uint64_t(w) * share >= total_blocks) {
-        return;
-    }
-    const uint32_t begin = w * share;
-    uint32_t left = total_blocks - begin < share ? total_blocks - begin : share, b = 0, n = 0;
-    for (uint32_t before = 0, b0 = 0; b0 < a.sequences; b0 += kWave) {
-        const uint32_t own = b0 + lane < a.sequences ? paged_blocks<KEYS>(paged_range(a, b0 + lane)) : 0u;
-        const uint32_t upto = before + paged_scan(own);
-        const unsigned long long past = __ballot(upto > begin);
-        if (past) {
-            const uint32_t at = __builtin_ctzll(past);
-            b = b0 + at;
-            n = begin - __builtin_amdgcn_readlane(upto - own, at);
-            break;
-        }
-        before = __builtin_amdgcn_readlane(upto, kWave - 1);
-    }
-    if (chunks < PER_ROW) {
-        for (uint32_t c = lane; c < 2u * KEYS * PER_ROW; c += 64u) {
-            *reinterpret_cast<uint4*>(ks + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
-        }
-        __builtin_amdgcn_s_waitcnt(0);  // before copies into the same places
-    }
-    const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
-    const T* k_pages = a.k + kv * a.head_stride;
-    const T* v_pages = a.v + kv * a.head_stride;
+    float peak, total;
+    f32x4_t o[DP / 16];
 
-    for (; left; ++b, n = 0) {
-        const PagedRange range = paged_range(a, b);
+    // Zeros behind the rows' ends, once, before the first copies.
+    static __device__ __forceinline__ void prepare(const PagedOperands<T>& a, T* ks) {
+        if (a.dim < uint32_t(DP)) {
+            for (uint32_t c = threadIdx.x % 64u; c < 2u * KEYS * PER_ROW; c += 64u) {
+                *reinterpret_cast<uint4*>(ks + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
+            }
+            __builtin_amdgcn_s_waitcnt(0);
+        }
+    }
+
+    // Blocks n, n + step, ... below stop of sequence b, KV head kv, query head ``head`` in this lane's column.
+    __device__ __forceinline__ void run(const PagedOperands<T>& a, const PagedRange& range, uint32_t b, uint32_t kv, uint32_t head, uint32_t n,
+                                        uint32_t stop, uint32_t step, T* ks, T* vs) {
+        const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u, chunks = a.dim / CHUNK;
+        const float neg_inf = -__builtin_inff();
+        const T* k_pages = a.k + kv * a.head_stride;
+        const T* v_pages = a.v + kv * a.head_stride;
         const T* q = a.q + b * a.q_stride + uint64_t(head) * a.dim;
         const T* k_new = a.k_new + b * a.new_stride + uint64_t(kv) * a.dim;
         const T* v_new = a.v_new + b * a.new_stride + uint64_t(kv) * a.dim;
         const int64_t* table = a.table + b * a.table_stride;
-        const uint32_t head_blocks = (range.head + KEYS - 1u) / KEYS, blocks = paged_blocks<KEYS>(range);
-        const uint32_t count = blocks - n < left ? blocks - n : left, stop = n + count;
-        left -= count;
+        const uint32_t head_blocks = (range.head + KEYS - 1u) / KEYS;
         auto block_begin = [&](uint32_t x) { return x < head_blocks ? x * KEYS : range.low + (x - head_blocks) * KEYS; };
         auto block_end = [&](uint32_t x) { return x < head_blocks ? range.head : range.end; };
         // The page of this lane's row of block x (-1: none).
@@ -197,7 +195,9 @@ __device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint3
                 }
             }
         };
-        copy(n, page_of(n));
+        if (n < stop) {
+            copy(n, page_of(n));
+        }
         uint4 qf[PARTS];
 #pragma unroll
         for (int c = 0; c < PARTS; ++c) {
@@ -206,14 +206,14 @@ __device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint3
                 qf[c] = *reinterpret_cast<const uint4*>(q + (c * 4u + quad) * CHUNK);
             }
         }
-        float peak = neg_inf, total = 0.0f;
-        f32x4_t o[DP / 16];
+        peak = neg_inf;
+        total = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DP / 16; ++dt) {
             o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
         while (n < stop) {
-            const uint32_t next = n + 1u;
+            const uint32_t next = n + step;
             int64_t next_page = -1;
             if (next < stop) {
                 next_page = page_of(next);
@@ -324,28 +324,129 @@ __device__ __forceinline__ void attention_paged(const PagedOperands<T>& a, uint3
         }
         total += __shfl_xor(total, 16, kWave);
         total += __shfl_xor(total, 32, kWave);
-        const bool mine = row0 + col < a.group;
+    }
+
+    // The finished row of this lane's head, the sink added, in place.
+    __device__ __forceinline__ void finish(const PagedOperands<T>& a, uint32_t b, uint32_t head) {
+        const uint32_t quad = threadIdx.x % 64u / 16u;
+        const float sink = a.sinks ? paged_widen<T>(a.sinks[head]) : -__builtin_inff();
+        const FlashMerge merge{__builtin_fmaxf(peak, sink), 0.0f};
+        const float weight = merge.weight(peak), sum = weight * total + (a.sinks ? merge.weight(sink) : 0.0f);
+        const float factor = sum == 0.0f ? 0.0f : weight / sum;
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; ++dt) {
+            if (dt * 16u + quad * 4u < a.dim) {
+                paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + dt * 16u + quad * 4u, o[dt] * factor);
+            }
+        }
+    }
+};
+
+// One workgroup of WAVES waves for all blocks of a sequence and KV head: the waves take blocks in turn and meet in LDS.
+// grid: (KV heads x row tiles, sequences)
+template <class T, int DP, uint32_t KEYS, uint32_t WAVES> __device__ __forceinline__ void attention_paged_whole(const PagedOperands<T>& a) {
+    using Wave = PagedWave<T, DP, KEYS>;
+    constexpr uint32_t OPAD = DP + 4u, PART = Wave::ELEMENTS * sizeof(T) / 4u;  // floats of a wave's LDS
+    static_assert(16u * (OPAD + 2u) <= PART, "a wave's sums fit its LDS");
+    __shared__ __attribute__((aligned(1024))) T lds[WAVES * Wave::ELEMENTS];
+    const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t tiles = (a.group + 15u) / 16u, kv = blockIdx.x / tiles, row0 = blockIdx.x % tiles * 16u, b = blockIdx.y;
+    const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
+    T* ks = lds + wave * Wave::ELEMENTS;
+    const PagedRange range = paged_range(a, b);
+    Wave x;
+    Wave::prepare(a, ks);
+    x.run(a, range, b, kv, head, wave, paged_blocks<KEYS>(range), WAVES, ks, ks + KEYS * DP);
+    float* mine = reinterpret_cast<float*>(ks);
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+        *reinterpret_cast<f32x4_t*>(mine + col * OPAD + dt * 16u + quad * 4u) = x.o[dt];
+    }
+    if (quad == 0) {
+        mine[16u * OPAD + 2u * col] = x.peak;
+        mine[16u * OPAD + 2u * col + 1u] = x.total;
+    }
+    __syncthreads();
+    const float* parts = reinterpret_cast<const float*>(lds);
+    for (uint32_t i = threadIdx.x; i < 16u * (DP / 4u); i += 64u * WAVES) {
+        const uint32_t r = i / (DP / 4u), d = i % (DP / 4u) * 4u;
+        if (row0 + r >= a.group || d >= a.dim) {
+            continue;
+        }
+        const uint32_t row = kv * a.group + row0 + r;
+        const float sink = a.sinks ? paged_widen<T>(a.sinks[row]) : -__builtin_inff();
+        FlashMerge merge{sink, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            merge.top = __builtin_fmaxf(merge.top, parts[w * PART + 16u * OPAD + 2u * r]);
+        }
+        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            const float weight = merge.weight(parts[w * PART + 16u * OPAD + 2u * r]);
+            merge.total += weight * parts[w * PART + 16u * OPAD + 2u * r + 1u];
+            sum += weight * *reinterpret_cast<const f32x4_t*>(parts + w * PART + r * OPAD + d);
+        }
+        merge.total += a.sinks ? merge.weight(sink) : 0.0f;
+        paged_store4<T>(a.out + b * a.out_stride + uint64_t(row) * a.dim + d, sum * (merge.total == 0.0f ? 0.0f : 1.0f / merge.total));
+    }
+}
+
+// The blocks of all sequences in equal shares.
+// grid: ceil(ranges x KV heads x row tiles / kPagedWaves), 256 threads
+template <class T, int DP, uint32_t KEYS>
+__device__ __forceinline__ void attention_paged_shares(const PagedOperands<T>& a, uint32_t ranges, float* __restrict__ scratch) {
+    using Wave = PagedWave<T, DP, KEYS>;
+    __shared__ __attribute__((aligned(1024))) T lds[kPagedWaves * Wave::ELEMENTS];
+    const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t tiles = (a.group + 15u) / 16u, heads = a.kv_heads * tiles, worker = blockIdx.x * kPagedWaves + wave;
+    const uint32_t w = worker / heads, kv = worker % heads / tiles, row0 = worker % heads % tiles * 16u;
+    T* ks = lds + wave * Wave::ELEMENTS;
+    const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, uint64_t(a.kv_heads) * a.group);
+
+    // This wave's share of the blocks, and the sequence b and its block n at which it begins.
+    const PagedShares shares(paged_total<KEYS>(a), ranges);
+    if (w >= shares.ranges) {
+        return;
+    }
+    const uint32_t begin = shares.begin(w);
+    uint32_t left = shares.begin(w + 1u) - begin, b = 0, n = 0;
+    for (uint32_t before = 0, b0 = 0; b0 < a.sequences; b0 += kWave) {
+        const uint32_t own = b0 + lane < a.sequences ? paged_blocks<KEYS>(paged_range(a, b0 + lane)) : 0u;
+        const uint32_t upto = before + paged_scan(own);
+        const unsigned long long past = __ballot(upto > begin);
+        if (past) {
+            const uint32_t at = __builtin_ctzll(past);
+            b = b0 + at;
+            n = begin - __builtin_amdgcn_readlane(upto - own, at);
+            break;
+        }
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    Wave::prepare(a, ks);
+    const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
+    for (; left; ++b, n = 0) {
+        const PagedRange range = paged_range(a, b);
+        const uint32_t blocks = paged_blocks<KEYS>(range), count = blocks - n < left ? blocks - n : left;
+        left -= count;
+        Wave x;
+        x.run(a, range, b, kv, head, n, n + count, 1u, ks, ks + KEYS * DP);
+        if (row0 + col >= a.group) {
+            continue;
+        }
         if (count == blocks) {
-            const FlashMerge merge{__builtin_fmaxf(peak, a.sinks ? paged_widen<T>(a.sinks[head]) : neg_inf), 0.0f};
-            const float weight = merge.weight(peak), sum = weight * total + (a.sinks ? merge.weight(paged_widen<T>(a.sinks[head])) : 0.0f);
-            const float factor = sum == 0.0f ? 0.0f : weight / sum;
+            x.finish(a, b, head);
+            continue;
+        }
+        const uint64_t at = uint64_t(w + b) * a.kv_heads * a.group + head;
 #pragma unroll
-            for (int dt = 0; dt < DP / 16; ++dt) {
-                if (mine && dt * 16u + quad * 4u < a.dim) {
-                    paged_store4<T>(a.out + b * a.out_stride + uint64_t(head) * a.dim + dt * 16u + quad * 4u, o[dt] * factor);
-                }
-            }
-        } else {
-            const uint64_t at = uint64_t(w + b) * a.kv_heads * a.group + head;
-#pragma unroll
-            for (int dt = 0; dt < DP / 16; ++dt) {
-                if (mine && dt * 16u + quad * 4u < a.dim) {
-                    *reinterpret_cast<f32x4_t*>(parts.sums + at * DP + dt * 16u + quad * 4u) = o[dt];
-                }
-            }
-            if (mine && quad == 0) {
-                *reinterpret_cast<float2*>(parts.stats + 2u * at) = float2{peak, total};
-            }
+        for (int dt = 0; dt < DP / 16; ++dt) {
+            *reinterpret_cast<f32x4_t*>(parts.sums + at * DP + dt * 16u + quad * 4u) = x.o[dt];
+        }
+        if (quad == 0) {
+            *reinterpret_cast<float2*>(parts.stats + 2u * at) = float2{x.peak, x.total};
         }
     }
 }
@@ -370,8 +471,8 @@ __device__ __forceinline__ void attention_paged_combine(const PagedOperands<T>& 
     }
     all = __builtin_amdgcn_readlane(paged_scan(all), kWave - 1);
     before = __builtin_amdgcn_readlane(paged_scan(before), kWave - 1);
-    const uint32_t share = (all + ranges - 1u) / ranges, own = paged_blocks<KEYS>(paged_range(a, b));
-    const uint32_t first = before / share, count = (before + own - 1u) / share - first + 1u;
+    const PagedShares shares(all, ranges);
+    const uint32_t first = shares.of(before), count = shares.of(before + paged_blocks<KEYS>(paged_range(a, b)) - 1u) - first + 1u;
     if (count == 1u) {
         return;  // written by its wave
     }

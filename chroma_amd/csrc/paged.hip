@@ -14,9 +14,14 @@ namespace {
 
 using Call = chroma_hip_paged_attention_call;
 
+template <class T, int DP, uint32_t KEYS, uint32_t WAVES>
+__global__ void __launch_bounds__(64 * WAVES) paged_attention_whole(chroma::PagedOperands<T> a) {
+    chroma::attention_paged_whole<T, DP, KEYS, WAVES>(a);
+}
+
 template <class T, int DP>
-__global__ void __launch_bounds__(256) paged_attention(chroma::PagedOperands<T> a, uint32_t ranges, float* scratch) {
-    chroma::attention_paged<T, DP, chroma::paged_keys<T, DP>()>(a, ranges, scratch);
+__global__ void __launch_bounds__(256) paged_attention_shares(chroma::PagedOperands<T> a, uint32_t ranges, float* scratch) {
+    chroma::attention_paged_shares<T, DP, chroma::paged_keys<T, DP>()>(a, ranges, scratch);
 }
 
 template <class T, int DP, uint32_t WAVES>
@@ -105,45 +110,55 @@ template <class T> chroma::PagedOperands<T> operands(const Call& c) {
 // Whether a call of these types and head dimension runs on the kernels of padded dimension DP.
 template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP == (sizeof(T) == 2 ? 32 : 16) || c.dim > DP / 2); }
 
-// How a call is cut: the most blocks a sequence can have, and the shares that all of them are cut into, as many as bring
-// kWaves waves.
-constexpr int64_t kWaves = 2048;
+// How a call is cut. Up to kPasses key blocks for every wave of a sequence's workgroup one launch takes whole sequences: 8 KV
+// heads of 8 heads of 64, us for whole sequences and for shares: one of 900 rows 8.9 and 11.3, of 1400 10.5 and 10.7, of
+// 2000 14.2 and 10.8; 8 mixed ones up to 900 9.2 and 11.8, up to 2000 15.8 and 14.8; 32 up to 900 11.3 and 16.5, up to 4096 36.8
+// and 33.2; 128 up to 1000 31 and 37, up to 2000 69 and 68. Beyond, all blocks are cut into as many shares as bring kWaves
+// waves, those that the chip holds at once: 1024 / 2048 / 4096 waves take 64 sequences of 8192 216 / 192 / 198 us and 32
+// mixed ones up to 4096 40 / 37 / 42.
+constexpr int64_t kPasses = 6, kWaves = 2048;
 struct Cut {
-    int64_t blocks, ranges, heads, tiles;
-    bool joined() const { return blocks > 1; }  // whether a sequence can lie in more than one share
+    int64_t heads, tiles;
+    int64_t ranges;  // shares; 0: whole sequences
 };
 template <class T, int DP> Cut cut_of(const Call& c) {
-    const int64_t keys = chroma::paged_keys<T, DP>();
     Cut cut;
     cut.tiles = (c.group + 15) / 16;
     cut.heads = c.kv_heads * c.group;
-    const int64_t rows = c.longest + 1;
-    cut.blocks = (rows + keys - 1) / keys;
-    if (c.window) {
-        const int64_t head = std::min(c.first, c.longest), seen = std::min(c.window, rows);
-        cut.blocks = std::min(cut.blocks + 1, (head + keys - 1) / keys + (seen + keys - 1) / keys);
-    }
+    // the most blocks of ``keys`` rows that a sequence can have
+    const auto most_blocks = [&](int64_t keys) {
+        const int64_t rows = c.longest + 1, blocks = (rows + keys - 1) / keys;
+        if (!c.window) {
+            return blocks;
+        }
+        return std::min(blocks + 1, (std::min(c.first, c.longest) + keys - 1) / keys + (std::min(c.window, rows) + keys - 1) / keys);
+    };
     const int64_t wanted = (kWaves + c.kv_heads * cut.tiles - 1) / (c.kv_heads * cut.tiles);
-    cut.ranges = std::min(wanted, c.sequences * cut.blocks);
+    cut.ranges = most_blocks(chroma::paged_whole_keys<T, DP>()) <= kPasses * int64_t(chroma::paged_whole_waves<T, DP>())
+                     ? 0
+                     : std::min(wanted, c.sequences * most_blocks(chroma::paged_keys<T, DP>()));
     return cut;
 }
 
 template <class T, int DP> size_t scratch_bytes(const Call& c) {
     const Cut cut = cut_of<T, DP>(c);
-    return cut.joined() ? size_t((cut.ranges + c.sequences) * cut.heads) * (DP + 2) * sizeof(float) : 0;
+    return cut.ranges ? size_t(cut.ranges + c.sequences) * size_t(cut.heads) * (DP + 2) * sizeof(float) : 0;
 }
 
 template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_t stream) {
     const Cut cut = cut_of<T, DP>(c);
     const chroma::PagedOperands<T> a = operands<T>(c);
-    const uint32_t ranges = uint32_t(cut.ranges);
-    const int64_t waves = cut.ranges * c.kv_heads * cut.tiles;
-    paged_attention<T, DP><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
-    if (!cut.joined()) {
+    if (!cut.ranges) {
+        const dim3 grid(unsigned(c.kv_heads * cut.tiles), unsigned(c.sequences));
+        constexpr uint32_t keys = chroma::paged_whole_keys<T, DP>(), waves = chroma::paged_whole_waves<T, DP>();
+        paged_attention_whole<T, DP, keys, waves><<<grid, 64 * waves, 0, stream>>>(a);
         return;
     }
+    const uint32_t ranges = uint32_t(cut.ranges);
+    const int64_t waves = cut.ranges * c.kv_heads * cut.tiles;
+    paged_attention_shares<T, DP><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
     const int64_t units = c.sequences * cut.heads;
-    if (cut.blocks > 64 && units < 2048) {
+    if (cut.ranges > 32 * c.sequences && units < 2048) {  // many parts and few heads: a workgroup for a head
         paged_attention_combine<T, DP, 4><<<unsigned(units), 256, 0, stream>>>(a, ranges, scratch);
     } else {
         paged_attention_combine<T, DP, 1><<<unsigned((units + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
