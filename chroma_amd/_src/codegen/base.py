@@ -181,6 +181,9 @@ class Codegen:
     def output(self, index: int, value: Value) -> None:
         raise NotImplementedError
 
+    def paged_attention(self, meta: torch.Tensor, *operands) -> Value:
+        raise NotImplementedError(f"paged attention on the {self.backend} backend")
+
 
 def literal(value: float) -> str:
     """A C++ float literal that round-trips ``value`` through float32."""

@@ -185,6 +185,7 @@ ERROR_REGION = 1024  # bytes of the error region: error word, router tickets, de
 ATTENTION_TICKETS = 64  # (query row, head) rows a split-key decode attention can serve (chroma::kAttentionTickets)
 NARROW_COLUMNS = 64  # linears of at most this many columns over many rows take one workgroup per 16 rows
 SMALL_INPUT_BYTES = 64 << 10  # inputs up to this size are staged ahead of the larger ones
+PAGED_PASSES, PAGED_WAVES = 6, 2048  # how attention over a paged cache is cut (kPasses and kWaves of csrc/paged.hip)
 MATRIX_ATTENTION_TOKENS = 64  # bfloat16 attention over at least this many queries runs on the matrix cores
 # query heads per wave of the grouped prefill attention (attention_heads): two share each K and V^T fragment
 # read from LDS, whose bandwidth bounds the one-head form; compiled for 3 resident workgroups per compute unit
@@ -2445,6 +2446,110 @@ class HIPCodegen(Codegen):
             table = k.slot(partial.name, torch.float32, extent=self.extents[partial.name])
             k.line(f"chroma::attention_combine<{dim}, {group}>({table} + {row} * {group * dim}u, {splits}u, store);")
             self.launch(k, (tokens, kv_heads, 1), 256, [partial], kind="attention_combine")
+        self.fused_attentions += 1
+        return out
+
+    @staticmethod
+    def _paged_keys(dim: int, item: int) -> Tuple[int, int, int, int]:
+        """(padded head dimension, keys of a block, keys and waves where a workgroup takes a whole sequence) of
+        ``attention_paged.h``."""
+        padded = next(n for n in (16, 32, 64, 128, 256) if n * item >= 64 and dim <= n)
+        least = 32 if item == 2 else 16
+        keys = max(least, min(64, 16384 // (2 * padded * item)))
+        half = max(least, keys // 2)
+        return padded, keys, half, 4 if half * padded * item > 8192 else 8
+
+    def paged_attention(self, meta, q: Value, k_pages: Value, v_pages: Value, k_new: Optional[Value], v_new: Optional[Value], table: Value,
+                        lengths: Value, sinks: Optional[Value], scale: float, window: int, first: int) -> Value:
+        """Attention of one new token per sequence over a paged cache (``chroma_amd::paged_attention``), cut as
+        ``chroma_hip_paged_attention`` cuts its calls (csrc/paged.hip, which says what each way measured)."""
+        sequences, kv_heads, group, dim = q.shape
+        pages, rows = k_pages.shape[:2]
+        if dim % 8 or dim > 256 or group > 1024 or max(sequences, kv_heads) > 65535:
+            raise NotImplementedError(f"paged attention of {sequences} sequences, {kv_heads} KV heads of {group} heads of {dim}")
+        item = ITEMSIZE[meta.dtype]
+        chunk = 16 // item
+
+        def in_place(value: Value) -> Value:
+            """``value`` where its rows can be read as they lie, else a row-major copy."""
+            stored, strides = self._in_place(value)
+            if stored is not None:
+                offset = stored.view.offset if stored.view.base is not None else 0
+                strides = [0 if size == 1 else stride for size, stride in zip(value.shape, strides)]
+                if (dim == 1 or strides[-1] == 1) and not any(x % chunk for x in [*strides[:-1], offset]):
+                    return value
+            return rows_of(value)
+
+        def rows_of(value: Value) -> Value:
+            """A row-major ``value`` that starts on 16 bytes."""
+            value = self.contiguous(value)
+            if value.view.base is not None and value.view.offset % chunk:
+                copied = self.allocate(value.shape, value.dtype)
+                self.map_kernel(copied, value)
+                return copied
+            return value
+
+        # K and V lie alike (strides of K serve both); q's and the new rows' heads are adjacent
+        k_pages, v_pages = in_place(k_pages), in_place(v_pages)
+        if list(self._operand(k_pages, k_pages.shape)[1]) != list(self._operand(v_pages, v_pages.shape)[1]):
+            k_pages, v_pages = rows_of(k_pages), rows_of(v_pages)
+        q, k_new, v_new = (None if value is None else rows_of(value) for value in (q, k_new, v_new))
+        table, lengths, sinks = (None if value is None else self.contiguous(value) for value in (table, lengths, sinks))
+        out = self.allocate(tuple(meta.shape), meta.dtype)
+        operands = {"q": q, "k": k_pages, "v": v_pages, "k_new": k_new, "v_new": v_new, "sinks": sinks, "table": table, "lengths": lengths}
+        plan = {name: self._operand(value, value.shape) for name, value in operands.items() if value is not None}
+        page_stride, row_stride, head_stride, _ = plan["k"][1]
+        longest = table.shape[1] * rows
+        most = 2**31 - 1
+        if sequences * (longest // 16 + 2) > most or pages > most or longest > most - 4096 or sequences * kv_heads * group > most:
+            raise NotImplementedError("paged attention of more rows than the kernels count")
+        ctype = ctype_of(meta.dtype)
+        padded, keys, half, waves = self._paged_keys(dim, item)
+        tiles = -(-group // 16)
+
+        def kernel() -> Kernel:
+            k = Kernel(1)
+            k.line(f"chroma::PagedOperands<{ctype}> a;")
+            slot = k.slot(out.name, out.dtype, writable=True, extent=self.extents[out.name])
+            k.line(f"a.out = {slot}; a.out_stride = {kv_heads * group * dim}u;")
+            for name in operands:
+                if name not in plan:
+                    k.line(f"a.{name} = nullptr;")
+                    continue
+                value, _, offset = plan[name]
+                base = k.slot(value.root.name, value.root.dtype, extent=self.extents[value.root.name])
+                k.line(f"a.{name} = {base} + {offset}ull;")
+            k.line(f"a.page_stride = {page_stride}ull; a.row_stride = {row_stride}ull; a.head_stride = {head_stride}ull;")
+            k.line(f"a.q_stride = {kv_heads * group * dim}u; a.new_stride = {kv_heads * dim}u; a.table_stride = {table.shape[1]}u;")
+            k.line(f"a.pages = {pages}u; a.page_rows = {rows}u; a.longest = {longest}u; a.window = {min(window, most)}u; a.first = {min(first, most)}u;")
+            k.line(f"a.sequences = {sequences}u; a.kv_heads = {kv_heads}u; a.group = {group}u; a.dim = {dim}u; a.scale = {float_literal(scale)};")
+            return k
+
+        def most_blocks(size: int) -> int:
+            blocks = -(-(longest + 1) // size)
+            if not window:
+                return blocks
+            return min(blocks + 1, -(-min(first, longest) // size) + -(-min(window, longest + 1) // size))
+
+        inputs = [entry[0] for entry in plan.values()]
+        if most_blocks(half) <= PAGED_PASSES * waves:
+            k = kernel()
+            k.line(f"chroma::attention_paged_whole<{ctype}, {padded}, {half}u, {waves}u>(a);")
+            self.launch(k, (kv_heads * tiles, sequences, 1), 64 * waves, inputs, kind="attention_paged")
+        else:
+            ranges = min(-(-PAGED_WAVES // (kv_heads * tiles)), sequences * most_blocks(keys))
+            partial = self.allocate(((ranges + sequences) * kv_heads * group * (padded + 2),), torch.float32)
+            for combine in (False, True):
+                k = kernel()
+                scratch = k.slot(partial.name, torch.float32, writable=True, extent=self.extents[partial.name])
+                if combine:
+                    units = sequences * kv_heads * group
+                    per = 4 if ranges > 32 * sequences and units < 2048 else 1
+                    k.line(f"chroma::attention_paged_combine<{ctype}, {padded}, {keys}u, {per}u>(a, {ranges}u, {scratch});")
+                    self.launch(k, (units if per == 4 else -(-units // 4), 1, 1), 256, inputs + [partial], kind="attention_paged_combine")
+                else:
+                    k.line(f"chroma::attention_paged_shares<{ctype}, {padded}, {keys}u>(a, {ranges}u, {scratch});")
+                    self.launch(k, (-(-ranges * kv_heads * tiles // 4), 1, 1), 256, inputs, kind="attention_paged")
         self.fused_attentions += 1
         return out
 

@@ -37,6 +37,7 @@ import numpy as np
 from chroma_amd._src import host
 from chroma_amd._src.dtypes import BFLOAT16, numpy_dtype
 from chroma_amd._src.program import NativeModel, Program
+from chroma_amd._src.rules import TokenRules
 
 SELECT_MAX_K = 1024  # largest k the runtime's row selection takes (chroma_hip_rows_topk)
 
@@ -343,10 +344,13 @@ class Decoder:
         logits, _, _ = self._consume(tokens, keep_logits=False)
         return logits
 
-    def append_top(self, tokens: Any, k: int = 1, *, allowed: Any = None) -> Tuple[np.ndarray, np.ndarray]:
+    def append_top(self, tokens: Any, k: int = 1, *, allowed: Any = None, rules: Optional[TokenRules] = None) -> Tuple[np.ndarray, np.ndarray]:
         """Consume new token ids like ``append`` and return the ``k`` largest logits after the last one
         with their token ids, largest first: NaN outranks every number and ties go to the lower id (the
-        reference GPU backend's top-k rule). ``allowed`` (token ids) restricts the choice to those ids.
+        reference GPU backend's top-k rule). ``allowed`` (token ids) restricts the choice to those ids;
+        ``rules`` (penalties for repeated tokens, biases, allowed tokens) adjust the logits first, and the
+        values returned are the adjusted ones. The two are given one at a time (rules have an ``allowed`` of
+        their own: its other tokens count as -inf and can still be returned where k exceeds it).
 
         With hip programs the logits never leave the device: the runtime's row selection runs on the step's
         own stream right after it, under the step's one synchronization, and only the ``k`` values and ids
@@ -356,6 +360,10 @@ class Decoder:
         the reference API: its chat script samples from the downloaded row, scripts/chat.py:82-98.)"""
         if not isinstance(k, (int, np.integer)) or k < 1:
             raise ValueError(f"k must be a positive integer, got {k!r}")
+        if rules is not None:
+            if allowed is not None:
+                raise ValueError("allowed tokens go into the rules where rules are given")
+            rules.check(self.vocab_size)
         ids = None
         if allowed is not None:
             ids = np.unique(np.asarray(allowed))
@@ -369,8 +377,11 @@ class Decoder:
         device = self._on_device and isinstance(self._models[1].native, NativeModel)
         with self._lock:  # the step's device logits stay this step's until the selection has read them
             if device and ids is None and k <= SELECT_MAX_K:
-                _, _, (values, picks) = self._consume(tokens, keep_logits=True, top=int(k))
+                _, _, (values, picks) = self._consume(tokens, keep_logits=True, top=int(k), rules=rules)
                 return values[0].copy(), picks[0].copy()
+            if rules is not None:  # other programs, or more tokens than the row selection takes
+                logits, _, _ = self._consume(tokens, keep_logits=False)
+                return _select_host(rules.apply(logits[0]), int(k), None)
             logits, which, _ = self._consume(tokens, keep_logits=device)
             if not device:
                 return _select_host(logits[0], int(k), ids)
@@ -388,10 +399,10 @@ class Decoder:
             selector.run_resident([None, ids], [values, picks])
             return values[0].copy(), ids[picks[0]]
 
-    def greedy(self, tokens: Any, *, allowed: Any = None) -> int:
+    def greedy(self, tokens: Any, *, allowed: Any = None, rules: Optional[TokenRules] = None) -> int:
         """Consume new token ids and return the id of the largest logit after the last one (``append_top``
         with k = 1)."""
-        return int(self.append_top(tokens, 1, allowed=allowed)[1][0])
+        return int(self.append_top(tokens, 1, allowed=allowed, rules=rules)[1][0])
 
     def _selector(self, k: int, candidates: Optional[int]) -> Program:
         """The hip program selecting the top ``k`` of a logits row (of ``candidates`` gathered ids), compiled
@@ -416,11 +427,12 @@ class Decoder:
             self._selectors[key] = program
         return program
 
-    def _consume(self, tokens: Any, *, keep_logits: bool, top: Optional[int] = None) -> Tuple[Optional[np.ndarray], int, Any]:
+    def _consume(self, tokens: Any, *, keep_logits: bool, top: Optional[int] = None,
+                 rules: Optional[TokenRules] = None) -> Tuple[Optional[np.ndarray], int, Any]:
         """Run the steps for ``tokens``; return the last step's logits (None when ``keep_logits`` leaves
         them in the device output of the program that ran it), that program's index, and, when ``top`` is
-        given (device mode), the (values, ids) of the last step's ``top`` largest logits selected on the
-        device after it."""
+        given (device mode), the (values, ids) of the last step's ``top`` largest logits, adjusted by
+        ``rules``, selected on the device after it."""
         ids = np.asarray(tokens)
         if ids.ndim != 1 or not len(ids):
             raise ValueError(f"append wants a nonempty 1-D sequence of token IDs, got shape {ids.shape}")
@@ -475,7 +487,8 @@ class Decoder:
                         inputs = list(args)
                         inputs[4] = inputs[5] = None  # the masks built on the device above
                     if top is not None and offset + count == len(ids):
-                        selection = self._models[which].run_top_resident(inputs, [logits, *updates, *extras], 0, top)
+                        chosen = {} if rules is None else {"rules": [rules]}
+                        selection = self._models[which].run_top_resident(inputs, [logits, *updates, *extras], 0, top, **chosen)
                     else:
                         self._models[which].run_resident(inputs, [logits, *updates, *extras])
                     with _interrupts_deferred():

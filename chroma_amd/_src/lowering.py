@@ -28,6 +28,7 @@ from typing import Any, Dict, List, Sequence, Tuple, Union
 
 import torch
 
+import chroma_amd.ops  # noqa: F401  (registers the operators that exported files may hold)
 from chroma_amd._src.dtypes import round_bf16
 from chroma_amd._src.value import FLOAT_DTYPES, Value, View, axis, contiguous_strides
 
@@ -95,6 +96,7 @@ OPERATIONS.update(
         "aten.triu.default": "triangular",
         "aten.tril.default": "triangular",
         "aten._assert_tensor_metadata.default": "metadata",
+        "chroma_amd.paged_attention.default": "paged_attention",  # the package's own operator (chroma_amd/ops.py)
     }
 )
 
@@ -300,6 +302,12 @@ def lower(codegen, target: Any, meta: Any, args: Tuple[Any, ...], kwargs: Dict[s
         vector = meta[0].new_empty((1,), dtype=x.dtype)
         values, indices = codegen.topk([part.new_empty((1,)) for part in meta], codegen.reshape(vector, x), 0, largest, sort)
         return codegen.reshape(meta[0], values), codegen.reshape(meta[1], indices)
+    if family == "paged_attention":
+        if meta.dtype not in FLOAT_DTYPES:
+            raise NotImplementedError(name)
+        names = ("q", "k_pages", "v_pages", "k_new", "v_new", "table", "lengths", "sinks", "scale", "window", "first")
+        *operands, scale, window, first = (_arg(args, kwargs, i, n, 0 if n in ("window", "first") else None) for i, n in enumerate(names))
+        return codegen.paged_attention(meta, *operands, float(scale), window, first)
     if family == "cat":
         return codegen.concatenate(meta, args[0], axis(_arg(args, kwargs, 1, "dim", 0), len(meta.shape)))
     if family == "triangular":

@@ -151,6 +151,10 @@ def library() -> ctypes.CDLL:
         lib.chroma_hip_cache_move.argtypes = [c.POINTER(CacheRows), c.POINTER(CacheRows), c.c_int64, c.c_int64, c.c_void_p, c.c_int64, c.c_void_p,
                                               c.c_char_p, c.c_size_t]
         lib.chroma_hip_rows_adjust.argtypes = [c.POINTER(Adjust), c.c_void_p, c.c_char_p, c.c_size_t]
+        lib.chroma_hip_cache_move_queued.argtypes = [c.c_void_p, c.POINTER(CacheRows), c.POINTER(CacheRows), c.c_int64, c.c_int64, c.c_void_p,
+                                                     c.c_int64, c.c_char_p, c.c_size_t]
+        lib.chroma_hip_run_top_adjusted.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_int, c.c_int, c.c_size_t, c.c_size_t,
+                                                    c.POINTER(Adjust), c.c_int, c.c_void_p, c.c_void_p, c.c_char_p, c.c_size_t]
         _library = lib
         return lib
 
@@ -185,7 +189,9 @@ EXPORTED = (
     "chroma_hip_paged_attention_workspace",
     "chroma_hip_paged_attention",
     "chroma_hip_cache_move",
+    "chroma_hip_cache_move_queued",
     "chroma_hip_rows_adjust",
+    "chroma_hip_run_top_adjusted",
 )
 
 

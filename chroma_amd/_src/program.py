@@ -22,6 +22,7 @@ import numpy as np
 
 from chroma_amd._src import host, native
 from chroma_amd._src.dtypes import BFLOAT16, numpy_dtype
+from chroma_amd._src.rules import TokenRules, pack
 from chroma_amd._src.spec import MANIFEST_VERSION, signature
 
 Array = np.ndarray
@@ -106,11 +107,13 @@ class NativeModel:
         error = ctypes.create_string_buffer(1024)
         native.check(self._lib.chroma_hip_run(self._handle, ins, outs, error, len(error)), error)
 
-    def run_top(self, inputs: List[Optional[np.ndarray]], outputs: List[Optional[np.ndarray]], index: int, k: int) -> Tuple[np.ndarray, np.ndarray]:
+    def run_top(self, inputs: List[Optional[np.ndarray]], outputs: List[Optional[np.ndarray]], index: int, k: int,
+                rules: Optional[Sequence[TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
         """``run`` (resident: None keeps an input's device copy, and leaves an output on the device) that also
         selects the ``k`` largest values of each row of output ``index`` on the device, after the plan on
         the same stream and under the same synchronization; returns (values [rows, k], int64 ids [rows, k])
-        in page-locked host arrays."""
+        in page-locked host arrays. ``rules`` (one for each row) adjust the rows that the selection reads;
+        the output itself stays as it is."""
         spec = self._outputs[index]
         dtype = numpy_dtype(spec["dtype"])
         if dtype not in (np.dtype(np.float32), BFLOAT16) or not spec["shape"]:
@@ -122,8 +125,21 @@ class NativeModel:
         ids = host.empty((rows, k), np.int64)
         code = native.FLOAT32 if dtype == np.dtype(np.float32) else native.BFLOAT16
         error = ctypes.create_string_buffer(1024)
-        status = self._lib.chroma_hip_run_top(self._handle, ins, outs, index, code, rows, width, k, values.ctypes.data, ids.ctypes.data,
-                                              error, len(error))
+        if rules is None:
+            status = self._lib.chroma_hip_run_top(self._handle, ins, outs, index, code, rows, width, k, values.ctypes.data, ids.ctypes.data,
+                                                  error, len(error))
+        else:
+            if len(rules) != rows:
+                raise ValueError(f"{len(rules)} rules for {rows} rows")
+            arrays = pack(rules, width)
+            call = native.Adjust(**{name: None if array is None else array.ctypes.data for name, array in arrays.items()})
+            if arrays["history"] is not None:
+                call.history_stride = call.history_width = arrays["history"].shape[1]
+            for name in ("bias", "mask"):
+                if arrays[name] is not None and len(arrays[name]) > 1:
+                    setattr(call, f"{name}_stride", arrays[name].shape[1])
+            status = self._lib.chroma_hip_run_top_adjusted(self._handle, ins, outs, index, code, rows, width, ctypes.byref(call), k,
+                                                           values.ctypes.data, ids.ctypes.data, error, len(error))
         native.check(status, error)
         return values, ids
 
@@ -146,6 +162,15 @@ class NativeModel:
         array = (native.Rect * len(rects))(*[native.Rect(*rect) for rect in rects])
         error = ctypes.create_string_buffer(256)
         native.check(self._lib.chroma_hip_copy_2d_batch_queued(self._handle, array, len(rects), error, len(error)), error)
+
+    def cache_move(self, to: native.CacheRows, source: native.CacheRows, layers: int, row_bytes: int, moves: np.ndarray) -> None:
+        """Copy rows of keys and values, in every layer, queued on this program's stream: ``moves`` [n, 3] holds
+        (first source row, first destination row, rows)."""
+        moves = np.ascontiguousarray(moves, dtype=np.int64).reshape(-1, 3)
+        error = ctypes.create_string_buffer(256)
+        status = self._lib.chroma_hip_cache_move_queued(self._handle, ctypes.byref(to), ctypes.byref(source), layers, row_bytes,
+                                                        moves.ctypes.data, len(moves), error, len(error))
+        native.check(status, error)
 
     def clear_input(self, index: int) -> None:
         """Zero input ``index``'s device staging, queued on this program's stream (see ``synchronize``)."""
@@ -294,14 +319,15 @@ class Program:
                 raise RuntimeError("Model is closed")
             self._model.run(arrays, list(outputs), resident=True)
 
-    def run_top_resident(self, inputs: Sequence[Optional[Array]], outputs: Sequence[Optional[Array]], index: int, k: int) -> Tuple[Array, Array]:
-        """``run_resident`` that also returns the ``k`` largest values of each row of output ``index`` and
-        their ids, selected on the device (``NativeModel.run_top``)."""
+    def run_top_resident(self, inputs: Sequence[Optional[Array]], outputs: Sequence[Optional[Array]], index: int, k: int,
+                         rules: Optional[Sequence[TokenRules]] = None) -> Tuple[Array, Array]:
+        """``run_resident`` that also returns the ``k`` largest values of each row of output ``index`` (adjusted by
+        ``rules``, if given) and their ids, selected on the device (``NativeModel.run_top``)."""
         arrays = [None if value is None else self._array(value) for value in inputs]
         with self._lock:
             if self._model is None:
                 raise RuntimeError("Model is closed")
-            return self._model.run_top(arrays, list(outputs), index, k)
+            return self._model.run_top(arrays, list(outputs), index, k) if rules is None else self._model.run_top(arrays, list(outputs), index, k, rules)
 
     @property
     def native(self) -> NativeModel:

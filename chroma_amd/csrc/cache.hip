@@ -2,7 +2,7 @@
 //
 // The moves travel as kernel arguments (up to kMoves a launch), so that nothing is uploaded and a captured call replays
 // them. What bounds it: a step's rows the launch, pages the memory (each byte read and written once).
-#include "../../include/chroma_hip.h"
+#include "cache.h"
 
 #include <hip/hip_runtime.h>
 
@@ -169,15 +169,24 @@ int move(const chroma_hip_cache_rows& to, const chroma_hip_cache_rows& from, int
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) int chroma_hip_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from,
-                                                                            int64_t layers, int64_t row_bytes, const int64_t* moves,
-                                                                            int64_t count, void* stream, char* error, size_t error_size) {
+namespace chroma_cache {
+
+int launch_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes,
+                      const int64_t* moves, int64_t count, hipStream_t stream, char* error, size_t error_size) {
     if (!to || !from) {
         return refuse("null cache", error, error_size);
     }
     try {
-        return move(*to, *from, layers, row_bytes, moves, count, static_cast<hipStream_t>(stream), error, error_size);
+        return move(*to, *from, layers, row_bytes, moves, count, stream, error, error_size);
     } catch (const std::exception& e) {
         return refuse(e.what(), error, error_size);
     }
+}
+
+}  // namespace chroma_cache
+
+extern "C" __attribute__((visibility("default"))) int chroma_hip_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from,
+                                                                            int64_t layers, int64_t row_bytes, const int64_t* moves,
+                                                                            int64_t count, void* stream, char* error, size_t error_size) {
+    return chroma_cache::launch_cache_move(to, from, layers, row_bytes, moves, count, static_cast<hipStream_t>(stream), error, error_size);
 }

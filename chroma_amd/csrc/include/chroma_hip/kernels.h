@@ -5,4 +5,5 @@
 #include "linear.h"
 #include "attention.h"
 #include "attention_flash.h"
+#include "attention_paged.h"
 #include "kwave.h"

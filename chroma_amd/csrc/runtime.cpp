@@ -5,6 +5,8 @@
 // arguments are pre-resolved device pointers. ``run`` uploads inputs, launches every kernel (or replays
 // the captured hipGraph), downloads the error word and the outputs, and synchronizes once.
 #include "../../include/chroma_hip.h"
+#include "adjust.h"
+#include "cache.h"
 #include "copy.h"
 #include "masks.h"
 #include "select.h"
@@ -366,10 +368,57 @@ public:
         }
     }
 
+    // The host arrays of ``rules`` (rows of ``width`` logits) one after another in page-locked memory, and the call that
+    // reads them at their places behind ``device``.
+    struct StagedRules {
+        size_t bytes = 0;
+        std::vector<std::pair<const void*, size_t>> pieces;  // host array (one row at a time where rows lie apart), bytes
+        chroma_hip_adjust_call call{};
+    };
+    static StagedRules stage_rules(const chroma_hip_adjust_call& rules, size_t rows, size_t width, char* device) {
+        StagedRules staged;
+        staged.call = rules;
+        auto place = [&](const void* array, size_t count, int64_t stride, size_t row_bytes, size_t item) -> char* {
+            if (!array) {
+                return nullptr;
+            }
+            char* at = device + staged.bytes;
+            for (size_t r = 0; r < count; ++r) {
+                staged.pieces.emplace_back(static_cast<const char*>(array) + r * size_t(stride) * item, row_bytes);
+            }
+            const size_t bytes = count * row_bytes, padding = (bytes + 15) / 16 * 16 - bytes;
+            if (padding) {
+                staged.pieces.emplace_back(nullptr, padding);
+            }
+            staged.bytes += bytes + padding;
+            return at;
+        };
+        if (rules.history && (rules.history_width < 0 || rules.history_stride < rules.history_width)) {
+            throw std::runtime_error("run_top_adjusted: a history row is longer than its stride");
+        }
+        const size_t words = (width + 31) / 32, history = rules.history ? size_t(rules.history_width) : 0;
+        if ((rules.bias && rules.bias_stride && (rules.bias_stride < 0 || size_t(rules.bias_stride) < width)) ||
+            (rules.mask && rules.mask_stride && (rules.mask_stride < 0 || size_t(rules.mask_stride) < words))) {
+            throw std::runtime_error("run_top_adjusted: a stride is smaller than its row");
+        }
+        staged.call.history = reinterpret_cast<const int64_t*>(place(rules.history, rows, rules.history_stride, history * 8, 8));
+        staged.call.history_stride = staged.call.history_width = int64_t(history);
+        staged.call.history_lengths = reinterpret_cast<const int64_t*>(place(rules.history_lengths, 1, 0, rows * 8, 8));
+        staged.call.repetition = reinterpret_cast<const float*>(place(rules.repetition, 1, 0, rows * 4, 4));
+        staged.call.presence = reinterpret_cast<const float*>(place(rules.presence, 1, 0, rows * 4, 4));
+        staged.call.frequency = reinterpret_cast<const float*>(place(rules.frequency, 1, 0, rows * 4, 4));
+        staged.call.bias = reinterpret_cast<const float*>(place(rules.bias, rules.bias_stride ? rows : 1, rules.bias_stride, width * 4, 4));
+        staged.call.bias_stride = rules.bias_stride ? int64_t(width) : 0;
+        staged.call.mask = reinterpret_cast<const uint32_t*>(place(rules.mask, rules.mask_stride ? rows : 1, rules.mask_stride, words * 4, 4));
+        staged.call.mask_stride = rules.mask_stride ? int64_t(words) : 0;
+        return staged;
+    }
+
     // ``run`` with a row selection over output ``index`` queued after the plan: only the k values and ids
     // of each row come back (and the outputs whose host pointers are non-null), after one synchronization.
-    void run_top(const void* const* inputs, void* const* outputs, int index, int dtype, size_t rows, size_t width, int k, void* values,
-                 int64_t* ids) {
+    // With ``rules`` the selection reads the output's rows adjusted by them.
+    void run_top(const void* const* inputs, void* const* outputs, int index, int dtype, size_t rows, size_t width,
+                 const chroma_hip_adjust_call* rules, int k, void* values, int64_t* ids) {
         DeviceGuard guard(device_);
         if (index < 0 || size_t(index) >= plan_.outputs.size()) {
             throw std::runtime_error("run_top: output index out of range");
@@ -389,8 +438,12 @@ public:
         const size_t value_bytes = rows * size_t(k) * item, id_bytes = rows * size_t(k) * sizeof(int64_t);
         // ids then values, adjacent, so one copy brings both back
         const size_t result_bytes = id_bytes + value_bytes;
-        const size_t need = align(scratch) + result_bytes;
-        if (need > select_bytes_ || result_bytes > select_host_bytes_) {
+        // behind them, with rules: the adjusted rows and the rules' arrays (these behind the results on the host too)
+        const size_t adjusted_at = align(align(scratch) + result_bytes), rules_at = adjusted_at + (rules ? align(rows * width * item) : 0);
+        const size_t rule_bytes = rules ? stage_rules(*rules, rows, width, nullptr).bytes : 0;
+        const size_t need = rules ? rules_at + rule_bytes : align(scratch) + result_bytes;
+        const size_t host_need = rules ? align(result_bytes) + rule_bytes : result_bytes;
+        if (need > select_bytes_ || host_need > select_host_bytes_) {
             check(hipStreamSynchronize(stream_), "Selection scratch");
             if (select_) {
                 check(hipFree(select_), "hipFree selection scratch");
@@ -405,22 +458,50 @@ public:
             drop_select_graph();
             check(hipMalloc(&select_, need), "hipMalloc selection scratch");
             select_bytes_ = need;
-            check(hipHostMalloc(&select_host_, result_bytes, hipHostMallocDefault), "hipHostMalloc selection results");
-            select_host_bytes_ = result_bytes;
+            check(hipHostMalloc(&select_host_, host_need, hipHostMallocDefault), "hipHostMalloc selection results");
+            select_host_bytes_ = host_need;
         }
         char* base = static_cast<char*>(select_);
         int64_t* device_ids = reinterpret_cast<int64_t*>(base + align(scratch));
         void* device_values = base + align(scratch) + id_bytes;
         try {
             upload(inputs);
-            const std::array<size_t, 6> key{size_t(index), size_t(dtype), rows, width, size_t(k), reinterpret_cast<size_t>(select_)};
-            launch_all_then(key, [&]() {
+            char* logits = static_cast<char*>(base_) + plan_.outputs[index].offset;
+            auto select = [&](const char* from) {
                 char message[256] = {0};
-                if (chroma_select::launch_rows_topk(static_cast<char*>(base_) + plan_.outputs[index].offset, dtype, rows, width, k, 1,
-                                                    device_values, device_ids, select_, scratch, stream_, message, sizeof(message))) {
+                if (chroma_select::launch_rows_topk(from, dtype, rows, width, k, 1, device_values, device_ids, select_, scratch, stream_,
+                                                    message, sizeof(message))) {
                     throw HipError(message);
                 }
-            });
+            };
+            if (rules) {
+                StagedRules staged = stage_rules(*rules, rows, width, base + rules_at);
+                char* at = static_cast<char*>(select_host_) + align(result_bytes);
+                for (const auto& piece : staged.pieces) {
+                    if (piece.first) {
+                        std::memcpy(at, piece.first, piece.second);
+                    }
+                    at += piece.second;
+                }
+                if (rule_bytes) {
+                    check(hipMemcpyAsync(base + rules_at, static_cast<char*>(select_host_) + align(result_bytes), rule_bytes,
+                                         hipMemcpyHostToDevice, stream_), "Upload rules");
+                }
+                launch_all();
+                staged.call.x = logits;
+                staged.call.y = base + adjusted_at;
+                staged.call.rows = int64_t(rows);
+                staged.call.width = staged.call.x_stride = staged.call.y_stride = int64_t(width);
+                staged.call.dtype = dtype;
+                char message[256] = {0};
+                if (chroma_adjust::launch_rows_adjust(staged.call, stream_, message, sizeof(message))) {
+                    throw HipError(message);
+                }
+                select(base + adjusted_at);
+            } else {
+                const std::array<size_t, 6> key{size_t(index), size_t(dtype), rows, width, size_t(k), reinterpret_cast<size_t>(select_)};
+                launch_all_then(key, [&]() { select(logits); });
+            }
             check(hipMemcpyAsync(error_host_, static_cast<char*>(base_) + plan_.error, sizeof(unsigned), hipMemcpyDeviceToHost, stream_),
                   "Read index error");
             check(hipMemcpyAsync(select_host_, device_ids, result_bytes, hipMemcpyDeviceToHost, stream_), "Download selection");
@@ -519,6 +600,16 @@ public:
         }
         if (plan_.inputs[index].bytes) {
             check(hipMemsetAsync(input_pointer(index), 0, plan_.inputs[index].bytes, stream_), "hipMemsetAsync");
+        }
+    }
+
+    // Queued copies of cache rows (cache.hip).
+    void cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes, const int64_t* moves,
+                    int64_t count) {
+        DeviceGuard guard(device_);
+        char message[256] = {0};
+        if (chroma_cache::launch_cache_move(to, from, layers, row_bytes, moves, count, stream_, message, sizeof(message))) {
+            throw std::runtime_error(message);
         }
     }
 
@@ -923,7 +1014,26 @@ __attribute__((visibility("default"))) int chroma_hip_run(void* handle, const vo
 __attribute__((visibility("default"))) int chroma_hip_run_top(void* handle, const void* const* inputs, void* const* outputs, int output_index,
                                                               int dtype, size_t rows, size_t width, int k, void* values, int64_t* ids,
                                                               char* error, size_t error_size) {
-    return guarded(error, error_size, [&] { program(handle)->run_top(inputs, outputs, output_index, dtype, rows, width, k, values, ids); });
+    return guarded(error, error_size,
+                   [&] { program(handle)->run_top(inputs, outputs, output_index, dtype, rows, width, nullptr, k, values, ids); });
+}
+
+__attribute__((visibility("default"))) int chroma_hip_run_top_adjusted(void* handle, const void* const* inputs, void* const* outputs,
+                                                                       int output_index, int dtype, size_t rows, size_t width,
+                                                                       const chroma_hip_adjust_call* rules, int k, void* values, int64_t* ids,
+                                                                       char* error, size_t error_size) {
+    return guarded(error, error_size, [&] {
+        if (!rules) {
+            throw std::runtime_error("run_top_adjusted: null rules");
+        }
+        program(handle)->run_top(inputs, outputs, output_index, dtype, rows, width, rules, k, values, ids);
+    });
+}
+
+__attribute__((visibility("default"))) int chroma_hip_cache_move_queued(void* handle, const chroma_hip_cache_rows* to,
+                                                                        const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes,
+                                                                        const int64_t* moves, int64_t count, char* error, size_t error_size) {
+    return guarded(error, error_size, [&] { program(handle)->cache_move(to, from, layers, row_bytes, moves, count); });
 }
 
 __attribute__((visibility("default"))) const char* chroma_hip_device_name(void* handle) { return program(handle)->name().c_str(); }

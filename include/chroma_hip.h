@@ -244,6 +244,11 @@ typedef struct chroma_hip_cache_rows {
 int chroma_hip_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes,
                           const int64_t* moves, int64_t count, void* stream, char* error, size_t error_size);
 
+/* The same moves queued on the program's stream, as ``chroma_hip_copy_2d_batch_queued``: they run before the program's
+ * later runs. Both caches lie in device memory of the program's device. */
+int chroma_hip_cache_move_queued(void* handle, const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers,
+                                 int64_t row_bytes, const int64_t* moves, int64_t count, char* error, size_t error_size);
+
 /* Logits made ready for the choice of a token, row by row, y = x with, in this order:
  *   - tokens that occur c > 0 times among the row's history: x > 0 ? x / repetition : x * repetition, then
  *     minus (presence + frequency * c);
@@ -270,6 +275,13 @@ typedef struct chroma_hip_adjust_call {
     int32_t dtype; /* of x and y: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
 } chroma_hip_adjust_call;
 int chroma_hip_rows_adjust(const chroma_hip_adjust_call* call, void* stream, char* error, size_t error_size);
+
+/* ``chroma_hip_run_top`` over adjusted logits: the rows of output ``output_index`` go through ``rules`` into scratch of the
+ * program (the output itself stays as it is), and the selection reads that. The arrays of ``rules`` are host memory, read
+ * before the call returns; its x, y, rows, width, x_stride, y_stride and dtype are the output's and are not read. */
+int chroma_hip_run_top_adjusted(void* handle, const void* const* inputs, void* const* outputs, int output_index, int dtype, size_t rows,
+                                size_t width, const chroma_hip_adjust_call* rules, int k, void* values, int64_t* ids, char* error,
+                                size_t error_size);
 
 #ifdef __cplusplus
 }
