@@ -2501,7 +2501,7 @@ class HIPCodegen(Codegen):
         page_stride, row_stride, head_stride, _ = plan["k"][1]
         longest = table.shape[1] * rows
         most = 2**31 - 1
-        if sequences * (longest // 16 + 2) > most or pages > most or longest > most - 4096 or sequences * kv_heads * group > most:
+        if sequences * (longest // 16 + 2) > most or pages > most or longest > most - 4096 or sequences * kv_heads * group > 2**24:
             raise NotImplementedError("paged attention of more rows than the kernels count")
         ctype = ctype_of(meta.dtype)
         padded, keys, half, waves = self._paged_keys(dim, item)
@@ -2548,7 +2548,8 @@ class HIPCodegen(Codegen):
                     k.line(f"chroma::attention_paged_combine<{ctype}, {padded}, {keys}u, {per}u>(a, {ranges}u, {scratch});")
                     self.launch(k, (units if per == 4 else -(-units // 4), 1, 1), 256, inputs + [partial], kind="attention_paged_combine")
                 else:
-                    k.line(f"chroma::attention_paged_shares<{ctype}, {padded}, {keys}u>(a, {ranges}u, {scratch});")
+                    stream = str(tiles == 1 and dim * item % 128 == 0).lower()
+                    k.line(f"chroma::attention_paged_shares<{ctype}, {padded}, {keys}u, {stream}>(a, {ranges}u, {scratch});")
                     self.launch(k, (-(-ranges * kv_heads * tiles // 4), 1, 1), 256, inputs, kind="attention_paged")
         self.fused_attentions += 1
         return out

@@ -250,6 +250,10 @@ const char* mistake(const chroma_hip_adjust_call& c) {
     if (c.rows < 1 || c.rows > 65535 || c.width < 1 || c.width >= int64_t(1) << 31) {
         return "want 1 to 65535 rows of 1 to 2147483647 logits";
     }
+    constexpr int64_t kStride = int64_t(1) << 40;
+    if (c.x_stride > kStride || c.y_stride > kStride || c.history_stride > kStride || c.bias_stride > kStride || c.mask_stride > kStride) {
+        return "a stride is out of range";
+    }
     if (c.x_stride < c.width || c.y_stride < c.width || (c.history && (c.history_width < 0 || c.history_stride < c.history_width)) ||
         (c.bias && c.bias_stride && c.bias_stride < c.width) || (c.mask && c.mask_stride && c.mask_stride < (c.width + 31) / 32)) {
         return "a stride is smaller than its row";

@@ -136,12 +136,14 @@ template <class T> __device__ __forceinline__ void paged_store4(T* to, const f32
 // One wave's pass over key blocks of one sequence, 16 query heads of a KV head: (maximum, sum, p . v) of what they hold.
 // ``ks`` and ``vs``: LDS of KEYS rows of DP values each. Lane (quad, col) ends up with values 16 dt + 4 quad .. + 3 of head
 // ``col`` in o[dt], and that head's maximum and sum.
-template <class T, int DP, uint32_t KEYS> struct PagedWave {
+// STREAM: the copies leave no room in the caches to what they bring (it is read once).
+template <class T, int DP, uint32_t KEYS, bool STREAM> struct PagedWave {
     static constexpr bool BF16 = sizeof(T) == 2;
     static constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
     static constexpr int COPIES = KEYS * DP * sizeof(T) / 1024, PARTS = PER_ROW / 4u, TILES = KEYS / 16;
     static constexpr uint32_t SWZ = PER_ROW % 8u == 0 ? 7u : 3u;  // chunk c of row r lies at c ^ ((r / 2) & SWZ)
     static constexpr uint32_t ELEMENTS = 2u * KEYS * DP;          // of LDS
+    static constexpr int AUX = STREAM ? 2 : 0;                    // the copies' cache policy
     static_assert(PER_ROW % 4u == 0 && 64u % PER_ROW == 0 && KEYS <= 64u && KEYS % (BF16 ? 32u : 16u) == 0, "block");
 
     float peak, total;
@@ -190,8 +192,8 @@ template <class T, int DP, uint32_t KEYS> struct PagedWave {
                 const T* k = (fresh ? k_new : k_pages + from) + chunk * CHUNK;
                 const T* v = (fresh ? v_new : v_pages + from) + chunk * CHUNK;
                 if (chunk < chunks) {
-                    __builtin_amdgcn_global_load_lds((global_void*)k, (lds_void*)(ks + i * (1024u / sizeof(T))), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((global_void*)v, (lds_void*)(vs + i * (1024u / sizeof(T))), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((global_void*)k, (lds_void*)(ks + i * (1024u / sizeof(T))), 16, 0, AUX);
+                    __builtin_amdgcn_global_load_lds((global_void*)v, (lds_void*)(vs + i * (1024u / sizeof(T))), 16, 0, AUX);
                 }
             }
         };
@@ -345,7 +347,7 @@ template <class T, int DP, uint32_t KEYS> struct PagedWave {
 // One workgroup of WAVES waves for all blocks of a sequence and KV head: the waves take blocks in turn and meet in LDS.
 // grid: (KV heads x row tiles, sequences)
 template <class T, int DP, uint32_t KEYS, uint32_t WAVES> __device__ __forceinline__ void attention_paged_whole(const PagedOperands<T>& a) {
-    using Wave = PagedWave<T, DP, KEYS>;
+    using Wave = PagedWave<T, DP, KEYS, false>;
     constexpr uint32_t OPAD = DP + 4u, PART = Wave::ELEMENTS * sizeof(T) / 4u;  // floats of a wave's LDS
     static_assert(16u * (OPAD + 2u) <= PART, "a wave's sums fit its LDS");
     __shared__ __attribute__((aligned(1024))) T lds[WAVES * Wave::ELEMENTS];
@@ -393,11 +395,13 @@ template <class T, int DP, uint32_t KEYS, uint32_t WAVES> __device__ __forceinli
     }
 }
 
-// The blocks of all sequences in equal shares.
+// The blocks of all sequences in equal shares. STREAM where a head's row is whole 128-byte lines and one wave reads it (the
+// other heads or row tiles of a line would fetch it again): 64 sequences of 8192 rows 206 -> 184 us (5.8 TB/s), six up to 131072
+// with heads of 128 345 -> 305 (6.3 TB/s; heads of 32, two to a line, 32 -> 36 us for 32 of 16384).
 // grid: ceil(ranges x KV heads x row tiles / kPagedWaves), 256 threads
-template <class T, int DP, uint32_t KEYS>
+template <class T, int DP, uint32_t KEYS, bool STREAM>
 __device__ __forceinline__ void attention_paged_shares(const PagedOperands<T>& a, uint32_t ranges, float* __restrict__ scratch) {
-    using Wave = PagedWave<T, DP, KEYS>;
+    using Wave = PagedWave<T, DP, KEYS, STREAM>;
     __shared__ __attribute__((aligned(1024))) T lds[kPagedWaves * Wave::ELEMENTS];
     const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);

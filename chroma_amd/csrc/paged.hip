@@ -19,9 +19,9 @@ __global__ void __launch_bounds__(64 * WAVES) paged_attention_whole(chroma::Page
     chroma::attention_paged_whole<T, DP, KEYS, WAVES>(a);
 }
 
-template <class T, int DP>
+template <class T, int DP, bool STREAM>
 __global__ void __launch_bounds__(256) paged_attention_shares(chroma::PagedOperands<T> a, uint32_t ranges, float* scratch) {
-    chroma::attention_paged_shares<T, DP, chroma::paged_keys<T, DP>()>(a, ranges, scratch);
+    chroma::attention_paged_shares<T, DP, chroma::paged_keys<T, DP>(), STREAM>(a, ranges, scratch);
 }
 
 template <class T, int DP, uint32_t WAVES>
@@ -52,7 +52,7 @@ const char* mistake(const Call& c) {
     if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest >= kMost - 4096) {
         return "pages, page_rows or longest out of range";
     }
-    if (c.sequences * (c.longest / 16 + 2) >= kMost || c.sequences * c.kv_heads * c.group >= kMost) {
+    if (c.sequences * (c.longest / 16 + 2) >= kMost || c.sequences * c.kv_heads * c.group > (int64_t(1) << 24)) {
         return "more sequences of this length, or more query heads, than the kernels count";
     }
     if (c.window < 0 || c.first < 0) {
@@ -156,7 +156,11 @@ template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_
     }
     const uint32_t ranges = uint32_t(cut.ranges);
     const int64_t waves = cut.ranges * c.kv_heads * cut.tiles;
-    paged_attention_shares<T, DP><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
+    if (cut.tiles == 1 && c.dim * sizeof(T) % 128 == 0) {
+        paged_attention_shares<T, DP, true><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
+    } else {
+        paged_attention_shares<T, DP, false><<<unsigned((waves + 3) / 4), 256, 0, stream>>>(a, ranges, scratch);
+    }
     const int64_t units = c.sequences * cut.heads;
     if (cut.ranges > 32 * c.sequences && units < 2048) {  // many parts and few heads: a workgroup for a head
         paged_attention_combine<T, DP, 4><<<unsigned(units), 256, 0, stream>>>(a, ranges, scratch);

@@ -220,7 +220,7 @@ typedef struct chroma_hip_paged_attention_call {
     int32_t dtype; /* of every value: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
 } chroma_hip_paged_attention_call;
 
-/* Scratch bytes the call needs (it depends on the extents only; 0 when none is needed or the call would be refused).
+/* Scratch bytes the call needs (no pointer matters; 0 when none is needed or the extents would be refused).
  * Calls that may run at the same time need workspaces of their own. */
 size_t chroma_hip_paged_attention_workspace(const chroma_hip_paged_attention_call* call);
 int chroma_hip_paged_attention(const chroma_hip_paged_attention_call* call, void* workspace, size_t workspace_bytes, void* stream,

@@ -303,6 +303,7 @@ def plain_attention_call(**changes):
     (dict(group=-1), "query heads"), (dict(dim=0), "head dimension"), (dict(dim=20), "head dimension"), (dict(dim=264), "head dimension"),
     (dict(pages=0), "pages"), (dict(page_rows=0), "page_rows"), (dict(longest=-1), "longest"), (dict(longest=2**31), "longest"),
     (dict(window=-1), "window"), (dict(first=-2), "first"), (dict(k_new=None), "k_new and v_new"), (dict(v_new=None), "k_new and v_new"),
+    (dict(sequences=60000, kv_heads=300), "more query heads"), (dict(sequences=40000, longest=2**21, table_stride=2**17), "more sequences"),
     (dict(table_stride=3), "table row"), (dict(longest=65), "table row"), (dict(q_stride=511), "stride"), (dict(out_stride=504), "stride"),
     (dict(new_stride=64), "stride"), (dict(row_stride=32), "stride"), (dict(head_stride=32), "stride"), (dict(page_stride=-2048), "stride"),
     (dict(q_stride=516), "16-byte"), (dict(page_stride=2052), "16-byte"), (dict(q=None), "null"), (dict(k_pages=None), "null"),
@@ -592,7 +593,7 @@ def plain_adjust_call(**changes):
 
 @pytest.mark.parametrize("changes,message", [
     (dict(dtype=5), "dtype"), (dict(rows=0), "rows"), (dict(rows=65536), "rows"), (dict(width=0), "logits"), (dict(width=2**31), "logits"),
-    (dict(x_stride=99), "stride"), (dict(y_stride=99), "stride"), (dict(history_stride=7), "stride"), (dict(history_width=-1), "stride"),
+    (dict(x_stride=2**62), "out of range"), (dict(history_stride=2**41), "out of range"), (dict(x_stride=99), "stride"), (dict(y_stride=99), "stride"), (dict(history_stride=7), "stride"), (dict(history_width=-1), "stride"),
     (dict(bias_stride=50), "stride"), (dict(mask_stride=3), "stride"), (dict(x=None), "null"), (dict(y=None), "null"),
     (dict(x=(1 << 20) + 2), "own size"), (dict(y=(1 << 20) + 400), "apart"), (dict(y=1 << 20, y_stride=101), "apart"),
 ])
