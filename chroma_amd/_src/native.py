@@ -98,6 +98,8 @@ class Adjust(ctypes.Structure):
 
 def library() -> ctypes.CDLL:
     global _library
+    if _library is not None:
+        return _library
     with _lock:
         if _library is not None:
             return _library
