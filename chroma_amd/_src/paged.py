@@ -225,7 +225,8 @@ class PagedDecoder:
         logits = host.empty((self._slots, self.vocab_size), self._logit_dtype)
         with self._lock:
             slots, _ = self._run(tokens, [logits, None, None], None, None)
-            return logits[slots]
+            adjacent = slots == list(range(slots[0], slots[0] + len(slots)))
+            return logits[slots[0] : slots[0] + len(slots)] if adjacent else logits[slots]
 
     def step_top(self, tokens: Mapping[int, int], k: int = 1, *, rules: Optional[Mapping[int, TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
         """``step`` that returns the ``k`` largest logits after each token and their ids (both [n, k]), chosen on
