@@ -69,8 +69,9 @@ class PagedDecoder:
     """Sequences are named by integers that ``add`` and ``fork`` return. Calls are serialized by one lock."""
 
     def __init__(self, decoder: Decoder, step: Program) -> None:
-        """``decoder`` (a ``Decoder`` of hip programs) consumes the prompts, at most its context long; ``step`` is a
-        compiled ``export_paged`` of the same model. Both are closed with the paged decoder."""
+        """``decoder`` (a ``Decoder`` of hip programs, made with the model's own sliding window, which the step program
+        holds) consumes the prompts, at most its context long, and is reset by each; ``step`` is a compiled
+        ``export_paged`` of the same model. Both are closed with the paged decoder."""
         if len(step.inputs) != 6 or len(step.outputs) != 3:
             raise ValueError(f"PagedDecoder step wants six inputs and three outputs, not {len(step.inputs)} and {len(step.outputs)}")
         cache, table = step.inputs[2], step.inputs[4]

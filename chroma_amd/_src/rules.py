@@ -70,6 +70,8 @@ class TokenRules:
         for name, array in (("bias", self.bias), ("allowed", self.allowed)):
             if isinstance(array, np.ndarray) and (name == "bias" or array.dtype == np.bool_) and len(array) != vocab_size:
                 raise ValueError(f"{name} holds {len(array)} values, the vocabulary {vocab_size}")
+        if self.allowed is not None and not (self.allowed.any() if self.allowed.dtype == np.bool_ else len(self.allowed)):
+            raise ValueError("no token is allowed")
 
     def bias_row(self, vocab_size: int) -> np.ndarray:
         if isinstance(self.bias, np.ndarray):

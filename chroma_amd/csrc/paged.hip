@@ -112,10 +112,10 @@ template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP 
 
 // How a call is cut. Up to kPasses key blocks for every wave of a sequence's workgroup one launch takes whole sequences: 8 KV
 // heads of 8 heads of 64, us for whole sequences and for shares: one of 900 rows 8.9 and 11.3, of 1400 10.5 and 10.7, of
-// 2000 14.2 and 10.8; 8 mixed ones up to 900 9.2 and 11.8, up to 2000 15.8 and 14.8; 32 up to 900 11.3 and 16.5, up to 4096 36.8
-// and 33.2; 128 up to 1000 31 and 37, up to 2000 69 and 68. Beyond, all blocks are cut into as many shares as bring kWaves
-// waves, those that the chip holds at once: 1024 / 2048 / 4096 waves take 64 sequences of 8192 216 / 192 / 198 us and 32
-// mixed ones up to 4096 40 / 37 / 42.
+// 2000 14.2 and 10.7; 8 mixed ones up to 900 9.1 and 11.8, up to 2000 15.8 and 14.2; 32 up to 900 11.3 and 16.5, up to 2000
+// 18.5 and 23.5, up to 4096 36.8 and 34.8; 128 up to 1000 31 and 37, up to 2000 69 and 62. Beyond, all blocks are cut into as
+// many shares as bring kWaves waves, those that the chip holds at once: 1024 / 2048 / 4096 waves take 64 sequences of 8192
+// 201 / 185 / 192 us and 32 mixed ones up to 4096 37 / 35 / 40.
 constexpr int64_t kPasses = 6, kWaves = 2048;
 struct Cut {
     int64_t heads, tiles;

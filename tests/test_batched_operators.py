@@ -605,3 +605,99 @@ def test_rows_adjust_refusals(changes, message):
 def test_rows_adjust_refuses_no_call():
     error = ctypes.create_string_buffer(64)
     assert native.library().chroma_hip_rows_adjust(None, None, error, len(error)) == native.RUNTIME_ERROR
+
+
+@gpu
+def test_rows_adjust_in_a_graph():
+    """A captured call reads the history, lengths and logits that lie there when it is replayed."""
+    x, inputs = adjust_inputs(3, 5000, 40, torch.bfloat16, 8, bias="shared", mask="rows")
+    device, source = on_gpu(inputs), x.cuda()
+    y = torch.empty_like(source)
+    adjust(adjust_call(source, y, **device))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adjust(adjust_call(source, y, **device), torch.cuda.current_stream().cuda_stream)
+    for turn in range(4):
+        device["history"][:, turn] = 4999 - turn
+        device["lengths"].fill_(10 * turn)
+        y.fill_(0.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.empty_like(source)
+        adjust(adjust_call(source, eager, **device))
+        torch.cuda.synchronize()
+        assert torch.equal(y.view(torch.int16), eager.view(torch.int16))
+        inputs["history"], inputs["lengths"] = device["history"].cpu(), device["lengths"].cpu()
+        want, bound = adjust_reference(x, **inputs)
+        got, fine = y.cpu().double(), torch.isfinite(want)
+        assert torch.equal(torch.isinf(got), torch.isinf(want)) and ((got - want).abs()[fine] <= bound[fine]).all()
+
+
+# ------------------------------------------------------------------------------------------------ a run of them together
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_decode_steps_of_the_operators(dtype):
+    """Steps as a serving loop makes them, on a stream of its own: attention with the new rows, these rows stored into their
+    pages (a branch's shared page copied first), logits from the result, adjusted by the tokens so far, the token chosen.
+    Each attention against 64 bits over the text of its sequence, the stored rows bit for bit."""
+    lib, g = native.library(), torch.Generator().manual_seed(6)
+    kv, group, dim, page, pages, span, vocabulary = 2, 4, 32, 4, 40, 12, 2000
+    lengths = [5, 8, 5]  # sequence 2 is a branch of sequence 0
+    table = torch.full((3, span), -1, dtype=torch.int64)
+    table[0, :2], table[1, :2], table[2, :2] = torch.tensor([7, 3]), torch.tensor([20, 11]), torch.tensor([7, 3])
+    free = [page_id for page_id in range(pages) if page_id not in (7, 3, 20, 11)]
+    k, v = (torch.randn(pages, page, kv, dim, generator=g).to(dtype) for _ in range(2))
+    head = torch.randn(vocabulary, kv * group * dim, generator=g).to(dtype).cuda()
+    k_device, v_device = k.cuda(), v.cuda()
+    row_bytes = kv * dim * k.element_size()
+    cache = native.CacheRows(keys=k_device.data_ptr(), values=v_device.data_ptr(), rows=pages * page, layer_pitch=pages * page * row_bytes)
+    texts = [[1, 2, 3, 4, 5], [9] * 8, [1, 2, 3, 4, 5]]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for step in range(6):
+            q = torch.randn(3, kv, group, dim, generator=g).to(dtype)
+            k_new, v_new = (torch.randn(3, kv, dim, generator=g).to(dtype) for _ in range(2))
+            inputs = {"q": q, "k_pages": k, "v_pages": v, "table": table, "lengths": torch.tensor(lengths), "k_new": k_new, "v_new": v_new}
+            want, bound = attention_reference(**inputs, window=9, first=2)
+            device = on_gpu({**inputs, "k_pages": None, "v_pages": None})
+            out = torch.empty_like(device["q"])
+            kept = attend(attention_call(**{**device, "k_pages": k_device, "v_pages": v_device}, out=out, window=9, first=2), stream.cuda_stream)
+            moves = []
+            for b in range(3):  # the pages of this step's rows
+                i = lengths[b] // page
+                if lengths[b] % page == 0:
+                    table[b, i] = free.pop(0)
+                elif b == 2 and step == 0:
+                    moves.append((int(table[b, i]) * page, free[0] * page, lengths[b] % page))
+                    k[free[0], : lengths[b] % page], v[free[0], : lengths[b] % page] = k[table[b, i], : lengths[b] % page], v[table[b, i], : lengths[b] % page]
+                    table[b, i] = free.pop(0)
+            move(cache, cache, moves, 1, row_bytes, stream.cuda_stream)
+            fresh = native.CacheRows(keys=device["k_new"].data_ptr(), values=device["v_new"].data_ptr(), rows=3, layer_pitch=3 * row_bytes)
+            move(cache, fresh, [(b, int(table[b, lengths[b] // page]) * page + lengths[b] % page, 1) for b in range(3)], 1, row_bytes, stream.cuda_stream)
+            for b in range(3):
+                k[table[b, lengths[b] // page], lengths[b] % page], v[table[b, lengths[b] // page], lengths[b] % page] = k_new[b], v_new[b]
+            logits = out.reshape(3, -1) @ head.t().contiguous()
+            longest = max(map(len, texts))
+            history = torch.tensor([text + [-1] * (longest - len(text)) for text in texts])
+            rules = {"history": history, "repetition": torch.full((3,), 1.3), "presence": torch.full((3,), 0.4),
+                     "mask": torch.randint(-(2**31), 2**31, (3, -(-vocabulary // 32)), generator=g).to(torch.int32)}
+            adjusted, on_device = torch.empty_like(logits), on_gpu(rules)
+            adjust(adjust_call(logits, adjusted, **on_device), stream.cuda_stream)
+            values, ids = torch.empty(3, 1, dtype=dtype, device="cuda"), torch.empty(3, 1, dtype=torch.int64, device="cuda")
+            need, error = lib.chroma_hip_rows_topk_workspace(3, vocabulary, 1), ctypes.create_string_buffer(256)
+            scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+            checked(lib.chroma_hip_rows_topk(adjusted.data_ptr(), DTYPES[dtype], 3, vocabulary, 1, 1, values.data_ptr(), ids.data_ptr(),
+                                             scratch.data_ptr(), need, stream.cuda_stream, error, len(error)), error)
+            stream.synchronize()
+            assert ((out.cpu().double() - want).abs() <= bound).all(), step
+            assert torch.equal(k_device.cpu(), k) and torch.equal(v_device.cpu(), v)
+            exact, off = adjust_reference(logits.cpu(), **rules)
+            got, fine = adjusted.cpu().double(), torch.isfinite(exact)
+            assert torch.equal(torch.isinf(got), torch.isinf(exact)) and ((got - exact).abs()[fine] <= off[fine]).all()
+            for b in range(3):
+                assert int(ids[b]) == int(torch.nonzero(got[b] == got[b].max())[0])
+                texts[b].append(int(ids[b]))
+                lengths[b] += 1
+            del kept

@@ -446,7 +446,8 @@ def test_rules_refuse(arguments, kind):
 
 
 @pytest.mark.parametrize("arguments,kind", [(dict(history=[10]), IndexError), (dict(history=[-1]), IndexError), (dict(bias={10: 1.0}), IndexError),
-                                            (dict(bias=np.zeros(9)), ValueError), (dict(allowed=[10]), IndexError), (dict(allowed=np.ones(11, bool)), ValueError)])
+                                            (dict(bias=np.zeros(9)), ValueError), (dict(allowed=[10]), IndexError), (dict(allowed=np.ones(11, bool)), ValueError),
+                                            (dict(allowed=[]), ValueError), (dict(allowed=np.zeros(10, bool)), ValueError)])
 def test_rules_refuse_another_vocabulary(arguments, kind):
     rules = TokenRules(**arguments)
     with pytest.raises(kind):
