@@ -67,6 +67,8 @@ def _check(q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, window, fir
     if q.dim() != 4 or k_pages.dim() != 4 or tuple(v_pages.shape) != tuple(k_pages.shape):
         raise ValueError("paged_attention wants q [sequences, KV heads, group, dim] and pages [pages, rows, KV heads, dim]")
     sequences, kv_heads, group, dim = q.shape
+    if 0 in q.shape or 0 in k_pages.shape:
+        raise ValueError(f"empty q {tuple(q.shape)} or pages {tuple(k_pages.shape)}")
     if tuple(k_pages.shape[2:]) != (kv_heads, dim):
         raise ValueError(f"pages of {tuple(k_pages.shape[2:])} heads and dimensions, q of {(kv_heads, dim)}")
     if (k_new is None) != (v_new is None) or (k_new is not None and not tuple(k_new.shape) == tuple(v_new.shape) == (sequences, kv_heads, dim)):

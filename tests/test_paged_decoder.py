@@ -56,7 +56,7 @@ def test_operator_refusals():
     good = operator_arguments(paged_inputs([5, 9], kv=2, group=2, dim=8, page=4, dtype=torch.float32))
     paged_attention(*good, 1.0)
     for index, value, kind in ((0, good[0][0], ValueError), (1, good[1][:, :, :1], ValueError), (3, None, ValueError), (3, good[3][:1], ValueError),
-                               (5, good[5].int(), TypeError), (5, good[5][:1], ValueError), (6, good[6][:1], ValueError), (7, good[7][:3], ValueError),
+                               (0, good[0][:0], ValueError), (5, good[5].int(), TypeError), (5, good[5][:1], ValueError), (6, good[6][:1], ValueError), (7, good[7][:3], ValueError),
                                (2, good[2].bfloat16(), TypeError), (7, good[7].double(), TypeError)):
         changed = list(good)
         changed[index] = value
@@ -65,6 +65,9 @@ def test_operator_refusals():
     for window, first in ((-1, 0), (0, -1)):
         with pytest.raises(ValueError):
             paged_attention(*good, 1.0, window, first)
+    for empty in (good[1][:0], good[1][:, :0]):
+        with pytest.raises(ValueError, match="empty"):
+            paged_attention(good[0], empty, empty, *good[3:], 1.0)
 
 
 class Attention(torch.nn.Module):
