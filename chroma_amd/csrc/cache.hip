@@ -9,8 +9,8 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
-#include <type_traits>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -95,13 +95,13 @@ const char* mistake(const chroma_hip_cache_rows& to, const chroma_hip_cache_rows
             return "a cache's layer pitch is smaller than its rows";
         }
     }
-    const bool same = to.keys == from.keys && to.values == from.values && to.layer_pitch == from.layer_pitch;
+    const bool same = to.keys == from.keys && to.values == from.values && (layers == 1 || to.layer_pitch == from.layer_pitch);
     const auto begin = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
     const auto bytes = [&](const chroma_hip_cache_rows& c) { return uintptr_t((layers - 1) * c.layer_pitch + c.rows * row_bytes); };
     const auto meet = [&](const void* a, uintptr_t size_a, const void* b, uintptr_t size_b) {
         return begin(a) < begin(b) + size_b && begin(b) < begin(a) + size_a;
     };
-    if (meet(to.keys, bytes(to), to.values, bytes(to))) {
+    if (meet(to.keys, bytes(to), to.values, bytes(to)) || (same && meet(from.keys, bytes(from), from.values, bytes(from)))) {
         return "keys and values overlap";
     }
     if (!same && (meet(to.keys, bytes(to), from.keys, bytes(from)) || meet(to.keys, bytes(to), from.values, bytes(from)) ||

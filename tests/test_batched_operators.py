@@ -440,7 +440,8 @@ def host_cache(**changes):
     ({}, dict(keys=1 << 28, values=1 << 29, rows=3), 2, 64, [(2, 5, 2)], "leaves"),
     ({}, None, 2, 64, [(0, 5, 2), (10, 6, 1)], "twice"), ({}, None, 2, 64, [(0, 1, 2)], "twice"), ({}, None, 2, 64, [(0, 5, 1), (5, 9, 1)], "twice"),
     ({}, None, 2, 64, [(7, 7, 1)], "twice"), ({}, dict(keys=1 << 28, values=1 << 29), 2, 64, [(0, 5, 2), (10, 5, 2)], "twice"),
-    ({}, None, 2, 64, [(60, 0, 30), (20, 40, 5), (41, 95, 1)], "twice"),
+    ({}, None, 2, 64, [(60, 0, 30), (20, 40, 5), (41, 95, 1)], "twice"), ({}, dict(layer_pitch=9999), 1, 64, [(7, 7, 1)], "twice"),
+    ({}, dict(layer_pitch=9999), 2, 64, [], "must be the same"), ({}, dict(rows=1 << 18, layer_pitch=1 << 24), 1, 64, [], "keys and values overlap"),
 ])
 def test_cache_move_refusals(to, source, layers, row_bytes, moves, message):
     target = host_cache(**to)
