@@ -76,16 +76,21 @@ class PagedDecoder:
             raise ValueError(f"PagedDecoder step wants six inputs and three outputs, not {len(step.inputs)} and {len(step.outputs)}")
         cache, table = step.inputs[2], step.inputs[4]
         layers, pages, rows, heads, dim = cache["shape"] if len(cache["shape"]) == 5 else (0,) * 5
+        slots, span = table["shape"] if len(table["shape"]) == 2 else (0, 0)
         prompts = decoder._models[1].inputs[2]
-        if [layers, heads, dim] != [prompts["shape"][0], *prompts["shape"][2:]] or cache["dtype"] != prompts["dtype"] or \
-                step.outputs[0]["shape"] != [step.inputs[0]["shape"][0], decoder.vocab_size] or len(table["shape"]) != 2:
+        # rows move by these extents, so every input and output must have them
+        fresh = ([layers, slots, heads, dim], prompts["dtype"])
+        wanted = [([slots], "int64"), ([slots], "float32"), *[([layers, pages, rows, heads, dim], prompts["dtype"])] * 2, ([slots, span], "int64"),
+                  ([slots], "int64"), ([slots, decoder.vocab_size], step.outputs[0]["dtype"]), fresh, fresh]
+        if [layers, heads, dim] != [prompts["shape"][0], *prompts["shape"][2:]] or \
+                [(list(spec["shape"]), spec["dtype"]) for spec in (*step.inputs, *step.outputs)] != wanted:
             raise ValueError("PagedDecoder decoder and step were not exported from the same model")
         if not decoder.stats["cache_on_device"] or decoder.device != step.device:
             raise ValueError("PagedDecoder wants a decoder of hip programs on the step's device")
         self._decoder, self._step = decoder, step
         self._layers, self._page_rows = layers, rows
         self._row_bytes = heads * dim * numpy_dtype(cache["dtype"]).itemsize
-        self._slots, self._span = table["shape"]
+        self._slots, self._span = slots, span
         self.vocab_size = decoder.vocab_size
         self._logit_dtype = numpy_dtype(step.outputs[0]["dtype"])
         self._pool = PagePool(pages)

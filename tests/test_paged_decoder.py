@@ -366,6 +366,12 @@ def test_paged_decoder_refuses_programs_that_do_not_belong_together():
     for graph in (export_paged(other, SLOTS, PAGES, ROWS, SPAN), export_cached(model, CONTEXT, 1)):
         with pytest.raises(ValueError, match="PagedDecoder"):
             PagedDecoder(prompts, FakePagedProgram(graph, device))
+    for part, index, shape in (("inputs", 3, [2, PAGES - 1, ROWS, 2, 8]), ("inputs", 5, [SLOTS + 1]), ("outputs", 1, [2, SLOTS - 1, 2, 8]),
+                               ("outputs", 2, [1, SLOTS, 2, 8]), ("inputs", 0, [SLOTS + 1])):
+        step = FakePagedProgram(export_paged(model, SLOTS, PAGES, ROWS, SPAN), device)
+        getattr(step, part)[index]["shape"] = shape
+        with pytest.raises(ValueError, match="same model"):
+            PagedDecoder(prompts, step)
     for extents in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
         with pytest.raises(ValueError):
             export_paged(model, *extents)
