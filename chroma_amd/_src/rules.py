@@ -8,7 +8,6 @@ samples from the raw row, scripts/chat.py:82-98.)
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 from typing import Any, Dict, Mapping, Optional, Sequence, Union
 
@@ -43,11 +42,13 @@ class TokenRules:
     allowed: Optional[Any] = None
 
     def __post_init__(self) -> None:
-        for name in ("repetition", "presence", "frequency"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
-        if self.repetition <= 0:
-            raise ValueError(f"repetition must be positive, got {self.repetition}")
+        with np.errstate(over="ignore"):
+            factors = {name: np.float32(getattr(self, name)) for name in ("repetition", "presence", "frequency")}
+        for name, factor in factors.items():
+            if not np.isfinite(factor):
+                raise ValueError(f"{name} must be finite in float32, got {getattr(self, name)}")
+        if factors["repetition"] <= 0:
+            raise ValueError(f"repetition must be positive in float32, got {self.repetition}")
         object.__setattr__(self, "history", _ids(self.history, "history"))
         if self.bias is not None and not isinstance(self.bias, Mapping):
             bias = np.asarray(self.bias, dtype=np.float32)

@@ -448,7 +448,8 @@ def test_packed_rules_share_rows():
 @pytest.mark.parametrize("arguments,kind", [
     (dict(repetition=0.0), ValueError), (dict(repetition=-1.0), ValueError), (dict(repetition=math.inf), ValueError), (dict(presence=math.nan), ValueError),
     (dict(frequency=math.inf), ValueError), (dict(history=[1.5]), TypeError), (dict(history=[[1]]), TypeError), (dict(bias=np.zeros((2, 2))), ValueError),
-    (dict(allowed=[0.5]), TypeError), (dict(allowed=np.zeros((2, 2), bool)), TypeError)])
+    (dict(allowed=[0.5]), TypeError), (dict(allowed=np.zeros((2, 2), bool)), TypeError),
+    (dict(repetition=1e-60), ValueError), (dict(frequency=-1e39), ValueError)])
 def test_rules_refuse(arguments, kind):
     with pytest.raises(kind):
         TokenRules(**arguments)
