@@ -257,7 +257,7 @@ int chroma_hip_cache_move_queued(void* handle, const chroma_hip_cache_rows* to, 
  * The arithmetic is float's, one rounding per operation, and the result is rounded to y's type once. ``history`` holds
  * token ids; of row r the first history_lengths[r] count (all history_width when null; less than 0 counts as 0, more
  * than history_width as history_width), and ids outside [0, width) count for nothing. A null parameter array changes
- * nothing. y may be x itself with the same stride (then only what changes is written); otherwise it must not overlap x. */
+ * nothing. y may be x itself with the same stride (then only what changes is written); otherwise it must not overlap x, nor in either case another array. */
 typedef struct chroma_hip_adjust_call {
     const void* x; /* [rows, width] at x_stride elements */
     void* y;       /* [rows, width] at y_stride elements */
