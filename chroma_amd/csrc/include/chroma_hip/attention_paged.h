@@ -34,10 +34,14 @@ struct PagedRange {
     uint32_t length, head, low, end;
 };
 
-template <class T> __device__ __forceinline__ PagedRange paged_range(const PagedOperands<T>& a, uint32_t b) {
+template <class T> __device__ __forceinline__ uint32_t paged_length(const PagedOperands<T>& a, uint32_t b) {
     const int64_t given = a.lengths[b];
+    return given < 0 ? 0u : given > int64_t(a.longest) ? a.longest : uint32_t(given);
+}
+
+template <class T> __device__ __forceinline__ PagedRange paged_range(const PagedOperands<T>& a, uint32_t length) {
     PagedRange r;
-    r.length = given < 0 ? 0u : given > int64_t(a.longest) ? a.longest : uint32_t(given);
+    r.length = length;
     const uint32_t fresh = a.k_new ? 1u : 0u;
     r.end = r.length + fresh;
     // the token's position is end - 1; the cached rows after end - 1 - window are in its window (the new row always is)
@@ -99,14 +103,25 @@ __device__ __forceinline__ uint32_t paged_scan(uint32_t v) {  // inclusive sums 
     return v;
 }
 
-// The number of blocks of all sequences.
-template <uint32_t KEYS, class T> __device__ __forceinline__ uint32_t paged_total(const PagedOperands<T>& a) {
-    uint32_t mine = 0;
-    for (uint32_t b = threadIdx.x % kWave; b < a.sequences; b += kWave) {
-        mine += paged_blocks<KEYS>(paged_range(a, b));
+// The sequences' lengths, the first 64 in registers, one to a lane (what is read once more waits once more).
+template <uint32_t KEYS, class T> struct PagedLengths {
+    const PagedOperands<T>& a;
+    uint32_t own, own_blocks;
+    __device__ __forceinline__ explicit PagedLengths(const PagedOperands<T>& a) : a(a) {
+        const uint32_t lane = threadIdx.x % kWave;
+        own = lane < a.sequences ? paged_length(a, lane) : 0u;
+        own_blocks = lane < a.sequences ? paged_blocks<KEYS>(paged_range(a, own)) : 0u;
     }
-    return __builtin_amdgcn_readlane(paged_scan(mine), kWave - 1);
-}
+    // blocks of this lane's sequence b0 + lane (0 past the last); b0 a multiple of 64
+    __device__ __forceinline__ uint32_t blocks(uint32_t b0) const {
+        const uint32_t b = b0 + threadIdx.x % kWave;
+        return b0 == 0 ? own_blocks : b < a.sequences ? paged_blocks<KEYS>(paged_range(a, paged_length(a, b))) : 0u;
+    }
+    // of sequence b, the same in all lanes
+    __device__ __forceinline__ PagedRange range(uint32_t b) const {
+        return paged_range(a, b < uint32_t(kWave) ? uint32_t(__builtin_amdgcn_readlane(own, b)) : paged_length(a, b));
+    }
+};
 
 // Share w < ranges holds blocks [begin(w), begin(w + 1)) of ``total``, one at least; ``of`` gives the share that holds a block.
 struct PagedShares {
@@ -356,7 +371,7 @@ template <class T, int DP, uint32_t KEYS, uint32_t WAVES> __device__ __forceinli
     const uint32_t tiles = (a.group + 15u) / 16u, kv = blockIdx.x / tiles, row0 = blockIdx.x % tiles * 16u, b = blockIdx.y;
     const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
     T* ks = lds + wave * Wave::ELEMENTS;
-    const PagedRange range = paged_range(a, b);
+    const PagedRange range = paged_range(a, paged_length(a, b));
     Wave x;
     Wave::prepare(a, ks);
     x.run(a, range, b, kv, head, wave, paged_blocks<KEYS>(range), WAVES, ks, ks + KEYS * DP);
@@ -411,15 +426,21 @@ __device__ __forceinline__ void attention_paged_shares(const PagedOperands<T>& a
     const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, uint64_t(a.kv_heads) * a.group);
 
     // This wave's share of the blocks, and the sequence b and its block n at which it begins.
-    const PagedShares shares(paged_total<KEYS>(a), ranges);
+    const PagedLengths<KEYS, T> lengths(a);
+    uint32_t all = 0;
+    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWave) {
+        all += lengths.blocks(b0);
+    }
+    const uint32_t upto0 = paged_scan(all);
+    const PagedShares shares(__builtin_amdgcn_readlane(upto0, kWave - 1), ranges);
     if (w >= shares.ranges) {
         return;
     }
     const uint32_t begin = shares.begin(w);
     uint32_t left = shares.begin(w + 1u) - begin, b = 0, n = 0;
     for (uint32_t before = 0, b0 = 0; b0 < a.sequences; b0 += kWave) {
-        const uint32_t own = b0 + lane < a.sequences ? paged_blocks<KEYS>(paged_range(a, b0 + lane)) : 0u;
-        const uint32_t upto = before + paged_scan(own);
+        const uint32_t own = lengths.blocks(b0);
+        const uint32_t upto = a.sequences <= uint32_t(kWave) ? upto0 : before + paged_scan(own);
         const unsigned long long past = __ballot(upto > begin);
         if (past) {
             const uint32_t at = __builtin_ctzll(past);
@@ -432,7 +453,7 @@ __device__ __forceinline__ void attention_paged_shares(const PagedOperands<T>& a
     Wave::prepare(a, ks);
     const uint32_t head = kv * a.group + (row0 + col < a.group ? row0 + col : a.group - 1u);
     for (; left; ++b, n = 0) {
-        const PagedRange range = paged_range(a, b);
+        const PagedRange range = lengths.range(b);
         const uint32_t blocks = paged_blocks<KEYS>(range), count = blocks - n < left ? blocks - n : left;
         left -= count;
         Wave x;
@@ -467,16 +488,17 @@ __device__ __forceinline__ void attention_paged_combine(const PagedOperands<T>& 
         return;
     }
     const PagedScratch<DP> parts(scratch, uint64_t(ranges) + a.sequences, heads);
+    const PagedLengths<KEYS, T> lengths(a);
     uint32_t all = 0, before = 0;
-    for (uint32_t x = lane; x < a.sequences; x += kWave) {
-        const uint32_t own = paged_blocks<KEYS>(paged_range(a, x));
+    for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWave) {
+        const uint32_t own = lengths.blocks(b0);
         all += own;
-        before += x < b ? own : 0u;
+        before += b0 + lane < b ? own : 0u;
     }
     all = __builtin_amdgcn_readlane(paged_scan(all), kWave - 1);
     before = __builtin_amdgcn_readlane(paged_scan(before), kWave - 1);
     const PagedShares shares(all, ranges);
-    const uint32_t first = shares.of(before), count = shares.of(before + paged_blocks<KEYS>(paged_range(a, b)) - 1u) - first + 1u;
+    const uint32_t first = shares.of(before), count = shares.of(before + paged_blocks<KEYS>(lengths.range(b)) - 1u) - first + 1u;
     if (count == 1u) {
         return;  // written by its wave
     }

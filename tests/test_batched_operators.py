@@ -151,6 +151,27 @@ SHAPES = [  # (lengths, kv, group, dim, page)
 ]
 
 
+LONG_SHAPES = [  # more key blocks than one workgroup takes; a wave knows the lengths of 64 sequences from one load
+    ([4000], 1, 3, 64, 16),
+    ([2100, 1900], 1, 8, 8, 5),
+    ([9000, 0, 1], 2, 2, 256, 64),
+    ([1, 2500, 0, 700] * 18, 2, 4, 32, 16),
+    ([0] * 63 + [3200, 3000, 0, 1, 40] + [10] * 60 + [2000, 0], 1, 17, 16, 12),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("window,first", [(0, 0), (1800, 3)])
+@pytest.mark.parametrize("shape", LONG_SHAPES, ids=lambda s: f"{len(s[0])}x{max(s[0])}-{s[1]}x{s[2]}x{s[3]}-{s[4]}")
+def test_paged_attention_of_long_sequences(shape, window, first, dtype):
+    lengths, kv, group, dim, page = shape
+    inputs = paged_inputs(lengths, kv=kv, group=group, dim=dim, page=page, dtype=dtype, fresh=not window, sinks=bool(window), seed=dim)
+    call = attention_call(**inputs, out=torch.empty_like(inputs["q"]), window=window, first=first)
+    assert native.library().chroma_hip_paged_attention_workspace(ctypes.byref(call)) > 0
+    check_attention(inputs, window=window, first=first)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
