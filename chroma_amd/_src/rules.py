@@ -74,13 +74,13 @@ class TokenRules:
         if self.allowed is not None and not (self.allowed.any() if self.allowed.dtype == np.bool_ else len(self.allowed)):
             raise ValueError("no token is allowed")
 
-    def bias_row(self, vocab_size: int) -> np.ndarray:
+    def write_bias(self, row: np.ndarray) -> None:
+        """Write the bias into a row of zeros."""
         if isinstance(self.bias, np.ndarray):
-            return self.bias
-        row = np.zeros(vocab_size, dtype=np.float32)
-        for token, value in (self.bias or {}).items():
-            row[token] = value
-        return row
+            row[:] = self.bias
+        else:
+            for token, value in (self.bias or {}).items():
+                row[token] = value
 
     def allowed_row(self, vocab_size: int) -> np.ndarray:
         if self.allowed is None:
@@ -102,7 +102,9 @@ class TokenRules:
             repetition, presence, frequency = (np.float32(v) for v in (self.repetition, self.presence, self.frequency))
             x[ids] = np.where(old > 0, old / repetition, old * repetition) - (presence + frequency * counts.astype(np.float32))
             if self.bias is not None:
-                x += self.bias_row(vocab_size)
+                bias = np.zeros(vocab_size, dtype=np.float32)
+                self.write_bias(bias)
+                x += bias
         x[~self.allowed_row(vocab_size)] = -np.inf
         return float32_to_bf16(x) if row.dtype == BFLOAT16 else x
 
@@ -129,11 +131,16 @@ def pack(rules: Sequence[TokenRules], vocab_size: int) -> Dict[str, Optional[np.
 
     arrays["bias"] = arrays["mask"] = None
     if any(rule.bias is not None for rule in rules):
-        arrays["bias"] = np.stack([rules[i].bias_row(vocab_size) for i in rows_of([rule.bias for rule in rules])])
+        chosen = rows_of([rule.bias for rule in rules])
+        arrays["bias"] = np.zeros((len(chosen), vocab_size), dtype=np.float32)
+        for row, i in zip(arrays["bias"], chosen):
+            rules[i].write_bias(row)
     if any(rule.allowed is not None for rule in rules):
         chosen = rows_of([rule.allowed for rule in rules])
-        bits = np.zeros((len(chosen), -(-vocab_size // 32) * 32), dtype=np.bool_)
-        for row, i in zip(bits, chosen):
-            row[:vocab_size] = rules[i].allowed_row(vocab_size)
-        arrays["mask"] = np.packbits(bits, axis=1, bitorder="little").view(np.uint32)
+        words = arrays["mask"] = np.full((len(chosen), -(-vocab_size // 32)), 0xFFFFFFFF, dtype=np.uint32)
+        bits = np.zeros(words.shape[1] * 32, dtype=np.bool_)
+        for row, i in zip(words, chosen):
+            if rules[i].allowed is not None:
+                bits[:vocab_size] = rules[i].allowed_row(vocab_size)
+                row[:] = np.packbits(bits, bitorder="little").view(np.uint32)
     return arrays
