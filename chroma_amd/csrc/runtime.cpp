@@ -75,6 +75,7 @@ struct Region {
 constexpr size_t kDirectBytes = size_t(256) << 10;
 constexpr size_t kErrorRegion = 1024;  // bytes the plan reserves at its error offset
 constexpr size_t kStagingSlot = size_t(2) << 20;
+constexpr size_t kLeastRules = size_t(64) << 10;  // least room for a selection's rules
 
 std::mutex pinned_mutex;
 std::map<uintptr_t, size_t> pinned_blocks;  // start -> bytes of each block from chroma_hip_host_alloc
@@ -287,6 +288,15 @@ public:
         if (select_host_) {
             hipHostFree(select_host_);
         }
+        if (adjusted_) {
+            hipFree(adjusted_);
+        }
+        if (rules_) {
+            hipFree(rules_);
+        }
+        if (rules_host_) {
+            hipHostFree(rules_host_);
+        }
         if (error_host_) {
             hipHostFree(error_host_);
         }
@@ -328,6 +338,11 @@ public:
         select_bytes_ = 0;
         select_host_ = nullptr;
         select_host_bytes_ = 0;
+        adjusted_ = nullptr;
+        adjusted_bytes_ = 0;
+        rules_ = nullptr;
+        rules_host_ = nullptr;
+        rules_bytes_ = 0;
         slots_ = nullptr;
         slots_host_ = nullptr;
         slots_capacity_ = 0;
@@ -414,6 +429,38 @@ public:
         return staged;
     }
 
+    // Room for the adjusted logits and for the rules' arrays (on the device and page-locked), apart from the selection's
+    // scratch, whose address a captured selection holds. The rules get half as much again as they need: a history that
+    // grows by a token a step moves them a logarithmic number of times.
+    void ensure_rules(size_t logits, size_t bytes) {
+        if (logits > adjusted_bytes_) {
+            check(hipStreamSynchronize(stream_), "Adjusted logits");
+            if (adjusted_) {
+                check(hipFree(adjusted_), "hipFree adjusted logits");
+                adjusted_ = nullptr;
+                adjusted_bytes_ = 0;
+            }
+            check(hipMalloc(&adjusted_, logits), "hipMalloc adjusted logits");
+            adjusted_bytes_ = logits;
+        }
+        if (bytes > rules_bytes_) {
+            const size_t capacity = std::max(bytes + bytes / 2, kLeastRules);
+            check(hipStreamSynchronize(stream_), "Rules");
+            rules_bytes_ = 0;
+            if (rules_) {
+                check(hipFree(rules_), "hipFree rules");
+                rules_ = nullptr;
+            }
+            if (rules_host_) {
+                check(hipHostFree(rules_host_), "hipHostFree rules");
+                rules_host_ = nullptr;
+            }
+            check(hipMalloc(&rules_, capacity), "hipMalloc rules");
+            check(hipHostMalloc(&rules_host_, capacity, hipHostMallocDefault), "hipHostMalloc rules");
+            rules_bytes_ = capacity;
+        }
+    }
+
     // ``run`` with a row selection over output ``index`` queued after the plan: only the k values and ids
     // of each row come back (and the outputs whose host pointers are non-null), after one synchronization.
     // With ``rules`` the selection reads the output's rows adjusted by them.
@@ -438,12 +485,8 @@ public:
         const size_t value_bytes = rows * size_t(k) * item, id_bytes = rows * size_t(k) * sizeof(int64_t);
         // ids then values, adjacent, so one copy brings both back
         const size_t result_bytes = id_bytes + value_bytes;
-        // behind them, with rules: the adjusted rows and the rules' arrays (these behind the results on the host too)
-        const size_t adjusted_at = align(align(scratch) + result_bytes), rules_at = adjusted_at + (rules ? align(rows * width * item) : 0);
-        const size_t rule_bytes = rules ? stage_rules(*rules, rows, width, nullptr).bytes : 0;
-        const size_t need = rules ? rules_at + rule_bytes : align(scratch) + result_bytes;
-        const size_t host_need = rules ? align(result_bytes) + rule_bytes : result_bytes;
-        if (need > select_bytes_ || host_need > select_host_bytes_) {
+        const size_t need = align(scratch) + result_bytes;
+        if (need > select_bytes_ || result_bytes > select_host_bytes_) {
             check(hipStreamSynchronize(stream_), "Selection scratch");
             if (select_) {
                 check(hipFree(select_), "hipFree selection scratch");
@@ -458,8 +501,13 @@ public:
             drop_select_graph();
             check(hipMalloc(&select_, need), "hipMalloc selection scratch");
             select_bytes_ = need;
-            check(hipHostMalloc(&select_host_, host_need, hipHostMallocDefault), "hipHostMalloc selection results");
-            select_host_bytes_ = host_need;
+            check(hipHostMalloc(&select_host_, result_bytes, hipHostMallocDefault), "hipHostMalloc selection results");
+            select_host_bytes_ = result_bytes;
+        }
+        StagedRules staged;
+        if (rules) {
+            ensure_rules(rows * width * item, stage_rules(*rules, rows, width, nullptr).bytes);
+            staged = stage_rules(*rules, rows, width, static_cast<char*>(rules_));
         }
         char* base = static_cast<char*>(select_);
         int64_t* device_ids = reinterpret_cast<int64_t*>(base + align(scratch));
@@ -475,21 +523,19 @@ public:
                 }
             };
             if (rules) {
-                StagedRules staged = stage_rules(*rules, rows, width, base + rules_at);
-                char* at = static_cast<char*>(select_host_) + align(result_bytes);
+                char* at = static_cast<char*>(rules_host_);
                 for (const auto& piece : staged.pieces) {
                     if (piece.first) {
                         std::memcpy(at, piece.first, piece.second);
                     }
                     at += piece.second;
                 }
-                if (rule_bytes) {
-                    check(hipMemcpyAsync(base + rules_at, static_cast<char*>(select_host_) + align(result_bytes), rule_bytes,
-                                         hipMemcpyHostToDevice, stream_), "Upload rules");
+                if (staged.bytes) {
+                    check(hipMemcpyAsync(rules_, rules_host_, staged.bytes, hipMemcpyHostToDevice, stream_), "Upload rules");
                 }
                 launch_all();
                 staged.call.x = logits;
-                staged.call.y = base + adjusted_at;
+                staged.call.y = adjusted_;
                 staged.call.rows = int64_t(rows);
                 staged.call.width = staged.call.x_stride = staged.call.y_stride = int64_t(width);
                 staged.call.dtype = dtype;
@@ -497,7 +543,7 @@ public:
                 if (chroma_adjust::launch_rows_adjust(staged.call, stream_, message, sizeof(message))) {
                     throw HipError(message);
                 }
-                select(base + adjusted_at);
+                select(static_cast<const char*>(adjusted_));
             } else {
                 const std::array<size_t, 6> key{size_t(index), size_t(dtype), rows, width, size_t(k), reinterpret_cast<size_t>(select_)};
                 launch_all_then(key, [&]() { select(logits); });
@@ -966,6 +1012,11 @@ private:
     size_t select_bytes_ = 0;
     void* select_host_ = nullptr;  // pinned landing area of run_top's ids and values
     size_t select_host_bytes_ = 0;
+    void* adjusted_ = nullptr;  // run_top's adjusted logits (allocated on first use with rules)
+    size_t adjusted_bytes_ = 0;
+    void* rules_ = nullptr;       // the rules' arrays on the device
+    void* rules_host_ = nullptr;  // and page-locked
+    size_t rules_bytes_ = 0;      // bytes both hold
     // run_top's plan and selection captured as one graph, for the selection it was captured with
     hipGraph_t select_graph_ = nullptr;
     hipGraphExec_t select_exec_ = nullptr;

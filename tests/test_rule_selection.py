@@ -1,0 +1,126 @@
+"""Selection of tokens from adjusted logits over many steps (``run_top`` with rules): histories that grow, rules whose rows
+lie apart, plain selections between them.
+
+CPU: the runtime itself, built over a stand-in for HIP (``runtime_stub.cpp``) that counts what it allocates and captures.
+GPU (marked): compiled programs against the host rule."""
+
+from __future__ import annotations
+
+import ctypes
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import chroma_amd
+from chroma_amd import TokenRules
+from chroma_amd._src import host, native
+from chroma_amd._src.decoder import _select_host
+from chroma_amd._src.program import NativeModel
+from chroma_amd._src.rules import pack
+from tests.conftest import ROOT
+from tests.helpers import Function, as_float, numpy_of
+
+gpu = pytest.mark.gpu
+
+
+class StubModel(NativeModel):
+    """A program of one kernel that hands its input rows [rows, width] on as output 0."""
+
+    def __init__(self, library, directory, rows, width):
+        size = rows * width * 4
+        room = -(-size // 256) * 256
+        (directory / "weights.bin").write_bytes(b"")
+        (directory / "model.plan").write_text("\n".join([
+            "chroma-hip-plan 2", "signature none", "code_object none", "weights_file weights.bin", f"arena {2 * room + 1024}", "weights 0",
+            f"error {2 * room}", f"input 0 0 {size}", f"output 0 {room} {size}", f"launch copy_{size} 1 1 1 64 0 2 0 {room}", ""]))
+        spec = [{"name": "logits", "shape": [rows, width], "dtype": "float32"}]
+        self.counted = library
+        super().__init__(directory, spec, spec)
+
+    def counts(self):
+        """[device allocations, page-locked allocations, instantiated graphs, plan kernels run] so far."""
+        values = np.zeros(4, np.int64)
+        self.counted.stub_counts(values.ctypes.data_as(ctypes.c_void_p))
+        return values
+
+
+@pytest.fixture(scope="module")
+def stub_library(tmp_path_factory):
+    path = tmp_path_factory.mktemp("stub") / "libstub.so"
+    sources = [native.RUNTIME_SOURCE, ROOT / "tests" / "runtime_stub.cpp"]
+    subprocess.run(["g++", "-std=c++17", "-O1", "-ffp-contract=off", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-w", "-D__HIP_PLATFORM_AMD__",
+                    f"-I{native.ROCM / 'include'}", *map(str, sources), "-o", str(path)], check=True)
+    library = ctypes.CDLL(str(path))
+    for name in ("chroma_hip_create", "chroma_hip_run", "chroma_hip_device_name", "chroma_hip_signature", "chroma_hip_destroy", "chroma_hip_run_top",
+                 "chroma_hip_run_top_adjusted"):
+        function, known = getattr(library, name), getattr(native.library(), name)
+        function.argtypes, function.restype = known.argtypes, known.restype
+    return library
+
+
+@pytest.fixture
+def stub_model(stub_library, tmp_path, monkeypatch):
+    def make(rows, width):
+        with monkeypatch.context() as patch:
+            patch.setattr(native, "library", lambda: stub_library)
+            return StubModel(stub_library, tmp_path, rows, width)
+
+    monkeypatch.setattr(host, "empty", lambda shape, dtype: np.empty(shape, dtype))
+    return make
+
+
+def chosen(rows, rules, k):
+    """The host rule: the ``k`` largest adjusted values of each row and their ids."""
+    picked = [_select_host(rule.apply(row), k, None) for row, rule in zip(rows, rules)]
+    return np.stack([values for values, _ in picked]), np.stack([ids for _, ids in picked])
+
+
+def test_growing_histories_keep_their_buffers_and_the_captured_selection(stub_model):
+    """200 steps whose histories grow by 300 ids each (10 KB to 2 MB): buffers move a logarithmic number of times, and the
+    plain selections between them replay the graph that the first one captured."""
+    model, rng = stub_model(4, 100), np.random.default_rng(1)
+    texts = [list(rng.integers(0, 100, 17 * i)) for i in range(4)]
+    first = None
+    for step in range(200):
+        logits = rng.normal(size=(4, 100)).astype(np.float32) * 4
+        for text in texts:
+            text.extend(rng.integers(0, 100, 300))
+        rules = [TokenRules(text, 1.0 + 0.1 * i, 0.01 * i, 0.001 * i) for i, text in enumerate(texts)]
+        values, ids = model.run_top([logits], [None], 0, 3, rules)
+        want_values, want_ids = chosen(logits, rules, 3)
+        np.testing.assert_array_equal(ids, want_ids)
+        np.testing.assert_array_equal(values, want_values)
+        if step % 10 == 0:
+            values, ids = model.run_top([logits], [None], 0, 3)
+            np.testing.assert_array_equal(ids, chosen(logits, [TokenRules()] * 4, 3)[1])
+        if first is None:
+            first = model.counts()
+    grown = model.counts() - first
+    # half as much again each time: log(2 MB / 64 KiB) / log(1.5) = 8.5 moves, one buffer of each kind
+    assert grown[0] <= 9 and grown[1] <= 9 and grown[2] == 0, grown
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_growing_histories_on_the_device(tmp_path, dtype):
+    """60 steps whose histories grow by 200 ids each, past the first room for rules, plain selections and their graph
+    between them: values and ids bit for bit by the host rule (the same float operations)."""
+    graph = torch.export.export(Function(lambda x: x * 0.5), (torch.zeros(3, 3001, dtype=dtype),))
+    g, rng = torch.Generator().manual_seed(3), np.random.default_rng(3)
+    texts, mask = [[], [1], [2, 3]], rng.random(3001) < 0.5
+    with chroma_amd.compile(graph, tmp_path) as program:
+        for step in range(60):
+            x = (torch.randn(3, 3001, generator=g) * 8).to(dtype)
+            rows = numpy_of(x * 0.5)
+            for text in texts:
+                text.extend(rng.integers(0, 3001, 200))
+            rules = [TokenRules(text, 1.0 + 0.2 * i, 0.1 * i, 0.01 * i, None, mask if step % 2 else None) for i, text in enumerate(texts)]
+            for given in ((rules, None) if step % 4 == 0 else (rules,)):
+                values, ids = program.run_top_resident([numpy_of(x)], [None], 0, 5, rules=given)
+                adjusted = [rule.apply(row) for rule, row in zip(given or [TokenRules()] * 3, rows)]
+                for got_values, got_ids, row in zip(values, ids, adjusted):
+                    order = _select_host(as_float(row), 5, None)[1]
+                    np.testing.assert_array_equal(got_ids, order)
+                    np.testing.assert_array_equal(got_values.view(np.uint8), row[order].view(np.uint8))
