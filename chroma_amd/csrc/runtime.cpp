@@ -383,14 +383,15 @@ public:
         }
     }
 
-    // The host arrays of ``rules`` (rows of ``width`` logits) one after another in page-locked memory, and the call that
-    // reads them at their places behind ``device``.
+    // The host arrays of ``rules`` (a call without mistakes) one after another in page-locked memory, and the call that reads
+    // them at their places behind ``device``.
     struct StagedRules {
         size_t bytes = 0;
         std::vector<std::pair<const void*, size_t>> pieces;  // host array (one row at a time where rows lie apart), bytes
         chroma_hip_adjust_call call{};
     };
-    static StagedRules stage_rules(const chroma_hip_adjust_call& rules, size_t rows, size_t width, char* device) {
+    static StagedRules stage_rules(const chroma_hip_adjust_call& rules, char* device) {
+        const size_t rows = size_t(rules.rows), width = size_t(rules.width);
         StagedRules staged;
         staged.call = rules;
         auto place = [&](const void* array, size_t count, int64_t stride, size_t row_bytes, size_t item) -> char* {
@@ -408,14 +409,7 @@ public:
             staged.bytes += bytes + padding;
             return at;
         };
-        if (rules.history && (rules.history_width < 0 || rules.history_stride < rules.history_width)) {
-            throw std::runtime_error("run_top_adjusted: a history row is longer than its stride");
-        }
         const size_t words = (width + 31) / 32, history = rules.history ? size_t(rules.history_width) : 0;
-        if ((rules.bias && rules.bias_stride && (rules.bias_stride < 0 || size_t(rules.bias_stride) < width)) ||
-            (rules.mask && rules.mask_stride && (rules.mask_stride < 0 || size_t(rules.mask_stride) < words))) {
-            throw std::runtime_error("run_top_adjusted: a stride is smaller than its row");
-        }
         staged.call.history = reinterpret_cast<const int64_t*>(place(rules.history, rows, rules.history_stride, history * 8, 8));
         staged.call.history_stride = staged.call.history_width = int64_t(history);
         staged.call.history_lengths = reinterpret_cast<const int64_t*>(place(rules.history_lengths, 1, 0, rows * 8, 8));
@@ -481,6 +475,21 @@ public:
         if (!scratch) {
             throw std::runtime_error("run_top: want 1 <= k <= min(width, 1024) and width <= 524288");
         }
+        char* logits = static_cast<char*>(base_) + plan_.outputs[index].offset;
+        chroma_hip_adjust_call call{};
+        if (rules) {  // checked here, before anything runs
+            call = *rules;
+            call.x = call.y = logits;
+            call.rows = int64_t(rows);
+            call.width = call.x_stride = call.y_stride = int64_t(width);
+            call.dtype = dtype;
+            call.history_stride = call.history ? call.history_stride : 0;
+            call.bias_stride = call.bias ? call.bias_stride : 0;
+            call.mask_stride = call.mask ? call.mask_stride : 0;
+            if (const char* wrong = chroma_adjust::mistake(call)) {
+                throw std::runtime_error(std::string("run_top_adjusted: ") + wrong);
+            }
+        }
         auto align = [](size_t n) { return (n + 255) / 256 * 256; };
         const size_t value_bytes = rows * size_t(k) * item, id_bytes = rows * size_t(k) * sizeof(int64_t);
         // ids then values, adjacent, so one copy brings both back
@@ -506,15 +515,15 @@ public:
         }
         StagedRules staged;
         if (rules) {
-            ensure_rules(rows * width * item, stage_rules(*rules, rows, width, nullptr).bytes);
-            staged = stage_rules(*rules, rows, width, static_cast<char*>(rules_));
+            ensure_rules(rows * width * item, stage_rules(call, nullptr).bytes);
+            staged = stage_rules(call, static_cast<char*>(rules_));
+            staged.call.y = adjusted_;
         }
         char* base = static_cast<char*>(select_);
         int64_t* device_ids = reinterpret_cast<int64_t*>(base + align(scratch));
         void* device_values = base + align(scratch) + id_bytes;
         try {
             upload(inputs);
-            char* logits = static_cast<char*>(base_) + plan_.outputs[index].offset;
             auto select = [&](const char* from) {
                 char message[256] = {0};
                 if (chroma_select::launch_rows_topk(from, dtype, rows, width, k, 1, device_values, device_ids, select_, scratch, stream_,
@@ -534,11 +543,6 @@ public:
                     check(hipMemcpyAsync(rules_, rules_host_, staged.bytes, hipMemcpyHostToDevice, stream_), "Upload rules");
                 }
                 launch_all();
-                staged.call.x = logits;
-                staged.call.y = adjusted_;
-                staged.call.rows = int64_t(rows);
-                staged.call.width = staged.call.x_stride = staged.call.y_stride = int64_t(width);
-                staged.call.dtype = dtype;
                 char message[256] = {0};
                 if (chroma_adjust::launch_rows_adjust(staged.call, stream_, message, sizeof(message))) {
                     throw HipError(message);

@@ -111,8 +111,8 @@ int launch_rows_topk(const void* x, int, size_t rows, size_t width, int k, int, 
 
 namespace chroma_adjust {
 int launch_rows_adjust(const chroma_hip_adjust_call& c, hipStream_t, char* error, size_t size) {
-    if (c.rows > 65535) {
-        return std::snprintf(error, size, "too many rows"), CHROMA_HIP_RUNTIME_ERROR;
+    if (const char* wrong = mistake(c)) {
+        return std::snprintf(error, size, "%s", wrong), CHROMA_HIP_RUNTIME_ERROR;
     }
     for (int64_t r = 0; r < c.rows; ++r) {
         const float* x = static_cast<const float*>(c.x) + r * c.x_stride;

@@ -38,6 +38,7 @@ class StubModel(NativeModel):
         spec = [{"name": "logits", "shape": [rows, width], "dtype": "float32"}]
         self.counted = library
         super().__init__(directory, spec, spec)
+        self.started = self.counts()[3]
 
     def counts(self):
         """[device allocations, page-locked allocations, instantiated graphs, plan kernels run] so far."""
@@ -100,6 +101,30 @@ def test_growing_histories_keep_their_buffers_and_the_captured_selection(stub_mo
     grown = model.counts() - first
     # half as much again each time: log(2 MB / 64 KiB) / log(1.5) = 8.5 moves, one buffer of each kind
     assert grown[0] <= 9 and grown[1] <= 9 and grown[2] == 0, grown
+
+
+def adjusted_status(model, rules, rows, width, **strides):
+    """(status, message) of a direct call with packed ``rules``, some strides or extents replaced."""
+    arrays = pack(rules, width)
+    call = native.Adjust(**{name: None if array is None else array.ctypes.data for name, array in arrays.items()})
+    call.history_stride = call.history_width = arrays["history"].shape[1]
+    for name, value in strides.items():
+        setattr(call, name, value)
+    logits, values, ids = np.ones((rows, width), np.float32), np.zeros((rows, 1), np.float32), np.zeros((rows, 1), np.int64)
+    error = ctypes.create_string_buffer(256)
+    status = model._lib.chroma_hip_run_top_adjusted(model._handle, native.pointer_array([logits.ctypes.data]), native.pointer_array([None]), 0, native.FLOAT32,
+                                                    rows, width, ctypes.byref(call), 1, values.ctypes.data, ids.ctypes.data, error, len(error))
+    return status, error.value.decode()
+
+
+@pytest.mark.parametrize("rows,changes,message", [
+    (65536, {}, "65535 rows"), (2, dict(history_width=-1), "stride"), (2, dict(history_stride=1), "stride"), (2, dict(bias_stride=3), "stride"),
+    (2, dict(bias_stride=-4), "stride"), (2, dict(history_width=2**61, history_stride=2**61), "out of range")])
+def test_refused_rules_run_nothing(stub_model, rows, changes, message):
+    model = stub_model(rows, 4)
+    status, text = adjusted_status(model, [TokenRules([1, 2], 1.5, bias={3: 1.0})] * rows, rows, 4, **changes)
+    assert status == native.RUNTIME_ERROR and message in text
+    assert model.counts()[3] == model.started, "the plan ran"
 
 
 @gpu
