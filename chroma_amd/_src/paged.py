@@ -4,17 +4,18 @@
 consumes one token of every sequence at a time. The cache lies in the step program's input staging; a
 sequence is a list of its pages (``PagePool``). Rows move on the device (``chroma_hip_cache_move``): a prompt's
 from the decoder's cache, a step's new rows into their pages, the last page of a forked sequence when it is
-first written to, live pages to the front of the cache. A step commits only after its program returned, in a
-section that defers SIGINT, so an interrupt leaves the last committed state.
+first written to, live pages to the front of the cache. A step commits only after its program returned and its moves are
+queued, in a section that defers SIGINT, so an interrupt or an error leaves the last committed state.
 
 (No counterpart in the reference, whose decoder holds one sequence, chroma/_src/decoder.py:44-152.)
 """
 
 from __future__ import annotations
 
+import contextlib
 import heapq
 import threading
-from typing import Any, Dict, Iterable, List, Mapping, Optional, Sequence, Tuple
+from typing import Any, Dict, Iterable, Iterator, List, Mapping, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -145,6 +146,16 @@ class PagedDecoder:
         if moves:
             self._step.native.cache_move(self._cache(), source, self._layers, self._row_bytes, np.array(moves, dtype=np.int64))
 
+    @contextlib.contextmanager
+    def _taking(self, count: int) -> Iterator[List[int]]:
+        """``count`` pages from the pool, which go back to it if the block fails."""
+        pages = [self._pool.take() for _ in range(count)]
+        try:
+            yield pages
+        except BaseException:
+            self._pool.release(pages)
+            raise
+
     def _new_slot(self) -> int:
         used = set(self._slot_of.values())
         slot = next((slot for slot in range(self._slots) if slot not in used), None)
@@ -181,12 +192,12 @@ class PagedDecoder:
                 # the prompt starts a fresh cache, so row i holds position i
                 owner = self._decoder._models[self._decoder._state.owner].native
                 owner.synchronize()  # its queued commits have landed
-                pages = [self._pool.take() for _ in range(needed)]
                 rows = self._decoder.context
                 source = native.CacheRows(keys=owner.input_pointer(2), values=owner.input_pointer(3), rows=rows, layer_pitch=rows * self._row_bytes)
                 size = self._page_rows
-                self._move(source, [(i * size, page * size, min(size, count - i * size)) for i, page in enumerate(pages)])
-                self._step.native.synchronize()  # before the decoder's next prompt overwrites the rows
+                with self._taking(needed) as pages:
+                    self._move(source, [(i * size, page * size, min(size, count - i * size)) for i, page in enumerate(pages)])
+                    self._step.native.synchronize()  # before the decoder's next prompt overwrites the rows
                 return self._enter(slot, pages, count), logits
 
     def fork(self, sequence: int) -> int:
@@ -289,19 +300,18 @@ class PagedDecoder:
         else:
             selection = self._step.run_top_resident(self._args, outputs, 0, k)
         with _interrupts_deferred():
-            copied = []
+            with self._taking(len(copies) + len(starts)) as taken:
+                pages = {s: self._pages[s][-1] for s in tokens} | dict(zip((*copies, *starts), taken))
+                self._move(self._cache(), [(self._pages[s][-1] * size, pages[s] * size, self._lengths[s] % size) for s in copies])
+                model = self._step.native
+                fresh = native.CacheRows(keys=model.output_pointer(1), values=model.output_pointer(2), rows=self._slots,
+                                         layer_pitch=self._slots * self._row_bytes)
+                self._move(fresh, [(self._slot_of[s], pages[s] * size + self._lengths[s] % size, 1) for s in tokens])
             for sequence in copies:
-                shared, page = self._pages[sequence][-1], self._pool.take()
-                copied.append((shared * size, page * size, self._lengths[sequence] % size))
-                self._pool.release([shared])
-                self._pages[sequence][-1] = page
+                self._pool.release(self._pages[sequence][-1:])
+                self._pages[sequence][-1] = pages[sequence]
             for sequence in starts:
-                self._pages[sequence].append(self._pool.take())
-            self._move(self._cache(), copied)
-            model = self._step.native
-            fresh = native.CacheRows(keys=model.output_pointer(1), values=model.output_pointer(2), rows=self._slots,
-                                     layer_pitch=self._slots * self._row_bytes)
-            self._move(fresh, [(self._slot_of[s], self._pages[s][-1] * size + self._lengths[s] % size, 1) for s in tokens])
+                self._pages[sequence].append(pages[sequence])
             for sequence in tokens:
                 self._lengths[sequence] += 1
                 self._set_row(sequence)
