@@ -177,7 +177,7 @@ class PagedDecoder:
     # ------------------------------------------------------------------------------------ sequences
     def add(self, tokens: Any) -> Tuple[int, np.ndarray]:
         """Consume a prompt; returns the new sequence and the logits [1, vocab] after the prompt's last token."""
-        with self._lock:
+        with self._lock, self._decoder._lock:  # the decoder's cache stays this prompt's until its rows have been taken
             if self._closed:
                 raise RuntimeError("PagedDecoder is closed")
             count = len(tokens)

@@ -3,6 +3,8 @@ are the sequences before the call, and the next calls answer as if it had not be
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 
 from tests.test_paged_decoder import Twin, fake_paged_decoder, small_model
@@ -62,3 +64,32 @@ def test_a_prompt_whose_rows_cannot_be_stored_takes_no_pages():
     twin.texts[b] = [1, 2, 3, 4, 5]
     twin.check(b, logits[0])
     twin.step(decoder, {b: 6, a: 2})
+
+
+def test_another_thread_cannot_use_the_decoder_in_the_middle_of_a_prompt():
+    """A prompt's rows are taken from the decoder's cache after it consumed them: another user of the same decoder waits."""
+    model = small_model()
+    decoder, twin = fake_paged_decoder(model), Twin(model, 2e-5, 2e-6)
+    prompts, append = decoder._decoder, decoder._decoder.append
+    threads = []
+
+    def consume(tokens):
+        logits = append(tokens)
+
+        def other():
+            prompts.reset()
+            append([16, 16, 16, 16, 16])
+
+        threads.append(threading.Thread(target=other))
+        threads[-1].start()
+        threads[-1].join(0.5)  # ends here only if it is let in
+        return logits
+
+    prompts.append = consume
+    a, logits = decoder.add([1, 2, 3, 4, 5])
+    threads[0].join(30)
+    assert not threads[0].is_alive() and prompts.position == 5
+    prompts.append = append
+    twin.texts[a] = [1, 2, 3, 4, 5]
+    twin.check(a, logits[0])
+    twin.step(decoder, {a: 6})
