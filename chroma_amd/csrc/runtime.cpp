@@ -653,10 +653,21 @@ public:
         }
     }
 
-    // Queued copies of cache rows (cache.hip).
+    // Queued copies of cache rows (cache.hip). A kernel that follows an address of another device's memory faults, and two
+    // programs of one process may lie on two devices of the same name, so such caches are refused.
     void cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers, int64_t row_bytes, const int64_t* moves,
                     int64_t count) {
         DeviceGuard guard(device_);
+        for (const chroma_hip_cache_rows* cache : {to, from}) {
+            for (const void* rows : {cache ? cache->keys : nullptr, cache ? cache->values : nullptr}) {
+                hipPointerAttribute_t attributes{};
+                if (rows && hipPointerGetAttributes(&attributes, rows) != hipSuccess) {
+                    static_cast<void>(hipGetLastError());
+                } else if (rows && attributes.type == hipMemoryTypeDevice && attributes.device != device_) {
+                    throw std::runtime_error("cache_move: a cache lies on another device than the program");
+                }
+            }
+        }
         char message[256] = {0};
         if (chroma_cache::launch_cache_move(to, from, layers, row_bytes, moves, count, stream_, message, sizeof(message))) {
             throw std::runtime_error(message);

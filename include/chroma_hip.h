@@ -245,7 +245,7 @@ int chroma_hip_cache_move(const chroma_hip_cache_rows* to, const chroma_hip_cach
                           const int64_t* moves, int64_t count, void* stream, char* error, size_t error_size);
 
 /* The same moves queued on the program's stream, as ``chroma_hip_copy_2d_batch_queued``: they run before the program's
- * later runs. Both caches lie in device memory of the program's device. */
+ * later runs. Both caches lie in device memory of the program's device; memory that HIP knows as another device's is refused. */
 int chroma_hip_cache_move_queued(void* handle, const chroma_hip_cache_rows* to, const chroma_hip_cache_rows* from, int64_t layers,
                                  int64_t row_bytes, const int64_t* moves, int64_t count, char* error, size_t error_size);
 

@@ -1,5 +1,5 @@
 """Selection of tokens from adjusted logits over many steps (``run_top`` with rules): histories that grow, rules whose rows
-lie apart, plain selections between them.
+lie apart, plain selections between them; and what the runtime refuses for the paged cache.
 
 CPU: the runtime itself, built over a stand-in for HIP (``runtime_stub.cpp``) that counts what it allocates and captures.
 GPU (marked): compiled programs against the host rule."""
@@ -41,7 +41,7 @@ class StubModel(NativeModel):
         self.started = self.counts()[3]
 
     def counts(self):
-        """[device allocations, page-locked allocations, instantiated graphs, plan kernels run] so far."""
+        """[device allocations, page-locked allocations, instantiated graphs, plan kernels and moves run] so far."""
         values = np.zeros(4, np.int64)
         self.counted.stub_counts(values.ctypes.data_as(ctypes.c_void_p))
         return values
@@ -55,7 +55,7 @@ def stub_library(tmp_path_factory):
                     f"-I{native.ROCM / 'include'}", *map(str, sources), "-o", str(path)], check=True)
     library = ctypes.CDLL(str(path))
     for name in ("chroma_hip_create", "chroma_hip_run", "chroma_hip_device_name", "chroma_hip_signature", "chroma_hip_destroy", "chroma_hip_run_top",
-                 "chroma_hip_run_top_adjusted"):
+                 "chroma_hip_run_top_adjusted", "chroma_hip_cache_move_queued"):
         function, known = getattr(library, name), getattr(native.library(), name)
         function.argtypes, function.restype = known.argtypes, known.restype
     return library
@@ -125,6 +125,21 @@ def test_refused_rules_run_nothing(stub_model, rows, changes, message):
     status, text = adjusted_status(model, [TokenRules([1, 2], 1.5, bias={3: 1.0})] * rows, rows, 4, **changes)
     assert status == native.RUNTIME_ERROR and message in text
     assert model.counts()[3] == model.started, "the plan ran"
+
+
+@pytest.mark.parametrize("away", [None, ("to", "keys"), ("to", "values"), ("source", "keys"), ("source", "values")])
+def test_queued_moves_of_memory_on_another_device_are_refused(stub_model, away):
+    model, moves = stub_model(1, 4), np.array([[0, 1, 1]], dtype=np.int64)
+    caches = {name: native.CacheRows(keys=base, values=base + 4096, rows=4, layer_pitch=64) for name, base in (("to", 1 << 20), ("source", 1 << 24))}
+    if away is None:
+        caches["source"].keys = 256  # what HIP does not know is left to the caller
+        model.cache_move(caches["to"], caches["source"], 1, 16, moves)
+        assert model.counts()[3] == model.started + 1
+        return
+    setattr(caches[away[0]], away[1], 1 << 60)
+    with pytest.raises(RuntimeError, match="another device"):
+        model.cache_move(caches["to"], caches["source"], 1, 16, moves)
+    assert model.counts()[3] == model.started
 
 
 @gpu
