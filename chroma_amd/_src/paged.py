@@ -23,7 +23,7 @@ from chroma_amd._src import host, native
 from chroma_amd._src.decoder import SELECT_MAX_K, Decoder, _interrupts_deferred, _staging_mirror
 from chroma_amd._src.dtypes import numpy_dtype
 from chroma_amd._src.program import Program
-from chroma_amd._src.rules import TokenRules
+from chroma_amd._src.rules import TokenRules, unread
 
 
 class PagePool:
@@ -295,8 +295,9 @@ class PagedDecoder:
             self._step.run_resident(self._args, outputs)
         elif rules:
             plain = TokenRules()
-            by_slot = {self._slot_of[sequence]: rule for sequence, rule in rules.items()}
-            selection = self._step.run_top_resident(self._args, outputs, 0, k, [by_slot.get(slot, plain) for slot in range(self._slots)])
+            by_slot = {self._slot_of[sequence]: rules.get(sequence, plain) for sequence in tokens}
+            idle = unread(list(by_slot.values()))
+            selection = self._step.run_top_resident(self._args, outputs, 0, k, [by_slot.get(slot, idle) for slot in range(self._slots)])
         else:
             selection = self._step.run_top_resident(self._args, outputs, 0, k)
         with _interrupts_deferred():

@@ -109,6 +109,17 @@ class TokenRules:
         return float32_to_bf16(x) if row.dtype == BFLOAT16 else x
 
 
+def unread(rules: Sequence[TokenRules]) -> TokenRules:
+    """What a row that nobody reads is given beside ``rules``: the bias and the allowed tokens that all of them share, so
+    that it does not end the sharing, and nothing else."""
+    row = TokenRules()
+    for name in ("bias", "allowed"):
+        value = getattr(rules[0], name)
+        if all(getattr(rule, name) is value for rule in rules):
+            object.__setattr__(row, name, value)
+    return row
+
+
 def pack(rules: Sequence[TokenRules], vocab_size: int) -> Dict[str, Optional[np.ndarray]]:
     """The rows' rules as the arrays of ``chroma_hip_adjust_call``: history [rows, longest] padded with -1, its
     lengths, the three factors, bias [rows, vocab] and mask words [rows, ceil(vocab / 32)] (bias and mask as one

@@ -21,6 +21,7 @@ from chroma_amd._src.program import NativeModel
 from chroma_amd._src.rules import pack
 from tests.conftest import ROOT
 from tests.helpers import Function, as_float, numpy_of
+from tests.test_paged_decoder import SLOTS, fake_paged_decoder, small_model
 
 gpu = pytest.mark.gpu
 
@@ -125,6 +126,30 @@ def test_refused_rules_run_nothing(stub_model, rows, changes, message):
     status, text = adjusted_status(model, [TokenRules([1, 2], 1.5, bias={3: 1.0})] * rows, rows, 4, **changes)
     assert status == native.RUNTIME_ERROR and message in text
     assert model.counts()[3] == model.started, "the plan ran"
+
+
+@pytest.mark.parametrize("tokens", [{0: 1, 1: 2, 2: 3}, {2: 5}], ids=["a-free-slot", "idle-sequences"])
+def test_slots_without_a_token_do_not_end_the_sharing_of_a_bias_and_a_mask(tokens, monkeypatch):
+    """Rules that all sequences of a step share are laid out as one row, whatever the other slots of the step program hold."""
+    decoder = fake_paged_decoder(small_model())
+    for prompt in ([1, 2], [3], [4, 5, 6]):
+        decoder.add(prompt)
+    bias, allowed = np.linspace(-1, 1, 17).astype(np.float32), np.arange(17) % 3 == 0
+    rules = {s: TokenRules([s, s + 1], 1.5, bias=bias, allowed=allowed) for s in tokens}
+    run_top, seen = decoder._step.native.run_top, []
+
+    def watched(inputs, outputs, index, k, given):
+        seen.append(pack(given, 17))
+        return run_top(inputs, outputs, index, k, given)
+
+    monkeypatch.setattr(decoder._step.native, "run_top", watched)
+    values, ids = decoder.step_top(tokens, 2, rules=rules)
+    assert (ids % 3 == 0).all() and np.isfinite(values).all()
+    assert len(seen[0]["history"]) == SLOTS and seen[0]["bias"].shape == (1, 17) and seen[0]["mask"].shape == (1, 1)
+    # a sequence with a token and without rules keeps its plain row, and a slot without a token then has one too
+    if len(tokens) == 3:
+        decoder.step_top(tokens, 2, rules={0: rules[0]})
+        assert seen[1]["bias"].shape == (SLOTS, 17) and not seen[1]["bias"][1:].any() and (seen[1]["mask"][1:] == 0xFFFFFFFF).all()
 
 
 @pytest.mark.parametrize("away", [None, ("to", "keys"), ("to", "values"), ("source", "keys"), ("source", "values")])
