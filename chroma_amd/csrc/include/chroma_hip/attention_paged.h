@@ -2,8 +2,8 @@
 //
 //     o = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)),   s_j = scale * (q . k_j),
 //
-// j over the cached rows that the sequence's page table holds and its window leaves, and the new row. Scores, sums and
-// products stay in float; the result is rounded once.
+// j over the cached rows that the sequence's page table holds and its window leaves, and the new row. Scores and sums stay
+// in float and the result is rounded once; a bfloat16 weight meets V as two halves (below).
 #pragma once
 
 #include "attention_flash.h"

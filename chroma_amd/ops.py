@@ -24,7 +24,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_new: Optional
     head, or None. Row j < lengths[b] of sequence b is row j % R of page table[b, j // R]. ``window`` > 0 leaves
     out the rows at least ``window`` before the token's position, but for the ``first`` first ones. Lengths
     below 0 count as 0 and above N * R as N * R, rows on pages outside [0, P) are not seen, and a token that
-    sees no row gets zeros. Scores, sums and products are float's, rounded once."""
+    sees no row gets zeros. Scores and sums are float's, the result is rounded once; compiled with bfloat16, a weight
+    meets the values as two bfloat16 halves (within 2^-16 of it)."""
     _check(q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, window, first)
     sequences, kv_heads, group, dim = q.shape
     pages, rows = k_pages.shape[:2]

@@ -190,14 +190,15 @@ int chroma_hip_run_top(void* handle, const void* const* inputs, void* const* out
  * table[b][j / page_rows], and, when ``k_new`` / ``v_new`` are given, one new row at position lengths[b]. The token's
  * position t is lengths[b] with a new row and lengths[b] - 1 without. ``window`` > 0 leaves out the cached rows
  * j <= t - window except the ``first`` first ones. The sink term (a learned logit per query head) is left out when ``sinks`` is null.
- * A token that sees no row gets zeros. Scores, sums and products are kept in float and rounded once, at the end.
+ * A token that sees no row gets zeros. Scores and sums are kept in float and the result is rounded once, at the end; with
+ * bfloat16 values each weight exp(s_j - m) meets v_j as two bfloat16 halves, which leaves out at most 2^-16 of it.
  *
  * Lengths are read on the device: one below 0 counts as 0 and one above ``longest`` as ``longest``, and only the first
  * ceil(longest / page_rows) entries of a table row are read. A row on a page outside [0, pages) is not seen.
  *
  * The head dimension is innermost and contiguous; strides count elements. Each query head of KV head h, h * group + g,
  * lies at (h * group + g) * dim of its sequence's q and out. q, out, k_pages, v_pages, k_new and v_new start on 16 bytes
- * and their strides are whole 16-byte chunks. out must not overlap an input. */
+ * and their strides are whole 16-byte chunks. out and the workspace must not overlap an input, nor each other. */
 typedef struct chroma_hip_paged_attention_call {
     const void* q;          /* [sequences, kv_heads, group, dim] */
     const void* k_pages;    /* [pages, page_rows, kv_heads, dim] at page_stride, row_stride, head_stride */
@@ -226,8 +227,9 @@ size_t chroma_hip_paged_attention_workspace(const chroma_hip_paged_attention_cal
 int chroma_hip_paged_attention(const chroma_hip_paged_attention_call* call, void* workspace, size_t workspace_bytes, void* stream,
                                char* error, size_t error_size);
 
-/* Rows of a cache: ``keys`` and ``values`` hold [layers, rows, row bytes], layers ``layer_pitch`` bytes apart. The pages of a
- * paged cache are runs of page_rows rows. */
+/* Rows of a cache: ``keys`` and ``values`` hold [layers, rows, row bytes], layers ``layer_pitch`` bytes apart. In a cache that
+ * is written, all layers of one lie behind the last of the other (keys and values that take turns by layer are refused).
+ * The pages of a paged cache are runs of page_rows rows. */
 typedef struct chroma_hip_cache_rows {
     void* keys;
     void* values;
@@ -256,8 +258,10 @@ int chroma_hip_cache_move_queued(void* handle, const chroma_hip_cache_rows* to, 
  *   - -inf where the token's bit of ``mask`` (bit i % 32 of word i / 32) is 0.
  * The arithmetic is float's, one rounding per operation, and the result is rounded to y's type once. ``history`` holds
  * token ids; of row r the first history_lengths[r] count (all history_width when null; less than 0 counts as 0, more
- * than history_width as history_width), and ids outside [0, width) count for nothing. A null parameter array changes
- * nothing. y may be x itself with the same stride (then only what changes is written); otherwise it must not overlap x, nor in either case another array. */
+ * than history_width as history_width), and ids outside [0, width) count for nothing. Each row has a history of its own
+ * (history_stride >= history_width); biases and masks can be one row for all. A null parameter array changes nothing. y may
+ * be x itself with the same stride (then only what changes is written); otherwise it must not overlap x, nor in either case
+ * another array. */
 typedef struct chroma_hip_adjust_call {
     const void* x; /* [rows, width] at x_stride elements */
     void* y;       /* [rows, width] at y_stride elements */
@@ -278,7 +282,8 @@ int chroma_hip_rows_adjust(const chroma_hip_adjust_call* call, void* stream, cha
 
 /* ``chroma_hip_run_top`` over adjusted logits: the rows of output ``output_index`` go through ``rules`` into scratch of the
  * program (the output itself stays as it is), and the selection reads that. The arrays of ``rules`` are host memory, read
- * before the call returns; its x, y, rows, width, x_stride, y_stride and dtype are the output's and are not read. */
+ * before the call returns; its x, y, rows, width, x_stride, y_stride and dtype are the output's and are not read. What the
+ * adjustment refuses (more than 65535 rows, a stride smaller than its row) is refused before anything runs. */
 int chroma_hip_run_top_adjusted(void* handle, const void* const* inputs, void* const* outputs, int output_index, int dtype, size_t rows,
                                 size_t width, const chroma_hip_adjust_call* rules, int k, void* values, int64_t* ids, char* error,
                                 size_t error_size);
