@@ -104,6 +104,29 @@ def test_growing_histories_keep_their_buffers_and_the_captured_selection(stub_mo
     assert grown[0] <= 9 and grown[1] <= 9 and grown[2] == 0, grown
 
 
+def test_rules_whose_rows_lie_apart(stub_model):
+    """Rows of the rules' arrays further apart than they are long; what lies between them is nobody's."""
+    rows, width, k, rng = 3, 70, 4, np.random.default_rng(5)
+    model = stub_model(rows, width)
+    rules = [TokenRules(rng.integers(0, width, 5 + i), 1.5, 0.25, 0.125, rng.normal(size=width).astype(np.float32), rng.random(width) < 0.6) for i in range(rows)]
+    arrays = pack(rules, width)
+    spread = {name: np.full((rows, arrays[name].shape[1] + gap), fill, arrays[name].dtype)
+              for name, gap, fill in (("history", 3, 9), ("bias", 13, np.nan), ("mask", 2, 0))}
+    for name, room in spread.items():
+        room[:, : arrays[name].shape[1]] = arrays[name]
+    call = native.Adjust(**{name: spread.get(name, array).ctypes.data for name, array in arrays.items()})
+    call.history_width = arrays["history"].shape[1]
+    call.history_stride, call.bias_stride, call.mask_stride = (spread[name].shape[1] for name in ("history", "bias", "mask"))
+    logits = rng.normal(size=(rows, width)).astype(np.float32)
+    values, ids, error = np.zeros((rows, k), np.float32), np.zeros((rows, k), np.int64), ctypes.create_string_buffer(256)
+    native.check(model._lib.chroma_hip_run_top_adjusted(
+        model._handle, native.pointer_array([logits.ctypes.data]), native.pointer_array([None]), 0, native.FLOAT32, rows, width, ctypes.byref(call), k,
+        values.ctypes.data, ids.ctypes.data, error, len(error)), error)
+    want_values, want_ids = chosen(logits, rules, k)
+    np.testing.assert_array_equal(ids, want_ids)
+    np.testing.assert_array_equal(values, want_values)
+
+
 def adjusted_status(model, rules, rows, width, **strides):
     """(status, message) of a direct call with packed ``rules``, some strides or extents replaced."""
     arrays = pack(rules, width)
