@@ -37,7 +37,7 @@ typedef Aligned Bytes __attribute__((aligned(1)));             // at any address
 
 // grid: (pieces of the longest move, moves, layers x keys or values). A thread copies 16 bytes, and what a move's length
 // leaves of its last 16 bytes goes byte by byte. Loads and stores are non-temporal: 1500 pages of 16 rows of 1 KiB in 24
-// layers (4.7 GB read and written) 387 us against 454 through the caches (64 threads: 370 and 437, but 100 pages of
+// layers (2.4 GB read and written in all) 387 us against 454 through the caches (64 threads: 370 and 437, but 100 pages of
 // differing fill 21 us against 12; 4 loads under way a thread: 421 and 478).
 template <bool ALIGNED> __global__ void __launch_bounds__(kThreads) move_rows(Moves m) {
     using Unit = std::conditional_t<ALIGNED, Aligned, Bytes>;
