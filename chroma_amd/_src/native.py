@@ -19,7 +19,7 @@ PACKAGE = Path(__file__).resolve().parents[1]
 REPO = PACKAGE.parent
 LIBRARY = PACKAGE / "lib" / "libchroma_hip.so"
 RUNTIME_SOURCE = PACKAGE / "csrc" / "runtime.cpp"
-DEVICE_SOURCES = [PACKAGE / "csrc" / f"{name}.hip" for name in ("select", "copy", "masks", "paged", "cache", "adjust")]
+DEVICE_SOURCES = [PACKAGE / "csrc" / f"{name}.hip" for name in ("select", "copy", "masks", "paged", "cache", "adjust", "plan", "store", "chunk", "sample")]
 DEVICE_INCLUDE = PACKAGE / "csrc" / "include"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
@@ -96,6 +96,46 @@ class Adjust(ctypes.Structure):
     ]
 
 
+class PagedPlan(ctypes.Structure):
+    """``chroma_hip_paged_plan_call``: a step's page tables, slots and positions from its requests' lengths."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("lengths", "counts", "free_pages", "cursor", "table", "starts", "slots", "positions", "owners",
+                                               "new_lengths", "taken")),
+        *((name, ctypes.c_int64) for name in ("sequences", "tokens", "pages", "page_rows", "span", "table_stride", "free_count")),
+    ]
+
+
+class CacheStore(ctypes.Structure):
+    """``chroma_hip_cache_store_call``: new rows of keys and values stored at their slots."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("keys", "values", "new_keys", "new_values", "slots")),
+        *((name, ctypes.c_int64) for name in ("layers", "rows", "count", "row_bytes", "layer_pitch", "new_layer_pitch", "new_row_pitch")),
+    ]
+
+
+class PagedChunk(ctypes.Structure):
+    """``chroma_hip_paged_chunk_call``: attention of a chunk of new tokens of every sequence over a paged cache."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("q", "k_pages", "v_pages", "k_new", "v_new", "sinks", "table", "lengths", "starts", "out")),
+        *((name, ctypes.c_int64) for name in ("tokens", "sequences", "kv_heads", "group", "dim", "pages", "page_rows", "page_stride", "row_stride",
+                                              "head_stride", "q_stride", "new_stride", "out_stride", "table_stride", "longest", "window", "first")),
+        ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class Sample(ctypes.Structure):
+    """``chroma_hip_sample_call``: a token drawn from each row of logits."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p), *((name, ctypes.c_int64) for name in ("rows", "width", "x_stride")),
+        *((name, ctypes.c_void_p) for name in ("temperature", "top_k", "top_p", "min_p", "uniform", "ids", "logprobs")),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 def library() -> ctypes.CDLL:
     global _library
     if _library is not None:
@@ -157,6 +197,12 @@ def library() -> ctypes.CDLL:
                                                      c.c_int64, c.c_char_p, c.c_size_t]
         lib.chroma_hip_run_top_adjusted.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_int, c.c_int, c.c_size_t, c.c_size_t,
                                                     c.POINTER(Adjust), c.c_int, c.c_void_p, c.c_void_p, c.c_char_p, c.c_size_t]
+        for name, call in (("chroma_hip_paged_chunk_attention", PagedChunk), ("chroma_hip_rows_sample", Sample)):
+            getattr(lib, name + "_workspace").argtypes = [c.POINTER(call)]
+            getattr(lib, name + "_workspace").restype = c.c_size_t
+            getattr(lib, name).argtypes = [c.POINTER(call), c.c_void_p, c.c_size_t, c.c_void_p, c.c_char_p, c.c_size_t]
+        for name, call in (("chroma_hip_paged_plan", PagedPlan), ("chroma_hip_cache_store", CacheStore)):
+            getattr(lib, name).argtypes = [c.POINTER(call), c.c_void_p, c.c_char_p, c.c_size_t]
         _library = lib
         return lib
 
@@ -194,6 +240,12 @@ EXPORTED = (
     "chroma_hip_cache_move_queued",
     "chroma_hip_rows_adjust",
     "chroma_hip_run_top_adjusted",
+    "chroma_hip_paged_plan",
+    "chroma_hip_cache_store",
+    "chroma_hip_paged_chunk_attention_workspace",
+    "chroma_hip_paged_chunk_attention",
+    "chroma_hip_rows_sample_workspace",
+    "chroma_hip_rows_sample",
 )
 
 

@@ -288,6 +288,138 @@ int chroma_hip_run_top_adjusted(void* handle, const void* const* inputs, void* c
                                 size_t width, const chroma_hip_adjust_call* rules, int k, void* values, int64_t* ids, char* error,
                                 size_t error_size);
 
+/* --- steps in which every sequence takes any number of tokens ---
+ * A prompt's chunk, a second turn or one decoded token of each sequence in one step: planned, stored, attended and sampled on
+ * the device, on the caller's stream (no counterpart in the reference, whose decoder holds one sequence and is planned on the
+ * host, chroma/_src/decoder.py:57-152, and whose chat script samples on the host, scripts/chat.py:82-98). All pointers are
+ * device memory of the current device; each call queues its kernels, allocates nothing and can be captured into a graph. What
+ * a call writes must not overlap what it reads, nor what else it writes, unless it says so. */
+
+/* The plan of a step from its requests' lengths. Sequence b holds lengths[b] rows and takes n_b = counts[b] new tokens, in the
+ * sequences' order, as long as the step has room for ``tokens`` of them:
+ *
+ *   starts[0] = 0, starts[b + 1] = min(starts[b] + counts[b], tokens), n_b = starts[b + 1] - starts[b]
+ *
+ * Its rows lengths[b] .. lengths[b] + n_b - 1 lie on the pages of its table row. Those that begin a page take one from
+ * ``free_pages``, in the order of sequences and rows, from entry *cursor on (0 when null): the table gets them, and *taken is
+ * the entry after the last one that the step needs. More than free_count means that there were too few: the pages that are
+ * missing are -1 in the table. For token t = starts[b] + i of the step: positions[t] = lengths[b] + i, owners[t] = b, and
+ * slots[t] is the row of the cache that holds it, table[b][p / page_rows] * page_rows + p % page_rows with p = positions[t], or
+ * -1 where p lies behind the table row or its page outside [0, pages). Tokens that no sequence takes get -1 in all three.
+ * new_lengths[b] = lengths[b] + n_b, at most span * page_rows.
+ *
+ * Lengths below 0 count as 0 and above span * page_rows as that, counts below 0 as 0, a cursor below 0 as 0. Table entries
+ * before the new pages are read and keep what they hold. positions, owners and new_lengths may be null. */
+typedef struct chroma_hip_paged_plan_call {
+    const int64_t* lengths;    /* [sequences] */
+    const int64_t* counts;     /* [sequences] */
+    const int64_t* free_pages; /* [free_count], or null when free_count is 0 */
+    const int64_t* cursor;     /* [1] or null */
+    int64_t* table;            /* [sequences, span] at table_stride, read and written */
+    int64_t* starts;           /* [sequences + 1] */
+    int64_t* slots;            /* [tokens] */
+    int64_t* positions;        /* [tokens] or null */
+    int64_t* owners;           /* [tokens] or null */
+    int64_t* new_lengths;      /* [sequences] or null */
+    int64_t* taken;            /* [1] */
+    int64_t sequences, tokens;
+    int64_t pages, page_rows, span, table_stride, free_count;
+} chroma_hip_paged_plan_call;
+int chroma_hip_paged_plan(const chroma_hip_paged_plan_call* call, void* stream, char* error, size_t error_size);
+
+/* New rows of keys and values stored in a cache, in every layer: row i of ``new_keys`` / ``new_values`` becomes row slots[i] of
+ * ``keys`` / ``values``. A slot outside [0, rows) stores nothing. The slots inside must differ (of two rows with one slot, bytes
+ * of either may stay). Rows that no slot names keep their bytes. Layers of the cache lie layer_pitch bytes apart (its rows one
+ * behind the other), those of the new rows new_layer_pitch, and the new rows new_row_pitch: they can be columns of a wider
+ * matrix. Any alignment is taken. */
+typedef struct chroma_hip_cache_store_call {
+    void* keys;             /* [layers, rows, row_bytes] */
+    void* values;
+    const void* new_keys;   /* [layers, count, row_bytes] at the new pitches */
+    const void* new_values;
+    const int64_t* slots;   /* [count] */
+    int64_t layers, rows, count;
+    int64_t row_bytes;
+    int64_t layer_pitch, new_layer_pitch, new_row_pitch;
+} chroma_hip_cache_store_call;
+int chroma_hip_cache_store(const chroma_hip_cache_store_call* call, void* stream, char* error, size_t error_size);
+
+/* Attention of a chunk of new tokens of every sequence over its cached keys and values, which lie in pages, as
+ * ``chroma_hip_paged_attention`` has it for one token each. Sequence b's tokens are rows starts[b] .. starts[b + 1] - 1 of q and
+ * out, none or any number of them. With ``k_new`` / ``v_new`` the chunk's own rows lie there, row by row as in q, and token i
+ * of a sequence has position lengths[b] + i; without, they have been stored: the last n_b of the lengths[b] cached rows are
+ * the chunk's, and token i has position lengths[b] - n_b + i (below 0: it sees nothing). A token at position t sees the rows
+ * j <= t, cached or new; ``window`` > 0 leaves out those with j <= t - window except the ``first`` first ones. A token that sees no
+ * row gets zeros, and rows of out that belong to no sequence stay as they are.
+ *
+ * Scores and sums are kept in float and the result is rounded once, at the end; with bfloat16 values each weight exp(s_j - m)
+ * meets v_j rounded to bfloat16 (within 2^-8 of it). A value that is not finite reaches only the tokens that see its row.
+ *
+ * ``starts`` must ascend within [0, tokens]; entries outside count as the nearest bound, a range that descends as empty. Lengths,
+ * table rows, bad pages, strides and alignments are as for ``chroma_hip_paged_attention``; new_stride and q_stride count from token to
+ * token. */
+typedef struct chroma_hip_paged_chunk_call {
+    const void* q;          /* [tokens, kv_heads, group, dim] */
+    const void* k_pages;    /* [pages, page_rows, kv_heads, dim] at page_stride, row_stride, head_stride */
+    const void* v_pages;    /* laid out as k_pages */
+    const void* k_new;      /* [tokens, kv_heads, dim], or null (then v_new is null too) */
+    const void* v_new;
+    const void* sinks;      /* [kv_heads * group] or null */
+    const int64_t* table;   /* [sequences, table_stride] */
+    const int64_t* lengths; /* [sequences] */
+    const int64_t* starts;  /* [sequences + 1] */
+    void* out;              /* [tokens, kv_heads, group, dim] */
+    int64_t tokens, sequences, kv_heads, group;
+    int64_t dim; /* a multiple of 8, at most 256 */
+    int64_t pages, page_rows;
+    int64_t page_stride, row_stride, head_stride;
+    int64_t q_stride, new_stride, out_stride; /* between tokens */
+    int64_t table_stride;
+    int64_t longest; /* bound of the lengths */
+    int64_t window, first; /* 0: no window, no first rows */
+    float scale;
+    int32_t dtype; /* of every value: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
+} chroma_hip_paged_chunk_call;
+
+/* Scratch bytes the call needs (no pointer but k_new matters; 0 when none is needed or the extents would be refused).
+ * Calls that may run at the same time need workspaces of their own. */
+size_t chroma_hip_paged_chunk_attention_workspace(const chroma_hip_paged_chunk_call* call);
+int chroma_hip_paged_chunk_attention(const chroma_hip_paged_chunk_call* call, void* workspace, size_t workspace_bytes, void* stream,
+                                     char* error, size_t error_size);
+
+/* A token drawn from each row of logits. In descending order of the logits, ties to the lower id, token i has the weight
+ * w_i = exp((x_i - x_max) / temperature), and of the row's tokens are kept
+ *   - the first top_k (0 or less: all);
+ *   - of those, the fewest first ones whose weights reach top_p of the sum of them (1 or more: all; 0 or less: one);
+ *   - of those, the ones with w_i >= min_p (0 or less: all), one at least.
+ * The chosen token is the first whose running sum of weights exceeds ``uniform`` times the kept sum: ids[r], and logprobs[r] is
+ * the logarithm of its share of the kept sum. ``uniform`` is a random number from [0, 1): below 0 it counts as 0, from 1 on as
+ * the largest below. A temperature of 0 or less chooses the largest logit (logprob 0). NaN settings count as those that
+ * change nothing: a temperature or uniform of 0, a top_p of 1, a min_p of 0. A row with a NaN gives the first NaN's id, as the
+ * row selection ranks it (logprob NaN); with an infinite logit, the infinite ones share the row; with nothing but -inf, -1 (logprob
+ * -inf).
+ *
+ * Weights are evaluated and summed in 64 bits, in units of 2^-44 of the largest: sums do not depend on any order, and a token
+ * of less than half a unit is never drawn. */
+typedef struct chroma_hip_sample_call {
+    const void* x; /* [rows, width] at x_stride elements */
+    int64_t rows, width, x_stride;
+    const float* temperature; /* [rows] each, or null: 1 */
+    const int64_t* top_k;     /* or null: 0 */
+    const float* top_p;       /* or null: 1 */
+    const float* min_p;       /* or null: 0 */
+    const float* uniform;     /* [rows] */
+    int64_t* ids;             /* [rows] */
+    float* logprobs;          /* [rows] or null */
+    int32_t dtype; /* of x: CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16 */
+} chroma_hip_sample_call;
+
+/* Scratch bytes the call needs (no pointer matters; 0 when none is needed or the extents would be refused). Calls that may
+ * run at the same time need workspaces of their own. */
+size_t chroma_hip_rows_sample_workspace(const chroma_hip_sample_call* call);
+int chroma_hip_rows_sample(const chroma_hip_sample_call* call, void* workspace, size_t workspace_bytes, void* stream, char* error,
+                           size_t error_size);
+
 #ifdef __cplusplus
 }
 #endif
