@@ -21,8 +21,14 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk_tiles(chroma::ChunkOpe
     chroma::attention_chunk_tiles<T, DP, KEYS, WAVES>(a, splits, scratch);
 }
 
-template <class T, int DP> __global__ void __launch_bounds__(256) paged_chunk_combine(chroma::ChunkOperands<T> a, uint32_t splits, float* scratch) {
-    chroma::attention_chunk_combine<T, DP>(a, splits, scratch);
+template <int DP, uint32_t KEYS, bool FULL, int MIN>
+__global__ void __launch_bounds__(256, MIN) paged_chunk_wide(chroma::ChunkOperands<uint16_t> a, uint32_t splits, float* scratch) {
+    chroma::attention_chunk_wide<DP, KEYS, FULL>(a, splits, scratch);
+}
+
+template <class T, int DP, uint32_t ROWS, bool LOG2>
+__global__ void __launch_bounds__(256) paged_chunk_combine(chroma::ChunkOperands<T> a, uint32_t splits, float* scratch) {
+    chroma::attention_chunk_combine<T, DP, ROWS, LOG2>(a, splits, scratch);
 }
 
 constexpr int64_t kMost = int64_t(1) << 31;  // extents that the kernels count in 32 bits stay below this
@@ -116,34 +122,56 @@ template <class T> chroma::ChunkOperands<T> operands(const Call& c) {
 // Whether a call of these types and head dimension runs on the kernels of padded dimension DP.
 template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP == (sizeof(T) == 2 ? 32 : 16) || c.dim > DP / 2); }
 
-// How a call is cut: at most this many tiles of all sequences, and workgroups for each of them.
+// How a call is cut: tiles of 128 rows or of 16, at most this many of all sequences, and workgroups for each of them.
 struct Cut {
+    bool wide;
     int64_t tiles, splits;
 };
 template <class T, int DP> Cut cut_of(const Call& c) {
     Cut cut;
-    cut.tiles = c.tokens * c.group / 16 + std::min(c.sequences, c.tokens);
-    const int64_t keys = chroma::paged_whole_keys<T, DP>(), waves = chroma::paged_whole_waves<T, DP>();
-    const int64_t rows = c.longest + (c.k_new ? c.tokens : 0), blocks = (rows + keys - 1) / keys + 1;
-    const int64_t most = c.window ? std::min(blocks, (std::min(c.first, rows) + std::min(c.window, rows)) / keys + 3) : blocks;
+    const auto tiles_of = [&](int64_t rows) { return c.tokens * c.group / rows + std::min(c.sequences, c.tokens); };
+    const int64_t rows = c.longest + (c.k_new ? c.tokens : 0);
+    const auto most_blocks = [&](int64_t keys) {
+        const int64_t blocks = (rows + keys - 1) / keys + 1;
+        return c.window ? std::min(blocks, (std::min(c.first, rows) + std::min(c.window, rows)) / keys + 3) : blocks;
+    };
+    cut.wide = sizeof(T) == 2 && c.tokens * c.group >= 64 * c.sequences && c.tokens * c.group * c.kv_heads >= 128 * 64;
+    const int64_t keys = cut.wide ? chroma::chunk_wide_keys<DP>() : chroma::paged_whole_keys<T, DP>();
+    const int64_t waves = cut.wide ? 1 : chroma::paged_whole_waves<T, DP>();
+    cut.tiles = tiles_of(cut.wide ? chroma::kChunkRows : 16);
     const int64_t wanted = (512 + cut.tiles * c.kv_heads - 1) / (cut.tiles * c.kv_heads);
-    cut.splits = std::max<int64_t>(1, std::min(wanted, most / (2 * waves)));
+    cut.splits = std::max<int64_t>(1, std::min(wanted, most_blocks(keys) / (2 * waves)));
     return cut;
 }
 
 template <class T, int DP> size_t scratch_bytes(const Call& c) {
     const Cut cut = cut_of<T, DP>(c);
-    return cut.splits > 1 ? size_t(cut.tiles * c.kv_heads * cut.splits) * chroma::chunk_partial_floats<DP>() * sizeof(float) : 0;
+    const size_t floats = cut.wide ? chroma::chunk_partial_floats<DP, chroma::kChunkRows>() : chroma::chunk_partial_floats<DP, 16u>();
+    return cut.splits > 1 ? size_t(cut.tiles * c.kv_heads * cut.splits) * floats * sizeof(float) : 0;
 }
 
 template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_t stream) {
     const Cut cut = cut_of<T, DP>(c);
     const chroma::ChunkOperands<T> a = operands<T>(c);
-    constexpr uint32_t keys = chroma::paged_whole_keys<T, DP>(), waves = chroma::paged_whole_waves<T, DP>();
     const uint32_t groups = uint32_t(cut.tiles * c.kv_heads), splits = uint32_t(cut.splits);
+    if constexpr (sizeof(T) == 2) {
+        if (cut.wide) {
+            constexpr int MIN = DP > 128 ? 1 : 2;
+            if (c.dim == DP) {
+                paged_chunk_wide<DP, chroma::chunk_wide_keys<DP>(), true, MIN><<<dim3(groups, splits), 256, 0, stream>>>(a, splits, scratch);
+            } else {
+                paged_chunk_wide<DP, chroma::chunk_wide_keys<DP>(), false, MIN><<<dim3(groups, splits), 256, 0, stream>>>(a, splits, scratch);
+            }
+            if (splits > 1) {
+                paged_chunk_combine<T, DP, chroma::kChunkRows, true><<<groups, 256, 0, stream>>>(a, splits, scratch);
+            }
+            return;
+        }
+    }
+    constexpr uint32_t keys = chroma::paged_whole_keys<T, DP>(), waves = chroma::paged_whole_waves<T, DP>();
     paged_chunk_tiles<T, DP, keys, waves><<<dim3(groups, splits), 64 * waves, 0, stream>>>(a, splits, scratch);
     if (splits > 1) {
-        paged_chunk_combine<T, DP><<<groups, 256, 0, stream>>>(a, splits, scratch);
+        paged_chunk_combine<T, DP, 16u, false><<<groups, 256, 0, stream>>>(a, splits, scratch);
     }
 }
 

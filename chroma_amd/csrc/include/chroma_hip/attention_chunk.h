@@ -42,10 +42,6 @@ struct ChunkTile {
     int32_t first_position, last_position;  // of the tile's tokens
     uint32_t head, low, end;
 
-    // Whether position p sees row j.
-    template <class T> __device__ __forceinline__ bool sees(const ChunkOperands<T>& a, int32_t p, uint32_t j) const {
-        return int32_t(j) <= p && (!a.window || int64_t(j) + a.window > int64_t(p) || j < a.first);
-    }
     template <uint32_t KEYS> __device__ __forceinline__ uint32_t head_blocks() const { return (head + KEYS - 1u) / KEYS; }
     template <uint32_t KEYS> __device__ __forceinline__ uint32_t blocks() const { return head_blocks<KEYS>() + (end - low + KEYS - 1u) / KEYS; }
     template <uint32_t KEYS> __device__ __forceinline__ uint32_t block_begin(uint32_t x) const {
@@ -93,6 +89,18 @@ template <uint32_t ROWS, class T> __device__ __forceinline__ bool chunk_tile(con
     return false;
 }
 
+// The rows that a token sees: ``span`` + 1 from ``low`` on, and those below ``head``.
+struct ChunkSight {
+    uint32_t low, span, head;
+    template <class T> __device__ __forceinline__ ChunkSight(const ChunkOperands<T>& a, int32_t position) {
+        const int64_t begin = int64_t(position) - int64_t(a.window) + 1;
+        low = position < 0 ? ~0u : a.window && begin > 0 ? uint32_t(begin) : 0u;
+        span = position < 0 ? 0u : uint32_t(position) - low;
+        head = position < 0 ? 0u : a.first <= uint32_t(position) ? a.first : uint32_t(position) + 1u;
+    }
+    __device__ __forceinline__ bool operator()(uint32_t j) const { return j - low <= span || j < head; }
+};
+
 template <class T> __device__ __forceinline__ bool chunk_not_finite(T v) {
     if constexpr (sizeof(T) == 2) {
         return (v & 0x7f80u) == 0x7f80u;
@@ -132,7 +140,7 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
         const uint32_t lane = threadIdx.x % 64u, quad = lane / 16u, col = lane % 16u, chunks = a.dim / CHUNK, stop = tile.template blocks<KEYS>();
         const float neg_inf = -__builtin_inff();
         const uint32_t row = tile.row + col < tile.rows ? tile.row + col : tile.rows - 1u, token = row / a.group;
-        const int32_t position = tile.base + int32_t(token);
+        const ChunkSight sight(a, tile.base + int32_t(token));
         const T* k_pages = a.k + kv * a.head_stride;
         const T* v_pages = a.v + kv * a.head_stride;
         const T* q = a.q + (tile.begin + token) * a.q_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim;
@@ -209,7 +217,7 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                 }
                 if (__ballot(odd) != 0ull) {
                     for (uint32_t r = 0; r < KEYS; ++r) {
-                        const bool sees = ((seen >> r) & 1ull) && tile.sees(a, position, begin + r);
+                        const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
 #pragma unroll
                         for (int dt = 0; dt < DP / 16; ++dt) {
 #pragma unroll
@@ -245,7 +253,7 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                 const uint32_t bits = uint32_t(seen >> (t * 16u + quad * 4u)) & 15u;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const bool sees = ((bits >> r) & 1u) && (whole || tile.sees(a, position, begin + t * 16u + quad * 4u + r));
+                    const bool sees = ((bits >> r) & 1u) && (whole || sight(begin + t * 16u + quad * 4u + r));
                     u[t][r] = sees ? s[r] * a.scale : neg_inf;
                     top = __builtin_fmaxf(top, u[t][r]);
                 }
@@ -335,8 +343,8 @@ __device__ __forceinline__ void chunk_store(const ChunkOperands<T>& a, const Chu
                     sum * (total == 0.0f ? 0.0f : 1.0f / total));
 }
 
-// Floats of one (tile, KV head, split): 16 rows of DP sums, then each row's maximum and sum.
-template <int DP> constexpr uint32_t chunk_partial_floats() { return 16u * (DP + 2u); }
+// Floats of one (tile, KV head, split): ROWS rows of DP sums, then each row's maximum and sum.
+template <int DP, uint32_t ROWS> constexpr uint32_t chunk_partial_floats() { return ROWS * (DP + 2u); }
 
 // A workgroup of WAVES waves takes every ``splits``-th of a tile's blocks; its waves take blocks in turn and meet in LDS.
 // grid: (tiles x KV heads, splits)
@@ -390,7 +398,7 @@ __device__ __forceinline__ void attention_chunk_tiles(const ChunkOperands<T>& a,
         if (splits == 1u) {
             chunk_store(a, tile, kv, r, d, sum, merge.total + (sinks ? merge.weight(sink) : 0.0f));
         } else {
-            float* to = partial + (uint64_t(blockIdx.x) * splits + split) * chunk_partial_floats<DP>();
+            float* to = partial + (uint64_t(blockIdx.x) * splits + split) * chunk_partial_floats<DP, 16u>();
             *reinterpret_cast<f32x4_t*>(to + r * DP + d) = sum;
             if (d == 0) {
                 to[16u * DP + 2u * r] = merge.top;
@@ -400,33 +408,357 @@ __device__ __forceinline__ void attention_chunk_tiles(const ChunkOperands<T>& a,
     }
 }
 
-// The splits of a tile, in order, and the sink. grid: tiles x KV heads, 256 threads
-template <class T, int DP>
+// FlashMerge with the maxima in units of log2 or not.
+constexpr float kLog2e = 1.44269504088896341f;
+template <bool LOG2> struct ChunkMerge {
+    float top, total;
+    __device__ __forceinline__ float weight(float peak) const {
+        return peak == -__builtin_inff() ? 0.0f : LOG2 ? __builtin_amdgcn_exp2f(peak - top) : fast_exp(peak - top);
+    }
+};
+
+// The splits of a tile of ROWS rows, in order, and the sink; LOG2: the maxima are of scores in units of log2.
+// grid: tiles x KV heads, 256 threads
+template <class T, int DP, uint32_t ROWS, bool LOG2>
 __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& a, uint32_t splits, const float* __restrict__ partial) {
+    constexpr uint32_t PART = chunk_partial_floats<DP, ROWS>();
     const uint32_t kv = blockIdx.x % a.kv_heads;
     ChunkTile tile;
-    if (!chunk_tile<16u>(a, blockIdx.x / a.kv_heads, tile)) {
+    if (!chunk_tile<ROWS>(a, blockIdx.x / a.kv_heads, tile)) {
         return;
     }
-    const float* parts = partial + uint64_t(blockIdx.x) * splits * chunk_partial_floats<DP>();
-    for (uint32_t i = threadIdx.x; i < 16u * (DP / 4u); i += 256u) {
+    const float* parts = partial + uint64_t(blockIdx.x) * splits * PART;
+    for (uint32_t i = threadIdx.x; i < ROWS * (DP / 4u); i += 256u) {
         const uint32_t r = i / (DP / 4u), d = i % (DP / 4u) * 4u;
         if (tile.row + r >= tile.rows || d >= a.dim) {
             continue;
         }
-        const float sink = a.sinks ? paged_widen<T>(a.sinks[kv * a.group + (tile.row + r) % a.group]) : -__builtin_inff();
-        FlashMerge merge{sink, 0.0f};
+        const float sink = a.sinks ? paged_widen<T>(a.sinks[kv * a.group + (tile.row + r) % a.group]) * (LOG2 ? kLog2e : 1.0f) : -__builtin_inff();
+        ChunkMerge<LOG2> merge{sink, 0.0f};
         for (uint32_t s = 0; s < splits; ++s) {
-            merge.top = __builtin_fmaxf(merge.top, parts[s * chunk_partial_floats<DP>() + 16u * DP + 2u * r]);
+            merge.top = __builtin_fmaxf(merge.top, parts[uint64_t(s) * PART + ROWS * DP + 2u * r]);
         }
         f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
         for (uint32_t s = 0; s < splits; ++s) {
-            const float* part = parts + s * chunk_partial_floats<DP>();
-            const float weight = merge.weight(part[16u * DP + 2u * r]);
-            merge.total += weight * part[16u * DP + 2u * r + 1u];
+            const float* part = parts + uint64_t(s) * PART;
+            const float weight = merge.weight(part[ROWS * DP + 2u * r]);
+            merge.total += weight * part[ROWS * DP + 2u * r + 1u];
             sum += weight * *reinterpret_cast<const f32x4_t*>(part + r * DP + d);
         }
         chunk_store(a, tile, kv, r, d, sum, merge.total + (a.sinks ? merge.weight(sink) : 0.0f));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Long chunks of bfloat16: a tile is 128 rows, 32 to a wave, and a workgroup's four waves share blocks of K and V in LDS (two
+// buffers of each, one barrier a block). Scores are K Q^T, so that a lane holds 16 of 32 keys of one row, and its
+// weights are the second product's operand as they are: key slot (h, i) of 16 stands for key 8 (i / 4) + 4 h + i % 4 on both
+// sides (V's comes from transposing reads).
+//
+// Scores are kept in units of log2: t = s * (scale log2 e), p = 2^(t - m). A lane's maximum is raised only past a headroom, so
+// that most blocks change no sums.
+
+constexpr uint32_t kChunkRows = 128, kChunkWaves = 4;
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+static __device__ const uint4 chunk_zeros[32] = {};  // a row of V for keys that nothing sees
+
+template <int DP> constexpr uint32_t chunk_wide_keys() { return DP > 128 ? 32u : 64u; }
+
+// FULL: the head dimension is DP.
+// grid: (tiles x KV heads, splits), 256 threads
+template <int DP, uint32_t KEYS, bool FULL>
+__device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_t>& a, uint32_t splits, float* __restrict__ partial) {
+    constexpr uint32_t PER_ROW = DP / 8u, BLOCK = KEYS * DP;          // 16-byte chunks of a row; elements of K or V of a block
+    constexpr int COPIES = BLOCK / 512 / kChunkWaves;                 // 1 KiB pieces of K, and of V, that a wave copies
+    constexpr int STEPS = DP / 16, TILES = KEYS / 32, DEEP = DP / 32;
+    constexpr unsigned long long EVERY = KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull;
+    static_assert(COPIES >= 1 && BLOCK % (512 * kChunkWaves) == 0, "whole pieces for every wave");
+    // Chunk c of K's row r lies at c ^ swizzle: 16 rows of one chunk, that one read's pass takes, fill the banks once; so do four
+    // rows of V's 64 bytes.
+    const auto k_swizzle = [](uint32_t r) { return PER_ROW >= 16u ? r & 15u : PER_ROW == 8u ? (r / 2u) & 7u : (r / 4u) & 3u; };
+    const auto v_swizzle = [](uint32_t r) { return PER_ROW >= 16u ? (r & 3u) * 4u : PER_ROW == 8u ? ((r / 2u) & 1u) * 4u : 0u; };
+    __shared__ __attribute__((aligned(1024))) uint16_t lds[4u * BLOCK];
+    const uint32_t lane = threadIdx.x % 64u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), half = lane / 32u, col = lane % 32u;
+    const uint32_t kv = blockIdx.x % a.kv_heads, split = blockIdx.y, chunks = FULL ? PER_ROW : a.dim / 8u;
+    const float neg_inf = -__builtin_inff();
+    ChunkTile tile;
+    if (!chunk_tile<kChunkRows>(a, blockIdx.x / a.kv_heads, tile)) {
+        return;
+    }
+    // this wave's rows (none: it only copies) and this lane's
+    const uint32_t row0 = tile.row + wave * 32u, last_row = (row0 + 32u < tile.rows ? row0 + 32u : tile.rows) - 1u;
+    const bool idle = row0 >= tile.rows;
+    const uint32_t row = row0 + col < tile.rows ? row0 + col : tile.rows - 1u, token = row / a.group;
+    const ChunkSight sight(a, tile.base + int32_t(token));
+    const int32_t first_position = tile.base + int32_t((idle ? last_row : row0) / a.group), last_position = tile.base + int32_t(last_row / a.group);
+    const uint64_t k_pages = uint64_t(a.k + kv * a.head_stride), v_pages = uint64_t(a.v + kv * a.head_stride);  // addresses
+    const uint64_t k_new = uint64_t(a.k_new + uint64_t(kv) * a.dim), v_new = uint64_t(a.v_new + uint64_t(kv) * a.dim);
+    const int64_t* table = a.table + tile.b * a.table_stride;
+    const uint32_t stop = tile.template blocks<KEYS>(), page_rows = a.page_rows, inverse = 0xffffffffu / page_rows;
+    // j / page_rows: the rounded reciprocal is right or one too small
+    const auto page_index = [&](uint32_t j) {
+        const uint32_t q = __umulhi(j, inverse);
+        return q + (j - q * page_rows >= page_rows ? 1u : 0u);
+    };
+    auto page_of = [&](uint32_t x) -> int64_t {  // of this lane's row of block x (-1: none)
+        const uint32_t j = tile.template block_begin<KEYS>(x) + lane;
+        return j < tile.template block_end<KEYS>(x) && j < tile.length ? table[page_index(j)] : -1;
+    };
+    if constexpr (!FULL) {  // zeros behind the rows' ends
+        for (uint32_t c = threadIdx.x; c < 4u * BLOCK / 8u; c += 64u * kChunkWaves) {
+            *reinterpret_cast<uint4*>(lds + c * 8u) = uint4{0u, 0u, 0u, 0u};
+        }
+        __syncthreads();
+    }
+    // Copies block x into buffer ``to``; returns which of its rows there are.
+    auto copy = [&](uint32_t x, uint32_t to, int64_t page) -> unsigned long long {
+        const uint32_t j = tile.template block_begin<KEYS>(x) + lane;
+        const bool held = page >= 0 && uint64_t(page) < a.pages;
+        const bool is_new = j >= tile.length && j < tile.template block_end<KEYS>(x);
+        const uint64_t place = 2u * (held ? uint64_t(page) * a.page_stride + uint64_t(j - page_index(j) * page_rows) * a.row_stride
+                                     : is_new ? uint64_t(tile.begin + (j - tile.length)) * a.new_stride : 0u);
+        const unsigned long long here = __ballot(held || is_new), fresh = __ballot(is_new);
+        uint16_t* ks = lds + to * 2u * BLOCK;
+        uint16_t* vs = ks + BLOCK;
+        const auto pieces = [&](auto addresses) {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+                const uint32_t piece = wave * COPIES + i, r = piece * (64u / PER_ROW) + lane / PER_ROW;
+                const uint32_t k_chunk = (lane % PER_ROW) ^ k_swizzle(r), v_chunk = (lane % PER_ROW) ^ v_swizzle(r);
+                uint64_t k, v;
+                addresses(r, __shfl(place, r, kWave), k, v);
+                if (k_chunk < chunks) {
+                    __builtin_amdgcn_global_load_lds((global_void*)(k + k_chunk * 16u), (lds_void*)(ks + piece * 512u), 16, 0, 0);
+                }
+                if (v_chunk < chunks) {
+                    __builtin_amdgcn_global_load_lds((global_void*)(v + v_chunk * 16u), (lds_void*)(vs + piece * 512u), 16, 0, 0);
+                }
+            }
+        };
+        if (here == EVERY && fresh == 0ull) {
+            pieces([&](uint32_t, uint64_t from, uint64_t& k, uint64_t& v) { k = k_pages + from, v = v_pages + from; });
+        } else {
+            pieces([&](uint32_t r, uint64_t from, uint64_t& k, uint64_t& v) {
+                const bool beside = (fresh >> r) & 1ull, there = (here >> r) & 1ull;
+                k = (beside ? k_new : k_pages) + from;
+                v = there ? (beside ? v_new : v_pages) + from : uint64_t(chunk_zeros);
+            });
+        }
+        return here;
+    };
+
+    // Scores are taken with |scale|, a negative one's sign in Q, and one of 0 as a Q of zeros.
+    const float factor = a.scale == 0.0f ? 1.0f : __builtin_fabsf(a.scale) * kLog2e;
+    const uint32_t keep = a.scale == 0.0f ? 0u : ~0u, flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    uint4 qf[STEPS];
+#pragma unroll
+    for (int c = 0; c < STEPS; ++c) {
+        qf[c] = uint4{0u, 0u, 0u, 0u};
+        if (c * 2u + half < chunks) {
+            qf[c] = *reinterpret_cast<const uint4*>(a.q + (tile.begin + token) * a.q_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim + (c * 2u + half) * 8u);
+            qf[c] = uint4{(qf[c].x ^ flip) & keep, (qf[c].y ^ flip) & keep, (qf[c].z ^ flip) & keep, (qf[c].w ^ flip) & keep};
+        }
+    }
+    float peak, total;
+    f32x16_t o[DEEP];
+    // The pass over the blocks, and a second one where a result is not finite (``careful``), in which the values that are not
+    // finite leave V's block and join the rows that see them by themselves (ChunkWave).
+    for (bool careful = false;; careful = true) {
+        peak = neg_inf;
+        total = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DEEP; ++dt) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[dt][e] = 0.0f;
+            }
+        }
+        uint32_t n = split, buffer = 0;
+        unsigned long long seen = 0;
+        int64_t ahead = -1;
+        if (n < stop) {
+            seen = copy(n, 0u, page_of(n));
+            ahead = n + splits < stop ? page_of(n + splits) : -1;
+        }
+        for (; n < stop; n += splits, buffer ^= 1u) {
+            const uint32_t begin = tile.template block_begin<KEYS>(n), next = n + splits;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+            __builtin_amdgcn_s_barrier();  // block n has landed, and every wave is done with the other buffer
+            __builtin_amdgcn_sched_barrier(0);
+            const unsigned long long here = seen;
+            if (next < stop) {
+                seen = copy(next, buffer ^ 1u, ahead);
+                ahead = next + splits < stop ? page_of(next + splits) : -1;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const uint16_t* ks = lds + buffer * 2u * BLOCK;
+            uint16_t* vs = lds + buffer * 2u * BLOCK + BLOCK;
+            if (careful) {
+                for (uint32_t r = 0; r < KEYS; ++r) {
+                    const bool sees = ((here >> r) & 1ull) && sight(begin + r);
+#pragma unroll
+                    for (int dt = 0; dt < DEEP; ++dt) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t d = dt * 32u + 8u * (e / 4) + 4u * half + e % 4;
+                            const uint16_t v = vs[r * DP + ((d / 8u) ^ v_swizzle(r)) * 8u + d % 8u];
+                            o[dt][e] += sees && chunk_not_finite<uint16_t>(v) ? bf16_to_f32(v) : 0.0f;
+                        }
+                    }
+                }
+                __syncthreads();  // every wave has read them
+                for (uint32_t c = threadIdx.x; c < BLOCK; c += 64u * kChunkWaves) {
+                    if (chunk_not_finite<uint16_t>(vs[c])) {
+                        vs[c] = 0;
+                    }
+                }
+                __syncthreads();
+            }
+            // what none of this wave's rows sees is skipped
+            if (idle || int32_t(begin) > last_position ||
+                (a.window && int64_t(begin) + KEYS - 1 + a.window <= int64_t(first_position) && begin >= a.first)) {
+                continue;
+            }
+            f32x16_t s[TILES];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[t][e] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const uint32_t r = t * 32u + col;
+                    const uint4 kf = *reinterpret_cast<const uint4*>(ks + r * DP + ((c * 2u + half) ^ k_swizzle(r)) * 8u);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[c]), s[t], 0, 0, 0);
+                }
+            }
+            // rows that some of the wave's tokens do not see (the chunk's own, the window's first), and rows that are not there
+            if (int32_t(begin + KEYS - 1u) > first_position ||
+                (a.window && int64_t(begin) + a.window <= int64_t(last_position) && begin + KEYS > a.first)) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[t][e] = sight(begin + t * 32u + 8u * (e / 4) + 4u * half + e % 4) ? s[t][e] : neg_inf;
+                    }
+                }
+            }
+            if (here != EVERY) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const uint32_t bits = uint32_t(here >> (32 * t)) >> (4u * half);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[t][e] = (bits >> (8 * (e / 4) + e % 4)) & 1u ? s[t][e] : neg_inf;
+                    }
+                }
+            }
+            float top = neg_inf;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    top = __builtin_fmaxf(top, s[t][e]);
+                }
+            }
+            top *= factor;
+            if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
+                const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = __builtin_fmaxf(__builtin_fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1])), peak);
+                const float shrink = peak == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(peak - top);
+                total *= shrink;
+#pragma unroll
+                for (int dt = 0; dt < DEEP; ++dt) {
+                    o[dt] *= shrink;
+                }
+                peak = top;
+            }
+            const float base = peak == neg_inf ? 0.0f : -peak;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], factor, base));
+                    total += s[t][e];
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2 * TILES; ++g) {
+                bf16x8_t weights;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const bf16x2_t pair = __builtin_convertvector(f32x2_t{s[g / 2][g % 2 * 8 + e], s[g / 2][g % 2 * 8 + e + 1]}, bf16x2_t);
+                    weights[e] = pair[0];
+                    weights[e + 1] = pair[1];
+                }
+#pragma unroll
+                for (int dt = 0; dt < DEEP; ++dt) {
+                    s16x4_t four[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t r = g * 16u + x * 8u + half * 4u + (lane % 16u) / 4u;
+                        const uint32_t chunk = (dt * 4u + (lane / 16u) % 2u * 2u + (lane % 4u) / 2u) ^ v_swizzle(r);
+                        four[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + r * DP + chunk * 8u + (lane % 2u) * 4u));
+                    }
+                    const uint2 lo = __builtin_bit_cast(uint2, four[0]), hi = __builtin_bit_cast(uint2, four[1]);
+                    const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, uint4{lo.x, lo.y, hi.x, hi.y});
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, weights, o[dt], 0, 0, 0);
+                }
+            }
+        }
+        bool odd = false;
+#pragma unroll
+        for (int dt = 0; dt < DEEP; ++dt) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                odd |= !(__builtin_fabsf(o[dt][e]) < __builtin_inff());
+            }
+        }
+        if (careful || !__syncthreads_or(odd)) {
+            break;
+        }
+    }
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(total), __float_as_uint(total), false, false);
+    total = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+    if (row0 + col >= tile.rows) {
+        return;
+    }
+    if (splits == 1u) {
+        const float sink = a.sinks ? bf16_to_f32(a.sinks[kv * a.group + row % a.group]) * kLog2e : neg_inf;
+        const ChunkMerge<true> merge{__builtin_fmaxf(peak, sink), 0.0f};
+        const float weight = merge.weight(peak), sum = weight * total + (a.sinks ? merge.weight(sink) : 0.0f), scaled = sum == 0.0f ? 0.0f : weight / sum;
+        uint16_t* to = a.out + (tile.begin + token) * a.out_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim;
+#pragma unroll
+        for (int dt = 0; dt < DEEP; ++dt) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t d = dt * 32u + 2u * e + 4u * half;
+                if (FULL || d < a.dim) {
+                    paged_store4<uint16_t>(to + d, f32x4_t{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * scaled);
+                }
+            }
+        }
+    } else {
+        const uint32_t r = wave * 32u + col;
+        float* to = partial + (uint64_t(blockIdx.x) * splits + split) * chunk_partial_floats<DP, kChunkRows>();
+#pragma unroll
+        for (int dt = 0; dt < DEEP; ++dt) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                *reinterpret_cast<f32x4_t*>(to + r * DP + dt * 32u + 2u * e + 4u * half) = f32x4_t{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
+            }
+        }
+        if (half == 0u) {
+            to[kChunkRows * DP + 2u * r] = peak;
+            to[kChunkRows * DP + 2u * r + 1u] = total;
+        }
     }
 }
 

@@ -412,6 +412,51 @@ def test_chunk(shape, fresh, dtype):
     check_chunk(chunk_inputs(counts, lengths, kv=kv, group=group, dim=dim, page=page, dtype=dtype, fresh=fresh, sinks=fresh, seed=dim + page))
 
 
+LONG_CHUNKS = [  # as many rows as the matrix-core tiles of 128 rows take
+    ([130, 0, 1], [200, 5, 300], 8, 8, 64, 16),
+    ([300, 35], [64, 100], 8, 4, 128, 64),
+    ([70], [257], 16, 8, 32, 12),
+    ([260], [40], 4, 8, 256, 7),
+    ([300, 5], [90, 3], 4, 7, 80, 32),
+    ([1100], [0], 1, 8, 64, 16),
+    ([700], [130], 4, 3, 200, 9),
+    ([40, 30], [129, 64], 3, 40, 64, 16),
+    ([33, 47, 60], [1, 64, 63], 60, 1, 104, 1),
+]
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
+@pytest.mark.parametrize("shape", LONG_CHUNKS, ids=lambda s: f"{sum(s[0])}after{max(s[1])}-{s[2]}x{s[3]}x{s[4]}-{s[5]}")
+def test_long_chunk(shape, fresh, dtype):
+    counts, lengths, kv, group, dim, page = shape
+    if not fresh:
+        lengths = [n + c for n, c in zip(lengths, counts)]
+    inputs = chunk_inputs(counts, lengths, kv=kv, group=group, dim=dim, page=page, dtype=dtype, fresh=fresh, sinks=fresh, seed=dim + page)
+    check_chunk(inputs)
+    check_chunk(inputs, window=100, first=3)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+@pytest.mark.parametrize("tokens", [9, 140])
+def test_chunk_scales(tokens, scale, dtype):
+    check_chunk(chunk_inputs([tokens], [50], kv=8, group=8, dim=64, page=16, dtype=dtype, seed=2), scale=scale)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("window", [0, 500])
+def test_long_chunk_over_a_long_cache(window, dtype):
+    """Few tiles of 128 rows over many keys: a tile's keys are split over workgroups."""
+    inputs = chunk_inputs([150], [2500], kv=4, group=16, dim=64, page=16, dtype=dtype, seed=3)
+    call = chunk_call(**inputs, out=torch.empty_like(inputs["q"]))
+    assert dtype == torch.float32 or native.library().chroma_hip_paged_chunk_attention_workspace(ctypes.byref(call)) > 0
+    check_chunk(inputs, window=window, first=2)
+
+
 @gpu
 @BOTH
 @pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
@@ -447,10 +492,11 @@ def test_chunk_of_many_sequences(dtype):
 @gpu
 @BOTH
 @pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
-def test_chunk_rows_on_bad_pages_are_not_seen(fresh, dtype):
+@pytest.mark.parametrize("kv", [2, 80])
+def test_chunk_rows_on_bad_pages_are_not_seen(kv, fresh, dtype):
     """Table entries outside the pages, lengths outside [0, longest], tokens before the first position, sequences that see
     nothing."""
-    inputs = chunk_inputs([20, 6, 5, 3, 4], [100, 40, 64, 0, 90], kv=2, group=3, dim=64, page=16, dtype=dtype, fresh=fresh, sinks=False, seed=4)
+    inputs = chunk_inputs([20, 6, 5, 3, 4], [100, 40, 64, 0, 90], kv=kv, group=9, dim=64, page=16, dtype=dtype, fresh=fresh, sinks=False, seed=4)
     pages = len(inputs["k_pages"])
     inputs["table"][0, 2], inputs["table"][0, 4] = -1, pages
     inputs["table"][1, :] = 2**40
@@ -478,9 +524,10 @@ def test_chunk_of_starts_out_of_order(dtype):
 @gpu
 @BOTH
 @pytest.mark.parametrize("where", ["new", "window", "first"])
-def test_chunk_values_that_are_not_finite_reach_only_who_sees_them(where, dtype):
+@pytest.mark.parametrize("kv", [2, 17])
+def test_chunk_values_that_are_not_finite_reach_only_who_sees_them(kv, where, dtype):
     """A value of infinity or NaN in a row that some tokens of a tile see and others do not."""
-    inputs = chunk_inputs([70], [200], kv=2, group=8, dim=64, page=16, dtype=dtype, seed=11)
+    inputs = chunk_inputs([70], [200], kv=kv, group=8, dim=64, page=16, dtype=dtype, seed=11)
     options = {} if where == "new" else {"window": 60, "first": 0 if where == "window" else 9}
     if where == "new":
         inputs["v_new"][20, 0, 3], inputs["v_new"][41, 1, 7], inputs["v_new"][41, 0, 60] = math.inf, math.nan, -math.inf
@@ -493,14 +540,15 @@ def test_chunk_values_that_are_not_finite_reach_only_who_sees_them(where, dtype)
 
 @gpu
 @BOTH
-def test_chunk_of_large_and_equal_scores(dtype):
+@pytest.mark.parametrize("tokens", [30, 600])
+def test_chunk_of_large_and_equal_scores(tokens, dtype):
     """Scores of some hundreds (sums need the running maximum), equal ones, sinks of -inf and of the lowest value."""
-    inputs = chunk_inputs([30, 5], [300, 65], kv=1, group=4, dim=64, page=16, dtype=dtype, seed=9, spread=6.0)
-    inputs["sinks"] = torch.tensor([-math.inf, torch.finfo(dtype).min, 0.0, 300.0], dtype=dtype)
+    inputs = chunk_inputs([tokens, 5], [300, 65], kv=4, group=4, dim=64, page=16, dtype=dtype, seed=9, spread=6.0)
+    inputs["sinks"] = torch.tensor([-math.inf, torch.finfo(dtype).min, 0.0, 300.0] * 4, dtype=dtype)
     check_chunk(inputs)
     inputs["k_pages"].nan_to_num_(0.0)
     inputs["k_pages"].fill_(0.25)
-    inputs["k_new"][:35] = 0.25
+    inputs["k_new"][:-2] = 0.25
     check_chunk(inputs, scale=1.0)
 
 
