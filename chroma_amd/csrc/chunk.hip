@@ -21,9 +21,11 @@ __global__ void __launch_bounds__(64 * WAVES) paged_chunk_tiles(chroma::ChunkOpe
     chroma::attention_chunk_tiles<T, DP, KEYS, WAVES>(a, splits, scratch);
 }
 
-template <int DP, uint32_t KEYS, bool FULL, int MIN>
-__global__ void __launch_bounds__(256, MIN) paged_chunk_wide(chroma::ChunkOperands<uint16_t> a, uint32_t splits, float* scratch) {
-    chroma::attention_chunk_wide<DP, KEYS, FULL>(a, splits, scratch);
+// (two waves a SIMD, or three with heads up to 64)
+template <int DP, uint32_t KEYS, uint32_t WAVES, bool FULL>
+__global__ void __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : DP == 256 ? 1 : 2) paged_chunk_wide(chroma::ChunkOperands<uint16_t> a, uint32_t splits,
+                                                                                                 float* scratch) {
+    chroma::attention_chunk_wide<DP, KEYS, WAVES, FULL>(a, splits, scratch);
 }
 
 template <class T, int DP, uint32_t ROWS, bool LOG2>
@@ -122,10 +124,12 @@ template <class T> chroma::ChunkOperands<T> operands(const Call& c) {
 // Whether a call of these types and head dimension runs on the kernels of padded dimension DP.
 template <class T, int DP> bool fits(const Call& c) { return c.dim <= DP && (DP == (sizeof(T) == 2 ? 32 : 16) || c.dim > DP / 2); }
 
-// How a call is cut: tiles of 128 rows or of 16, at most this many of all sequences, and workgroups for each of them.
+// How a call is cut: tiles of 32 rows a wave (``waves`` 4 or 8, bfloat16) or of 16 rows (``waves`` 0), at most this many of all
+// sequences, and workgroups for each of them.
 struct Cut {
-    bool wide;
+    int waves;
     int64_t tiles, splits;
+    int64_t rows() const { return waves ? 32 * waves : 16; }
 };
 template <class T, int DP> Cut cut_of(const Call& c) {
     Cut cut;
@@ -135,43 +139,51 @@ template <class T, int DP> Cut cut_of(const Call& c) {
         const int64_t blocks = (rows + keys - 1) / keys + 1;
         return c.window ? std::min(blocks, (std::min(c.first, rows) + std::min(c.window, rows)) / keys + 3) : blocks;
     };
-    cut.wide = sizeof(T) == 2 && c.tokens * c.group >= 64 * c.sequences && c.tokens * c.group * c.kv_heads >= 128 * 64;
-    const int64_t keys = cut.wide ? chroma::chunk_wide_keys<DP>() : chroma::paged_whole_keys<T, DP>();
-    const int64_t waves = cut.wide ? 1 : chroma::paged_whole_waves<T, DP>();
-    cut.tiles = tiles_of(cut.wide ? chroma::kChunkRows : 16);
-    const int64_t wanted = (512 + cut.tiles * c.kv_heads - 1) / (cut.tiles * c.kv_heads);
-    cut.splits = std::max<int64_t>(1, std::min(wanted, most_blocks(keys) / (2 * waves)));
+    cut.waves = sizeof(T) != 2 || c.tokens * c.group < 64 * c.sequences || c.tokens * c.group * c.kv_heads < 128 * 64 ? 0
+              : DP == 128 && tiles_of(256) * c.kv_heads >= 512 ? 8 : 4;
+    cut.tiles = tiles_of(cut.rows());
+    const int64_t units = cut.tiles * c.kv_heads, wanted = (512 + units - 1) / units;
+    cut.splits = std::max<int64_t>(1, std::min(wanted, cut.waves ? most_blocks(chroma::chunk_wide_keys<DP>()) / 4
+                                                                : most_blocks(chroma::paged_whole_keys<T, DP>()) / (2 * chroma::paged_whole_waves<T, DP>())));
     return cut;
 }
 
 template <class T, int DP> size_t scratch_bytes(const Call& c) {
     const Cut cut = cut_of<T, DP>(c);
-    const size_t floats = cut.wide ? chroma::chunk_partial_floats<DP, chroma::kChunkRows>() : chroma::chunk_partial_floats<DP, 16u>();
-    return cut.splits > 1 ? size_t(cut.tiles * c.kv_heads * cut.splits) * floats * sizeof(float) : 0;
+    return cut.splits > 1 ? size_t(cut.tiles * c.kv_heads * cut.splits) * size_t(cut.rows() * (DP + 2)) * sizeof(float) : 0;
+}
+
+template <int DP, uint32_t WAVES, bool FULL, class A> void launch_wide(const A& a, dim3 grid, float* scratch, hipStream_t stream) {
+    paged_chunk_wide<DP, chroma::chunk_wide_keys<DP>(), WAVES, FULL><<<grid, 64 * WAVES, 0, stream>>>(a, grid.y, scratch);
 }
 
 template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_t stream) {
     const Cut cut = cut_of<T, DP>(c);
     const chroma::ChunkOperands<T> a = operands<T>(c);
-    const uint32_t groups = uint32_t(cut.tiles * c.kv_heads), splits = uint32_t(cut.splits);
+    const dim3 grid(unsigned(cut.tiles * c.kv_heads), unsigned(cut.splits));
+    const auto combine = [&](auto kernel) { kernel<<<dim3(grid.x, unsigned(cut.rows() / 16)), 256, 0, stream>>>(a, grid.y, scratch); };
     if constexpr (sizeof(T) == 2) {
-        if (cut.wide) {
-            constexpr int MIN = DP > 128 ? 1 : 2;
-            if (c.dim == DP) {
-                paged_chunk_wide<DP, chroma::chunk_wide_keys<DP>(), true, MIN><<<dim3(groups, splits), 256, 0, stream>>>(a, splits, scratch);
-            } else {
-                paged_chunk_wide<DP, chroma::chunk_wide_keys<DP>(), false, MIN><<<dim3(groups, splits), 256, 0, stream>>>(a, splits, scratch);
+        if constexpr (DP == 128) {
+            if (cut.waves == 8) {
+                c.dim == DP ? launch_wide<DP, 8, true>(a, grid, scratch, stream) : launch_wide<DP, 8, false>(a, grid, scratch, stream);
+                if (grid.y > 1) {
+                    combine(paged_chunk_combine<T, DP, 256u, true>);
+                }
+                return;
             }
-            if (splits > 1) {
-                paged_chunk_combine<T, DP, chroma::kChunkRows, true><<<groups, 256, 0, stream>>>(a, splits, scratch);
+        }
+        if (cut.waves) {
+            c.dim == DP ? launch_wide<DP, 4, true>(a, grid, scratch, stream) : launch_wide<DP, 4, false>(a, grid, scratch, stream);
+            if (grid.y > 1) {
+                combine(paged_chunk_combine<T, DP, 128u, true>);
             }
             return;
         }
     }
     constexpr uint32_t keys = chroma::paged_whole_keys<T, DP>(), waves = chroma::paged_whole_waves<T, DP>();
-    paged_chunk_tiles<T, DP, keys, waves><<<dim3(groups, splits), 64 * waves, 0, stream>>>(a, splits, scratch);
-    if (splits > 1) {
-        paged_chunk_combine<T, DP, 16u, false><<<groups, 256, 0, stream>>>(a, splits, scratch);
+    paged_chunk_tiles<T, DP, keys, waves><<<grid, 64 * waves, 0, stream>>>(a, grid.y, scratch);
+    if (grid.y > 1) {
+        combine(paged_chunk_combine<T, DP, 16u, false>);
     }
 }
 

@@ -53,26 +53,39 @@ struct ChunkTile {
     }
 };
 
-// Tile ``index`` of the call in the sequences' order, the same in all lanes of a wave; false past the last.
-template <uint32_t ROWS, class T> __device__ __forceinline__ bool chunk_tile(const ChunkOperands<T>& a, uint32_t index, ChunkTile& tile) {
+// Tile ``index`` of the call, the same in all lanes of a wave; false past the last. The sequences come in their order;
+// LONGEST: up to 64 of them by the rows that they hold, and a sequence's last tile first, so that what takes longest starts
+// first (workgroups start in the order of their indices).
+template <uint32_t ROWS, bool LONGEST, class T> __device__ __forceinline__ bool chunk_tile(const ChunkOperands<T>& a, uint32_t index, ChunkTile& tile) {
     const uint32_t lane = threadIdx.x % kWave;
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWave) {
         ChunkRows rows{0u, 0u};
-        uint32_t own = 0;
+        uint32_t own = 0, order = lane;
         if (b0 + lane < a.sequences) {
             rows = chunk_rows(a, b0 + lane);
             own = ((rows.end - rows.begin) * a.group + ROWS - 1u) / ROWS;
         }
+        if (LONGEST && a.sequences <= uint32_t(kWave)) {
+            const uint32_t held = lane < a.sequences ? paged_length(a, lane) : 0u;
+            uint32_t rank = 0;
+            for (uint32_t i = 0; i < a.sequences; ++i) {
+                const uint32_t other = __builtin_amdgcn_readlane(held, i);
+                rank += other > held || (other == held && i < lane) ? 1u : 0u;
+            }
+            rank = lane < a.sequences ? rank : lane;
+            order = __builtin_amdgcn_ds_permute(int(rank * 4u), int(lane));  // the sequence of this lane's rank
+            own = __shfl(own, order, kWave);
+        }
         const uint32_t upto = before + paged_scan(own);
         const unsigned long long past = __ballot(upto > index);
         if (past) {
-            const uint32_t at = __builtin_ctzll(past);
-            tile.b = b0 + at;
-            tile.begin = __builtin_amdgcn_readlane(rows.begin, at);
-            const uint32_t count = __builtin_amdgcn_readlane(rows.end, at) - tile.begin;
+            const uint32_t at = __builtin_ctzll(past), sequence = __builtin_amdgcn_readlane(order, at);
+            tile.b = b0 + sequence;
+            tile.begin = __builtin_amdgcn_readlane(rows.begin, sequence);
+            const uint32_t count = __builtin_amdgcn_readlane(rows.end, sequence) - tile.begin, place = index - __builtin_amdgcn_readlane(upto - own, at);
             tile.rows = count * a.group;
-            tile.row = (index - __builtin_amdgcn_readlane(upto - own, at)) * ROWS;
+            tile.row = (LONGEST ? __builtin_amdgcn_readlane(own, at) - 1u - place : place) * ROWS;
             tile.length = paged_length(a, tile.b);
             tile.base = int32_t(tile.length) - (a.k_new ? 0 : int32_t(count));
             const uint32_t last = (tile.row + ROWS < tile.rows ? tile.row + ROWS : tile.rows) - 1u;
@@ -358,7 +371,7 @@ __device__ __forceinline__ void attention_chunk_tiles(const ChunkOperands<T>& a,
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
     const uint32_t kv = blockIdx.x % a.kv_heads, split = blockIdx.y;
     ChunkTile tile;
-    if (!chunk_tile<16u>(a, blockIdx.x / a.kv_heads, tile)) {
+    if (!chunk_tile<16u, false>(a, blockIdx.x / a.kv_heads, tile)) {
         return;
     }
     T* ks = lds + wave * Wave::ELEMENTS;
@@ -418,18 +431,18 @@ template <bool LOG2> struct ChunkMerge {
 };
 
 // The splits of a tile of ROWS rows, in order, and the sink; LOG2: the maxima are of scores in units of log2.
-// grid: tiles x KV heads, 256 threads
+// grid: (tiles x KV heads, ROWS / 16), 256 threads
 template <class T, int DP, uint32_t ROWS, bool LOG2>
 __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& a, uint32_t splits, const float* __restrict__ partial) {
     constexpr uint32_t PART = chunk_partial_floats<DP, ROWS>();
     const uint32_t kv = blockIdx.x % a.kv_heads;
     ChunkTile tile;
-    if (!chunk_tile<ROWS>(a, blockIdx.x / a.kv_heads, tile)) {
+    if (!chunk_tile<ROWS, LOG2>(a, blockIdx.x / a.kv_heads, tile)) {
         return;
     }
     const float* parts = partial + uint64_t(blockIdx.x) * splits * PART;
-    for (uint32_t i = threadIdx.x; i < ROWS * (DP / 4u); i += 256u) {
-        const uint32_t r = i / (DP / 4u), d = i % (DP / 4u) * 4u;
+    for (uint32_t i = threadIdx.x; i < 16u * (DP / 4u); i += 256u) {
+        const uint32_t r = blockIdx.y * 16u + i / (DP / 4u), d = i % (DP / 4u) * 4u;
         if (tile.row + r >= tile.rows || d >= a.dim) {
             continue;
         }
@@ -439,6 +452,7 @@ __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& 
             merge.top = __builtin_fmaxf(merge.top, parts[uint64_t(s) * PART + ROWS * DP + 2u * r]);
         }
         f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
         for (uint32_t s = 0; s < splits; ++s) {
             const float* part = parts + uint64_t(s) * PART;
             const float weight = merge.weight(part[ROWS * DP + 2u * r]);
@@ -450,15 +464,13 @@ __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Long chunks of bfloat16: a tile is 128 rows, 32 to a wave, and a workgroup's four waves share blocks of K and V in LDS (two
+// Long chunks of bfloat16: a tile is 32 rows a wave, and a workgroup's four or eight waves share blocks of K and V in LDS (two
 // buffers of each, one barrier a block). Scores are K Q^T, so that a lane holds 16 of 32 keys of one row, and its
 // weights are the second product's operand as they are: key slot (h, i) of 16 stands for key 8 (i / 4) + 4 h + i % 4 on both
 // sides (V's comes from transposing reads).
 //
 // Scores are kept in units of log2: t = s * (scale log2 e), p = 2^(t - m). A lane's maximum is raised only past a headroom, so
 // that most blocks change no sums.
-
-constexpr uint32_t kChunkRows = 128, kChunkWaves = 4;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -467,14 +479,15 @@ static __device__ const uint4 chunk_zeros[32] = {};  // a row of V for keys that
 template <int DP> constexpr uint32_t chunk_wide_keys() { return DP > 128 ? 32u : 64u; }
 
 // FULL: the head dimension is DP.
-// grid: (tiles x KV heads, splits), 256 threads
-template <int DP, uint32_t KEYS, bool FULL>
+// grid: (tiles x KV heads, splits), WAVES waves
+template <int DP, uint32_t KEYS, uint32_t WAVES, bool FULL>
 __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_t>& a, uint32_t splits, float* __restrict__ partial) {
     constexpr uint32_t PER_ROW = DP / 8u, BLOCK = KEYS * DP;          // 16-byte chunks of a row; elements of K or V of a block
-    constexpr int COPIES = BLOCK / 512 / kChunkWaves;                 // 1 KiB pieces of K, and of V, that a wave copies
+    constexpr uint32_t ROWS = 32u * WAVES;
+    constexpr int COPIES = BLOCK / 512 / WAVES;                 // 1 KiB pieces of K, and of V, that a wave copies
     constexpr int STEPS = DP / 16, TILES = KEYS / 32, DEEP = DP / 32;
     constexpr unsigned long long EVERY = KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull;
-    static_assert(COPIES >= 1 && BLOCK % (512 * kChunkWaves) == 0, "whole pieces for every wave");
+    static_assert(COPIES >= 1 && BLOCK % (512 * WAVES) == 0, "whole pieces for every wave");
     // Chunk c of K's row r lies at c ^ swizzle: 16 rows of one chunk, that one read's pass takes, fill the banks once; so do four
     // rows of V's 64 bytes.
     const auto k_swizzle = [](uint32_t r) { return PER_ROW >= 16u ? r & 15u : PER_ROW == 8u ? (r / 2u) & 7u : (r / 4u) & 3u; };
@@ -484,7 +497,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
     const uint32_t kv = blockIdx.x % a.kv_heads, split = blockIdx.y, chunks = FULL ? PER_ROW : a.dim / 8u;
     const float neg_inf = -__builtin_inff();
     ChunkTile tile;
-    if (!chunk_tile<kChunkRows>(a, blockIdx.x / a.kv_heads, tile)) {
+    if (!chunk_tile<ROWS, true>(a, blockIdx.x / a.kv_heads, tile)) {
         return;
     }
     // this wave's rows (none: it only copies) and this lane's
@@ -507,7 +520,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
         return j < tile.template block_end<KEYS>(x) && j < tile.length ? table[page_index(j)] : -1;
     };
     if constexpr (!FULL) {  // zeros behind the rows' ends
-        for (uint32_t c = threadIdx.x; c < 4u * BLOCK / 8u; c += 64u * kChunkWaves) {
+        for (uint32_t c = threadIdx.x; c < 4u * BLOCK / 8u; c += 64u * WAVES) {
             *reinterpret_cast<uint4*>(lds + c * 8u) = uint4{0u, 0u, 0u, 0u};
         }
         __syncthreads();
@@ -610,7 +623,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                     }
                 }
                 __syncthreads();  // every wave has read them
-                for (uint32_t c = threadIdx.x; c < BLOCK; c += 64u * kChunkWaves) {
+                for (uint32_t c = threadIdx.x; c < BLOCK; c += 64u * WAVES) {
                     if (chunk_not_finite<uint16_t>(vs[c])) {
                         vs[c] = 0;
                     }
@@ -660,14 +673,15 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                     }
                 }
             }
-            float top = neg_inf;
+            float tops[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    top = __builtin_fmaxf(top, s[t][e]);
+                    tops[e % 4] = __builtin_fmaxf(tops[e % 4], s[t][e]);
                 }
             }
+            float top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
             top *= factor;
             if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
                 const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
@@ -681,20 +695,17 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                 peak = top;
             }
             const float base = peak == neg_inf ? 0.0f : -peak;
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], factor, base));
-                    total += s[t][e];
-                }
-            }
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < 2 * TILES; ++g) {
                 bf16x8_t weights;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const bf16x2_t pair = __builtin_convertvector(f32x2_t{s[g / 2][g % 2 * 8 + e], s[g / 2][g % 2 * 8 + e + 1]}, bf16x2_t);
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + e], factor, base));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g / 2][g % 2 * 8 + e + 1], factor, base));
+                    sums[e % 4] += x;
+                    sums[e % 4 + 1] += y;
+                    const bf16x2_t pair = __builtin_convertvector(f32x2_t{x, y}, bf16x2_t);
                     weights[e] = pair[0];
                     weights[e + 1] = pair[1];
                 }
@@ -712,6 +723,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                     o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, weights, o[dt], 0, 0, 0);
                 }
             }
+            total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         }
         bool odd = false;
 #pragma unroll
@@ -721,7 +733,23 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                 odd |= !(__builtin_fabsf(o[dt][e]) < __builtin_inff());
             }
         }
-        if (careful || !__syncthreads_or(odd)) {
+        // (asked in the same LDS array: beside a second one every read above would wait for all copies)
+        uint32_t* flags = reinterpret_cast<uint32_t*>(lds);
+        __syncthreads();
+        if (lane == 0u) {
+            flags[wave] = 0u;
+        }
+        if (odd) {
+            flags[wave] = 1u;
+        }
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) {
+            any |= flags[w];
+        }
+        __syncthreads();
+        if (careful || !any) {
             break;
         }
     }
@@ -747,7 +775,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
         }
     } else {
         const uint32_t r = wave * 32u + col;
-        float* to = partial + (uint64_t(blockIdx.x) * splits + split) * chunk_partial_floats<DP, kChunkRows>();
+        float* to = partial + (uint64_t(blockIdx.x) * splits + split) * chunk_partial_floats<DP, ROWS>();
 #pragma unroll
         for (int dt = 0; dt < DEEP; ++dt) {
 #pragma unroll
@@ -756,8 +784,8 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
             }
         }
         if (half == 0u) {
-            to[kChunkRows * DP + 2u * r] = peak;
-            to[kChunkRows * DP + 2u * r + 1u] = total;
+            to[ROWS * DP + 2u * r] = peak;
+            to[ROWS * DP + 2u * r + 1u] = total;
         }
     }
 }
