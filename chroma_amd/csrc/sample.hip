@@ -1,8 +1,15 @@
 // ``chroma_hip_rows_sample``: a token drawn from each row of logits under temperature, top-k, top-p and min-p.
 //
 // Every filter keeps a prefix of the row's descending order, and the drawn token is a place in it, so that all of them ask the
-// same question: after which token does a running count, or a running sum of weights, reach a goal. It is answered by
-// descending on the order's 32-bit key (larger means earlier), a histogram of counts and weights per step.
+// same question: after which token does a running count, or a running sum of weights, reach a goal. A histogram of weights
+// (of counts where a top-k cuts the row) over the depths below the maximum answers it but for the tokens of a few buckets;
+// those are listed, and the places among them found by descending on their keys. A row is read three times: for its maximum,
+// for the histogram, for the list; the second and third time it lies in the caches.
+//
+// Rows enough to fill the chip have a workgroup each and one launch. Fewer rows are cut into spans, and the three readings are
+// three launches; the workgroup that comes last with a row's histogram, or list, goes on with them. Rows of up to kList tokens
+// are listed whole. Where the listed buckets hold more than kList tokens (rows of equal values, temperatures that leave
+// few depths), a workgroup descends on the keys of the whole row.
 //
 // A weight exp((x - max) / temperature) is evaluated in 64 bits and rounded to units of 2^-44: sums are integers, and the same
 // in whatever order they are taken. In 32 bits the place that a random number names among 200,000 tokens moves by more than
@@ -22,8 +29,15 @@ namespace {
 
 using Call = chroma_hip_sample_call;
 
-constexpr int kOne = 44;  // a weight of 1 is 2^kOne
+constexpr int kOne = 44;                        // a weight of 1 is 2^kOne
+constexpr uint64_t kWhole = uint64_t(1) << kOne;
 constexpr uint32_t kThreads = 1024, kBuckets = 2048;
+constexpr uint32_t kList = 4096;   // listed tokens of a row
+constexpr int64_t kMostTop = 1024;  // a larger top_k descends on the whole row
+constexpr float kDepths = 44.0f;   // buckets of the histogram for a factor of 2; the last one holds what weighs nothing
+
+__device__ __forceinline__ uint64_t lesser(uint64_t a, uint64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ uint64_t greater(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 template <class T> __device__ __forceinline__ float widen(T v);
 template <> __device__ __forceinline__ float widen<float>(float v) { return v; }
@@ -96,19 +110,134 @@ struct Place {
     __device__ __forceinline__ uint64_t weight() const { return before.weight + each * ties; }
 };
 
+// LDS of a workgroup.
+struct Shared {
+    uint64_t weight[kBuckets];
+    uint64_t before[kBuckets + 1];  // sums before each bucket, and of all
+    uint32_t count[kBuckets];
+    uint64_t list[kList];           // selection keys
+    Sums waves[kThreads / 64u];
+    Place found;
+    uint32_t listed, last;
+};
+
+// Sums over the workgroup.
+__device__ Sums sum_all(Shared& s, Sums own) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        own.weight += __shfl_xor(static_cast<unsigned long long>(own.weight), step, 64);
+        own.count += __shfl_xor(own.count, step, 64);
+    }
+    if (threadIdx.x % 64u == 0u) {
+        s.waves[threadIdx.x / 64u] = own;
+    }
+    __syncthreads();
+    Sums sum{0u, 0u};
+#pragma unroll
+    for (uint32_t v = 0; v < kThreads / 64u; ++v) {
+        sum.weight += s.waves[v].weight;
+        sum.count += s.waves[v].count;
+    }
+    __syncthreads();
+    return sum;
+}
+
+// The largest of the workgroup's values.
+__device__ uint64_t max_all(Shared& s, uint64_t own) {
+    own = chroma::wave_max_u64(own);
+    if (threadIdx.x % 64u == 0u) {
+        s.waves[threadIdx.x / 64u].weight = own;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t v = 0; v < kThreads / 64u; ++v) {
+        own = s.waves[v].weight > own ? s.waves[v].weight : own;
+    }
+    __syncthreads();
+    return own;
+}
+
+// Inclusive sums over the workgroup's threads, in their order.
+__device__ Sums scan_all(Shared& s, Sums own) {
+    const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const uint64_t weight = __shfl_up(static_cast<unsigned long long>(own.weight), step, 64);
+        const uint32_t count = __shfl_up(own.count, step, 64);
+        own.weight += lane >= uint32_t(step) ? weight : 0u;
+        own.count += lane >= uint32_t(step) ? count : 0u;
+    }
+    if (lane == 63u) {
+        s.waves[wave] = own;
+    }
+    __syncthreads();
+    for (uint32_t v = 0; v < wave; ++v) {
+        own.weight += s.waves[v].weight;
+        own.count += s.waves[v].count;
+    }
+    __syncthreads();
+    return own;
+}
+
+// f(value, id) of the tokens [begin, end), 16 bytes of them a load, several under way.
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Several {
+    T v[N];
+};
+template <class T, class F> __device__ __forceinline__ void visit(const T* x, uint32_t begin, uint32_t end, F f) {
+    constexpr uint32_t N = 16u / sizeof(T), AHEAD = 4u;
+    using Vector = Several<T, N>;
+    const uint32_t vectors = (end - begin) / N;
+    const auto at = [&](uint32_t v) { return *reinterpret_cast<const Vector*>(x + begin + v * N); };
+    const auto take = [&](const Vector& some, uint32_t v) {
+#pragma unroll
+        for (uint32_t e = 0; e < N; ++e) {
+            f(widen<T>(some.v[e]), begin + v * N + e);
+        }
+    };
+    uint32_t v = threadIdx.x;
+    for (; v + (AHEAD - 1u) * kThreads < vectors; v += AHEAD * kThreads) {
+        Vector some[AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            some[k] = at(v + k * kThreads);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            take(some[k], v + k * kThreads);
+        }
+    }
+    for (; v < vectors; v += kThreads) {
+        take(at(v), v);
+    }
+    if (const uint32_t i = begin + vectors * N + threadIdx.x; i < end) {
+        f(widen<T>(x[i]), i);
+    }
+}
+
+// The largest logit's order and the lowest id that has it, as a selection key, of [begin, end).
+template <class T> __device__ uint64_t largest(Shared& s, const T* x, uint32_t begin, uint32_t end) {
+    uint32_t best = 0, id = 0xffffffffu;
+    visit(x, begin, end, [&](float v, uint32_t i) {
+        const uint32_t order = order_of(v);
+        id = order > best ? i : id;  // (a thread's ids ascend)
+        best = order > best ? order : best;
+    });
+    return max_all(s, uint64_t(best) << 32 | uint64_t(0xffffffffu - id));
+}
+
+// A whole row, for descending on its keys.
 template <class T> struct Row {
     const T* x;
     uint32_t width;
-    uint64_t (*weight)[kBuckets];  // [2][kBuckets], LDS: the first step's histogram and the later ones'
-    uint32_t (*count)[kBuckets];
-    Sums* waves;  // [kThreads / 64]
-    Place* found;
+    Shared& s;
+    __device__ uint64_t* weight(uint32_t which) const { return which ? s.before : s.weight; }
+    __device__ uint32_t* count(uint32_t which) const { return which ? reinterpret_cast<uint32_t*>(s.list) : s.count; }
 
     // Sums of the tokens whose order is ``prefix`` above its bits [shift, shift + bits), by those bits.
     __device__ void histogram(const Weights& w, uint32_t which, uint32_t prefix, uint32_t shift, uint32_t bits) {
         for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
-            weight[which][i] = 0u;
-            count[which][i] = 0u;
+            weight(which)[i] = 0u;
+            count(which)[i] = 0u;
         }
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < width; i += kThreads) {
@@ -117,9 +246,9 @@ template <class T> struct Row {
             if (uint64_t(order) >> (shift + bits) == prefix) {
                 const uint32_t bucket = (order >> shift) & ((1u << bits) - 1u);
                 const uint64_t mine = w(v);
-                atomicAdd(&count[which][bucket], 1u);
+                atomicAdd(&count(which)[bucket], 1u);
                 if (mine) {
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&weight[which][bucket]), static_cast<unsigned long long>(mine));
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&weight(which)[bucket]), static_cast<unsigned long long>(mine));
                 }
             }
         }
@@ -129,47 +258,28 @@ template <class T> struct Row {
     // The highest bucket at whose end the sums before it and those down to it reach the goal, and the sums above it.
     __device__ uint32_t descend(uint32_t which, bool by_count, uint64_t goal, Sums& before) {
         constexpr uint32_t PER = kBuckets / kThreads;
-        const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u, top = kBuckets - 1u - threadIdx.x * PER;
+        const uint32_t top = kBuckets - 1u - threadIdx.x * PER;
         Sums own{0u, 0u};
 #pragma unroll
         for (uint32_t k = 0; k < PER; ++k) {
-            own.weight += weight[which][top - k];
-            own.count += count[which][top - k];
+            own.weight += weight(which)[top - k];
+            own.count += count(which)[top - k];
         }
-        Sums upto = own;
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-            const uint64_t ww = __shfl_up(static_cast<unsigned long long>(upto.weight), step, 64);
-            const uint32_t cc = __shfl_up(upto.count, step, 64);
-            if (lane >= uint32_t(step)) {
-                upto.weight += ww;
-                upto.count += cc;
-            }
-        }
-        if (lane == 63u) {
-            waves[wave] = upto;
-        }
-        __syncthreads();
-        Sums at = before;
-        for (uint32_t w = 0; w < wave; ++w) {
-            at.weight += waves[w].weight;
-            at.count += waves[w].count;
-        }
-        at.weight += upto.weight - own.weight;
-        at.count += upto.count - own.count;
+        const Sums upto = scan_all(s, own);
+        Sums at{before.weight + upto.weight - own.weight, before.count + upto.count - own.count};
 #pragma unroll
         for (uint32_t k = 0; k < PER; ++k) {
-            const Sums next{at.weight + weight[which][top - k], at.count + count[which][top - k]};
+            const Sums next{at.weight + weight(which)[top - k], at.count + count(which)[top - k]};
             const uint64_t reached = by_count ? next.count : next.weight, short_of = by_count ? at.count : at.weight;
             if (reached >= goal && short_of < goal) {  // one thread
-                found->order = top - k;
-                found->before = at;
+                s.found.order = top - k;
+                s.found.before = at;
             }
             at = next;
         }
         __syncthreads();
-        before = found->before;
-        const uint32_t bucket = found->order;
+        before = s.found.before;
+        const uint32_t bucket = s.found.order;
         __syncthreads();
         return bucket;
     }
@@ -189,45 +299,6 @@ template <class T> struct Row {
         return p;
     }
 
-    // Sums over the workgroup.
-    __device__ Sums all(Sums own) {
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-            own.weight += __shfl_xor(static_cast<unsigned long long>(own.weight), step, 64);
-            own.count += __shfl_xor(own.count, step, 64);
-        }
-        if (threadIdx.x % 64u == 0u) {
-            waves[threadIdx.x / 64u] = own;
-        }
-        __syncthreads();
-        Sums sum{0u, 0u};
-        for (uint32_t v = 0; v < kThreads / 64u; ++v) {
-            sum.weight += waves[v].weight;
-            sum.count += waves[v].count;
-        }
-        __syncthreads();
-        return sum;
-    }
-
-    // The largest logit's order and id, as a selection key.
-    __device__ uint64_t largest() {
-        uint64_t best = 0;
-        for (uint32_t i = threadIdx.x; i < width; i += kThreads) {
-            const uint64_t key = chroma::topk_key(widen<T>(x[i]), i, true);
-            best = key > best ? key : best;
-        }
-        best = chroma::wave_max_u64(best);
-        if (threadIdx.x % 64u == 0u) {
-            waves[threadIdx.x / 64u].weight = best;
-        }
-        __syncthreads();
-        for (uint32_t v = 0; v < kThreads / 64u; ++v) {
-            best = waves[v].weight > best ? waves[v].weight : best;
-        }
-        __syncthreads();
-        return best;
-    }
-
     // The id of the ``nth`` token of this order, from 1 on, by id: every wave counts a span, one looks it up.
     __device__ void id_of(uint32_t order, uint32_t nth, int64_t* id) {
         const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u, span = (width + kThreads - 1u) / kThreads * 64u;
@@ -238,12 +309,12 @@ template <class T> struct Row {
             own += __popcll(matches(i));
         }
         if (lane == 0u) {
-            waves[wave].count = own;
+            s.waves[wave].count = own;
         }
         __syncthreads();
         uint32_t before = 0;
         for (uint32_t v = 0; v < wave; ++v) {
-            before += waves[v].count;
+            before += s.waves[v].count;
         }
         if (before < nth && nth <= before + own) {
             for (uint32_t i = begin; i < end; i += 64u) {
@@ -261,74 +332,513 @@ template <class T> struct Row {
     }
 };
 
-// grid: rows
-template <class T> __global__ void __launch_bounds__(kThreads) sample_rows(Call c) {
-    __shared__ uint64_t weight[2][kBuckets];
-    __shared__ uint32_t count[2][kBuckets];
-    __shared__ Sums waves[kThreads / 64u];
-    __shared__ Place found;
-    const uint64_t r = blockIdx.x;
-    Row<T> row{static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), uint32_t(c.width), weight, count, waves, &found};
-    const float temperature = c.temperature ? c.temperature[r] : 1.0f;
-    const uint64_t best = row.largest();
-    const uint32_t order = uint32_t(best >> 32);
-    const float top = value_of(order);
-    if (order == 0xffffffffu || top == -__builtin_inff() || !(temperature > 0.0f)) {
-        if (threadIdx.x == 0u) {
-            const bool nan = order == 0xffffffffu, nothing = !nan && top == -__builtin_inff();
-            c.ids[r] = nothing ? -1 : int64_t(0xffffffffu - uint32_t(best));
-            if (c.logprobs) {
-                c.logprobs[r] = nan ? __builtin_nanf("") : nothing ? top : 0.0f;
-            }
-        }
-        return;
+// A row's settings, and its weights.
+struct Settings {
+    float top, temperature, top_p, min_p, uniform;
+    int64_t top_k;
+    uint32_t best;  // id of the largest logit
+    bool nan;
+    __device__ __forceinline__ Settings(const Call& c, uint64_t r, uint64_t key)
+        : temperature(c.temperature ? c.temperature[r] : 1.0f), top_p(c.top_p ? c.top_p[r] : 1.0f), min_p(c.min_p ? c.min_p[r] : 0.0f),
+          uniform(c.uniform[r]), top_k(c.top_k ? c.top_k[r] : 0), best(0xffffffffu - uint32_t(key)), nan(key >> 32 == 0xffffffffu) {
+        top = value_of(uint32_t(key >> 32));
+        top_k = top_k >= c.width || top_k < 0 ? 0 : top_k;
     }
-    const Weights w(top, temperature);
+    // Whether the largest logit decides alone; ``finish`` then writes the result.
+    __device__ __forceinline__ bool greedy() const { return nan || top == -__builtin_inff() || !(temperature > 0.0f); }
+    __device__ __forceinline__ void finish(const Call& c, uint64_t r) const {
+        const bool nothing = !nan && top == -__builtin_inff();
+        c.ids[r] = nothing ? -1 : int64_t(best);
+        if (c.logprobs) {
+            c.logprobs[r] = nan ? __builtin_nanf("") : nothing ? top : 0.0f;
+        }
+    }
+    __device__ __forceinline__ Weights weights() const { return Weights(top, temperature); }
+    // The histogram's bucket of a logit: it never falls as the logit falls. (Halves: the difference itself may overflow.)
+    __device__ __forceinline__ uint32_t bucket(float x, float rate) const {
+        const float t = x == top ? 0.0f : (0.5f * top - 0.5f * x) * rate;
+        return t < float(kBuckets - 1u) ? uint32_t(t) : kBuckets - 1u;
+    }
+    __device__ __forceinline__ float rate() const { return 2.0f * kDepths * 1.44269504088896341f / temperature; }
+    // The sum of weights that the kept tokens of ``sum`` must reach under top_p (at least the first one's).
+    __device__ __forceinline__ uint64_t nucleus(uint64_t sum) const {
+        bool more = false;
+        const uint64_t whole = top_p > 0.0f ? share_of(sum, top_p, more) : 0u, goal = whole + (more ? 1u : 0u);
+        return goal ? goal : 1u;
+    }
+    // The least weight that min_p keeps.
+    __device__ __forceinline__ uint64_t least() const { return uint64_t(__builtin_ceil(double(min_p > 2.0f ? 2.0f : min_p) * double(kWhole))); }
+    // The sum of weights that reaches the drawn token.
+    __device__ __forceinline__ uint64_t place(uint64_t kept) const {
+        bool more = false;
+        return 1u + (uniform > 0.0f ? share_of(kept, uniform < 1.0f ? uniform : __uint_as_float(0x3f7fffffu), more) : 0u);
+    }
+    __device__ __forceinline__ float logprob(float x, uint64_t kept) const {
+        return float(-weights().depth(x) * 0.69314718055994530942 - log(double(kept) * (1.0 / double(kWhole))));
+    }
+};
+
+// The token of a whole row, by descending on its keys.
+template <class T> __device__ void descend_row(const Call& c, uint64_t r, const Settings& set, const T* x, Shared& s) {
+    Row<T> row{x, uint32_t(c.width), s};
+    const Weights w = set.weights();
     row.histogram(w, 0u, 0u, 21u, 11u);
     Sums own{0u, 0u};
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
-        own.weight += weight[0][i];
-        own.count += count[0][i];
+        own.weight += s.weight[i];
+        own.count += s.count[i];
     }
-    Sums kept = row.all(own);
-    const int64_t k = c.top_k ? c.top_k[r] : 0;
-    if (k > 0 && k < c.width) {
-        const Place p = row.reach(w, true, uint64_t(k));
-        kept = Sums{p.weight(), uint32_t(p.count())};
+    uint64_t kept = sum_all(s, own).weight;
+    if (set.top_k) {
+        kept = row.reach(w, true, uint64_t(set.top_k)).weight();
     }
-    const float top_p = c.top_p ? c.top_p[r] : 1.0f;
-    if (top_p < 1.0f) {
-        bool more = false;
-        const uint64_t whole = top_p > 0.0f ? share_of(kept.weight, top_p, more) : 0u;
-        const uint64_t goal = whole + (more ? 1u : 0u);
-        const Place p = row.reach(w, false, goal ? goal : 1u);
-        kept = Sums{p.weight(), uint32_t(p.count())};
+    if (set.top_p < 1.0f) {
+        kept = row.reach(w, false, set.nucleus(kept)).weight();
     }
-    const float min_p = c.min_p ? c.min_p[r] : 0.0f;
-    if (min_p > 0.0f) {
-        const double least = __builtin_ceil(double(min_p > 2.0f ? 2.0f : min_p) * double(1ull << kOne));
-        const uint64_t floor = uint64_t(least);
+    if (set.min_p > 0.0f) {
+        const uint64_t least = set.least();
         own = Sums{0u, 0u};
-        for (uint32_t i = threadIdx.x; i < row.width; i += kThreads) {
-            const uint64_t mine = w(widen<T>(row.x[i]));
-            own.weight += mine >= floor ? mine : 0u;
-            own.count += mine >= floor ? 1u : 0u;
-        }
-        Sums high = row.all(own);
-        if (!high.count) {
-            high = Sums{1ull << kOne, 1u};
-        }
-        kept = high.count < kept.count ? high : kept;
+        visit(x, 0u, row.width, [&](float v, uint32_t) {
+            const uint64_t mine = w(v);
+            own.weight += mine >= least ? mine : 0u;
+        });
+        const uint64_t high = sum_all(s, own).weight;
+        kept = lesser(kept, greater(high, kWhole));
     }
-    const float given = c.uniform[r];
-    bool more = false;
-    const uint64_t goal = 1u + (given > 0.0f ? share_of(kept.weight, given < 1.0f ? given : __uint_as_float(0x3f7fffffu), more) : 0u);
-    const Place drawn = row.reach(w, false, goal);
+    const Place drawn = row.reach(w, false, set.place(kept));
     row.id_of(drawn.order, drawn.ties, c.ids + r);
     if (threadIdx.x == 0u && c.logprobs) {
-        const double share = double(kept.weight) * (1.0 / double(1ull << kOne));
-        c.logprobs[r] = float(-w.depth(value_of(drawn.order)) * 0.69314718055994530942 - log(share));
+        c.logprobs[r] = set.logprob(value_of(drawn.order), kept);
     }
+}
+
+// Which tokens of a row are listed: those of buckets up to ``top`` (a top-k's), or those of three ranges of buckets, in which the
+// top-p's cut, the min-p's and the drawn token lie; ``whole``: none, the whole row is descended on.
+struct Listing {
+    uint32_t whole, by_count;
+    uint32_t nucleus, least_low, least_high, drawn_low, drawn_high;
+    __device__ __forceinline__ bool holds(uint32_t b) const {
+        return by_count ? b <= drawn_high : b == nucleus || (b >= least_low && b <= least_high) || (b >= drawn_low && b <= drawn_high);
+    }
+};
+constexpr uint32_t kNone = 0x7fffffffu;
+
+// The histogram of [begin, end) in s.weight: weights, or counts where a top-k cuts the row.
+template <class T> __device__ void depths(const Settings& set, const T* x, uint32_t begin, uint32_t end, Shared& s) {
+    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+        s.weight[i] = 0u;
+        s.count[i] = 0u;
+    }
+    __syncthreads();
+    const float rate = set.rate();
+    if (set.top_k) {
+        visit(x, begin, end, [&](float v, uint32_t) { atomicAdd(&s.count[set.bucket(v, rate)], 1u); });
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+            s.weight[i] = s.count[i];
+        }
+    } else {
+        const Weights w = set.weights();
+        visit(x, begin, end, [&](float v, uint32_t) {
+            const uint32_t bucket = set.bucket(v, rate);
+            if (bucket < kBuckets - 1u) {
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[bucket]), static_cast<unsigned long long>(w(v)));
+            }
+        });
+    }
+    __syncthreads();
+}
+
+// The bucket in which the sums reach ``goal``, from 1 to all there is.
+__device__ uint32_t bucket_of(Shared& s, uint64_t goal) {
+    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+        if (s.before[i] < goal && s.before[i + 1u] >= goal) {
+            s.last = i;
+        }
+    }
+    __syncthreads();
+    const uint32_t found = s.last;
+    __syncthreads();
+    return found;
+}
+
+// From the row's histogram in s.weight: its running sums in s.before, and what is listed.
+__device__ Listing list_of(const Settings& set, Shared& s) {
+    const uint32_t first = threadIdx.x * 2u;
+    const uint64_t one = s.weight[first], two = s.weight[first + 1u];
+    const uint64_t upto = scan_all(s, Sums{one + two, 0u}).weight;
+    s.before[first] = upto - one - two;
+    s.before[first + 1u] = upto - two;
+    if (threadIdx.x == kThreads - 1u) {
+        s.before[kBuckets] = upto;
+    }
+    __syncthreads();
+    Listing l{0u, 0u, kNone, kNone, 0u, kNone, 0u};
+    if (set.top_k) {
+        l.by_count = 1u;
+        l.drawn_high = bucket_of(s, uint64_t(set.top_k));
+        l.whole = set.top_k > kMostTop || s.before[l.drawn_high + 1u] > kList ? 1u : 0u;
+        return l;
+    }
+    const uint64_t all = s.before[kBuckets];
+    uint64_t low = all, high = all;  // bounds of the kept sum
+    if (set.top_p < 1.0f) {
+        const uint64_t goal = set.nucleus(all);
+        l.nucleus = bucket_of(s, goal);
+        low = goal;
+        high = s.before[l.nucleus + 1u];
+    }
+    if (set.min_p > 0.0f) {
+        // the least weight's bucket, and one on either side for the rounding of a logit's
+        const float t = -__log2f(set.min_p > 1.0f ? 1.0f : set.min_p) * kDepths;
+        const uint32_t bucket = t < float(kBuckets - 1u) ? uint32_t(t) : kBuckets - 1u;
+        l.least_low = bucket ? bucket - 1u : 0u;
+        l.least_high = min(bucket + 1u, kBuckets - 2u);
+        low = lesser(low, greater(s.before[l.least_low], kWhole));
+        high = lesser(high, greater(s.before[l.least_high + 1u], kWhole));
+    }
+    l.drawn_low = bucket_of(s, set.place(low));
+    l.drawn_high = bucket_of(s, set.place(high));
+    return l;
+}
+
+// A listed token at which sums reach a goal.
+struct Listed {
+    uint64_t key, before;  // before: the sum of weights (or the count) of the tokens before it
+};
+
+// Among the ``n`` keys of s.list in [low, high]: where counts or weights, ``before`` of them before the first, reach ``goal``.
+__device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_count, uint64_t before, uint64_t goal, uint64_t low, uint64_t high) {
+    for (int step = 0; step < 8; ++step) {  // (eleven bits a step)
+        uint64_t most = 0, least = 0;  // least: of the inverted keys
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const uint64_t key = s.list[i];
+            if (key >= low && key <= high) {
+                most = key > most ? key : most;
+                least = ~key > least ? ~key : least;
+            }
+        }
+        most = max_all(s, most);
+        least = ~max_all(s, least);
+        if (most == least) {  // one key
+            return Listed{most, before};
+        }
+        const int bits = 64 - __builtin_clzll(most ^ least), shift = bits > 11 ? bits - 11 : 0;
+        for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+            s.weight[i] = 0u;
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const uint64_t key = s.list[i];
+            if (key >= low && key <= high) {
+                const uint64_t mine = by_count ? 1u : w(value_of(uint32_t(key >> 32)));
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[(key >> shift) % kBuckets]), static_cast<unsigned long long>(mine));
+            }
+        }
+        __syncthreads();
+        const uint32_t top = kBuckets - 1u - threadIdx.x * 2u;
+        const uint64_t one = s.weight[top], two = s.weight[top - 1u];
+        const uint64_t at = before + scan_all(s, Sums{one + two, 0u}).weight - one - two;
+        if (at < goal && at + one >= goal) {
+            s.found.order = top;
+            s.found.before.weight = at;
+        } else if (at + one < goal && at + one + two >= goal) {
+            s.found.order = top - 1u;
+            s.found.before.weight = at + one;
+        }
+        __syncthreads();
+        before = s.found.before.weight;
+        const uint64_t above = most >> shift >> 11 << 11 | s.found.order;  // the keys' bits from ``shift`` on
+        low = greater(low, above << shift);  // (other buckets' keys may lie in the step's range)
+        high = lesser(high, above << shift | ((1ull << shift) - 1u));
+        __syncthreads();
+    }
+    return Listed{low, before};
+}
+
+// Lists the tokens of [begin, end): s.listed of them, the first kList to come in s.list.
+template <class T> __device__ void gather(const Settings& set, const Listing& l, const T* x, uint32_t begin, uint32_t end, Shared& s) {
+    if (threadIdx.x == 0u) {
+        s.listed = 0u;
+    }
+    __syncthreads();
+    const float rate = set.rate();
+    visit(x, begin, end, [&](float v, uint32_t i) {
+        if (l.holds(set.bucket(v, rate))) {
+            const uint32_t at = atomicAdd(&s.listed, 1u);
+            if (at < kList) {
+                s.list[at] = chroma::topk_key(v, i, true);
+            }
+        }
+    });
+    __syncthreads();
+}
+
+// The token, from the ``n`` listed keys in s.list; ``below(b)``: the histogram's sums before bucket b.
+template <class B> __device__ void choose(const Call& c, uint64_t r, const Settings& set, const Listing& l, uint32_t n, B below, Shared& s) {
+    const Weights w = set.weights();
+    const float rate = set.rate();
+    // the keys of bucket b: those of the list between its largest and its smallest
+    const auto reach = [&](uint32_t b, uint64_t goal) {
+        uint64_t most = 0, least = 0;
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const uint64_t key = s.list[i];
+            if (set.bucket(value_of(uint32_t(key >> 32)), rate) == b) {
+                most = key > most ? key : most;
+                least = ~key > least ? ~key : least;
+            }
+        }
+        most = max_all(s, most);
+        least = ~max_all(s, least);
+        return reach_list(w, s, n, false, below(b), goal, least, most);
+    };
+    const auto weight_of = [&](uint64_t key) { return w(value_of(uint32_t(key >> 32))); };
+    const auto at_least = [&](uint64_t least, uint32_t from, uint32_t to) {  // sum of the listed weights of these buckets
+        Sums own{0u, 0u};
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const float v = value_of(uint32_t(s.list[i] >> 32));
+            const uint32_t b = set.bucket(v, rate);
+            const uint64_t mine = w(v);
+            own.weight += mine >= least && b >= from && b <= to ? mine : 0u;
+        }
+        return sum_all(s, own).weight;
+    };
+    uint64_t kept;
+    Listed drawn;
+    if (l.by_count) {
+        const Listed last = reach_list(w, s, n, true, 0u, uint64_t(set.top_k), 0u, ~0ull);
+        Sums own{0u, 0u};
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            own.weight += s.list[i] >= last.key ? weight_of(s.list[i]) : 0u;
+        }
+        kept = sum_all(s, own).weight;
+        if (set.top_p < 1.0f) {
+            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), 0u, ~0ull);
+            kept = cut.before + weight_of(cut.key);
+        }
+        if (set.min_p > 0.0f) {
+            const uint64_t high = at_least(set.least(), 0u, kBuckets);
+            kept = lesser(kept, greater(high, kWhole));
+        }
+        drawn = reach_list(w, s, n, false, 0u, set.place(kept), 0u, ~0ull);
+    } else {
+        kept = below(kBuckets);
+        if (set.top_p < 1.0f) {
+            const Listed cut = reach(l.nucleus, set.nucleus(kept));
+            kept = cut.before + weight_of(cut.key);
+        }
+        if (set.min_p > 0.0f) {
+            const uint64_t high = below(l.least_low) + at_least(set.least(), l.least_low, l.least_high);
+            kept = lesser(kept, greater(high, kWhole));
+        }
+        const uint64_t goal = set.place(kept);
+        uint32_t b = l.drawn_low;
+        while (b < l.drawn_high && below(b + 1u) < goal) {
+            ++b;
+        }
+        drawn = reach(b, goal);
+    }
+    if (threadIdx.x == 0u) {
+        c.ids[r] = int64_t(0xffffffffu - uint32_t(drawn.key));
+        if (c.logprobs) {
+            c.logprobs[r] = set.logprob(value_of(uint32_t(drawn.key >> 32)), kept);
+        }
+    }
+}
+
+// One workgroup a row. grid: rows
+template <class T> __global__ void __launch_bounds__(kThreads) sample_rows(Call c) {
+    __shared__ Shared s;
+    const uint64_t r = blockIdx.x;
+    const T* x = static_cast<const T*>(c.x) + r * uint64_t(c.x_stride);
+    const uint32_t width = uint32_t(c.width);
+    const Settings set(c, r, largest(s, x, 0u, width));
+    if (set.greedy()) {
+        if (threadIdx.x == 0u) {
+            set.finish(c, r);
+        }
+        return;
+    }
+    depths(set, x, 0u, width, s);
+    const Listing l = list_of(set, s);
+    if (l.whole) {
+        descend_row(c, r, set, x, s);
+        return;
+    }
+    gather(set, l, x, 0u, width, s);
+    const uint32_t n = s.listed;
+    if (n > kList) {
+        descend_row(c, r, set, x, s);
+        return;
+    }
+    choose(c, r, set, l, n, [&](uint32_t b) { return s.before[b]; }, s);
+}
+
+// Scratch of a row that is cut into spans.
+struct Scratch {
+    uint64_t* best;       // [spans]
+    uint64_t* histogram;  // [spans, kBuckets]
+    uint64_t* before;     // [kBuckets + 1]
+    uint64_t* list;       // [kList]
+    Listing* listing;
+    uint32_t* tickets;  // workgroups that are done with the histogram, with the list; listed tokens
+    static __host__ __device__ uint64_t words(uint64_t spans) { return spans * (1u + kBuckets) + kBuckets + 1u + kList + 8u; }
+    __device__ Scratch(uint64_t* base, uint64_t r, uint32_t spans) {
+        best = base + r * words(spans);
+        histogram = best + spans;
+        before = histogram + uint64_t(spans) * kBuckets;
+        list = before + kBuckets + 1u;
+        listing = reinterpret_cast<Listing*>(list + kList);
+        tickets = reinterpret_cast<uint32_t*>(list + kList + 4u);
+    }
+};
+static_assert(sizeof(Listing) <= 32 && kBuckets == 2 * kThreads, "scratch and running sums");
+
+struct Span {
+    uint32_t begin, end;
+    __device__ Span(const Call& c, uint32_t spans, uint32_t i) {
+        const uint32_t width = uint32_t(c.width), each = ((width + spans - 1u) / spans + 7u) / 8u * 8u;
+        begin = min(i * each, width);
+        end = min(begin + each, width);
+    }
+};
+
+// The first reading: each span's largest logit. grid: (spans, rows)
+template <class T> __global__ void __launch_bounds__(kThreads) sample_best(Call c, uint64_t* scratch) {
+    __shared__ Shared s;
+    const uint64_t r = blockIdx.y;
+    const Scratch mine(scratch, r, gridDim.x);
+    const Span span(c, gridDim.x, blockIdx.x);
+    const uint64_t best = largest(s, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), span.begin, span.end);
+    if (threadIdx.x == 0u) {
+        mine.best[blockIdx.x] = best;
+        if (blockIdx.x == 0u) {
+            mine.tickets[0] = 0u;
+            mine.tickets[1] = 0u;
+            mine.tickets[2] = 0u;
+        }
+    }
+}
+
+__device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
+    uint64_t best = 0;
+    for (uint32_t i = 0; i < spans; ++i) {
+        best = mine.best[i] > best ? mine.best[i] : best;
+    }
+    return best;
+}
+
+// Whether this workgroup is the last of the row's to come here, after its device-scope stores.
+__device__ bool comes_last(uint32_t* ticket, Shared& s) {
+    chroma::device_stores_complete();
+    __syncthreads();
+    if (threadIdx.x == 0u) {
+        s.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    const bool last = s.last == gridDim.x - 1u;
+    __syncthreads();
+    return last;
+}
+
+// The second reading: the histogram, and what is listed. grid: (spans, rows)
+template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Call c, uint64_t* scratch) {
+    __shared__ Shared s;
+    const uint64_t r = blockIdx.y;
+    const uint32_t spans = gridDim.x;
+    const Scratch mine(scratch, r, spans);
+    const Settings set(c, r, best_of(mine, spans));
+    if (set.greedy()) {
+        if (blockIdx.x == 0u && threadIdx.x == 0u) {
+            set.finish(c, r);
+        }
+        return;
+    }
+    const Span span(c, spans, blockIdx.x);
+    depths(set, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), span.begin, span.end, s);
+    uint64_t* to = mine.histogram + uint64_t(blockIdx.x) * kBuckets;
+    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+        chroma::store_device(to + i, s.weight[i]);
+    }
+    if (!comes_last(mine.tickets, s)) {
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+        uint64_t sum = 0;
+        for (uint32_t k = 0; k < spans; ++k) {
+            sum += chroma::load_device(mine.histogram + uint64_t(k) * kBuckets + i);
+        }
+        s.weight[i] = sum;
+    }
+    __syncthreads();
+    const Listing l = list_of(set, s);
+    for (uint32_t i = threadIdx.x; i <= kBuckets; i += kThreads) {
+        mine.before[i] = s.before[i];
+    }
+    if (threadIdx.x == 0u) {
+        *mine.listing = l;
+    }
+}
+
+// The third reading: the list, and the token. grid: (spans, rows)
+template <class T> __global__ void __launch_bounds__(kThreads) sample_listed(Call c, uint64_t* scratch) {
+    __shared__ Shared s;
+    const uint64_t r = blockIdx.y;
+    const uint32_t spans = gridDim.x;
+    const Scratch mine(scratch, r, spans);
+    const Settings set(c, r, best_of(mine, spans));
+    if (set.greedy()) {
+        return;
+    }
+    const T* x = static_cast<const T*>(c.x) + r * uint64_t(c.x_stride);
+    const Listing l = *mine.listing;
+    if (l.whole) {
+        if (blockIdx.x == 0u) {
+            descend_row(c, r, set, x, s);
+        }
+        return;
+    }
+    const Span span(c, spans, blockIdx.x);
+    gather(set, l, x, span.begin, span.end, s);
+    if (threadIdx.x == 0u) {
+        s.last = __hip_atomic_fetch_add(mine.tickets + 2, s.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    const uint32_t begin = s.last, own = min(s.listed, kList);
+    for (uint32_t i = threadIdx.x; i < own && begin + i < kList; i += kThreads) {
+        chroma::store_device(mine.list + begin + i, s.list[i]);
+    }
+    if (!comes_last(mine.tickets + 1, s)) {
+        return;
+    }
+    const uint32_t n = chroma::load_device(mine.tickets + 2);
+    if (n > kList) {
+        descend_row(c, r, set, x, s);
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        s.list[i] = chroma::load_device(mine.list + i);
+    }
+    __syncthreads();
+    choose(c, r, set, l, n, [&](uint32_t b) { return mine.before[b]; }, s);
+}
+
+// Spans of a row: workgroups that fill the chip twice, of 8192 tokens at least; 1: one launch of a workgroup a row.
+uint32_t spans_of(const Call& c) {
+    const int64_t wanted = 512 / c.rows, most = c.width / 8192;
+    return uint32_t(wanted < 2 || most < 2 ? 1 : wanted < most ? wanted : most);
+}
+
+template <class T> void launch(const Call& c, uint64_t* scratch, hipStream_t stream) {
+    const uint32_t spans = spans_of(c);
+    if (spans == 1u) {
+        sample_rows<T><<<unsigned(c.rows), kThreads, 0, stream>>>(c);
+        return;
+    }
+    const dim3 grid(spans, unsigned(c.rows));
+    sample_best<T><<<grid, kThreads, 0, stream>>>(c, scratch);
+    sample_depths<T><<<grid, kThreads, 0, stream>>>(c, scratch);
+    sample_listed<T><<<grid, kThreads, 0, stream>>>(c, scratch);
 }
 
 int refuse(const char* message, char* error, size_t size) {
@@ -357,7 +867,11 @@ const char* mistake(const Call& c) {
 extern "C" {
 
 __attribute__((visibility("default"))) size_t chroma_hip_rows_sample_workspace(const Call* call) {
-    return 0;
+    if (!call || mistake(*call)) {
+        return 0;
+    }
+    const uint32_t spans = spans_of(*call);
+    return spans > 1u ? size_t(call->rows) * Scratch::words(spans) * sizeof(uint64_t) : 0;
 }
 
 __attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* call, void* workspace, size_t workspace_bytes, void* stream,
@@ -390,9 +904,9 @@ __attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* ca
         return refuse("ids, logprobs or the workspace overlap another array", error, error_size);
     }
     if (c.dtype == CHROMA_HIP_FLOAT32) {
-        sample_rows<float><<<unsigned(c.rows), kThreads, 0, static_cast<hipStream_t>(stream)>>>(c);
+        launch<float>(c, static_cast<uint64_t*>(workspace), static_cast<hipStream_t>(stream));
     } else {
-        sample_rows<uint16_t><<<unsigned(c.rows), kThreads, 0, static_cast<hipStream_t>(stream)>>>(c);
+        launch<uint16_t>(c, static_cast<uint64_t*>(workspace), static_cast<hipStream_t>(stream));
     }
     const hipError_t status = hipGetLastError();
     return status == hipSuccess ? CHROMA_HIP_OK : refuse(hipGetErrorString(status), error, error_size);

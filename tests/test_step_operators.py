@@ -782,6 +782,34 @@ def test_sample(rows, width, dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("rows,width", [(1, 16384), (2, 70001), (70, 16390), (300, 9001), (300, 4096), (5, 4097)])
+@pytest.mark.parametrize("spread", [0.001, 2.0, 40.0])
+def test_sample_cut_into_spans_or_not(rows, width, spread, dtype):
+    """Few rows are cut into spans; logits that lie close together or far apart."""
+    x = (torch.randn(rows, width, generator=torch.Generator().manual_seed(width)) * spread).to(dtype)
+    settings = row_settings(rows, seed=rows + 1)
+    check_sample(x, **settings)
+    check_sample(x, uniform=settings["uniform"], top_p=settings["top_p"], min_p=settings["min_p"])
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("rows,width", [(3, 40000), (200, 12000)])
+def test_sample_of_rows_that_no_list_holds(rows, width, dtype):
+    """Equal values, few distinct ones, a large top_k, high temperatures: a bucket holds more than a list."""
+    g = torch.Generator().manual_seed(width)
+    x = torch.randint(-3, 4, (rows, width), generator=g).to(dtype)
+    x[0] = 0.25
+    settings = row_settings(rows, seed=7)
+    check_sample(x, **settings)
+    check_sample(x, **{**settings, "top_k": torch.full((rows,), width - 5)})
+    x = torch.randn(rows, width, generator=g).to(dtype)
+    check_sample(x, uniform=settings["uniform"], top_k=torch.full((rows,), 3000))
+    check_sample(x, uniform=settings["uniform"], temperature=torch.full((rows,), 500.0), top_p=torch.full((rows,), 0.7))
+
+
+@gpu
+@BOTH
 def test_sample_of_ties_and_equal_rows(dtype):
     """Few distinct values, rows all equal, both zeros: ties go by id, and cuts fall among them."""
     g = torch.Generator().manual_seed(3)
