@@ -48,36 +48,54 @@ __device__ __forceinline__ float value_of(uint32_t order) {
     return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 
+// 2^-i / 256 and 2^-i / 65536 of i < 256, in LDS.
+struct Powers {
+    double high[256], low[256];
+    __device__ __forceinline__ void fill() {
+        if (threadIdx.x < 512u) {
+            const uint32_t i = threadIdx.x % 256u;
+            // the series of exp(-f ln 2), |f| <= 1/2, to the 12th power (the 13th is below 2^-52)
+            const double y = double(i) * (threadIdx.x < 256u ? 1.0 / 256.0 : 1.0 / 65536.0), n = __builtin_rint(y), f = (n - y) * 0.69314718055994530942;
+            double p = 1.0 / 479001600.0;
+            p = __builtin_fma(p, f, 1.0 / 39916800.0);
+            p = __builtin_fma(p, f, 1.0 / 3628800.0);
+            p = __builtin_fma(p, f, 1.0 / 362880.0);
+            p = __builtin_fma(p, f, 1.0 / 40320.0);
+            p = __builtin_fma(p, f, 1.0 / 5040.0);
+            p = __builtin_fma(p, f, 1.0 / 720.0);
+            p = __builtin_fma(p, f, 1.0 / 120.0);
+            p = __builtin_fma(p, f, 1.0 / 24.0);
+            p = __builtin_fma(p, f, 1.0 / 6.0);
+            p = __builtin_fma(p, f, 0.5);
+            p = __builtin_fma(p, f, 1.0);
+            p = __builtin_fma(p, f, 1.0);
+            (threadIdx.x < 256u ? high : low)[i] = n == 1.0 ? 0.5 * p : p;
+        }
+        __syncthreads();
+    }
+};
+
 // Weights of one row, relative to its largest logit. An infinite largest one leaves the others nothing.
 struct Weights {
-    double top, rate;  // rate: log2(e) / temperature
-    __device__ __forceinline__ Weights(float top, float temperature)
-        : top(double(top)), rate(1.4426950408889634074 / double(temperature)) {}
-    // log2 of the inverse weight, 0 or more
+    const Powers& powers;
+    double top, rate;  // rate: 65536 log2(e) / temperature
+    __device__ __forceinline__ Weights(const Powers& powers, float top, float temperature)
+        : powers(powers), top(double(top)), rate(65536.0 * 1.4426950408889634074 / double(temperature)) {}
+    // log2 of the inverse weight, 0 or more, in units of 2^-16
     __device__ __forceinline__ double depth(float x) const { return double(x) == top ? 0.0 : (top - double(x)) * rate; }
     __device__ __forceinline__ uint64_t operator()(float x) const {
         const double y = depth(x);
-        if (!(y < double(kOne + 1))) {
+        if (!(y < 65536.0 * double(kOne + 1))) {
             return 0u;
         }
-        // 2^-y = 2^-n 2^-f, |f| <= 1/2: the series of exp(-f ln 2) to the 12th power (the 13th is below 2^-52)
-        const double n = __builtin_rint(y), f = (n - y) * 0.69314718055994530942;
-        double p = 1.0 / 479001600.0;
-        p = __builtin_fma(p, f, 1.0 / 39916800.0);
-        p = __builtin_fma(p, f, 1.0 / 3628800.0);
-        p = __builtin_fma(p, f, 1.0 / 362880.0);
-        p = __builtin_fma(p, f, 1.0 / 40320.0);
-        p = __builtin_fma(p, f, 1.0 / 5040.0);
-        p = __builtin_fma(p, f, 1.0 / 720.0);
-        p = __builtin_fma(p, f, 1.0 / 120.0);
-        p = __builtin_fma(p, f, 1.0 / 24.0);
-        p = __builtin_fma(p, f, 1.0 / 6.0);
-        p = __builtin_fma(p, f, 0.5);
-        p = __builtin_fma(p, f, 1.0);
-        p = __builtin_fma(p, f, 1.0);
-        const double scale = __longlong_as_double(int64_t(1023 + kOne - int(n)) << 52);
+        // 2^-(n + i / 256 + k / 65536) from the powers, and exp(-f ln 2 / 65536) from three terms of its series
+        const int n = int(y);
+        constexpr double c = 0.69314718055994530942 / 65536.0;
+        const double f = y - double(n), p = __builtin_fma(f, __builtin_fma(f, 0.5 * c * c, -c), 1.0);
+        const double scale = __longlong_as_double(int64_t(1023 + kOne - (n >> 16)) << 52);
         // (adding 2^52 rounds to a whole number, which then lies in the low bits)
-        return uint64_t(__double_as_longlong(__builtin_fma(p, scale, 4503599627370496.0))) & 0xfffffffffffffull;
+        const double all = powers.high[(n >> 8) & 255] * powers.low[n & 255] * p;
+        return uint64_t(__double_as_longlong(__builtin_fma(all, scale, 4503599627370496.0))) & 0xfffffffffffffull;
     }
 };
 
@@ -116,10 +134,21 @@ struct Shared {
     uint64_t before[kBuckets + 1];  // sums before each bucket, and of all
     uint32_t count[kBuckets];
     uint64_t list[kList];           // selection keys
+    Powers powers;
+    uint64_t few[64];
     Sums waves[kThreads / 64u];
+    uint64_t ends[kThreads / 64u];
     Place found;
-    uint32_t listed, last;
+    uint32_t listed, last, fews;
 };
+
+__device__ __forceinline__ uint32_t wave_count(uint32_t v) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        v += __shfl_xor(v, step, 64);
+    }
+    return v;
+}
 
 // Sums over the workgroup.
 __device__ Sums sum_all(Shared& s, Sums own) {
@@ -184,7 +213,7 @@ template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Sev
     T v[N];
 };
 template <class T, class F> __device__ __forceinline__ void visit(const T* x, uint32_t begin, uint32_t end, F f) {
-    constexpr uint32_t N = 16u / sizeof(T), AHEAD = 4u;
+    constexpr uint32_t N = 16u / sizeof(T), AHEAD = 16u / N;
     using Vector = Several<T, N>;
     const uint32_t vectors = (end - begin) / N;
     const auto at = [&](uint32_t v) { return *reinterpret_cast<const Vector*>(x + begin + v * N); };
@@ -194,20 +223,18 @@ template <class T, class F> __device__ __forceinline__ void visit(const T* x, ui
             f(widen<T>(some.v[e]), begin + v * N + e);
         }
     };
-    uint32_t v = threadIdx.x;
-    for (; v + (AHEAD - 1u) * kThreads < vectors; v += AHEAD * kThreads) {
+    for (uint32_t v = threadIdx.x; v < vectors; v += AHEAD * kThreads) {
         Vector some[AHEAD];
 #pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            some[k] = at(v + k * kThreads);
+        for (uint32_t k = 0; k < AHEAD; ++k) {  // (clamped: a guarded load would end its branch with a wait)
+            some[k] = at(min(v + k * kThreads, vectors - 1u));
         }
 #pragma unroll
         for (uint32_t k = 0; k < AHEAD; ++k) {
-            take(some[k], v + k * kThreads);
+            if (v + k * kThreads < vectors) {
+                take(some[k], v + k * kThreads);
+            }
         }
-    }
-    for (; v < vectors; v += kThreads) {
-        take(at(v), v);
     }
     if (const uint32_t i = begin + vectors * N + threadIdx.x; i < end) {
         f(widen<T>(x[i]), i);
@@ -353,7 +380,7 @@ struct Settings {
             c.logprobs[r] = nan ? __builtin_nanf("") : nothing ? top : 0.0f;
         }
     }
-    __device__ __forceinline__ Weights weights() const { return Weights(top, temperature); }
+    __device__ __forceinline__ Weights weights(const Shared& s) const { return Weights(s.powers, top, temperature); }
     // The histogram's bucket of a logit: it never falls as the logit falls. (Halves: the difference itself may overflow.)
     __device__ __forceinline__ uint32_t bucket(float x, float rate) const {
         const float t = x == top ? 0.0f : (0.5f * top - 0.5f * x) * rate;
@@ -373,15 +400,15 @@ struct Settings {
         bool more = false;
         return 1u + (uniform > 0.0f ? share_of(kept, uniform < 1.0f ? uniform : __uint_as_float(0x3f7fffffu), more) : 0u);
     }
-    __device__ __forceinline__ float logprob(float x, uint64_t kept) const {
-        return float(-weights().depth(x) * 0.69314718055994530942 - log(double(kept) * (1.0 / double(kWhole))));
+    __device__ __forceinline__ float logprob(const Weights& w, float x, uint64_t kept) const {
+        return float(-w.depth(x) * (0.69314718055994530942 / 65536.0) - log(double(kept) * (1.0 / double(kWhole))));
     }
 };
 
 // The token of a whole row, by descending on its keys.
 template <class T> __device__ void descend_row(const Call& c, uint64_t r, const Settings& set, const T* x, Shared& s) {
     Row<T> row{x, uint32_t(c.width), s};
-    const Weights w = set.weights();
+    const Weights w = set.weights(s);
     row.histogram(w, 0u, 0u, 21u, 11u);
     Sums own{0u, 0u};
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
@@ -408,7 +435,7 @@ template <class T> __device__ void descend_row(const Call& c, uint64_t r, const 
     const Place drawn = row.reach(w, false, set.place(kept));
     row.id_of(drawn.order, drawn.ties, c.ids + r);
     if (threadIdx.x == 0u && c.logprobs) {
-        c.logprobs[r] = set.logprob(value_of(drawn.order), kept);
+        c.logprobs[r] = set.logprob(w, value_of(drawn.order), kept);
     }
 }
 
@@ -438,7 +465,7 @@ template <class T> __device__ void depths(const Settings& set, const T* x, uint3
             s.weight[i] = s.count[i];
         }
     } else {
-        const Weights w = set.weights();
+        const Weights w = set.weights(s);
         visit(x, begin, end, [&](float v, uint32_t) {
             const uint32_t bucket = set.bucket(v, rate);
             if (bucket < kBuckets - 1u) {
@@ -476,7 +503,7 @@ __device__ Listing list_of(const Settings& set, Shared& s) {
     Listing l{0u, 0u, kNone, kNone, 0u, kNone, 0u};
     if (set.top_k) {
         l.by_count = 1u;
-        l.drawn_high = bucket_of(s, uint64_t(set.top_k));
+        l.drawn_high = min(bucket_of(s, uint64_t(set.top_k)), kBuckets - 2u);  // (the last one's tokens weigh nothing)
         l.whole = set.top_k > kMostTop || s.before[l.drawn_high + 1u] > kList ? 1u : 0u;
         return l;
     }
@@ -508,20 +535,61 @@ struct Listed {
 };
 
 // Among the ``n`` keys of s.list in [low, high]: where counts or weights, ``before`` of them before the first, reach ``goal``.
+// Eleven bits of the keys a step, until 64 keys are left; each wave then compares those by itself.
 __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_count, uint64_t before, uint64_t goal, uint64_t low, uint64_t high) {
-    for (int step = 0; step < 8; ++step) {  // (eleven bits a step)
+    const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
+    const auto weight_of = [&](uint64_t key) { return by_count ? uint64_t(1) : w(value_of(uint32_t(key >> 32))); };
+    for (int step = 0; step < 8; ++step) {
         uint64_t most = 0, least = 0;  // least: of the inverted keys
+        uint32_t left = 0;
+        if (threadIdx.x == 0u) {
+            s.fews = 0u;
+        }
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t key = s.list[i];
             if (key >= low && key <= high) {
-                most = key > most ? key : most;
-                least = ~key > least ? ~key : least;
+                most = greater(key, most);
+                least = greater(~key, least);
+                ++left;
             }
         }
-        most = max_all(s, most);
-        least = ~max_all(s, least);
-        if (most == least) {  // one key
-            return Listed{most, before};
+        most = chroma::wave_max_u64(most);
+        least = chroma::wave_max_u64(least);
+        left = wave_count(left);
+        if (lane == 0u) {
+            s.waves[wave] = Sums{most, left};
+            s.ends[wave] = least;
+        }
+        __syncthreads();
+        left = 0u;
+#pragma unroll
+        for (uint32_t v = 0; v < kThreads / 64u; ++v) {
+            most = greater(most, s.waves[v].weight);
+            least = greater(least, s.ends[v]);
+            left += s.waves[v].count;
+        }
+        least = ~least;
+        if (left <= 64u) {
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                const uint64_t key = s.list[i];
+                if (key >= low && key <= high) {
+                    s.few[atomicAdd(&s.fews, 1u)] = key;
+                }
+            }
+            __syncthreads();
+            const uint64_t key = lane < left ? s.few[lane] : 0u, mine = lane < left ? weight_of(key) : 0u;
+            uint64_t above = before;
+            for (uint32_t i = 0; i < left; ++i) {
+                const uint64_t other = s.few[i];
+                const uint32_t weight_low = __builtin_amdgcn_readlane(uint32_t(mine), i), weight_high = __builtin_amdgcn_readlane(uint32_t(mine >> 32), i);
+                above += other > key ? uint64_t(weight_high) << 32 | weight_low : 0u;
+            }
+            const unsigned long long here = __ballot(lane < left && above < goal && above + mine >= goal);
+            const uint32_t at = here ? __builtin_ctzll(here) : 0u;  // (one lane)
+            __syncthreads();  // s.few and s.waves have been read
+            return Listed{uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(key >> 32), at))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(key), at)),
+                          uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(above >> 32), at))) << 32 |
+                              uint32_t(__builtin_amdgcn_readlane(uint32_t(above), at))};
         }
         const int bits = 64 - __builtin_clzll(most ^ least), shift = bits > 11 ? bits - 11 : 0;
         for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
@@ -531,8 +599,7 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t key = s.list[i];
             if (key >= low && key <= high) {
-                const uint64_t mine = by_count ? 1u : w(value_of(uint32_t(key >> 32)));
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[(key >> shift) % kBuckets]), static_cast<unsigned long long>(mine));
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[(key >> shift) % kBuckets]), static_cast<unsigned long long>(weight_of(key)));
             }
         }
         __syncthreads();
@@ -576,7 +643,7 @@ template <class T> __device__ void gather(const Settings& set, const Listing& l,
 
 // The token, from the ``n`` listed keys in s.list; ``below(b)``: the histogram's sums before bucket b.
 template <class B> __device__ void choose(const Call& c, uint64_t r, const Settings& set, const Listing& l, uint32_t n, B below, Shared& s) {
-    const Weights w = set.weights();
+    const Weights w = set.weights(s);
     const float rate = set.rate();
     // the keys of bucket b: those of the list between its largest and its smallest
     const auto reach = [&](uint32_t b, uint64_t goal) {
@@ -606,10 +673,11 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
     uint64_t kept;
     Listed drawn;
     if (l.by_count) {
-        const Listed last = reach_list(w, s, n, true, 0u, uint64_t(set.top_k), 0u, ~0ull);
+        // (fewer are listed where the top-k takes tokens that weigh nothing)
+        const uint64_t last = n > uint64_t(set.top_k) ? reach_list(w, s, n, true, 0u, uint64_t(set.top_k), 0u, ~0ull).key : 0u;
         Sums own{0u, 0u};
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            own.weight += s.list[i] >= last.key ? weight_of(s.list[i]) : 0u;
+            own.weight += s.list[i] >= last ? weight_of(s.list[i]) : 0u;
         }
         kept = sum_all(s, own).weight;
         if (set.top_p < 1.0f) {
@@ -641,7 +709,7 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
     if (threadIdx.x == 0u) {
         c.ids[r] = int64_t(0xffffffffu - uint32_t(drawn.key));
         if (c.logprobs) {
-            c.logprobs[r] = set.logprob(value_of(uint32_t(drawn.key >> 32)), kept);
+            c.logprobs[r] = set.logprob(w, value_of(uint32_t(drawn.key >> 32)), kept);
         }
     }
 }
@@ -649,6 +717,7 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
 // One workgroup a row. grid: rows
 template <class T> __global__ void __launch_bounds__(kThreads) sample_rows(Call c) {
     __shared__ Shared s;
+    s.powers.fill();
     const uint64_t r = blockIdx.x;
     const T* x = static_cast<const T*>(c.x) + r * uint64_t(c.x_stride);
     const uint32_t width = uint32_t(c.width);
@@ -722,10 +791,10 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_best(Call 
 
 __device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
     uint64_t best = 0;
-    for (uint32_t i = 0; i < spans; ++i) {
-        best = mine.best[i] > best ? mine.best[i] : best;
+    for (uint32_t i = threadIdx.x % 64u; i < spans; i += 64u) {
+        best = greater(best, mine.best[i]);
     }
-    return best;
+    return chroma::wave_max_u64(best);
 }
 
 // Whether this workgroup is the last of the row's to come here, after its device-scope stores.
@@ -744,6 +813,7 @@ __device__ bool comes_last(uint32_t* ticket, Shared& s) {
 // The second reading: the histogram, and what is listed. grid: (spans, rows)
 template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Call c, uint64_t* scratch) {
     __shared__ Shared s;
+    s.powers.fill();
     const uint64_t r = blockIdx.y;
     const uint32_t spans = gridDim.x;
     const Scratch mine(scratch, r, spans);
@@ -765,8 +835,16 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Cal
     }
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
         uint64_t sum = 0;
-        for (uint32_t k = 0; k < spans; ++k) {
-            sum += chroma::load_device(mine.histogram + uint64_t(k) * kBuckets + i);
+        for (uint32_t k0 = 0; k0 < spans; k0 += 8u) {
+            uint64_t some[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                some[k] = chroma::load_device(mine.histogram + uint64_t(min(k0 + k, spans - 1u)) * kBuckets + i);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                sum += k0 + k < spans ? some[k] : 0u;
+            }
         }
         s.weight[i] = sum;
     }
@@ -783,6 +861,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Cal
 // The third reading: the list, and the token. grid: (spans, rows)
 template <class T> __global__ void __launch_bounds__(kThreads) sample_listed(Call c, uint64_t* scratch) {
     __shared__ Shared s;
+    s.powers.fill();
     const uint64_t r = blockIdx.y;
     const uint32_t spans = gridDim.x;
     const Scratch mine(scratch, r, spans);
