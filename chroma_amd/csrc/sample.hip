@@ -6,8 +6,8 @@
 // those are listed, and the places among them found by descending on their keys. A row is read three times: for its maximum,
 // for the histogram, for the list; the second and third time it lies in the caches.
 //
-// Rows enough to fill the chip have a workgroup each and one launch. Fewer rows are cut into spans, and the three readings are
-// three launches; the workgroup that comes last with a row's histogram, or list, goes on with them. Rows of up to kList tokens
+// Narrow rows have a workgroup each and one launch. Wide ones are cut into spans, and the three readings are launches of their
+// own; the workgroup that comes last with a row's histogram decides what is listed, and a fourth launch draws. Rows of up to kList tokens
 // are listed whole. Where the listed buckets hold more than kList tokens (rows of equal values, temperatures that leave
 // few depths), a workgroup descends on the keys of the whole row.
 //
@@ -88,13 +88,13 @@ struct Weights {
         if (!(y < 65536.0 * double(kOne + 1))) {
             return 0u;
         }
-        // 2^-(n + i / 256 + k / 65536) from the powers, and exp(-f ln 2 / 65536) from three terms of its series
-        const int n = int(y);
-        constexpr double c = 0.69314718055994530942 / 65536.0;
-        const double f = y - double(n), p = __builtin_fma(f, __builtin_fma(f, 0.5 * c * c, -c), 1.0);
-        const double scale = __longlong_as_double(int64_t(1023 + kOne - (n >> 16)) << 52);
-        // (adding 2^52 rounds to a whole number, which then lies in the low bits)
-        const double all = powers.high[(n >> 8) & 255] * powers.low[n & 255] * p;
+        // 2^-(n >> 16), 2^-(its next 8 bits / 256) and 2^-(the last 8 / 65536) from the powers, exp(-f ln 2 / 65536) from three
+        // terms of its series. (Adding 1.5 2^52 rounds to a whole number, which then lies in the low bits: conversions are slow.)
+        constexpr double c = 0.69314718055994530942 / 65536.0, whole = 6755399441055744.0;
+        const double near = y + whole, f = y - (near - whole), p = __builtin_fma(f, __builtin_fma(f, 0.5 * c * c, -c), 1.0);
+        const uint32_t n = uint32_t(__double_as_longlong(near));
+        const double scale = __hiloint2double(int(1023u + kOne - (n >> 16)) << 20, 0);
+        const double all = powers.high[(n >> 8) & 255u] * powers.low[n & 255u] * p;
         return uint64_t(__double_as_longlong(__builtin_fma(all, scale, 4503599627370496.0))) & 0xfffffffffffffull;
     }
 };
@@ -149,6 +149,12 @@ __device__ __forceinline__ uint32_t wave_count(uint32_t v) {
     }
     return v;
 }
+
+// LDS of a workgroup that only lists.
+struct Gathered {
+    uint64_t list[kList];
+    uint32_t listed, begin;
+};
 
 // Sums over the workgroup.
 __device__ Sums sum_all(Shared& s, Sums own) {
@@ -450,7 +456,8 @@ struct Listing {
 };
 constexpr uint32_t kNone = 0x7fffffffu;
 
-// The histogram of [begin, end) in s.weight: weights, or counts where a top-k cuts the row.
+// The histogram of [begin, end) in s.weight: weights, or counts where a top-k cuts the row; the last bucket's are left out (its
+// tokens weigh nothing, and most of a row may lie there).
 template <class T> __device__ void depths(const Settings& set, const T* x, uint32_t begin, uint32_t end, Shared& s) {
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
         s.weight[i] = 0u;
@@ -459,7 +466,12 @@ template <class T> __device__ void depths(const Settings& set, const T* x, uint3
     __syncthreads();
     const float rate = set.rate();
     if (set.top_k) {
-        visit(x, begin, end, [&](float v, uint32_t) { atomicAdd(&s.count[set.bucket(v, rate)], 1u); });
+        visit(x, begin, end, [&](float v, uint32_t) {
+            const uint32_t bucket = set.bucket(v, rate);
+            if (bucket < kBuckets - 1u) {
+                atomicAdd(&s.count[bucket], 1u);
+            }
+        });
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
             s.weight[i] = s.count[i];
@@ -503,7 +515,8 @@ __device__ Listing list_of(const Settings& set, Shared& s) {
     Listing l{0u, 0u, kNone, kNone, 0u, kNone, 0u};
     if (set.top_k) {
         l.by_count = 1u;
-        l.drawn_high = min(bucket_of(s, uint64_t(set.top_k)), kBuckets - 2u);  // (the last one's tokens weigh nothing)
+        // (a top-k that takes tokens of the last bucket takes all the others)
+        l.drawn_high = bucket_of(s, lesser(uint64_t(set.top_k), s.before[kBuckets]));
         l.whole = set.top_k > kMostTop || s.before[l.drawn_high + 1u] > kList ? 1u : 0u;
         return l;
     }
@@ -527,6 +540,17 @@ __device__ Listing list_of(const Settings& set, Shared& s) {
     l.drawn_low = bucket_of(s, set.place(low));
     l.drawn_high = bucket_of(s, set.place(high));
     return l;
+}
+
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(v), lane));
+}
+__device__ __forceinline__ uint64_t wave_total(uint64_t v) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        v += __shfl_xor(static_cast<unsigned long long>(v), step, 64);
+    }
+    return v;
 }
 
 // A listed token at which sums reach a goal.
@@ -580,16 +604,11 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
             const uint64_t key = lane < left ? s.few[lane] : 0u, mine = lane < left ? weight_of(key) : 0u;
             uint64_t above = before;
             for (uint32_t i = 0; i < left; ++i) {
-                const uint64_t other = s.few[i];
-                const uint32_t weight_low = __builtin_amdgcn_readlane(uint32_t(mine), i), weight_high = __builtin_amdgcn_readlane(uint32_t(mine >> 32), i);
-                above += other > key ? uint64_t(weight_high) << 32 | weight_low : 0u;
+                above += lane_u64(key, i) > key ? lane_u64(mine, i) : 0u;
             }
-            const unsigned long long here = __ballot(lane < left && above < goal && above + mine >= goal);
-            const uint32_t at = here ? __builtin_ctzll(here) : 0u;  // (one lane)
+            const uint32_t at = __builtin_ctzll(__ballot(lane < left && above < goal && above + mine >= goal) | 1ull << 63);  // (one lane)
             __syncthreads();  // s.few and s.waves have been read
-            return Listed{uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(key >> 32), at))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(key), at)),
-                          uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(above >> 32), at))) << 32 |
-                              uint32_t(__builtin_amdgcn_readlane(uint32_t(above), at))};
+            return Listed{lane_u64(key, at), lane_u64(above, at)};
         }
         const int bits = 64 - __builtin_clzll(most ^ least), shift = bits > 11 ? bits - 11 : 0;
         for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
@@ -624,7 +643,7 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
 }
 
 // Lists the tokens of [begin, end): s.listed of them, the first kList to come in s.list.
-template <class T> __device__ void gather(const Settings& set, const Listing& l, const T* x, uint32_t begin, uint32_t end, Shared& s) {
+template <class T, class S> __device__ void gather(const Settings& set, const Listing& l, const T* x, uint32_t begin, uint32_t end, S& s) {
     if (threadIdx.x == 0u) {
         s.listed = 0u;
     }
@@ -639,6 +658,35 @@ template <class T> __device__ void gather(const Settings& set, const Listing& l,
         }
     });
     __syncthreads();
+}
+
+// The token of a row that a top-k cuts to what the first ``n`` <= 64 of ``keys`` hold, by each wave alone.
+__device__ void choose_few(const Call& c, uint64_t r, const Settings& set, const Weights& w, const uint64_t* keys, uint32_t n) {
+    const uint32_t lane = threadIdx.x % 64u;
+    const uint64_t key = lane < n ? keys[lane] : 0u, all = lane < n ? w(value_of(uint32_t(key >> 32))) : 0u;
+    uint32_t rank = 0;
+    uint64_t above = 0;  // weights of larger keys
+    for (uint32_t i = 0; i < n; ++i) {
+        const bool larger = lane_u64(key, i) > key;
+        above += larger ? lane_u64(all, i) : 0u;
+        rank += larger ? 1u : 0u;
+    }
+    const uint64_t mine = rank < uint64_t(set.top_k) ? all : 0u;
+    const auto at = [&](uint64_t goal) { return __builtin_ctzll(__ballot(above < goal && above + mine >= goal) | 1ull << 63); };
+    uint64_t kept = wave_total(mine);
+    if (set.top_p < 1.0f) {
+        kept = lane_u64(above + mine, at(set.nucleus(kept)));
+    }
+    if (set.min_p > 0.0f) {
+        kept = lesser(kept, greater(wave_total(mine >= set.least() ? mine : 0u), kWhole));
+    }
+    const uint64_t drawn = lane_u64(key, at(set.place(kept)));
+    if (threadIdx.x == 0u) {
+        c.ids[r] = int64_t(0xffffffffu - uint32_t(drawn));
+        if (c.logprobs) {
+            c.logprobs[r] = set.logprob(w, value_of(uint32_t(drawn >> 32)), kept);
+        }
+    }
 }
 
 // The token, from the ``n`` listed keys in s.list; ``below(b)``: the histogram's sums before bucket b.
@@ -673,22 +721,38 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
     uint64_t kept;
     Listed drawn;
     if (l.by_count) {
+        if (n <= 64u) {
+            choose_few(c, r, set, w, s.list, n);
+            return;
+        }
         // (fewer are listed where the top-k takes tokens that weigh nothing)
         const uint64_t last = n > uint64_t(set.top_k) ? reach_list(w, s, n, true, 0u, uint64_t(set.top_k), 0u, ~0ull).key : 0u;
+        if (threadIdx.x == 0u) {
+            s.fews = 0u;
+        }
+        __syncthreads();
         Sums own{0u, 0u};
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            own.weight += s.list[i] >= last ? weight_of(s.list[i]) : 0u;
+            if (s.list[i] >= last) {
+                own.weight += weight_of(s.list[i]);
+                if (set.top_k <= 64) {
+                    s.few[atomicAdd(&s.fews, 1u)] = s.list[i];
+                }
+            }
         }
         kept = sum_all(s, own).weight;
+        if (set.top_k <= 64) {
+            choose_few(c, r, set, w, s.few, uint32_t(set.top_k));
+            return;
+        }
         if (set.top_p < 1.0f) {
-            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), 0u, ~0ull);
+            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), last, ~0ull);
             kept = cut.before + weight_of(cut.key);
         }
         if (set.min_p > 0.0f) {
-            const uint64_t high = at_least(set.least(), 0u, kBuckets);
-            kept = lesser(kept, greater(high, kWhole));
+            kept = lesser(kept, greater(at_least(set.least(), 0u, kBuckets), kWhole));
         }
-        drawn = reach_list(w, s, n, false, 0u, set.place(kept), 0u, ~0ull);
+        drawn = reach_list(w, s, n, false, 0u, set.place(kept), last, ~0ull);
     } else {
         kept = below(kBuckets);
         if (set.top_p < 1.0f) {
@@ -750,7 +814,7 @@ struct Scratch {
     uint64_t* before;     // [kBuckets + 1]
     uint64_t* list;       // [kList]
     Listing* listing;
-    uint32_t* tickets;  // workgroups that are done with the histogram, with the list; listed tokens
+    uint32_t* tickets;  // workgroups that are done with the histogram; listed tokens
     static __host__ __device__ uint64_t words(uint64_t spans) { return spans * (1u + kBuckets) + kBuckets + 1u + kList + 8u; }
     __device__ Scratch(uint64_t* base, uint64_t r, uint32_t spans) {
         best = base + r * words(spans);
@@ -773,7 +837,7 @@ struct Span {
 };
 
 // The first reading: each span's largest logit. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads) sample_best(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_best(Call c, uint64_t* scratch) {
     __shared__ Shared s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
@@ -784,7 +848,6 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_best(Call 
         if (blockIdx.x == 0u) {
             mine.tickets[0] = 0u;
             mine.tickets[1] = 0u;
-            mine.tickets[2] = 0u;
         }
     }
 }
@@ -811,7 +874,7 @@ __device__ bool comes_last(uint32_t* ticket, Shared& s) {
 }
 
 // The second reading: the histogram, and what is listed. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(Call c, uint64_t* scratch) {
     __shared__ Shared s;
     s.powers.fill();
     const uint64_t r = blockIdx.y;
@@ -858,45 +921,46 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_depths(Cal
     }
 }
 
-// The third reading: the list, and the token. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads) sample_listed(Call c, uint64_t* scratch) {
-    __shared__ Shared s;
-    s.powers.fill();
+// The third reading: the list. grid: (spans, rows)
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_listed(Call c, uint64_t* scratch) {
+    __shared__ Gathered s;
     const uint64_t r = blockIdx.y;
-    const uint32_t spans = gridDim.x;
+    const Scratch mine(scratch, r, gridDim.x);
+    const Settings set(c, r, best_of(mine, gridDim.x));
+    const Listing l = *mine.listing;
+    if (set.greedy() || l.whole) {
+        return;
+    }
+    const Span span(c, gridDim.x, blockIdx.x);
+    gather(set, l, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), span.begin, span.end, s);
+    if (threadIdx.x == 0u) {
+        s.begin = atomicAdd(mine.tickets + 1, s.listed);
+    }
+    __syncthreads();
+    const uint32_t begin = s.begin, own = min(s.listed, kList);
+    for (uint32_t i = threadIdx.x; i < own && begin + i < kList; i += kThreads) {
+        mine.list[begin + i] = s.list[i];
+    }
+}
+
+// The token. grid: rows
+template <class T> __global__ void __launch_bounds__(kThreads) sample_token(Call c, uint64_t* scratch, uint32_t spans) {
+    __shared__ Shared s;
+    const uint64_t r = blockIdx.x;
     const Scratch mine(scratch, r, spans);
     const Settings set(c, r, best_of(mine, spans));
     if (set.greedy()) {
         return;
     }
-    const T* x = static_cast<const T*>(c.x) + r * uint64_t(c.x_stride);
+    s.powers.fill();
     const Listing l = *mine.listing;
-    if (l.whole) {
-        if (blockIdx.x == 0u) {
-            descend_row(c, r, set, x, s);
-        }
-        return;
-    }
-    const Span span(c, spans, blockIdx.x);
-    gather(set, l, x, span.begin, span.end, s);
-    if (threadIdx.x == 0u) {
-        s.last = __hip_atomic_fetch_add(mine.tickets + 2, s.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    const uint32_t begin = s.last, own = min(s.listed, kList);
-    for (uint32_t i = threadIdx.x; i < own && begin + i < kList; i += kThreads) {
-        chroma::store_device(mine.list + begin + i, s.list[i]);
-    }
-    if (!comes_last(mine.tickets + 1, s)) {
-        return;
-    }
-    const uint32_t n = chroma::load_device(mine.tickets + 2);
-    if (n > kList) {
-        descend_row(c, r, set, x, s);
+    const uint32_t n = mine.tickets[1];
+    if (l.whole || n > kList) {
+        descend_row(c, r, set, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), s);
         return;
     }
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        s.list[i] = chroma::load_device(mine.list + i);
+        s.list[i] = mine.list[i];
     }
     __syncthreads();
     choose(c, r, set, l, n, [&](uint32_t b) { return mine.before[b]; }, s);
@@ -918,6 +982,7 @@ template <class T> void launch(const Call& c, uint64_t* scratch, hipStream_t str
     sample_best<T><<<grid, kThreads, 0, stream>>>(c, scratch);
     sample_depths<T><<<grid, kThreads, 0, stream>>>(c, scratch);
     sample_listed<T><<<grid, kThreads, 0, stream>>>(c, scratch);
+    sample_token<T><<<unsigned(c.rows), kThreads, 0, stream>>>(c, scratch, spans);
 }
 
 int refuse(const char* message, char* error, size_t size) {
