@@ -31,7 +31,7 @@ using Call = chroma_hip_sample_call;
 
 constexpr int kOne = 44;                        // a weight of 1 is 2^kOne
 constexpr uint64_t kWhole = uint64_t(1) << kOne;
-constexpr uint32_t kThreads = 1024, kBuckets = 2048;
+constexpr uint32_t kThreads = 512, kBuckets = 2048, kPer = kBuckets / kThreads;
 constexpr uint32_t kList = 4096;   // listed tokens of a row
 constexpr int64_t kMostTop = 1024;  // a larger top_k descends on the whole row
 constexpr float kDepths = 44.0f;   // buckets of the histogram for a factor of 2; the last one holds what weighs nothing
@@ -142,29 +142,55 @@ struct Shared {
     uint32_t listed, last, fews;
 };
 
-__device__ __forceinline__ uint32_t wave_count(uint32_t v) {
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        v += __shfl_xor(v, step, 64);
-    }
-    return v;
-}
-
 // LDS of a workgroup that only lists.
 struct Gathered {
     uint64_t list[kList];
     uint32_t listed, begin;
 };
 
+// Running sums over a wave's lanes without LDS: DPP shifts inside rows of 16 lanes, then the last lane of the rows before.
+// (A shift's lanes without a source receive 0.)
+template <int Control, int Rows> __device__ __forceinline__ uint32_t dpp_from(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), Control, Rows, 0xF, false));
+}
+template <int Control, int Rows> __device__ __forceinline__ uint64_t dpp_from(uint64_t v) {
+    return uint64_t(dpp_from<Control, Rows>(uint32_t(v >> 32))) << 32 | dpp_from<Control, Rows>(uint32_t(v));
+}
+template <class V> __device__ __forceinline__ V wave_scan(V v) {
+    v += dpp_from<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_from<0x112, 0xF>(v);
+    v += dpp_from<0x114, 0xF>(v);
+    v += dpp_from<0x118, 0xF>(v);
+    v += dpp_from<0x142, 0xA>(v);  // row_bcast 15: rows 1 and 3
+    v += dpp_from<0x143, 0xC>(v);  // row_bcast 31: rows 2 and 3
+    return v;
+}
+// The largest of a wave's values, in all lanes (lanes without a source see 0, which is no larger).
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    const auto with = [&](uint32_t other) { v = other > v ? other : v; };
+    with(dpp_from<0x111, 0xF>(v));
+    with(dpp_from<0x112, 0xF>(v));
+    with(dpp_from<0x114, 0xF>(v));
+    with(dpp_from<0x118, 0xF>(v));
+    with(dpp_from<0x142, 0xA>(v));
+    with(dpp_from<0x143, 0xC>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(v), lane));
+}
+__device__ __forceinline__ uint64_t wave_total(uint64_t v) { return lane_u64(wave_scan(v), 63u); }
+// The largest: by the high words, then by the low words of those that have the largest one.
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+    const uint32_t high = wave_max(uint32_t(v >> 32)), low = wave_max(uint32_t(v >> 32) == high ? uint32_t(v) : 0u);
+    return uint64_t(high) << 32 | low;
+}
+
 // Sums over the workgroup.
 __device__ Sums sum_all(Shared& s, Sums own) {
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        own.weight += __shfl_xor(static_cast<unsigned long long>(own.weight), step, 64);
-        own.count += __shfl_xor(own.count, step, 64);
-    }
+    const Sums wave{wave_total(own.weight), uint32_t(__builtin_amdgcn_readlane(wave_scan(own.count), 63))};
     if (threadIdx.x % 64u == 0u) {
-        s.waves[threadIdx.x / 64u] = own;
+        s.waves[threadIdx.x / 64u] = wave;
     }
     __syncthreads();
     Sums sum{0u, 0u};
@@ -179,7 +205,7 @@ __device__ Sums sum_all(Shared& s, Sums own) {
 
 // The largest of the workgroup's values.
 __device__ uint64_t max_all(Shared& s, uint64_t own) {
-    own = chroma::wave_max_u64(own);
+    own = wave_max(own);
     if (threadIdx.x % 64u == 0u) {
         s.waves[threadIdx.x / 64u].weight = own;
     }
@@ -195,20 +221,16 @@ __device__ uint64_t max_all(Shared& s, uint64_t own) {
 // Inclusive sums over the workgroup's threads, in their order.
 __device__ Sums scan_all(Shared& s, Sums own) {
     const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        const uint64_t weight = __shfl_up(static_cast<unsigned long long>(own.weight), step, 64);
-        const uint32_t count = __shfl_up(own.count, step, 64);
-        own.weight += lane >= uint32_t(step) ? weight : 0u;
-        own.count += lane >= uint32_t(step) ? count : 0u;
-    }
+    own.weight = wave_scan(own.weight);
+    own.count = wave_scan(own.count);
     if (lane == 63u) {
         s.waves[wave] = own;
     }
     __syncthreads();
-    for (uint32_t v = 0; v < wave; ++v) {
-        own.weight += s.waves[v].weight;
-        own.count += s.waves[v].count;
+#pragma unroll
+    for (uint32_t v = 0; v + 1u < kThreads / 64u; ++v) {
+        own.weight += v < wave ? s.waves[v].weight : 0u;
+        own.count += v < wave ? s.waves[v].count : 0u;
     }
     __syncthreads();
     return own;
@@ -503,11 +525,19 @@ __device__ uint32_t bucket_of(Shared& s, uint64_t goal) {
 
 // From the row's histogram in s.weight: its running sums in s.before, and what is listed.
 __device__ Listing list_of(const Settings& set, Shared& s) {
-    const uint32_t first = threadIdx.x * 2u;
-    const uint64_t one = s.weight[first], two = s.weight[first + 1u];
-    const uint64_t upto = scan_all(s, Sums{one + two, 0u}).weight;
-    s.before[first] = upto - one - two;
-    s.before[first + 1u] = upto - two;
+    const uint32_t first = threadIdx.x * kPer;
+    uint64_t own = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kPer; ++k) {
+        own += s.weight[first + k];
+    }
+    const uint64_t upto = scan_all(s, Sums{own, 0u}).weight;
+    uint64_t sum = upto - own;
+#pragma unroll
+    for (uint32_t k = 0; k < kPer; ++k) {
+        s.before[first + k] = sum;
+        sum += s.weight[first + k];
+    }
     if (threadIdx.x == kThreads - 1u) {
         s.before[kBuckets] = upto;
     }
@@ -542,17 +572,6 @@ __device__ Listing list_of(const Settings& set, Shared& s) {
     return l;
 }
 
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t lane) {
-    return uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(v), lane));
-}
-__device__ __forceinline__ uint64_t wave_total(uint64_t v) {
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        v += __shfl_xor(static_cast<unsigned long long>(v), step, 64);
-    }
-    return v;
-}
-
 // A listed token at which sums reach a goal.
 struct Listed {
     uint64_t key, before;  // before: the sum of weights (or the count) of the tokens before it
@@ -577,9 +596,9 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
                 ++left;
             }
         }
-        most = chroma::wave_max_u64(most);
-        least = chroma::wave_max_u64(least);
-        left = wave_count(left);
+        most = wave_max(most);
+        least = wave_max(least);
+        left = uint32_t(__builtin_amdgcn_readlane(wave_scan(left), 63));
         if (lane == 0u) {
             s.waves[wave] = Sums{most, left};
             s.ends[wave] = least;
@@ -622,15 +641,21 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
             }
         }
         __syncthreads();
-        const uint32_t top = kBuckets - 1u - threadIdx.x * 2u;
-        const uint64_t one = s.weight[top], two = s.weight[top - 1u];
-        const uint64_t at = before + scan_all(s, Sums{one + two, 0u}).weight - one - two;
-        if (at < goal && at + one >= goal) {
-            s.found.order = top;
-            s.found.before.weight = at;
-        } else if (at + one < goal && at + one + two >= goal) {
-            s.found.order = top - 1u;
-            s.found.before.weight = at + one;
+        const uint32_t top = kBuckets - 1u - threadIdx.x * kPer;
+        uint64_t own = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {
+            own += s.weight[top - k];
+        }
+        uint64_t at = before + scan_all(s, Sums{own, 0u}).weight - own;
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {
+            const uint64_t next = at + s.weight[top - k];
+            if (at < goal && next >= goal) {  // one thread
+                s.found.order = top - k;
+                s.found.before.weight = at;
+            }
+            at = next;
         }
         __syncthreads();
         before = s.found.before.weight;
@@ -825,7 +850,7 @@ struct Scratch {
         tickets = reinterpret_cast<uint32_t*>(list + kList + 4u);
     }
 };
-static_assert(sizeof(Listing) <= 32 && kBuckets == 2 * kThreads, "scratch and running sums");
+static_assert(sizeof(Listing) <= 32, "scratch");
 
 struct Span {
     uint32_t begin, end;
@@ -837,7 +862,7 @@ struct Span {
 };
 
 // The first reading: each span's largest logit. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_best(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_best(Call c, uint64_t* scratch) {
     __shared__ Shared s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
@@ -857,7 +882,7 @@ __device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
     for (uint32_t i = threadIdx.x % 64u; i < spans; i += 64u) {
         best = greater(best, mine.best[i]);
     }
-    return chroma::wave_max_u64(best);
+    return wave_max(best);
 }
 
 // Whether this workgroup is the last of the row's to come here, after its device-scope stores.
@@ -874,7 +899,7 @@ __device__ bool comes_last(uint32_t* ticket, Shared& s) {
 }
 
 // The second reading: the histogram, and what is listed. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_depths(Call c, uint64_t* scratch) {
     __shared__ Shared s;
     s.powers.fill();
     const uint64_t r = blockIdx.y;
@@ -922,7 +947,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(
 }
 
 // The third reading: the list. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_listed(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_listed(Call c, uint64_t* scratch) {
     __shared__ Gathered s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
@@ -966,9 +991,11 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_token(Call
     choose(c, r, set, l, n, [&](uint32_t b) { return mine.before[b]; }, s);
 }
 
-// Spans of a row: workgroups that fill the chip twice, of 8192 tokens at least; 1: one launch of a workgroup a row.
+// Spans of a row, of 8192 tokens at least: two workgroups for each compute unit and four for a row; 1: one launch of a
+// workgroup a row. 64 rows of 201088 bfloat16 logits cut to 50 tokens: 8 spans 39 us, 16 48, 32 (of 4096) 80; 256 rows with
+// settings of their own: 2 spans 152 us, 4 123, 8 131. Thousands of rows fill the chip by themselves.
 uint32_t spans_of(const Call& c) {
-    const int64_t wanted = 512 / c.rows, most = c.width / 8192;
+    const int64_t wanted = c.rows > 2048 ? 1 : c.rows >= 128 ? 4 : 512 / c.rows, most = c.width / 8192;
     return uint32_t(wanted < 2 || most < 2 ? 1 : wanted < most ? wanted : most);
 }
 
