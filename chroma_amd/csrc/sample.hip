@@ -128,18 +128,21 @@ struct Place {
     __device__ __forceinline__ uint64_t weight() const { return before.weight + each * ties; }
 };
 
-// LDS of a workgroup.
-struct Shared {
+// LDS of a workgroup that takes a histogram, and of one that draws.
+struct Depths {
     uint64_t weight[kBuckets];
     uint64_t before[kBuckets + 1];  // sums before each bucket, and of all
     uint32_t count[kBuckets];
-    uint64_t list[kList];           // selection keys
     Powers powers;
-    uint64_t few[64];
     Sums waves[kThreads / 64u];
+    uint32_t last;
+};
+struct Shared : Depths {
+    uint64_t list[kList];  // selection keys
+    uint64_t few[64];
     uint64_t ends[kThreads / 64u];
     Place found;
-    uint32_t listed, last, fews;
+    uint32_t listed, fews;
 };
 
 // LDS of a workgroup that only lists.
@@ -187,7 +190,7 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 }
 
 // Sums over the workgroup.
-__device__ Sums sum_all(Shared& s, Sums own) {
+__device__ Sums sum_all(Depths& s, Sums own) {
     const Sums wave{wave_total(own.weight), uint32_t(__builtin_amdgcn_readlane(wave_scan(own.count), 63))};
     if (threadIdx.x % 64u == 0u) {
         s.waves[threadIdx.x / 64u] = wave;
@@ -204,7 +207,7 @@ __device__ Sums sum_all(Shared& s, Sums own) {
 }
 
 // The largest of the workgroup's values.
-__device__ uint64_t max_all(Shared& s, uint64_t own) {
+__device__ uint64_t max_all(Depths& s, uint64_t own) {
     own = wave_max(own);
     if (threadIdx.x % 64u == 0u) {
         s.waves[threadIdx.x / 64u].weight = own;
@@ -219,7 +222,7 @@ __device__ uint64_t max_all(Shared& s, uint64_t own) {
 }
 
 // Inclusive sums over the workgroup's threads, in their order.
-__device__ Sums scan_all(Shared& s, Sums own) {
+__device__ Sums scan_all(Depths& s, Sums own) {
     const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
     own.weight = wave_scan(own.weight);
     own.count = wave_scan(own.count);
@@ -270,7 +273,7 @@ template <class T, class F> __device__ __forceinline__ void visit(const T* x, ui
 }
 
 // The largest logit's order and the lowest id that has it, as a selection key, of [begin, end).
-template <class T> __device__ uint64_t largest(Shared& s, const T* x, uint32_t begin, uint32_t end) {
+template <class T> __device__ uint64_t largest(Depths& s, const T* x, uint32_t begin, uint32_t end) {
     uint32_t best = 0, id = 0xffffffffu;
     visit(x, begin, end, [&](float v, uint32_t i) {
         const uint32_t order = order_of(v);
@@ -408,7 +411,7 @@ struct Settings {
             c.logprobs[r] = nan ? __builtin_nanf("") : nothing ? top : 0.0f;
         }
     }
-    __device__ __forceinline__ Weights weights(const Shared& s) const { return Weights(s.powers, top, temperature); }
+    __device__ __forceinline__ Weights weights(const Depths& s) const { return Weights(s.powers, top, temperature); }
     // The histogram's bucket of a logit: it never falls as the logit falls. (Halves: the difference itself may overflow.)
     __device__ __forceinline__ uint32_t bucket(float x, float rate) const {
         const float t = x == top ? 0.0f : (0.5f * top - 0.5f * x) * rate;
@@ -480,7 +483,7 @@ constexpr uint32_t kNone = 0x7fffffffu;
 
 // The histogram of [begin, end) in s.weight: weights, or counts where a top-k cuts the row; the last bucket's are left out (its
 // tokens weigh nothing, and most of a row may lie there).
-template <class T> __device__ void depths(const Settings& set, const T* x, uint32_t begin, uint32_t end, Shared& s) {
+template <class T> __device__ void depths(const Settings& set, const T* x, uint32_t begin, uint32_t end, Depths& s) {
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
         s.weight[i] = 0u;
         s.count[i] = 0u;
@@ -511,7 +514,7 @@ template <class T> __device__ void depths(const Settings& set, const T* x, uint3
 }
 
 // The bucket in which the sums reach ``goal``, from 1 to all there is.
-__device__ uint32_t bucket_of(Shared& s, uint64_t goal) {
+__device__ uint32_t bucket_of(Depths& s, uint64_t goal) {
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
         if (s.before[i] < goal && s.before[i + 1u] >= goal) {
             s.last = i;
@@ -524,7 +527,7 @@ __device__ uint32_t bucket_of(Shared& s, uint64_t goal) {
 }
 
 // From the row's histogram in s.weight: its running sums in s.before, and what is listed.
-__device__ Listing list_of(const Settings& set, Shared& s) {
+__device__ Listing list_of(const Settings& set, Depths& s) {
     const uint32_t first = threadIdx.x * kPer;
     uint64_t own = 0;
 #pragma unroll
@@ -863,7 +866,7 @@ struct Span {
 
 // The first reading: each span's largest logit. grid: (spans, rows)
 template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_best(Call c, uint64_t* scratch) {
-    __shared__ Shared s;
+    __shared__ Depths s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
     const Span span(c, gridDim.x, blockIdx.x);
@@ -886,7 +889,7 @@ __device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
 }
 
 // Whether this workgroup is the last of the row's to come here, after its device-scope stores.
-__device__ bool comes_last(uint32_t* ticket, Shared& s) {
+__device__ bool comes_last(uint32_t* ticket, Depths& s) {
     chroma::device_stores_complete();
     __syncthreads();
     if (threadIdx.x == 0u) {
@@ -900,7 +903,7 @@ __device__ bool comes_last(uint32_t* ticket, Shared& s) {
 
 // The second reading: the histogram, and what is listed. grid: (spans, rows)
 template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_depths(Call c, uint64_t* scratch) {
-    __shared__ Shared s;
+    __shared__ Depths s;
     s.powers.fill();
     const uint64_t r = blockIdx.y;
     const uint32_t spans = gridDim.x;
