@@ -184,6 +184,9 @@ class Codegen:
     def paged_attention(self, meta: torch.Tensor, *operands) -> Value:
         raise NotImplementedError(f"paged attention on the {self.backend} backend")
 
+    def paged_chunk_attention(self, meta: torch.Tensor, *operands) -> Value:
+        raise NotImplementedError(f"paged chunk attention on the {self.backend} backend")
+
 
 def literal(value: float) -> str:
     """A C++ float literal that round-trips ``value`` through float32."""

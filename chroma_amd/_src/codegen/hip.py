@@ -2467,38 +2467,8 @@ class HIPCodegen(Codegen):
         pages, rows = k_pages.shape[:2]
         if dim % 8 or dim > 256 or group > 1024 or max(sequences, kv_heads) > 65535:
             raise NotImplementedError(f"paged attention of {sequences} sequences, {kv_heads} KV heads of {group} heads of {dim}")
+        out, plan, kernel = self._paged_operands(meta, "PagedOperands", q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, scale, window, first)
         item = ITEMSIZE[meta.dtype]
-        chunk = 16 // item
-
-        def in_place(value: Value) -> Value:
-            """``value`` where its rows can be read as they lie, else a row-major copy."""
-            stored, strides = self._in_place(value)
-            if stored is not None:
-                offset = stored.view.offset if stored.view.base is not None else 0
-                strides = [0 if size == 1 else stride for size, stride in zip(value.shape, strides)]
-                if (dim == 1 or strides[-1] == 1) and not any(x % chunk for x in [*strides[:-1], offset]):
-                    return value
-            return rows_of(value)
-
-        def rows_of(value: Value) -> Value:
-            """A row-major ``value`` that starts on 16 bytes."""
-            value = self.contiguous(value)
-            if value.view.base is not None and value.view.offset % chunk:
-                copied = self.allocate(value.shape, value.dtype)
-                self.map_kernel(copied, value)
-                return copied
-            return value
-
-        # K and V lie alike (strides of K serve both); q's and the new rows' heads are adjacent
-        k_pages, v_pages = in_place(k_pages), in_place(v_pages)
-        if list(self._operand(k_pages, k_pages.shape)[1]) != list(self._operand(v_pages, v_pages.shape)[1]):
-            k_pages, v_pages = rows_of(k_pages), rows_of(v_pages)
-        q, k_new, v_new = (None if value is None else rows_of(value) for value in (q, k_new, v_new))
-        table, lengths, sinks = (None if value is None else self.contiguous(value) for value in (table, lengths, sinks))
-        out = self.allocate(tuple(meta.shape), meta.dtype)
-        operands = {"q": q, "k": k_pages, "v": v_pages, "k_new": k_new, "v_new": v_new, "sinks": sinks, "table": table, "lengths": lengths}
-        plan = {name: self._operand(value, value.shape) for name, value in operands.items() if value is not None}
-        page_stride, row_stride, head_stride, _ = plan["k"][1]
         longest = table.shape[1] * rows
         most = 2**31 - 1
         if sequences * (longest // 16 + 2) > most or pages > most or longest > most - 4096 or sequences * kv_heads * group > 2**24:
@@ -2506,24 +2476,6 @@ class HIPCodegen(Codegen):
         ctype = ctype_of(meta.dtype)
         padded, keys, half, waves = self._paged_keys(dim, item)
         tiles = -(-group // 16)
-
-        def kernel() -> Kernel:
-            k = Kernel(1)
-            k.line(f"chroma::PagedOperands<{ctype}> a;")
-            slot = k.slot(out.name, out.dtype, writable=True, extent=self.extents[out.name])
-            k.line(f"a.out = {slot}; a.out_stride = {kv_heads * group * dim}u;")
-            for name in operands:
-                if name not in plan:
-                    k.line(f"a.{name} = nullptr;")
-                    continue
-                value, _, offset = plan[name]
-                base = k.slot(value.root.name, value.root.dtype, extent=self.extents[value.root.name])
-                k.line(f"a.{name} = {base} + {offset}ull;")
-            k.line(f"a.page_stride = {page_stride}ull; a.row_stride = {row_stride}ull; a.head_stride = {head_stride}ull;")
-            k.line(f"a.q_stride = {kv_heads * group * dim}u; a.new_stride = {kv_heads * dim}u; a.table_stride = {table.shape[1]}u;")
-            k.line(f"a.pages = {pages}u; a.page_rows = {rows}u; a.longest = {longest}u; a.window = {min(window, most)}u; a.first = {min(first, most)}u;")
-            k.line(f"a.sequences = {sequences}u; a.kv_heads = {kv_heads}u; a.group = {group}u; a.dim = {dim}u; a.scale = {float_literal(scale)};")
-            return k
 
         def most_blocks(size: int) -> int:
             blocks = -(-(longest + 1) // size)
@@ -2551,6 +2503,138 @@ class HIPCodegen(Codegen):
                     stream = str(tiles == 1 and dim * item % 128 == 0).lower()
                     k.line(f"chroma::attention_paged_shares<{ctype}, {padded}, {keys}u, {stream}>(a, {ranges}u, {scratch});")
                     self.launch(k, (-(-ranges * kv_heads * tiles // 4), 1, 1), 256, inputs, kind="attention_paged")
+        self.fused_attentions += 1
+        return out
+
+    def _paged_operands(self, meta, struct: str, q: Value, k_pages: Value, v_pages: Value, k_new: Optional[Value], v_new: Optional[Value],
+                        table: Value, lengths: Value, sinks: Optional[Value], scale: float, window: int, first: int, starts: Optional[Value] = None):
+        """(result, {operand: (value, strides, offset)}, a kernel that holds them as ``a`` of the struct) of attention over a
+        paged cache; q is [rows, KV heads, group, dim], a row for each sequence or, with ``starts``, for each token."""
+        kv_heads, group, dim = q.shape[1:]
+        pages, rows = k_pages.shape[:2]
+        item = ITEMSIZE[meta.dtype]
+        chunk = 16 // item
+
+        def in_place(value: Value) -> Value:
+            """``value`` where its rows can be read as they lie, else a row-major copy."""
+            stored, strides = self._in_place(value)
+            if stored is not None:
+                offset = stored.view.offset if stored.view.base is not None else 0
+                strides = [0 if size == 1 else stride for size, stride in zip(value.shape, strides)]
+                if (dim == 1 or strides[-1] == 1) and not any(x % chunk for x in [*strides[:-1], offset]):
+                    return value
+            return rows_of(value)
+
+        def rows_of(value: Value) -> Value:
+            """A row-major ``value`` that starts on 16 bytes."""
+            value = self.contiguous(value)
+            if value.view.base is not None and value.view.offset % chunk:
+                copied = self.allocate(value.shape, value.dtype)
+                self.map_kernel(copied, value)
+                return copied
+            return value
+
+        # K and V lie alike (strides of K serve both); q's and the new rows' heads are adjacent
+        k_pages, v_pages = in_place(k_pages), in_place(v_pages)
+        if list(self._operand(k_pages, k_pages.shape)[1]) != list(self._operand(v_pages, v_pages.shape)[1]):
+            k_pages, v_pages = rows_of(k_pages), rows_of(v_pages)
+        q, k_new, v_new = (None if value is None else rows_of(value) for value in (q, k_new, v_new))
+        table, lengths, sinks, starts = (None if value is None else self.contiguous(value) for value in (table, lengths, sinks, starts))
+        out = self.allocate(tuple(meta.shape), meta.dtype)
+        operands = {"q": q, "k": k_pages, "v": v_pages, "k_new": k_new, "v_new": v_new, "sinks": sinks, "table": table, "lengths": lengths}
+        if starts is not None:
+            operands["starts"] = starts
+        plan = {name: self._operand(value, value.shape) for name, value in operands.items() if value is not None}
+        page_stride, row_stride, head_stride, _ = plan["k"][1]
+        ctype, most = ctype_of(meta.dtype), 2**31 - 1
+
+        def kernel() -> Kernel:
+            k = Kernel(1)
+            k.line(f"chroma::{struct}<{ctype}> a;")
+            slot = k.slot(out.name, out.dtype, writable=True, extent=self.extents[out.name])
+            k.line(f"a.out = {slot}; a.out_stride = {kv_heads * group * dim}u;")
+            for name in operands:
+                if name not in plan:
+                    k.line(f"a.{name} = nullptr;")
+                    continue
+                value, _, offset = plan[name]
+                base = k.slot(value.root.name, value.root.dtype, extent=self.extents[value.root.name])
+                k.line(f"a.{name} = {base} + {offset}ull;")
+            k.line(f"a.page_stride = {page_stride}ull; a.row_stride = {row_stride}ull; a.head_stride = {head_stride}ull;")
+            k.line(f"a.q_stride = {kv_heads * group * dim}u; a.new_stride = {kv_heads * dim}u; a.table_stride = {table.shape[1]}u;")
+            k.line(f"a.pages = {pages}u; a.page_rows = {rows}u; a.longest = {table.shape[1] * rows}u; a.window = {min(window, most)}u; "
+                   f"a.first = {min(first, most)}u;")
+            k.line(f"a.sequences = {lengths.shape[0]}u; a.kv_heads = {kv_heads}u; a.group = {group}u; a.dim = {dim}u; a.scale = {float_literal(scale)};")
+            if starts is not None:
+                k.line(f"a.tokens = {q.shape[0]}u;")
+            return k
+
+        return out, plan, kernel
+
+    @classmethod
+    def chunk_cut(cls, tokens: int, sequences: int, kv_heads: int, group: int, dim: int, item: int, longest: int, fresh: bool, window: int,
+                  first: int) -> Tuple[int, int, int]:
+        """(waves of a tile of 32 rows each, or 0 for tiles of 16 rows; tiles; workgroups a tile) of attention of chunks:
+        ``cut_of`` of csrc/chunk.hip, which says what each way measured."""
+        padded, _, half, waves = cls._paged_keys(dim, item)
+        rows = longest + (tokens if fresh else 0)
+
+        def tiles_of(size: int) -> int:
+            return tokens * group // size + min(sequences, tokens)
+
+        def most_blocks(keys: int) -> int:
+            blocks = -(-rows // keys) + 1
+            return min(blocks, (min(first, rows) + min(window, rows)) // keys + 3) if window else blocks
+
+        if item != 2 or tokens * group < 64 * sequences or tokens * group * kv_heads < 128 * 64:
+            wide = 0
+        else:
+            wide = 8 if padded == 128 and tiles_of(256) * kv_heads >= 512 else 4
+        tiles = tiles_of(32 * wide if wide else 16)
+        wanted = -(-512 // (tiles * kv_heads))
+        most = most_blocks(32 if padded > 128 else 64) // 4 if wide else most_blocks(half) // (2 * waves)
+        return wide, tiles, max(1, min(wanted, most))
+
+    def paged_chunk_attention(self, meta, q: Value, k_pages: Value, v_pages: Value, k_new: Optional[Value], v_new: Optional[Value], table: Value,
+                              lengths: Value, starts: Value, sinks: Optional[Value], scale: float, window: int, first: int) -> Value:
+        """Attention of a chunk of new tokens of every sequence over a paged cache (``chroma_amd::paged_chunk_attention``), cut as
+        ``chroma_hip_paged_chunk_attention`` cuts its calls; rows of no sequence are cleared first."""
+        tokens, kv_heads, group, dim = q.shape
+        sequences, longest = lengths.shape[0], table.shape[1] * k_pages.shape[1]
+        if dim % 8 or dim > 256 or group > 1024 or max(sequences, kv_heads) > 65535:
+            raise NotImplementedError(f"paged attention of {tokens} tokens of {sequences} sequences, {kv_heads} KV heads of {group} heads of {dim}")
+        if tokens > 2**24 or tokens * kv_heads * group >= 2**30 or sequences * kv_heads > 2**24 or k_pages.shape[0] >= 2**31 or longest + tokens >= 2**31 - 4096:
+            raise NotImplementedError("paged attention of more rows than the kernels count")
+        out, plan, kernel = self._paged_operands(meta, "ChunkOperands", q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, scale, window, first,
+                                                 starts)
+        item, ctype = ITEMSIZE[meta.dtype], ctype_of(meta.dtype)
+        padded, _, half, few = self._paged_keys(dim, item)
+        waves, tiles, splits = self.chunk_cut(tokens, sequences, kv_heads, group, dim, item, longest, k_new is not None, window, first)
+        rows = 32 * waves if waves else 16
+        inputs = [entry[0] for entry in plan.values()]
+        k = Kernel(1)
+        slot = k.slot(out.name, out.dtype, writable=True, extent=self.extents[out.name])
+        units = tokens * kv_heads * group * dim * item // 16
+        k.line(f"for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < {units}u; i += gridDim.x * 256u) {{")
+        k.line(f"    reinterpret_cast<uint4*>({slot})[i] = uint4{{0u, 0u, 0u, 0u}};")
+        k.line("}")
+        self.launch(k, (min(-(-units // 256), 2048), 1, 1), 256, [], kind="attention_chunk_clear")
+        partial = self.allocate((tiles * kv_heads * splits * rows * (padded + 2),), torch.float32) if splits > 1 else None
+
+        def scratch(k: Kernel) -> str:
+            return "nullptr" if partial is None else str(k.slot(partial.name, torch.float32, writable=True, extent=self.extents[partial.name]))
+
+        k = kernel()
+        if waves:
+            k.line(f"chroma::attention_chunk_wide<{padded}, {32 if padded > 128 else 64}u, {waves}u, {str(dim == padded).lower()}>(a, {splits}u, {scratch(k)});")
+            self.launch(k, (tiles * kv_heads, splits, 1), 64 * waves, inputs, kind="attention_chunk")
+        else:
+            k.line(f"chroma::attention_chunk_tiles<{ctype}, {padded}, {half}u, {few}u>(a, {splits}u, {scratch(k)});")
+            self.launch(k, (tiles * kv_heads, splits, 1), 64 * few, inputs, kind="attention_chunk")
+        if partial is not None:
+            k = kernel()
+            k.line(f"chroma::attention_chunk_combine<{ctype}, {padded}, {rows}u, {str(waves > 0).lower()}>(a, {splits}u, {scratch(k)});")
+            self.launch(k, (tiles * kv_heads, rows // 16, 1), 256, inputs + [partial], kind="attention_chunk_combine")
         self.fused_attentions += 1
         return out
 

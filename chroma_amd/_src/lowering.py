@@ -96,7 +96,8 @@ OPERATIONS.update(
         "aten.triu.default": "triangular",
         "aten.tril.default": "triangular",
         "aten._assert_tensor_metadata.default": "metadata",
-        "chroma_amd.paged_attention.default": "paged_attention",  # the package's own operator (chroma_amd/ops.py)
+        "chroma_amd.paged_attention.default": "paged_attention",  # the package's own operators (chroma_amd/ops.py)
+        "chroma_amd.paged_chunk_attention.default": "paged_chunk_attention",
     }
 )
 
@@ -308,6 +309,12 @@ def lower(codegen, target: Any, meta: Any, args: Tuple[Any, ...], kwargs: Dict[s
         names = ("q", "k_pages", "v_pages", "k_new", "v_new", "table", "lengths", "sinks", "scale", "window", "first")
         *operands, scale, window, first = (_arg(args, kwargs, i, n, 0 if n in ("window", "first") else None) for i, n in enumerate(names))
         return codegen.paged_attention(meta, *operands, float(scale), window, first)
+    if family == "paged_chunk_attention":
+        if meta.dtype not in FLOAT_DTYPES:
+            raise NotImplementedError(name)
+        names = ("q", "k_pages", "v_pages", "k_new", "v_new", "table", "lengths", "starts", "sinks", "scale", "window", "first")
+        *operands, scale, window, first = (_arg(args, kwargs, i, n, 0 if n in ("window", "first") else None) for i, n in enumerate(names))
+        return codegen.paged_chunk_attention(meta, *operands, float(scale), window, first)
     if family == "cat":
         return codegen.concatenate(meta, args[0], axis(_arg(args, kwargs, 1, "dim", 0), len(meta.shape)))
     if family == "triangular":

@@ -157,8 +157,8 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
         const T* k_pages = a.k + kv * a.head_stride;
         const T* v_pages = a.v + kv * a.head_stride;
         const T* q = a.q + (tile.begin + token) * a.q_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim;
-        const T* k_new = a.k_new + uint64_t(kv) * a.dim;
-        const T* v_new = a.v_new + uint64_t(kv) * a.dim;
+        const T* k_new = a.k_new ? a.k_new + uint64_t(kv) * a.dim : k_pages;  // (never followed without new rows)
+        const T* v_new = a.v_new ? a.v_new + uint64_t(kv) * a.dim : v_pages;
         const int64_t* table = a.table + tile.b * a.table_stride;
         // The page of this lane's row of block x (-1: none).
         auto page_of = [&](uint32_t x) -> int64_t {

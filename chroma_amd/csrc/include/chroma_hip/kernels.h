@@ -6,4 +6,5 @@
 #include "attention.h"
 #include "attention_flash.h"
 #include "attention_paged.h"
+#include "attention_chunk.h"
 #include "kwave.h"

@@ -1,8 +1,8 @@
 """Operators for exported modules that ATen has none for.
 
-``torch.ops.chroma_amd.paged_attention`` (``paged_attention`` here) can be called in any module that is
-exported and compiled; eager calls and other devices compute the plain form below. Importing this module
-registers it (the compiler does, so exported files that hold it load there).
+``torch.ops.chroma_amd.paged_attention`` and ``paged_chunk_attention`` (the functions here) can be called in any module that is
+exported and compiled; eager calls and other devices compute the plain forms below. Importing this module
+registers them (the compiler does, so exported files that hold them load there).
 """
 
 from __future__ import annotations
@@ -86,4 +86,75 @@ def _check(q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, window, fir
         raise ValueError("window and first must not be negative")
 
 
-__all__ = ["paged_attention"]
+@torch.library.custom_op("chroma_amd::paged_chunk_attention", mutates_args=())
+def paged_chunk_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], table: Tensor, lengths: Tensor,
+                          starts: Tensor, sinks: Optional[Tensor], scale: float, window: int = 0, first: int = 0) -> Tensor:
+    """Attention of a chunk of new tokens of every sequence over its cached keys and values, which lie in pages.
+
+    q [T, KV, G, D], rows starts[b] .. starts[b + 1] - 1 of it sequence b's tokens; starts [S + 1] int64, ascending within
+    [0, T] (entries outside count as the nearest bound, a range that descends as empty). k_new and v_new [T, KV, D] are the tokens' own
+    rows, token i of a sequence at position lengths[b] + i; or None, where they are the last of the lengths[b] cached rows. A
+    token sees the rows up to its position, cached or new, less what ``window`` leaves out. Pages, table [S, N], lengths, sinks,
+    window and first are as for ``paged_attention``. A token that sees no row and a row of q that no sequence has get zeros. Scores
+    and sums are float's, the result is rounded once; compiled with bfloat16, a weight meets the values rounded to bfloat16."""
+    _check_chunk(q, k_pages, v_pages, k_new, v_new, table, lengths, starts, sinks, window, first)
+    tokens, kv_heads, group, dim = q.shape
+    pages, rows = k_pages.shape[:2]
+    out = torch.zeros_like(q)
+    for b in range(len(lengths)):
+        begin = min(max(int(starts[b]), 0), tokens)
+        end = min(max(int(starts[b + 1]), begin), tokens)
+        if begin == end:
+            continue
+        length = min(max(int(lengths[b]), 0), table.shape[1] * rows)
+        j = torch.arange(length, device=q.device)
+        page = table[b][j // rows]
+        held = (page >= 0) & (page < pages)
+        j, place = j[held], (page * rows + j % rows)[held]
+        k, v = (x.reshape(-1, kv_heads, dim)[place].float() for x in (k_pages, v_pages))
+        now = torch.arange(end - begin, device=q.device) + length
+        if k_new is None:
+            now = now - (end - begin)
+        else:
+            k, v, j = torch.cat([k, k_new[begin:end].float()]), torch.cat([v, v_new[begin:end].float()]), torch.cat([j, now])
+        seen = j[None, :] <= now[:, None]
+        if window:
+            seen = seen & ((j[None, :] > now[:, None] - window) | (j[None, :] < first))
+        # head by head: [tokens, G, rows]
+        for h in range(kv_heads):
+            scores = torch.mm((q[begin:end, h].float() * scale).reshape(-1, dim), k[:, h].t().contiguous()).reshape(end - begin, group, -1)
+            scores = scores.masked_fill(~seen[:, None, :], -math.inf)
+            joined = scores
+            if sinks is not None:
+                joined = torch.cat([scores, sinks.float()[h * group : (h + 1) * group].reshape(1, group, 1).expand(end - begin, -1, -1)], -1)
+            top = joined.amax(-1, keepdim=True) if joined.shape[-1] else joined.new_zeros(end - begin, group, 1)
+            top = torch.where(top == -math.inf, 0.0, top)
+            weights, total = torch.exp(scores - top), torch.exp(joined - top).sum(-1, keepdim=True)
+            mixed = torch.mm(weights.reshape(-1, weights.shape[-1]), v[:, h]).reshape(end - begin, group, dim)
+            out[begin:end, h] = torch.where(total == 0, 0.0, mixed / total).to(q.dtype)
+    return out
+
+
+@paged_chunk_attention.register_fake
+def _(q, k_pages, v_pages, k_new, v_new, table, lengths, starts, sinks, scale, window=0, first=0):
+    _check_chunk(q, k_pages, v_pages, k_new, v_new, table, lengths, starts, sinks, window, first)
+    return q.new_empty(q.shape)
+
+
+def _check_chunk(q, k_pages, v_pages, k_new, v_new, table, lengths, starts, sinks, window, first) -> None:
+    if q.dim() != 4 or table.dim() != 2 or lengths.dim() != 1 or len(lengths) == 0:
+        raise ValueError("paged_chunk_attention wants q [tokens, KV heads, group, dim], table [sequences, pages of the longest] and lengths [sequences]")
+    tokens, kv_heads, _, dim = q.shape
+    if (k_new is None) != (v_new is None) or (k_new is not None and not tuple(k_new.shape) == tuple(v_new.shape) == (tokens, kv_heads, dim)):
+        raise ValueError("k_new and v_new come together, [tokens, KV heads, dim]")
+    # the rest is as for a token of each sequence
+    _check(q.new_empty((len(lengths), *q.shape[1:])) if tokens else q, k_pages, v_pages, None, None, table, lengths, sinks, window, first)
+    if k_new is not None and (k_new.dtype != q.dtype or v_new.dtype != q.dtype):
+        raise TypeError("q, pages, new rows and sinks must have one dtype")
+    if tuple(starts.shape) != (len(lengths) + 1,):
+        raise ValueError("starts must hold one entry more than lengths")
+    if starts.dtype != torch.int64:
+        raise TypeError("starts must be int64")
+
+
+__all__ = ["paged_attention", "paged_chunk_attention"]
