@@ -11,6 +11,7 @@ Additions:
 
 * ``PagedDecoder(decoder, step)`` - many sequences over one paged cache (``models.paged.export_paged``)
 * ``TokenRules(...)`` - penalties, biases and allowed tokens for ``append_top`` / ``greedy`` / ``step_top``
+* ``Sampling(...)`` - temperature, top-k, top-p and min-p for ``append_sample`` / ``step_sample``
 * ``chroma_amd.ops`` - operators for exported modules that ATen has none for (``paged_attention``)
 """
 
@@ -21,6 +22,7 @@ from chroma_amd._src.jit import jit
 from chroma_amd._src.paged import PagedDecoder
 from chroma_amd._src.program import Program
 from chroma_amd._src.rules import TokenRules
+from chroma_amd._src.sampling import Sampling
 
 
 def compile(input, output, *, blas: bool = True, backend: str = "hip") -> Program:
@@ -29,4 +31,4 @@ def compile(input, output, *, blas: bool = True, backend: str = "hip") -> Progra
     return compile_for_backend(input, output, blas=blas, backend=backend)
 
 
-__all__ = ["Decoder", "PagedDecoder", "Program", "TokenRules", "compile", "jit"]
+__all__ = ["Decoder", "PagedDecoder", "Program", "Sampling", "TokenRules", "compile", "jit"]

@@ -38,8 +38,10 @@ from chroma_amd._src import host
 from chroma_amd._src.dtypes import BFLOAT16, numpy_dtype
 from chroma_amd._src.program import NativeModel, Program
 from chroma_amd._src.rules import TokenRules
+from chroma_amd._src.sampling import Sampling, check_uniform, draw
 
 SELECT_MAX_K = 1024  # largest k the runtime's row selection takes (chroma_hip_rows_topk)
+SAMPLE_MAX_WIDTH = 1 << 19  # widest row that tokens are drawn from on the device
 
 
 @dataclass(frozen=True)
@@ -404,6 +406,24 @@ class Decoder:
         with k = 1)."""
         return int(self.append_top(tokens, 1, allowed=allowed, rules=rules)[1][0])
 
+    def append_sample(self, tokens: Any, sampling: Sampling = Sampling(), *, uniform: float, rules: Optional[TokenRules] = None) -> Tuple[int, float]:
+        """Consume new token ids like ``append`` and return a token drawn from the logits after the last one, with the logarithm
+        of its share of the kept weights. ``sampling`` says how (temperature, top-k, top-p, min-p), ``uniform`` is the random
+        number from [0, 1) that it is drawn with, and ``rules`` adjust the logits first. With hip programs the token is drawn on
+        the device, under the step's one synchronization; other programs draw on the host by the same rule. (An addition to
+        the reference API, as ``append_top``.)"""
+        if not isinstance(sampling, Sampling):
+            raise TypeError(f"sampling must be a Sampling, got {type(sampling).__name__}")
+        check_uniform(uniform)
+        if rules is not None:
+            rules.check(self.vocab_size)
+        with self._lock:
+            if self._on_device and isinstance(self._models[1].native, NativeModel) and self.vocab_size <= SAMPLE_MAX_WIDTH:
+                _, _, (ids, logprobs) = self._consume(tokens, keep_logits=True, sample=(sampling, uniform), rules=rules)
+                return int(ids[0]), float(logprobs[0])
+            logits, _, _ = self._consume(tokens, keep_logits=False)
+            return draw(logits[0] if rules is None else rules.apply(logits[0]), sampling, uniform)
+
     def _selector(self, k: int, candidates: Optional[int]) -> Program:
         """The hip program selecting the top ``k`` of a logits row (of ``candidates`` gathered ids), compiled
         on first use next to the decoder's programs and kept until ``close``."""
@@ -427,12 +447,12 @@ class Decoder:
             self._selectors[key] = program
         return program
 
-    def _consume(self, tokens: Any, *, keep_logits: bool, top: Optional[int] = None,
+    def _consume(self, tokens: Any, *, keep_logits: bool, top: Optional[int] = None, sample: Optional[Tuple[Sampling, float]] = None,
                  rules: Optional[TokenRules] = None) -> Tuple[Optional[np.ndarray], int, Any]:
         """Run the steps for ``tokens``; return the last step's logits (None when ``keep_logits`` leaves
         them in the device output of the program that ran it), that program's index, and, when ``top`` is
         given (device mode), the (values, ids) of the last step's ``top`` largest logits, adjusted by
-        ``rules``, selected on the device after it."""
+        ``rules``, selected on the device after it; with ``sample`` the (ids, logprobs) of a token drawn there."""
         ids = np.asarray(tokens)
         if ids.ndim != 1 or not len(ids):
             raise ValueError(f"append wants a nonempty 1-D sequence of token IDs, got shape {ids.shape}")
@@ -486,7 +506,10 @@ class Decoder:
                     if self._device_masks[which]:
                         inputs = list(args)
                         inputs[4] = inputs[5] = None  # the masks built on the device above
-                    if top is not None and offset + count == len(ids):
+                    if sample is not None and offset + count == len(ids):
+                        selection = self._models[which].run_sample_resident(inputs, [logits, *updates, *extras], 0, [sample[0]], [sample[1]],
+                                                                            None if rules is None else [rules])
+                    elif top is not None and offset + count == len(ids):
                         chosen = {} if rules is None else {"rules": [rules]}
                         selection = self._models[which].run_top_resident(inputs, [logits, *updates, *extras], 0, top, **chosen)
                     else:

@@ -201,6 +201,8 @@ def library() -> ctypes.CDLL:
             getattr(lib, name + "_workspace").argtypes = [c.POINTER(call)]
             getattr(lib, name + "_workspace").restype = c.c_size_t
             getattr(lib, name).argtypes = [c.POINTER(call), c.c_void_p, c.c_size_t, c.c_void_p, c.c_char_p, c.c_size_t]
+        lib.chroma_hip_run_sample.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_int, c.c_int, c.c_size_t, c.c_size_t, c.POINTER(Adjust),
+                                              c.POINTER(Sample), c.c_void_p, c.c_void_p, c.c_char_p, c.c_size_t]
         for name, call in (("chroma_hip_paged_plan", PagedPlan), ("chroma_hip_cache_store", CacheStore)):
             getattr(lib, name).argtypes = [c.POINTER(call), c.c_void_p, c.c_char_p, c.c_size_t]
         _library = lib
@@ -246,6 +248,7 @@ EXPORTED = (
     "chroma_hip_paged_chunk_attention",
     "chroma_hip_rows_sample_workspace",
     "chroma_hip_rows_sample",
+    "chroma_hip_run_sample",
 )
 
 

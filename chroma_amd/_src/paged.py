@@ -1,7 +1,8 @@
 """Generation of many sequences over one paged key-value cache on the device.
 
 ``PagedDecoder`` pairs a ``Decoder``, which consumes prompts, with a step program of ``export_paged``, which
-consumes one token of every sequence at a time. The cache lies in the step program's input staging; a
+consumes one token of every sequence at a time; or it has a step program of ``export_paged_chunk`` alone, which consumes any
+number of tokens of each, prompts among them. The cache lies in the step program's input staging; a
 sequence is a list of its pages (``PagePool``). Rows move on the device (``chroma_hip_cache_move``): a prompt's
 from the decoder's cache, a step's new rows into their pages, the last page of a forked sequence when it is
 first written to, live pages to the front of the cache. A step commits only after its program returned and its moves are
@@ -15,7 +16,7 @@ from __future__ import annotations
 import contextlib
 import heapq
 import threading
-from typing import Any, Dict, Iterable, Iterator, List, Mapping, Optional, Sequence, Tuple
+from typing import Any, Dict, Iterable, Iterator, List, Mapping, Optional, Sequence, Tuple, Union
 
 import numpy as np
 
@@ -24,6 +25,9 @@ from chroma_amd._src.decoder import SELECT_MAX_K, Decoder, _interrupts_deferred,
 from chroma_amd._src.dtypes import numpy_dtype
 from chroma_amd._src.program import Program
 from chroma_amd._src.rules import TokenRules, unread
+from chroma_amd._src.sampling import Sampling, check_uniform
+
+Tokens = Union[int, Sequence[int]]
 
 
 class PagePool:
@@ -69,30 +73,43 @@ class PagePool:
 class PagedDecoder:
     """Sequences are named by integers that ``add`` and ``fork`` return. Calls are serialized by one lock."""
 
-    def __init__(self, decoder: Decoder, step: Program) -> None:
+    def __init__(self, decoder: Optional[Decoder], step: Program) -> None:
         """``decoder`` (a ``Decoder`` of hip programs, made with the model's own sliding window, which the step program
         holds) consumes the prompts, at most its context long, and is reset by each; ``step`` is a compiled
-        ``export_paged`` of the same model. Both are closed with the paged decoder."""
-        if len(step.inputs) != 6 or len(step.outputs) != 3:
-            raise ValueError(f"PagedDecoder step wants six inputs and three outputs, not {len(step.inputs)} and {len(step.outputs)}")
+        ``export_paged`` of the same model. Or ``decoder`` is None and ``step`` a compiled ``export_paged_chunk``, in whose steps
+        prompts are consumed. Both are closed with the paged decoder."""
+        chunked = decoder is None
+        if len(step.inputs) != (8 if chunked else 6) or len(step.outputs) != 3:
+            want = "eight" if chunked else "six"
+            raise ValueError(f"PagedDecoder step wants {want} inputs and three outputs, not {len(step.inputs)} and {len(step.outputs)}")
         cache, table = step.inputs[2], step.inputs[4]
         layers, pages, rows, heads, dim = cache["shape"] if len(cache["shape"]) == 5 else (0,) * 5
         slots, span = table["shape"] if len(table["shape"]) == 2 else (0, 0)
-        prompts = decoder._models[1].inputs[2]
         # rows move by these extents, so every input and output must have them
-        fresh = ([layers, slots, heads, dim], prompts["dtype"])
-        wanted = [([slots], "int64"), ([slots], "float32"), *[([layers, pages, rows, heads, dim], prompts["dtype"])] * 2, ([slots, span], "int64"),
-                  ([slots], "int64"), ([slots, decoder.vocab_size], step.outputs[0]["dtype"]), fresh, fresh]
-        if [layers, heads, dim] != [prompts["shape"][0], *prompts["shape"][2:]] or \
-                [(list(spec["shape"]), spec["dtype"]) for spec in (*step.inputs, *step.outputs)] != wanted:
-            raise ValueError("PagedDecoder decoder and step were not exported from the same model")
-        if not decoder.stats["cache_on_device"] or decoder.device != step.device:
-            raise ValueError("PagedDecoder wants a decoder of hip programs on the step's device")
+        room = step.inputs[0]["shape"][0] if chunked and len(step.inputs[0]["shape"]) == 1 else slots
+        vocab_size = step.outputs[0]["shape"][-1] if chunked and step.outputs[0]["shape"] else None if chunked else decoder.vocab_size
+        dtype = cache["dtype"] if chunked else decoder._models[1].inputs[2]["dtype"]
+        wanted = [([room], "int64"), ([room], "float32"), *[([layers, pages, rows, heads, dim], dtype)] * 2, ([slots, span], "int64"),
+                  ([slots], "int64"), *([([slots + 1], "int64"), ([slots], "int64")] if chunked else []),
+                  ([slots, vocab_size], step.outputs[0]["dtype"]), *[([layers, room, heads, dim], dtype)] * 2]
+        found = [(list(spec["shape"]), spec["dtype"]) for spec in (*step.inputs, *step.outputs)]
+        if chunked:
+            if found != wanted:
+                raise ValueError("PagedDecoder step was not exported by export_paged_chunk")
+            if not hasattr(getattr(step, "native", None), "cache_move"):
+                raise ValueError("PagedDecoder wants a hip program")
+        else:
+            prompts = decoder._models[1].inputs[2]
+            if [layers, heads, dim] != [prompts["shape"][0], *prompts["shape"][2:]] or found != wanted:
+                raise ValueError("PagedDecoder decoder and step were not exported from the same model")
+            if not decoder.stats["cache_on_device"] or decoder.device != step.device:
+                raise ValueError("PagedDecoder wants a decoder of hip programs on the step's device")
+        self._room = room  # tokens of a step
         self._decoder, self._step = decoder, step
         self._layers, self._page_rows = layers, rows
         self._row_bytes = heads * dim * numpy_dtype(cache["dtype"]).itemsize
         self._slots, self._span = slots, span
-        self.vocab_size = decoder.vocab_size
+        self.vocab_size = vocab_size
         self._logit_dtype = numpy_dtype(step.outputs[0]["dtype"])
         self._pool = PagePool(pages)
         self._slot_of: Dict[int, int] = {}  # sequence -> its row of the step program
@@ -121,6 +138,11 @@ class PagedDecoder:
     @property
     def free_pages(self) -> int:
         return self._pool.free
+
+    @property
+    def step_tokens(self) -> int:
+        """Tokens that a step takes: of all its sequences together where each can bring several."""
+        return self._room
 
     def position(self, sequence: int) -> int:
         return self._lengths[self._known(sequence)]
@@ -176,7 +198,10 @@ class PagedDecoder:
 
     # ------------------------------------------------------------------------------------ sequences
     def add(self, tokens: Any) -> Tuple[int, np.ndarray]:
-        """Consume a prompt; returns the new sequence and the logits [1, vocab] after the prompt's last token."""
+        """Consume a prompt; returns the new sequence and the logits [1, vocab] after the prompt's last token. Without a decoder the
+        prompt is consumed in steps of its own; to share a step with other sequences, ``begin`` one and ``step`` it."""
+        if self._decoder is None:
+            return self._add_in_steps(tokens)
         with self._lock, self._decoder._lock:  # the decoder's cache stays this prompt's until its rows have been taken
             if self._closed:
                 raise RuntimeError("PagedDecoder is closed")
@@ -199,6 +224,48 @@ class PagedDecoder:
                     self._move(source, [(i * size, page * size, min(size, count - i * size)) for i, page in enumerate(pages)])
                     self._step.native.synchronize()  # before the decoder's next prompt overwrites the rows
                 return self._enter(slot, pages, count), logits
+
+    def begin(self) -> int:
+        """A new sequence without rows, for steps that take several tokens of it."""
+        with self._lock:
+            if self._closed:
+                raise RuntimeError("PagedDecoder is closed")
+            if self._decoder is not None:
+                raise RuntimeError("the decoder consumes the prompts of this step program")
+            slot = self._new_slot()
+            with _interrupts_deferred():
+                return self._enter(slot, [], 0)
+
+    def _add_in_steps(self, tokens: Any) -> Tuple[int, np.ndarray]:
+        tokens = [int(token) for token in self._tokens_of(tokens)]
+        with self._lock:
+            if self._closed:
+                raise RuntimeError("PagedDecoder is closed")
+            count, needed = len(tokens), -(-len(tokens) // self._page_rows)
+            if count > self._span * self._page_rows:
+                raise ValueError(f"a prompt of {count} tokens; a sequence holds {self._span * self._page_rows}")
+            if needed > self._pool.free:
+                raise RuntimeError(f"a prompt of {count} tokens needs {needed} pages, {self._pool.free} are free")
+            sequence = self.begin()
+            try:
+                for i in range(0, count, self._room):
+                    part = {sequence: tokens[i : i + self._room]}
+                    if i + self._room >= count:
+                        return sequence, self.step(part)
+                    self._run(part, [None, None, None], None, None)
+            except BaseException:
+                self.free(sequence)
+                raise
+
+    @staticmethod
+    def _tokens_of(tokens: Any) -> np.ndarray:
+        """One token or several, as an array of one at least."""
+        ids = np.asarray(tokens)
+        if ids.ndim > 1 or not ids.size:
+            raise ValueError(f"a sequence takes a token or a nonempty 1-D sequence of them, got shape {ids.shape}")
+        if not np.issubdtype(ids.dtype, np.integer):
+            raise TypeError(f"token ids must be integers, got {tokens!r}")
+        return ids.reshape(-1)
 
     def fork(self, sequence: int) -> int:
         """A new sequence with the same rows: the pages are shared, and the last one is copied when either of
@@ -236,16 +303,17 @@ class PagedDecoder:
             return len(moves)
 
     # ------------------------------------------------------------------------------------ steps
-    def step(self, tokens: Mapping[int, int]) -> np.ndarray:
-        """Consume one token of each named sequence ({sequence: token}); returns the logits [n, vocab] after
-        them, in the mapping's order."""
+    def step(self, tokens: Mapping[int, Tokens]) -> np.ndarray:
+        """Consume one token of each named sequence ({sequence: token}), or several where the step program takes them
+        ({sequence: tokens}, ``step_tokens`` in all); returns the logits [n, vocab] after each one's last, in the mapping's
+        order."""
         logits = host.empty((self._slots, self.vocab_size), self._logit_dtype)
         with self._lock:
             slots, _ = self._run(tokens, [logits, None, None], None, None)
             adjacent = slots == list(range(slots[0], slots[0] + len(slots)))
             return logits[slots[0] : slots[0] + len(slots)] if adjacent else logits[slots]
 
-    def step_top(self, tokens: Mapping[int, int], k: int = 1, *, rules: Optional[Mapping[int, TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
+    def step_top(self, tokens: Mapping[int, Tokens], k: int = 1, *, rules: Optional[Mapping[int, TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
         """``step`` that returns the ``k`` largest logits after each token and their ids (both [n, k]), chosen on
         the device by the rule of ``Decoder.append_top``; ``rules`` ({sequence: rules}) adjust a sequence's logits
         first."""
@@ -255,24 +323,50 @@ class PagedDecoder:
             slots, (values, ids) = self._run(tokens, [None, None, None], int(k), rules)
             return values[slots], ids[slots]
 
-    def _run(self, tokens: Mapping[int, int], outputs: List[Optional[np.ndarray]], k: Optional[int],
-             rules: Optional[Mapping[int, TokenRules]]) -> Tuple[List[int], Any]:
+    def step_sample(self, tokens: Mapping[int, Tokens], uniform: Mapping[int, float], sampling: Union[Sampling, Mapping[int, Sampling]] = Sampling(), *,
+                    rules: Optional[Mapping[int, TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
+        """``step`` that returns a token drawn on the device after each token and its logprob (both [n]), by the rule of
+        ``Decoder.append_sample``: ``uniform`` holds a random number of each sequence, ``sampling`` the settings of all or of
+        each ({sequence: settings}; those without have the plain ones), and ``rules`` adjust a sequence's logits first."""
+        settings = sampling if isinstance(sampling, Mapping) else {sequence: sampling for sequence in tokens}
+        for sequence in (*settings, *uniform):
+            if sequence not in tokens:
+                raise KeyError(f"settings for sequence {sequence}, which has no token in this step")
+        for sequence in tokens:
+            if sequence not in uniform:
+                raise KeyError(f"no random number for sequence {sequence}")
+            check_uniform(uniform[sequence])
+        for one in settings.values():
+            if not isinstance(one, Sampling):
+                raise TypeError(f"sampling must be a Sampling, got {type(one).__name__}")
+        with self._lock:
+            slots, (ids, logprobs) = self._run(tokens, [None, None, None], None, rules, (settings, uniform))
+            return ids[slots], logprobs[slots]
+
+    def _run(self, tokens: Mapping[int, Tokens], outputs: List[Optional[np.ndarray]], k: Optional[int], rules: Optional[Mapping[int, TokenRules]],
+             sample: Optional[Tuple[Mapping[int, Sampling], Mapping[int, float]]] = None) -> Tuple[List[int], Any]:
         if self._closed:
             raise RuntimeError("PagedDecoder is closed")
         if not tokens:
             raise ValueError("a step wants a token of at least one sequence")
+        taken_of: Dict[int, np.ndarray] = {}
         for sequence, token in tokens.items():
             self._known(sequence)
-            if not isinstance(token, (int, np.integer)):
+            if self._decoder is not None and not isinstance(token, (int, np.integer)):
                 raise TypeError(f"token ids must be integers, got {token!r}")
-            if self._lengths[sequence] >= self._span * self._page_rows:
-                raise ValueError(f"sequence {sequence} holds {self._lengths[sequence]} rows, all that the step program has pages for")
+            taken_of[sequence] = self._tokens_of(token)
+            if self._lengths[sequence] + len(taken_of[sequence]) > self._span * self._page_rows:
+                raise ValueError(f"sequence {sequence} holds {self._lengths[sequence]} rows, "
+                                 + ("all that the step program has pages for" if len(taken_of[sequence]) == 1 else
+                                    f"{len(taken_of[sequence])} more are not what the step program has pages for"))
+        if self._decoder is None and sum(map(len, taken_of.values())) > self._room:
+            raise ValueError(f"{sum(map(len, taken_of.values()))} tokens, a step takes {self._room}")
         for sequence in rules or ():
             if sequence not in tokens:
                 raise KeyError(f"rules for sequence {sequence}, which has no token in this step")
-        # a page for a row that begins one, or for a copy of a last page that other sequences share
+        # pages for the rows that begin one, and for a copy of a last page that other sequences share
         size = self._page_rows
-        starts = [s for s in tokens if self._lengths[s] % size == 0]
+        starts = {s: -(-(self._lengths[s] + len(taken_of[s])) // size) - len(self._pages[s]) for s in tokens}
         leaving: Dict[int, int] = {}
         copies = []
         for s in tokens:
@@ -281,47 +375,82 @@ class PagedDecoder:
                 if self._pool.references[page] - leaving.get(page, 0) > 1:  # the last of its owners keeps it
                     leaving[page] = leaving.get(page, 0) + 1
                     copies.append(s)
-        if len(starts) + len(copies) > self._pool.free:
-            raise RuntimeError(f"the step needs {len(starts) + len(copies)} pages, {self._pool.free} are free")
-        ids, positions, _, _, _, lengths = self._args
+        needed = sum(starts.values()) + len(copies)
+        if needed > self._pool.free:
+            raise RuntimeError(f"the step needs {needed} pages, {self._pool.free} are free")
+        ids, positions, lengths = self._args[0], self._args[1], self._args[5]
         ids.fill(0)
         positions.fill(0)
         lengths.fill(0)
-        for sequence, token in tokens.items():
-            slot = self._slot_of[sequence]
-            ids[slot], positions[slot], lengths[slot] = token, self._lengths[sequence], self._lengths[sequence]
-        selection = None
-        if k is None:
-            self._step.run_resident(self._args, outputs)
-        elif rules:
+        rows: Dict[int, int] = {}  # a sequence's first token in the step: its slot, or behind those of the slots before
+        if self._decoder is None:
+            first = 0
+            begins, last = self._args[6], self._args[7]
+            last.fill(0)
+            by_place = {self._slot_of[sequence]: sequence for sequence in tokens}
+            for slot in range(self._slots):
+                begins[slot] = first
+                if slot in by_place:
+                    rows[by_place[slot]] = first
+                    first += len(taken_of[by_place[slot]])
+                    last[slot] = first - 1
+            begins[self._slots] = first
+        for sequence, some in taken_of.items():
+            slot, held = self._slot_of[sequence], self._lengths[sequence]
+            row = rows.setdefault(sequence, slot)
+            ids[row : row + len(some)] = some
+            positions[row : row + len(some)] = np.arange(held, held + len(some))
+            lengths[slot] = held
+        selection = row_rules = None
+        if rules:
             plain = TokenRules()
             by_slot = {self._slot_of[sequence]: rules.get(sequence, plain) for sequence in tokens}
             idle = unread(list(by_slot.values()))
-            selection = self._step.run_top_resident(self._args, outputs, 0, k, [by_slot.get(slot, idle) for slot in range(self._slots)])
+            row_rules = [by_slot.get(slot, idle) for slot in range(self._slots)]
+        if sample is not None:
+            settings, uniform = [Sampling(temperature=0.0)] * self._slots, [0.0] * self._slots
+            for sequence in tokens:
+                settings[self._slot_of[sequence]], uniform[self._slot_of[sequence]] = sample[0].get(sequence, Sampling()), sample[1][sequence]
+            selection = self._step.run_sample_resident(self._args, outputs, 0, settings, uniform, row_rules)
+        elif k is None:
+            self._step.run_resident(self._args, outputs)
+        elif row_rules:
+            selection = self._step.run_top_resident(self._args, outputs, 0, k, row_rules)
         else:
             selection = self._step.run_top_resident(self._args, outputs, 0, k)
         with _interrupts_deferred():
-            with self._taking(len(copies) + len(starts)) as taken:
-                pages = {s: self._pages[s][-1] for s in tokens} | dict(zip((*copies, *starts), taken))
-                self._move(self._cache(), [(self._pages[s][-1] * size, pages[s] * size, self._lengths[s] % size) for s in copies])
+            with self._taking(needed) as taken:
+                left = iter(taken)
+                pages = {s: list(self._pages[s]) for s in tokens}
+                for s in copies:
+                    pages[s][-1] = next(left)
+                self._move(self._cache(), [(self._pages[s][-1] * size, pages[s][-1] * size, self._lengths[s] % size) for s in copies])
+                for s in tokens:
+                    pages[s].extend(next(left) for _ in range(starts[s]))
                 model = self._step.native
-                fresh = native.CacheRows(keys=model.output_pointer(1), values=model.output_pointer(2), rows=self._slots,
-                                         layer_pitch=self._slots * self._row_bytes)
-                self._move(fresh, [(self._slot_of[s], pages[s] * size + self._lengths[s] % size, 1) for s in tokens])
+                fresh = native.CacheRows(keys=model.output_pointer(1), values=model.output_pointer(2), rows=self._room,
+                                         layer_pitch=self._room * self._row_bytes)
+                moves = []
+                for s in tokens:  # a sequence's rows, page by page
+                    at, stop = self._lengths[s], self._lengths[s] + len(taken_of[s])
+                    while at < stop:
+                        count = min(stop, (at // size + 1) * size) - at
+                        moves.append((rows[s] + at - self._lengths[s], pages[s][at // size] * size + at % size, count))
+                        at += count
+                self._move(fresh, moves)
             for sequence in copies:
                 self._pool.release(self._pages[sequence][-1:])
-                self._pages[sequence][-1] = pages[sequence]
-            for sequence in starts:
-                self._pages[sequence].append(pages[sequence])
             for sequence in tokens:
-                self._lengths[sequence] += 1
+                self._pages[sequence] = pages[sequence]
+                self._lengths[sequence] += len(taken_of[sequence])
                 self._set_row(sequence)
         return [self._slot_of[s] for s in tokens], selection
 
     def close(self) -> None:
         with self._lock:
             self._closed = True
-            self._decoder.close()
+            if self._decoder is not None:
+                self._decoder.close()
             self._step.close()
 
     def __enter__(self) -> "PagedDecoder":

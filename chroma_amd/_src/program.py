@@ -23,6 +23,8 @@ import numpy as np
 from chroma_amd._src import host, native
 from chroma_amd._src.dtypes import BFLOAT16, numpy_dtype
 from chroma_amd._src.rules import TokenRules, pack
+from chroma_amd._src.sampling import Sampling
+from chroma_amd._src.sampling import pack as pack_sampling
 from chroma_amd._src.spec import MANIFEST_VERSION, signature
 
 Array = np.ndarray
@@ -107,6 +109,29 @@ class NativeModel:
         error = ctypes.create_string_buffer(1024)
         native.check(self._lib.chroma_hip_run(self._handle, ins, outs, error, len(error)), error)
 
+    def _rows_of(self, index: int, name: str) -> Tuple[np.dtype, int, int, int]:
+        """(type, its native code, rows, width) of output ``index``, whose rows tokens are chosen from."""
+        spec = self._outputs[index]
+        dtype = numpy_dtype(spec["dtype"])
+        if dtype not in (np.dtype(np.float32), BFLOAT16) or not spec["shape"]:
+            raise TypeError(f"{name} selects over float32 or bfloat16 outputs of rank >= 1")
+        rows = int(np.prod(spec["shape"][:-1])) if len(spec["shape"]) > 1 else 1
+        return dtype, native.FLOAT32 if dtype == np.dtype(np.float32) else native.BFLOAT16, rows, int(spec["shape"][-1])
+
+    @staticmethod
+    def _adjust_call(rules: Sequence[TokenRules], rows: int, width: int) -> Tuple[native.Adjust, Any]:
+        """The rules of ``rows`` rows as a call, and the arrays that it points to."""
+        if len(rules) != rows:
+            raise ValueError(f"{len(rules)} rules for {rows} rows")
+        arrays = pack(rules, width)
+        call = native.Adjust(**{name: None if array is None else array.ctypes.data for name, array in arrays.items()})
+        if arrays["history"] is not None:
+            call.history_stride = call.history_width = arrays["history"].shape[1]
+        for name in ("bias", "mask"):
+            if arrays[name] is not None and len(arrays[name]) > 1:
+                setattr(call, f"{name}_stride", arrays[name].shape[1])
+        return call, arrays
+
     def run_top(self, inputs: List[Optional[np.ndarray]], outputs: List[Optional[np.ndarray]], index: int, k: int,
                 rules: Optional[Sequence[TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
         """``run`` (resident: None keeps an input's device copy, and leaves an output on the device) that also
@@ -114,34 +139,38 @@ class NativeModel:
         the same stream and under the same synchronization; returns (values [rows, k], int64 ids [rows, k])
         in page-locked host arrays. ``rules`` (one for each row) adjust the rows that the selection reads;
         the output itself stays as it is."""
-        spec = self._outputs[index]
-        dtype = numpy_dtype(spec["dtype"])
-        if dtype not in (np.dtype(np.float32), BFLOAT16) or not spec["shape"]:
-            raise TypeError("run_top selects over float32 or bfloat16 outputs of rank >= 1")
-        width = int(spec["shape"][-1])
-        rows = int(np.prod(spec["shape"][:-1])) if len(spec["shape"]) > 1 else 1
+        dtype, code, rows, width = self._rows_of(index, "run_top")
         ins, outs = self._pointers(inputs, outputs, True)
         values = host.empty((rows, k), dtype)
         ids = host.empty((rows, k), np.int64)
-        code = native.FLOAT32 if dtype == np.dtype(np.float32) else native.BFLOAT16
         error = ctypes.create_string_buffer(1024)
         if rules is None:
             status = self._lib.chroma_hip_run_top(self._handle, ins, outs, index, code, rows, width, k, values.ctypes.data, ids.ctypes.data,
                                                   error, len(error))
         else:
-            if len(rules) != rows:
-                raise ValueError(f"{len(rules)} rules for {rows} rows")
-            arrays = pack(rules, width)
-            call = native.Adjust(**{name: None if array is None else array.ctypes.data for name, array in arrays.items()})
-            if arrays["history"] is not None:
-                call.history_stride = call.history_width = arrays["history"].shape[1]
-            for name in ("bias", "mask"):
-                if arrays[name] is not None and len(arrays[name]) > 1:
-                    setattr(call, f"{name}_stride", arrays[name].shape[1])
+            call, _arrays = self._adjust_call(rules, rows, width)
             status = self._lib.chroma_hip_run_top_adjusted(self._handle, ins, outs, index, code, rows, width, ctypes.byref(call), k,
                                                            values.ctypes.data, ids.ctypes.data, error, len(error))
         native.check(status, error)
         return values, ids
+
+    def run_sample(self, inputs: List[Optional[np.ndarray]], outputs: List[Optional[np.ndarray]], index: int, sampling: Sequence[Sampling],
+                   uniform: Sequence[float], rules: Optional[Sequence[TokenRules]] = None) -> Tuple[np.ndarray, np.ndarray]:
+        """``run_top`` that draws a token from each row instead, by ``sampling`` and a random number for each of them; returns
+        (int64 ids [rows], float32 logprobs [rows])."""
+        _, code, rows, width = self._rows_of(index, "run_sample")
+        if len(sampling) != rows or len(uniform) != rows:
+            raise ValueError(f"{len(sampling)} settings and {len(uniform)} random numbers for {rows} rows")
+        ins, outs = self._pointers(inputs, outputs, True)
+        settings = pack_sampling(sampling, uniform)
+        ids, logprobs = np.empty(rows, np.int64), np.empty(rows, np.float32)
+        call = native.Sample(**{name: array.ctypes.data for name, array in settings.items()})
+        adjustment, _arrays = (None, None) if rules is None else self._adjust_call(rules, rows, width)
+        error = ctypes.create_string_buffer(1024)
+        native.check(self._lib.chroma_hip_run_sample(self._handle, ins, outs, index, code, rows, width,
+                                                     None if adjustment is None else ctypes.byref(adjustment), ctypes.byref(call), ids.ctypes.data,
+                                                     logprobs.ctypes.data, error, len(error)), error)
+        return ids, logprobs
 
     def input_pointer(self, index: int) -> int:
         return int(self._lib.chroma_hip_input_pointer(self._handle, index) or 0)
@@ -328,6 +357,16 @@ class Program:
             if self._model is None:
                 raise RuntimeError("Model is closed")
             return self._model.run_top(arrays, list(outputs), index, k) if rules is None else self._model.run_top(arrays, list(outputs), index, k, rules)
+
+    def run_sample_resident(self, inputs: Sequence[Optional[Array]], outputs: Sequence[Optional[Array]], index: int, sampling: Sequence[Sampling],
+                            uniform: Sequence[float], rules: Optional[Sequence[TokenRules]] = None) -> Tuple[Array, Array]:
+        """``run_resident`` that also returns a token drawn from each row of output ``index`` (adjusted by ``rules``, if given) and
+        its logprob, drawn on the device (``NativeModel.run_sample``)."""
+        arrays = [None if value is None else self._array(value) for value in inputs]
+        with self._lock:
+            if self._model is None:
+                raise RuntimeError("Model is closed")
+            return self._model.run_sample(arrays, list(outputs), index, sampling, uniform, rules)
 
     @property
     def native(self) -> NativeModel:

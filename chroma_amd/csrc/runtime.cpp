@@ -9,6 +9,7 @@
 #include "cache.h"
 #include "copy.h"
 #include "masks.h"
+#include "sample.h"
 #include "select.h"
 
 #include <hip/hip_runtime_api.h>
@@ -297,6 +298,12 @@ public:
         if (rules_host_) {
             hipHostFree(rules_host_);
         }
+        if (sample_) {
+            hipFree(sample_);
+        }
+        if (sample_host_) {
+            hipHostFree(sample_host_);
+        }
         if (error_host_) {
             hipHostFree(error_host_);
         }
@@ -343,6 +350,9 @@ public:
         rules_ = nullptr;
         rules_host_ = nullptr;
         rules_bytes_ = 0;
+        sample_ = nullptr;
+        sample_host_ = nullptr;
+        sample_bytes_ = sample_host_bytes_ = 0;
         slots_ = nullptr;
         slots_host_ = nullptr;
         slots_capacity_ = 0;
@@ -455,6 +465,138 @@ public:
         }
     }
 
+    // ``rules`` as the call over an output's rows (checked), or an empty one.
+    static chroma_hip_adjust_call rules_for(const chroma_hip_adjust_call* rules, char* logits, size_t rows, size_t width, int dtype, const char* name) {
+        chroma_hip_adjust_call call{};
+        if (rules) {
+            call = *rules;
+            call.x = call.y = logits;
+            call.rows = int64_t(rows);
+            call.width = call.x_stride = call.y_stride = int64_t(width);
+            call.dtype = dtype;
+            call.history_stride = call.history ? call.history_stride : 0;
+            call.bias_stride = call.bias ? call.bias_stride : 0;
+            call.mask_stride = call.mask ? call.mask_stride : 0;
+            if (const char* wrong = chroma_adjust::mistake(call)) {
+                throw std::runtime_error(std::string(name) + ": " + wrong);
+            }
+        }
+        return call;
+    }
+    void upload_rules(const StagedRules& staged) {
+        char* at = static_cast<char*>(rules_host_);
+        for (const auto& piece : staged.pieces) {
+            if (piece.first) {
+                std::memcpy(at, piece.first, piece.second);
+            }
+            at += piece.second;
+        }
+        if (staged.bytes) {
+            check(hipMemcpyAsync(rules_, rules_host_, staged.bytes, hipMemcpyHostToDevice, stream_), "Upload rules");
+        }
+    }
+    void adjust(const StagedRules& staged) {
+        char message[256] = {0};
+        if (chroma_adjust::launch_rows_adjust(staged.call, stream_, message, sizeof(message))) {
+            throw HipError(message);
+        }
+    }
+
+    // ``run`` with a token drawn from each row of output ``index`` after the plan (and after ``rules``, if any): only the ids and
+    // their logprobs come back. The settings' arrays are host memory and go up in one copy, beside the results' room.
+    void run_sample(const void* const* inputs, void* const* outputs, int index, int dtype, size_t rows, size_t width,
+                    const chroma_hip_adjust_call* rules, const chroma_hip_sample_call& settings, int64_t* ids, float* logprobs) {
+        DeviceGuard guard(device_);
+        if (!chroma_sample::launch_rows_sample) {
+            throw std::runtime_error("run_sample: this runtime was built without the sampling kernels");
+        }
+        if (index < 0 || size_t(index) >= plan_.outputs.size()) {
+            throw std::runtime_error("run_sample: output index out of range");
+        }
+        if (!settings.uniform || !ids || !logprobs) {
+            throw std::runtime_error("run_sample: null uniform, ids or logprobs");
+        }
+        char* logits = static_cast<char*>(base_) + plan_.outputs[index].offset;
+        chroma_hip_sample_call call = settings;
+        call.x = logits;
+        call.rows = int64_t(rows);
+        call.width = call.x_stride = int64_t(width);
+        call.dtype = dtype;
+        if (const char* wrong = rows < 65536 && width <= (size_t(1) << 19) ? chroma_sample::mistake(call) : "want 1 to 65535 rows of 1 to 524288 logits") {
+            throw std::runtime_error(std::string("run_sample: ") + wrong);
+        }
+        if (rows * width * (dtype == CHROMA_HIP_FLOAT32 ? 4 : 2) != plan_.outputs[index].bytes) {
+            throw std::runtime_error("run_sample: rows x width elements do not match the output's byte size");
+        }
+        const chroma_hip_adjust_call adjustment = rules_for(rules, logits, rows, width, dtype, "run_sample");
+        // on the device and page-locked alike: five settings of 8 bytes a row, ids, logprobs; behind them the kernels' scratch
+        const size_t row_bytes = (rows * 8 + 255) / 256 * 256, fixed = 7 * row_bytes, need = fixed + chroma_sample::workspace_bytes(call);
+        if (need > sample_bytes_ || fixed > sample_host_bytes_) {
+            check(hipStreamSynchronize(stream_), "Sampling scratch");
+            sample_bytes_ = sample_host_bytes_ = 0;
+            if (sample_) {
+                check(hipFree(sample_), "hipFree sampling scratch");
+                sample_ = nullptr;
+            }
+            if (sample_host_) {
+                check(hipHostFree(sample_host_), "hipHostFree sampling results");
+                sample_host_ = nullptr;
+            }
+            check(hipMalloc(&sample_, need), "hipMalloc sampling scratch");
+            check(hipHostMalloc(&sample_host_, fixed, hipHostMallocDefault), "hipHostMalloc sampling results");
+            sample_bytes_ = need;
+            sample_host_bytes_ = fixed;
+        }
+        StagedRules staged;
+        if (rules) {
+            ensure_rules(plan_.outputs[index].bytes, stage_rules(adjustment, nullptr).bytes);
+            staged = stage_rules(adjustment, static_cast<char*>(rules_));
+            staged.call.y = adjusted_;
+            call.x = adjusted_;
+        }
+        char* device = static_cast<char*>(sample_);
+        char* pinned = static_cast<char*>(sample_host_);
+        const auto place = [&](auto*& array, size_t slot) {
+            if (array) {
+                std::memcpy(pinned + slot * row_bytes, array, rows * sizeof(*array));
+                array = reinterpret_cast<std::remove_reference_t<decltype(array)>>(device + slot * row_bytes);
+            }
+        };
+        place(call.temperature, 0);
+        place(call.top_k, 1);
+        place(call.top_p, 2);
+        place(call.min_p, 3);
+        place(call.uniform, 4);
+        call.ids = reinterpret_cast<int64_t*>(device + 5 * row_bytes);
+        call.logprobs = reinterpret_cast<float*>(device + 6 * row_bytes);
+        try {
+            upload(inputs);
+            check(hipMemcpyAsync(device, pinned, 5 * row_bytes, hipMemcpyHostToDevice, stream_), "Upload sampling settings");
+            if (rules) {
+                upload_rules(staged);
+            }
+            launch_all();
+            if (rules) {
+                adjust(staged);
+            }
+            char message[256] = {0};
+            if (chroma_sample::launch_rows_sample(call, device + fixed, need - fixed, stream_, message, sizeof(message))) {
+                throw HipError(message);
+            }
+            check(hipMemcpyAsync(error_host_, static_cast<char*>(base_) + plan_.error, sizeof(unsigned), hipMemcpyDeviceToHost, stream_),
+                  "Read index error");
+            check(hipMemcpyAsync(pinned + 5 * row_bytes, device + 5 * row_bytes, 2 * row_bytes, hipMemcpyDeviceToHost, stream_), "Download tokens");
+            download(outputs);
+            check(hipStreamSynchronize(stream_), "HIP execution");
+            std::memcpy(ids, pinned + 5 * row_bytes, rows * sizeof(int64_t));
+            std::memcpy(logprobs, pinned + 6 * row_bytes, rows * sizeof(float));
+            raise_index_error();
+        } catch (const HipError&) {
+            hipStreamSynchronize(stream_);
+            throw;
+        }
+    }
+
     // ``run`` with a row selection over output ``index`` queued after the plan: only the k values and ids
     // of each row come back (and the outputs whose host pointers are non-null), after one synchronization.
     // With ``rules`` the selection reads the output's rows adjusted by them.
@@ -476,20 +618,7 @@ public:
             throw std::runtime_error("run_top: want 1 <= k <= min(width, 1024) and width <= 524288");
         }
         char* logits = static_cast<char*>(base_) + plan_.outputs[index].offset;
-        chroma_hip_adjust_call call{};
-        if (rules) {  // checked here, before anything runs
-            call = *rules;
-            call.x = call.y = logits;
-            call.rows = int64_t(rows);
-            call.width = call.x_stride = call.y_stride = int64_t(width);
-            call.dtype = dtype;
-            call.history_stride = call.history ? call.history_stride : 0;
-            call.bias_stride = call.bias ? call.bias_stride : 0;
-            call.mask_stride = call.mask ? call.mask_stride : 0;
-            if (const char* wrong = chroma_adjust::mistake(call)) {
-                throw std::runtime_error(std::string("run_top_adjusted: ") + wrong);
-            }
-        }
+        const chroma_hip_adjust_call call = rules_for(rules, logits, rows, width, dtype, "run_top_adjusted");  // before anything runs
         auto align = [](size_t n) { return (n + 255) / 256 * 256; };
         const size_t value_bytes = rows * size_t(k) * item, id_bytes = rows * size_t(k) * sizeof(int64_t);
         // ids then values, adjacent, so one copy brings both back
@@ -532,21 +661,9 @@ public:
                 }
             };
             if (rules) {
-                char* at = static_cast<char*>(rules_host_);
-                for (const auto& piece : staged.pieces) {
-                    if (piece.first) {
-                        std::memcpy(at, piece.first, piece.second);
-                    }
-                    at += piece.second;
-                }
-                if (staged.bytes) {
-                    check(hipMemcpyAsync(rules_, rules_host_, staged.bytes, hipMemcpyHostToDevice, stream_), "Upload rules");
-                }
+                upload_rules(staged);
                 launch_all();
-                char message[256] = {0};
-                if (chroma_adjust::launch_rows_adjust(staged.call, stream_, message, sizeof(message))) {
-                    throw HipError(message);
-                }
+                adjust(staged);
                 select(static_cast<const char*>(adjusted_));
             } else {
                 const std::array<size_t, 6> key{size_t(index), size_t(dtype), rows, width, size_t(k), reinterpret_cast<size_t>(select_)};
@@ -1032,6 +1149,10 @@ private:
     void* rules_ = nullptr;       // the rules' arrays on the device
     void* rules_host_ = nullptr;  // and page-locked
     size_t rules_bytes_ = 0;      // bytes both hold
+    void* sample_ = nullptr;  // run_sample's settings, results and scratch (allocated on first use)
+    size_t sample_bytes_ = 0;
+    void* sample_host_ = nullptr;  // and the settings and results page-locked
+    size_t sample_host_bytes_ = 0;
     // run_top's plan and selection captured as one graph, for the selection it was captured with
     hipGraph_t select_graph_ = nullptr;
     hipGraphExec_t select_exec_ = nullptr;
@@ -1093,6 +1214,18 @@ __attribute__((visibility("default"))) int chroma_hip_run_top_adjusted(void* han
             throw std::runtime_error("run_top_adjusted: null rules");
         }
         program(handle)->run_top(inputs, outputs, output_index, dtype, rows, width, rules, k, values, ids);
+    });
+}
+
+__attribute__((visibility("default"))) int chroma_hip_run_sample(void* handle, const void* const* inputs, void* const* outputs, int output_index,
+                                                                 int dtype, size_t rows, size_t width, const chroma_hip_adjust_call* rules,
+                                                                 const chroma_hip_sample_call* settings, int64_t* ids, float* logprobs,
+                                                                 char* error, size_t error_size) {
+    return guarded(error, error_size, [&] {
+        if (!settings) {
+            throw std::runtime_error("run_sample: null settings");
+        }
+        program(handle)->run_sample(inputs, outputs, output_index, dtype, rows, width, rules, *settings, ids, logprobs);
     });
 }
 

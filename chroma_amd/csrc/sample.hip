@@ -14,7 +14,7 @@
 // A weight exp((x - max) / temperature) is evaluated in 64 bits and rounded to units of 2^-44: sums are integers, and the same
 // in whatever order they are taken. In 32 bits the place that a random number names among 200,000 tokens moves by more than
 // some tokens hold.
-#include "../../include/chroma_hip.h"
+#include "sample.h"
 
 #include <hip/hip_runtime.h>
 
@@ -1022,38 +1022,16 @@ int refuse(const char* message, char* error, size_t size) {
     return CHROMA_HIP_RUNTIME_ERROR;
 }
 
-// What is wrong with the call's extents, or null.
-const char* mistake(const Call& c) {
-    if (c.dtype != CHROMA_HIP_FLOAT32 && c.dtype != CHROMA_HIP_BFLOAT16) {
-        return "dtype must be CHROMA_HIP_FLOAT32 or CHROMA_HIP_BFLOAT16";
-    }
-    if (c.rows < 1 || c.rows > 65535 || c.width < 1 || c.width > (int64_t(1) << 19)) {  // sums of 2^19 weights fit 64 bits
-        return "want 1 to 65535 rows of 1 to 524288 logits";
-    }
-    if (c.x_stride < c.width || c.x_stride > (int64_t(1) << 40)) {
-        return "x_stride out of range";
-    }
-    return nullptr;
-}
-
 }  // namespace
 
-extern "C" {
+namespace chroma_sample {
 
-__attribute__((visibility("default"))) size_t chroma_hip_rows_sample_workspace(const Call* call) {
-    if (!call || mistake(*call)) {
-        return 0;
-    }
-    const uint32_t spans = spans_of(*call);
-    return spans > 1u ? size_t(call->rows) * Scratch::words(spans) * sizeof(uint64_t) : 0;
+size_t workspace_bytes(const Call& c) {
+    const uint32_t spans = mistake(c) ? 1u : spans_of(c);
+    return spans > 1u ? size_t(c.rows) * Scratch::words(spans) * sizeof(uint64_t) : 0;
 }
 
-__attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* call, void* workspace, size_t workspace_bytes, void* stream,
-                                                                  char* error, size_t error_size) {
-    if (!call) {
-        return refuse("null call", error, error_size);
-    }
-    const Call& c = *call;
+int launch_rows_sample(const Call& c, void* workspace, size_t workspace_size, hipStream_t stream, char* error, size_t error_size) {
     if (const char* wrong = mistake(c)) {
         return refuse(wrong, error, error_size);
     }
@@ -1064,8 +1042,8 @@ __attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* ca
     if (reinterpret_cast<uintptr_t>(c.x) % size) {
         return refuse("logits must lie on their own size", error, error_size);
     }
-    const size_t need = chroma_hip_rows_sample_workspace(call);
-    if (need && (!workspace || workspace_bytes < need)) {
+    const size_t need = workspace_bytes(c);
+    if (need && (!workspace || workspace_size < need)) {
         return refuse("workspace smaller than chroma_hip_rows_sample_workspace", error, error_size);
     }
     if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) {
@@ -1078,12 +1056,26 @@ __attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* ca
         return refuse("ids, logprobs or the workspace overlap another array", error, error_size);
     }
     if (c.dtype == CHROMA_HIP_FLOAT32) {
-        launch<float>(c, static_cast<uint64_t*>(workspace), static_cast<hipStream_t>(stream));
+        launch<float>(c, static_cast<uint64_t*>(workspace), stream);
     } else {
-        launch<uint16_t>(c, static_cast<uint64_t*>(workspace), static_cast<hipStream_t>(stream));
+        launch<uint16_t>(c, static_cast<uint64_t*>(workspace), stream);
     }
     const hipError_t status = hipGetLastError();
     return status == hipSuccess ? CHROMA_HIP_OK : refuse(hipGetErrorString(status), error, error_size);
+}
+
+}  // namespace chroma_sample
+
+extern "C" {
+
+__attribute__((visibility("default"))) size_t chroma_hip_rows_sample_workspace(const Call* call) { return call ? chroma_sample::workspace_bytes(*call) : 0; }
+
+__attribute__((visibility("default"))) int chroma_hip_rows_sample(const Call* call, void* workspace, size_t workspace_bytes, void* stream,
+                                                                  char* error, size_t error_size) {
+    if (!call) {
+        return refuse("null call", error, error_size);
+    }
+    return chroma_sample::launch_rows_sample(*call, workspace, workspace_bytes, static_cast<hipStream_t>(stream), error, error_size);
 }
 
 }  // extern "C"

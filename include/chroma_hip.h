@@ -420,6 +420,15 @@ size_t chroma_hip_rows_sample_workspace(const chroma_hip_sample_call* call);
 int chroma_hip_rows_sample(const chroma_hip_sample_call* call, void* workspace, size_t workspace_bytes, void* stream, char* error,
                            size_t error_size);
 
+/* ``chroma_hip_run`` followed, on the program's stream and under the same single synchronization, by a token drawn from each of the
+ * ``rows`` rows of output ``output_index`` (``width`` elements of ``dtype`` each, which must be that output's byte size), adjusted by
+ * ``rules`` first unless they are null (as ``chroma_hip_run_top_adjusted`` does). The arrays of ``settings`` are host memory, read
+ * before the call returns; its x, rows, width, x_stride, dtype, ids and logprobs are the output's and not read. ``ids`` and
+ * ``logprobs`` are host buffers of ``rows`` elements. The scratch is allocated by the program on first use and kept. */
+int chroma_hip_run_sample(void* handle, const void* const* inputs, void* const* outputs, int output_index, int dtype, size_t rows,
+                          size_t width, const chroma_hip_adjust_call* rules, const chroma_hip_sample_call* settings, int64_t* ids,
+                          float* logprobs, char* error, size_t error_size);
+
 #ifdef __cplusplus
 }
 #endif
