@@ -2603,7 +2603,7 @@ class HIPCodegen(Codegen):
         sequences, longest = lengths.shape[0], table.shape[1] * k_pages.shape[1]
         if dim % 8 or dim > 256 or group > 1024 or max(sequences, kv_heads) > 65535:
             raise NotImplementedError(f"paged attention of {tokens} tokens of {sequences} sequences, {kv_heads} KV heads of {group} heads of {dim}")
-        if tokens > 2**24 or tokens * kv_heads * group >= 2**30 or sequences * kv_heads > 2**24 or k_pages.shape[0] >= 2**31 or longest + tokens >= 2**31 - 4096:
+        if tokens > 2**24 or tokens * kv_heads * group >= 2**26 or sequences * kv_heads > 2**22 or k_pages.shape[0] >= 2**31 or longest + tokens >= 2**31 - 4096:
             raise NotImplementedError("paged attention of more rows than the kernels count")
         out, plan, kernel = self._paged_operands(meta, "ChunkOperands", q, k_pages, v_pages, k_new, v_new, table, lengths, sinks, scale, window, first,
                                                  starts)
@@ -2615,7 +2615,7 @@ class HIPCodegen(Codegen):
         k = Kernel(1)
         slot = k.slot(out.name, out.dtype, writable=True, extent=self.extents[out.name])
         units = tokens * kv_heads * group * dim * item // 16
-        k.line(f"for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < {units}u; i += gridDim.x * 256u) {{")
+        k.line(f"for (uint64_t i = blockIdx.x * 256u + threadIdx.x; i < {units}ull; i += gridDim.x * 256u) {{")
         k.line(f"    reinterpret_cast<uint4*>({slot})[i] = uint4{{0u, 0u, 0u, 0u}};")
         k.line("}")
         self.launch(k, (min(-(-units // 256), 2048), 1, 1), 256, [], kind="attention_chunk_clear")

@@ -59,7 +59,8 @@ const char* mistake(const Call& c) {
     if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest + c.tokens >= kMost - 4096) {
         return "pages, page_rows or longest out of range";
     }
-    if (c.tokens * c.kv_heads * c.group >= (int64_t(1) << 30) || c.sequences * c.kv_heads > (int64_t(1) << 24)) {
+    // (a launch holds fewer than 2^32 threads: the most tiles, 2^22 full ones and 2^22 sequences' last ones, have 512 each)
+    if (c.tokens * c.kv_heads * c.group >= (int64_t(1) << 26) || c.sequences * c.kv_heads > (int64_t(1) << 22)) {
         return "more query rows, or KV heads of sequences, than the kernels count";
     }
     if (c.window < 0 || c.first < 0) {
@@ -234,12 +235,18 @@ __attribute__((visibility("default"))) int chroma_hip_paged_chunk_attention(cons
     if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) {
         return refuse("the workspace must start on 16 bytes", error, error_size);
     }
-    const uint64_t size = c.dtype == CHROMA_HIP_BFLOAT16 ? 2 : 4, row = uint64_t(c.kv_heads * c.group * c.dim), last = uint64_t(c.tokens - 1);
-    const uint64_t new_bytes = (last * uint64_t(c.new_stride) + uint64_t(c.kv_heads * c.dim)) * size;
+    using chroma_ranges::bytes_of;
+    const uint64_t size = c.dtype == CHROMA_HIP_BFLOAT16 ? 2 : 4;
+    const int64_t row = c.kv_heads * c.group * c.dim;
+    const uint64_t new_bytes = bytes_of({{c.tokens, c.new_stride}, {c.kv_heads * c.dim, 1}}, size);
+    const uint64_t page_bytes = bytes_of({{c.pages, c.page_stride}, {c.page_rows, c.row_stride}, {c.kv_heads, c.head_stride}, {c.dim, 1}}, size);
+    const int64_t span = (c.longest + c.page_rows - 1) / c.page_rows;
     const chroma_ranges::Range ranges[] = {
-        {c.out, (last * uint64_t(c.out_stride) + row) * size, true}, {workspace, need, true}, {c.q, (last * uint64_t(c.q_stride) + row) * size, false},
-        {c.k_new, new_bytes, false}, {c.v_new, new_bytes, false}, {c.starts, uint64_t(c.sequences + 1) * 8u, false},
-        {c.lengths, uint64_t(c.sequences) * 8u, false}};
+        {c.out, bytes_of({{c.tokens, c.out_stride}, {row, 1}}, size), true}, {workspace, need, true},
+        {c.q, bytes_of({{c.tokens, c.q_stride}, {row, 1}}, size), false}, {c.k_pages, page_bytes, false}, {c.v_pages, page_bytes, false},
+        {c.k_new, new_bytes, false}, {c.v_new, new_bytes, false}, {c.sinks, uint64_t(c.kv_heads * c.group) * size, false},
+        {c.table, span ? bytes_of({{c.sequences, c.table_stride}, {span, 1}}, 8) : 0, false},
+        {c.starts, uint64_t(c.sequences + 1) * 8u, false}, {c.lengths, uint64_t(c.sequences) * 8u, false}};
     if (chroma_ranges::overlap(ranges)) {
         return refuse("out or the workspace overlaps another array", error, error_size);
     }

@@ -357,7 +357,8 @@ int chroma_hip_cache_store(const chroma_hip_cache_store_call* call, void* stream
  *
  * ``starts`` must ascend within [0, tokens]; entries outside count as the nearest bound, a range that descends as empty. Lengths,
  * table rows, bad pages, strides and alignments are as for ``chroma_hip_paged_attention``; new_stride and q_stride count from token to
- * token. */
+ * token. A call has fewer than 2^26 query heads of all tokens and at most 2^22 KV heads of all sequences. ``out`` and the workspace
+ * overlap no other array. */
 typedef struct chroma_hip_paged_chunk_call {
     const void* q;          /* [tokens, kv_heads, group, dim] */
     const void* k_pages;    /* [pages, page_rows, kv_heads, dim] at page_stride, row_stride, head_stride */

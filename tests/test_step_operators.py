@@ -662,6 +662,9 @@ def refused(name, call, workspace=None, size=0):
     (dict(table=None), "null"), (dict(lengths=None), "null"), (dict(starts=None), "null"), (dict(out=None), "null"),
     (dict(q=(1 << 20) + 8), "16 bytes"), (dict(out=(10 << 20) + 4), "16 bytes"), (dict(k_new=(4 << 20) + 2), "16 bytes"),
     (dict(out=1 << 20), "overlaps"), (dict(out=(4 << 20) + 1024), "overlaps"), (dict(out=(8 << 20) - 4096), "overlaps"),
+    (dict(out=(2 << 20) + 32768), "overlaps"), (dict(out=(3 << 20) - 16), "overlaps"), (dict(out=(6 << 20) + 16 - 16), "overlaps"),
+    (dict(out=(7 << 20) + 48), "overlaps"), (dict(q_stride=2**40, out=1 << 30, tokens=2**17), "overlaps"),
+    (dict(page_stride=2**40, pages=2**30, out=1 << 40), "overlaps"), (dict(tokens=2**23), "more query rows"), (dict(sequences=2**15, kv_heads=129), "more query rows"),
 ])
 def test_chunk_refusals(changes, message):
     with pytest.raises(RuntimeError, match="paged_chunk_attention.*" + message):
