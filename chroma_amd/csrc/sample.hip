@@ -35,6 +35,8 @@ constexpr uint32_t kThreads = 512, kBuckets = 2048, kPer = kBuckets / kThreads;
 constexpr uint32_t kList = 4096;   // listed tokens of a row
 constexpr int64_t kMostTop = 1024;  // a larger top_k descends on the whole row
 constexpr float kDepths = 44.0f;   // buckets of the histogram for a factor of 2; the last one holds what weighs nothing
+constexpr int kDeepest = 64;       // depths (in factors of 2) past which weights are not evaluated; from kOne + 1 on they are 0
+static_assert(float(kBuckets) < kDepths * float(kDeepest - 1) && float(kBuckets - 1u) > kDepths * float(kOne + 2), "buckets");
 
 __device__ __forceinline__ uint64_t lesser(uint64_t a, uint64_t b) { return a < b ? a : b; }
 __device__ __forceinline__ uint64_t greater(uint64_t a, uint64_t b) { return a > b ? a : b; }
@@ -48,14 +50,14 @@ __device__ __forceinline__ float value_of(uint32_t order) {
     return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 
-// 2^-i / 256 and 2^-i / 65536 of i < 256, in LDS.
+// 2^(i / 256) and 2^(i / 65536) of i < 256, in LDS.
 struct Powers {
     double high[256], low[256];
     __device__ __forceinline__ void fill() {
         if (threadIdx.x < 512u) {
             const uint32_t i = threadIdx.x % 256u;
-            // the series of exp(-f ln 2), |f| <= 1/2, to the 12th power (the 13th is below 2^-52)
-            const double y = double(i) * (threadIdx.x < 256u ? 1.0 / 256.0 : 1.0 / 65536.0), n = __builtin_rint(y), f = (n - y) * 0.69314718055994530942;
+            // the series of exp(f ln 2), |f| <= 1/2, to the 12th power (the 13th is below 2^-52)
+            const double y = double(i) * (threadIdx.x < 256u ? 1.0 / 256.0 : 1.0 / 65536.0), n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
             double p = 1.0 / 479001600.0;
             p = __builtin_fma(p, f, 1.0 / 39916800.0);
             p = __builtin_fma(p, f, 1.0 / 3628800.0);
@@ -69,7 +71,7 @@ struct Powers {
             p = __builtin_fma(p, f, 0.5);
             p = __builtin_fma(p, f, 1.0);
             p = __builtin_fma(p, f, 1.0);
-            (threadIdx.x < 256u ? high : low)[i] = n == 1.0 ? 0.5 * p : p;
+            (threadIdx.x < 256u ? high : low)[i] = n == 1.0 ? 2.0 * p : p;
         }
         __syncthreads();
     }
@@ -81,21 +83,23 @@ struct Weights {
     double top, rate;  // rate: 65536 log2(e) / temperature
     __device__ __forceinline__ Weights(const Powers& powers, float top, float temperature)
         : powers(powers), top(double(top)), rate(65536.0 * 1.4426950408889634074 / double(temperature)) {}
-    // log2 of the inverse weight, 0 or more, in units of 2^-16
-    __device__ __forceinline__ double depth(float x) const { return double(x) == top ? 0.0 : (top - double(x)) * rate; }
-    __device__ __forceinline__ uint64_t operator()(float x) const {
-        const double y = depth(x);
-        if (!(y < 65536.0 * double(kOne + 1))) {
-            return 0u;
-        }
-        // 2^-(n >> 16), 2^-(its next 8 bits / 256) and 2^-(the last 8 / 65536) from the powers, exp(-f ln 2 / 65536) from three
-        // terms of its series. (Adding 1.5 2^52 rounds to a whole number, which then lies in the low bits: conversions are slow.)
+    // The weight of a logit of finite depth, at most kDeepest.
+    __device__ __forceinline__ uint64_t near(float x) const {
+        // log2 of the weight in units of 2^-16 is n + f, n whole (adding 1.5 2^52 rounds, and n then lies in the low bits:
+        // conversions are slow); 2^(n >> 16), 2^(its next 8 bits / 256) and 2^(the last 8 / 65536) from the powers,
+        // exp(f ln 2 / 65536) from three terms of its series.
         constexpr double c = 0.69314718055994530942 / 65536.0, whole = 6755399441055744.0;
-        const double near = y + whole, f = y - (near - whole), p = __builtin_fma(f, __builtin_fma(f, 0.5 * c * c, -c), 1.0);
-        const uint32_t n = uint32_t(__double_as_longlong(near));
-        const double scale = __hiloint2double(int(1023u + kOne - (n >> 16)) << 20, 0);
+        const double d = double(x) - top, sum = __builtin_fma(d, rate, whole), f = __builtin_fma(d, rate, whole - sum);
+        const double p = __builtin_fma(f, __builtin_fma(f, 0.5 * c * c, c), 1.0);
+        const uint32_t n = uint32_t(__double_as_longlong(sum));
+        const double scale = __hiloint2double(int(((n & 0xffff0000u) << 4) + ((1023u + kOne) << 20)), 0);
         const double all = powers.high[(n >> 8) & 255u] * powers.low[n & 255u] * p;
         return uint64_t(__double_as_longlong(__builtin_fma(all, scale, 4503599627370496.0))) & 0xfffffffffffffull;
+    }
+    // log2 of the inverse weight, 0 or more
+    __device__ __forceinline__ double depth(float x) const { return double(x) == top ? 0.0 : (top - double(x)) * (rate * (1.0 / 65536.0)); }
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        return double(x) == top ? kWhole : depth(x) < double(kDeepest) ? near(x) : 0u;
     }
 };
 
@@ -414,8 +418,10 @@ struct Settings {
     __device__ __forceinline__ Weights weights(const Depths& s) const { return Weights(s.powers, top, temperature); }
     // The histogram's bucket of a logit: it never falls as the logit falls. (Halves: the difference itself may overflow.)
     __device__ __forceinline__ uint32_t bucket(float x, float rate) const {
-        const float t = x == top ? 0.0f : (0.5f * top - 0.5f * x) * rate;
-        return t < float(kBuckets - 1u) ? uint32_t(t) : kBuckets - 1u;
+        return x == top ? 0u : bucket_of_finite(x, rate);
+    }
+    __device__ __forceinline__ uint32_t bucket_of_finite(float x, float rate) const {
+        return uint32_t(fminf((0.5f * top - 0.5f * x) * rate, float(kBuckets - 1u)));
     }
     __device__ __forceinline__ float rate() const { return 2.0f * kDepths * 1.44269504088896341f / temperature; }
     // The sum of weights that the kept tokens of ``sum`` must reach under top_p (at least the first one's).
@@ -432,7 +438,7 @@ struct Settings {
         return 1u + (uniform > 0.0f ? share_of(kept, uniform < 1.0f ? uniform : __uint_as_float(0x3f7fffffu), more) : 0u);
     }
     __device__ __forceinline__ float logprob(const Weights& w, float x, uint64_t kept) const {
-        return float(-w.depth(x) * (0.69314718055994530942 / 65536.0) - log(double(kept) * (1.0 / double(kWhole))));
+        return float(-w.depth(x) * 0.69314718055994530942 - log(double(kept) * (1.0 / double(kWhole))));
     }
 };
 
@@ -503,12 +509,23 @@ template <class T> __device__ void depths(const Settings& set, const T* x, uint3
         }
     } else {
         const Weights w = set.weights(s);
-        visit(x, begin, end, [&](float v, uint32_t) {
-            const uint32_t bucket = set.bucket(v, rate);
-            if (bucket < kBuckets - 1u) {
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[bucket]), static_cast<unsigned long long>(w(v)));
-            }
-        });
+        const auto add = [&](uint32_t bucket, uint64_t weight) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[bucket]), static_cast<unsigned long long>(weight));
+        };
+        if (set.top == __builtin_inff()) {
+            visit(x, begin, end, [&](float v, uint32_t) {
+                if (v == set.top) {
+                    add(0u, kWhole);
+                }
+            });
+        } else {
+            visit(x, begin, end, [&](float v, uint32_t) {
+                const uint32_t bucket = set.bucket_of_finite(v, rate);
+                if (bucket < kBuckets - 1u) {
+                    add(bucket, w.near(v));
+                }
+            });
+        }
     }
     __syncthreads();
 }
