@@ -133,15 +133,19 @@ struct Place {
 };
 
 // LDS of a workgroup that takes a histogram, and of one that draws.
-struct Depths {
-    uint64_t weight[kBuckets];
-    uint64_t before[kBuckets + 1];  // sums before each bucket, and of all
-    uint32_t count[kBuckets];
-    Powers powers;
+struct Waves {
     Sums waves[kThreads / 64u];
     uint32_t last;
 };
+struct Depths : Waves {  // (at most 40 KB: four workgroups of a compute unit)
+    uint64_t weight[kBuckets];
+    uint64_t before[kBuckets + 1];  // sums before each bucket, and of all
+    Powers powers;
+    __device__ __forceinline__ uint32_t* counts() { return reinterpret_cast<uint32_t*>(before); }
+};
+static_assert(sizeof(Depths) <= 40u * 1024u, "LDS");
 struct Shared : Depths {
+    uint32_t count[kBuckets];
     uint64_t list[kList];  // selection keys
     uint64_t few[64];
     uint64_t ends[kThreads / 64u];
@@ -194,7 +198,7 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 }
 
 // Sums over the workgroup.
-__device__ Sums sum_all(Depths& s, Sums own) {
+__device__ Sums sum_all(Waves& s, Sums own) {
     const Sums wave{wave_total(own.weight), uint32_t(__builtin_amdgcn_readlane(wave_scan(own.count), 63))};
     if (threadIdx.x % 64u == 0u) {
         s.waves[threadIdx.x / 64u] = wave;
@@ -211,7 +215,7 @@ __device__ Sums sum_all(Depths& s, Sums own) {
 }
 
 // The largest of the workgroup's values.
-__device__ uint64_t max_all(Depths& s, uint64_t own) {
+__device__ uint64_t max_all(Waves& s, uint64_t own) {
     own = wave_max(own);
     if (threadIdx.x % 64u == 0u) {
         s.waves[threadIdx.x / 64u].weight = own;
@@ -226,7 +230,7 @@ __device__ uint64_t max_all(Depths& s, uint64_t own) {
 }
 
 // Inclusive sums over the workgroup's threads, in their order.
-__device__ Sums scan_all(Depths& s, Sums own) {
+__device__ Sums scan_all(Waves& s, Sums own) {
     const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
     own.weight = wave_scan(own.weight);
     own.count = wave_scan(own.count);
@@ -277,7 +281,7 @@ template <class T, class F> __device__ __forceinline__ void visit(const T* x, ui
 }
 
 // The largest logit's order and the lowest id that has it, as a selection key, of [begin, end).
-template <class T> __device__ uint64_t largest(Depths& s, const T* x, uint32_t begin, uint32_t end) {
+template <class T> __device__ uint64_t largest(Waves& s, const T* x, uint32_t begin, uint32_t end) {
     uint32_t best = 0, id = 0xffffffffu;
     visit(x, begin, end, [&](float v, uint32_t i) {
         const uint32_t order = order_of(v);
@@ -490,9 +494,10 @@ constexpr uint32_t kNone = 0x7fffffffu;
 // The histogram of [begin, end) in s.weight: weights, or counts where a top-k cuts the row; the last bucket's are left out (its
 // tokens weigh nothing, and most of a row may lie there).
 template <class T> __device__ void depths(const Settings& set, const T* x, uint32_t begin, uint32_t end, Depths& s) {
+    uint32_t* counts = s.counts();
     for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
         s.weight[i] = 0u;
-        s.count[i] = 0u;
+        counts[i] = 0u;
     }
     __syncthreads();
     const float rate = set.rate();
@@ -500,12 +505,12 @@ template <class T> __device__ void depths(const Settings& set, const T* x, uint3
         visit(x, begin, end, [&](float v, uint32_t) {
             const uint32_t bucket = set.bucket(v, rate);
             if (bucket < kBuckets - 1u) {
-                atomicAdd(&s.count[bucket], 1u);
+                atomicAdd(&counts[bucket], 1u);
             }
         });
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
-            s.weight[i] = s.count[i];
+            s.weight[i] = counts[i];
         }
     } else {
         const Weights w = set.weights(s);
@@ -882,8 +887,8 @@ struct Span {
 };
 
 // The first reading: each span's largest logit. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_best(Call c, uint64_t* scratch) {
-    __shared__ Depths s;
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_best(Call c, uint64_t* scratch) {
+    __shared__ Waves s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
     const Span span(c, gridDim.x, blockIdx.x);
@@ -906,7 +911,7 @@ __device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
 }
 
 // Whether this workgroup is the last of the row's to come here, after its device-scope stores.
-__device__ bool comes_last(uint32_t* ticket, Depths& s) {
+__device__ bool comes_last(uint32_t* ticket, Waves& s) {
     chroma::device_stores_complete();
     __syncthreads();
     if (threadIdx.x == 0u) {
@@ -919,7 +924,7 @@ __device__ bool comes_last(uint32_t* ticket, Depths& s) {
 }
 
 // The second reading: the histogram, and what is listed. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_depths(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(Call c, uint64_t* scratch) {
     __shared__ Depths s;
     s.powers.fill();
     const uint64_t r = blockIdx.y;
@@ -967,7 +972,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_depths(
 }
 
 // The third reading: the list. grid: (spans, rows)
-template <class T> __global__ void __launch_bounds__(kThreads, 6) sample_listed(Call c, uint64_t* scratch) {
+template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_listed(Call c, uint64_t* scratch) {
     __shared__ Gathered s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
