@@ -602,9 +602,11 @@ struct Listed {
     uint64_t key, before;  // before: the sum of weights (or the count) of the tokens before it
 };
 
-// Among the ``n`` keys of s.list in [low, high]: where counts or weights, ``before`` of them before the first, reach ``goal``.
-// Eleven bits of the keys a step, until 64 keys are left; each wave then compares those by itself.
-__device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_count, uint64_t before, uint64_t goal, uint64_t low, uint64_t high) {
+// Among those of the ``n`` keys of s.list that ``in`` takes, all in some range of them: where counts or weights, ``before`` of
+// them before the first, reach ``goal``. Eleven bits of the keys a step, until 64 keys are left; each wave then compares those
+// by itself.
+template <class F> __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_count, uint64_t before, uint64_t goal, F in) {
+    uint64_t low = 0, high = ~0ull;
     const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u;
     const auto weight_of = [&](uint64_t key) { return by_count ? uint64_t(1) : w(value_of(uint32_t(key >> 32))); };
     for (int step = 0; step < 8; ++step) {
@@ -615,7 +617,7 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
         }
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t key = s.list[i];
-            if (key >= low && key <= high) {
+            if (step ? key >= low && key <= high : in(key)) {
                 most = greater(key, most);
                 least = greater(~key, least);
                 ++left;
@@ -637,6 +639,8 @@ __device__ Listed reach_list(const Weights& w, Shared& s, uint32_t n, bool by_co
             left += s.waves[v].count;
         }
         least = ~least;
+        low = greater(low, least);
+        high = lesser(high, most);
         if (left <= 64u) {
             for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
                 const uint64_t key = s.list[i];
@@ -743,19 +747,8 @@ __device__ void choose_few(const Call& c, uint64_t r, const Settings& set, const
 template <class B> __device__ void choose(const Call& c, uint64_t r, const Settings& set, const Listing& l, uint32_t n, B below, Shared& s) {
     const Weights w = set.weights(s);
     const float rate = set.rate();
-    // the keys of bucket b: those of the list between its largest and its smallest
     const auto reach = [&](uint32_t b, uint64_t goal) {
-        uint64_t most = 0, least = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const uint64_t key = s.list[i];
-            if (set.bucket(value_of(uint32_t(key >> 32)), rate) == b) {
-                most = key > most ? key : most;
-                least = ~key > least ? ~key : least;
-            }
-        }
-        most = max_all(s, most);
-        least = ~max_all(s, least);
-        return reach_list(w, s, n, false, below(b), goal, least, most);
+        return reach_list(w, s, n, false, below(b), goal, [&](uint64_t key) { return set.bucket(value_of(uint32_t(key >> 32)), rate) == b; });
     };
     const auto weight_of = [&](uint64_t key) { return w(value_of(uint32_t(key >> 32))); };
     const auto at_least = [&](uint64_t least, uint32_t from, uint32_t to) {  // sum of the listed weights of these buckets
@@ -776,7 +769,7 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
             return;
         }
         // (fewer are listed where the top-k takes tokens that weigh nothing)
-        const uint64_t last = n > uint64_t(set.top_k) ? reach_list(w, s, n, true, 0u, uint64_t(set.top_k), 0u, ~0ull).key : 0u;
+        const uint64_t last = n > uint64_t(set.top_k) ? reach_list(w, s, n, true, 0u, uint64_t(set.top_k), [](uint64_t) { return true; }).key : 0u;
         if (threadIdx.x == 0u) {
             s.fews = 0u;
         }
@@ -791,18 +784,19 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
             }
         }
         kept = sum_all(s, own).weight;
+        const auto counted = [&](uint64_t key) { return key >= last; };
         if (set.top_k <= 64) {
             choose_few(c, r, set, w, s.few, uint32_t(set.top_k));
             return;
         }
         if (set.top_p < 1.0f) {
-            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), last, ~0ull);
+            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), counted);
             kept = cut.before + weight_of(cut.key);
         }
         if (set.min_p > 0.0f) {
             kept = lesser(kept, greater(at_least(set.least(), 0u, kBuckets), kWhole));
         }
-        drawn = reach_list(w, s, n, false, 0u, set.place(kept), last, ~0ull);
+        drawn = reach_list(w, s, n, false, 0u, set.place(kept), counted);
     } else {
         kept = below(kBuckets);
         if (set.top_p < 1.0f) {
@@ -946,20 +940,27 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(
     if (!comes_last(mine.tickets, s)) {
         return;
     }
-    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
-        uint64_t sum = 0;
-        for (uint32_t k0 = 0; k0 < spans; k0 += 8u) {
-            uint64_t some[8];
+    uint64_t sums[kPer] = {};
+    for (uint32_t k0 = 0; k0 < spans; k0 += 4u) {  // (16 loads under way)
+        uint64_t some[4][kPer];
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k) {
-                some[k] = chroma::load_device(mine.histogram + uint64_t(min(k0 + k, spans - 1u)) * kBuckets + i);
-            }
+        for (uint32_t k = 0; k < 4u; ++k) {
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k) {
-                sum += k0 + k < spans ? some[k] : 0u;
+            for (uint32_t e = 0; e < kPer; ++e) {
+                some[k][e] = chroma::load_device(mine.histogram + uint64_t(min(k0 + k, spans - 1u)) * kBuckets + threadIdx.x + e * kThreads);
             }
         }
-        s.weight[i] = sum;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+#pragma unroll
+            for (uint32_t e = 0; e < kPer; ++e) {
+                sums[e] += k0 + k < spans ? some[k][e] : 0u;
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e) {
+        s.weight[threadIdx.x + e * kThreads] = sums[e];
     }
     __syncthreads();
     const Listing l = list_of(set, s);
