@@ -297,6 +297,36 @@ def test_drawing_on_the_host(width, dtype):
     assert draw(np.array([1, np.inf, np.inf, 0], np.float32), Sampling(), 0.75) == (2, pytest.approx(math.log(0.5)))
 
 
+def near_places():
+    """(row, random number, token) where the drawn place is the last of its token, in sums past 2^53: of n equal logits and a small
+    one, u n is 1 below a multiple of 2^24, and the small weight's share lifts the place to 1 below that token's end."""
+    found = []
+    for n in range(2001, 2601, 2):
+        u = -pow(n, -1, 2**24) % 2**24
+        x = np.float32(math.log((2**20 - 1) * 2**24 / u) - 44 * math.log(2))
+        small = int(np.rint(math.exp(float(x)) * 2.0**44))
+        place = u * (n * 2**44 + small) >> 24
+        if place % 2**44 == 2**44 - 1:
+            found.append((np.append(np.zeros(n, np.float32), x), u / 2**24, place >> 44))
+    return found
+
+
+def test_places_next_to_a_border_past_53_bits():
+    cases = near_places()
+    assert len(cases) >= 3
+    for row, u, token in cases:
+        assert draw(row, Sampling(), u)[0] == token
+
+
+@gpu
+def test_places_next_to_a_border_past_53_bits_on_the_device():
+    for row, u, token in near_places():
+        x = torch.from_numpy(row).cuda()[None]
+        ids, logprobs = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, device="cuda")
+        queue_in("chroma_hip_rows_sample", sample_call(x, ids, logprobs, uniform=torch.tensor([u], device="cuda")))
+        assert int(ids) == token
+
+
 def test_sampling_of_a_decoder_on_the_host(tmp_path):
     model = small_model()
     programs = [compile_cpu(export_cached(model, CONTEXT, steps), tmp_path / f"p{steps}") for steps in (CONTEXT, 1)]
