@@ -321,9 +321,9 @@ def test_places_next_to_a_border_past_53_bits():
 @gpu
 def test_places_next_to_a_border_past_53_bits_on_the_device():
     for row, u, token in near_places():
-        x = torch.from_numpy(row).cuda()[None]
+        x, uniform = torch.from_numpy(row).cuda()[None], torch.tensor([u], device="cuda")
         ids, logprobs = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, device="cuda")
-        queue_in("chroma_hip_rows_sample", sample_call(x, ids, logprobs, uniform=torch.tensor([u], device="cuda")))
+        queue_in("chroma_hip_rows_sample", sample_call(x, ids, logprobs, uniform=uniform))
         assert int(ids) == token
 
 
