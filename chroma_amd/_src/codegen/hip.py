@@ -2586,13 +2586,20 @@ class HIPCodegen(Codegen):
             blocks = -(-rows // keys) + 1
             return min(blocks, (min(first, rows) + min(window, rows)) // keys + 3) if window else blocks
 
-        if item != 2 or tokens * group < 64 * sequences or tokens * group * kv_heads < 128 * 64:
+        keys, heads = 32 if padded > 128 else 64, tokens * group * kv_heads
+        if item != 2 or tokens * group < 64 * sequences or (heads < 128 * 64 and heads * most_blocks(keys) * keys < 10000000):
             wide = 0
         else:
             wide = 8 if padded == 128 and tiles_of(256) * kv_heads >= 512 else 4
         tiles = tiles_of(32 * wide if wide else 16)
-        wanted = -(-512 // (tiles * kv_heads))
-        most = most_blocks(32 if padded > 128 else 64) // 4 if wide else most_blocks(half) // (2 * waves)
+        units, rounds = tiles * kv_heads, most_blocks(half) // waves
+        wanted = -(-512 // units)
+        if wide:
+            most = most_blocks(keys) // 5
+        elif units >= 256:
+            most = 1
+        else:
+            most = min(rounds // 2, 32) if padded < 128 else max(min(256 // units, rounds // 2), (rounds + 2) // 4)
         return wide, tiles, max(1, min(wanted, most))
 
     def paged_chunk_attention(self, meta, q: Value, k_pages: Value, v_pages: Value, k_new: Optional[Value], v_new: Optional[Value], table: Value,
