@@ -138,15 +138,16 @@ struct Cut {
 // The 16-row tiles have eight waves share a tile's keys: quick where there are few rows, while the tiles of 128 rows read each
 // key 8 times less often. 32 tokens over 900 rows 12.5 (16 rows) and 19.8 (128 rows), over 8000 33 and 25; 64 over 2000 20 and
 // 20, over 8000 54 and 32; 256 over 900 35 and 22; 32 sequences of 16 over 2000 100 and 52; but below 64 rows a sequence most of
-// a large tile is empty: 32 of 4 tokens over 2000 31 and 39. D 128, 64 tokens over 2000: 21 and 25; over 16000 58 and 54.
+// a large tile is empty: 32 of 4 tokens over 2000 31 and 39. D 128, 64 tokens over 2000: 21 and 25; 32 over
+// 16000 58 and 54.
 // Eight waves a tile read the keys half as often, once tiles are many: D 128, 2 x 2048 tokens over 4000 419 with four and 378;
 // 512 over 900 37 with four and 52. With D 64 they gain nothing.
 //
 // Keys are split for 512 workgroups (with 256, 8 x 32 tokens over 2000 take 41 instead of 35; with 1024, D 128, 4 x 512 over 900
-// 97 instead of 72), but not into so little that the second launch costs more: five blocks of a large tile (256
-// over 900 in three parts 24, in four 22), two blocks a wave of a small one and at most 32 parts (one token over 30000 rows, 58 parts 40, 32
-// parts 31), no parts for 256 small tiles or more (64 over 900 in two 16, in one 13), and with D 128, whose parts are larger, four
-// blocks a wave where there are 256 workgroups (64 over 2000 in four 25, in two 20).
+// 97 instead of 72), but not into so little that the second launch costs more: five blocks of a large tile (256 over 900 in
+// three parts 24, in four 22), two blocks a wave of a small one and at most 32 parts (one token over 30000 rows, 58 parts 40,
+// 32 parts 31), no parts for 256 small tiles or more (64 over 900 in two 16, in one 13), and with D 128, whose parts are
+// larger, four blocks a wave where there are 256 workgroups (64 over 2000 in four 25, in two 20).
 template <class T, int DP> Cut cut_of(const Call& c) {
     constexpr int64_t wide = chroma::chunk_wide_keys<DP>(), few = chroma::paged_whole_keys<T, DP>(), few_waves = chroma::paged_whole_waves<T, DP>();
     Cut cut;
