@@ -64,13 +64,13 @@ template <uint32_t ROWS, bool LONGEST, class T> __device__ __forceinline__ bool 
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.sequences; b0 += kWave) {
         ChunkRows rows{0u, 0u};
-        uint32_t own = 0, order = lane;
+        uint32_t own = 0, order = lane, held = 0;
         if (b0 + lane < a.sequences) {
             rows = chunk_rows(a, b0 + lane);
+            held = paged_length(a, b0 + lane);  // (under way together)
             own = ((rows.end - rows.begin) * a.group + ROWS - 1u) / ROWS;
         }
         if (LONGEST && a.sequences <= uint32_t(kWave)) {
-            const uint32_t held = lane < a.sequences ? paged_length(a, lane) : 0u;
             uint32_t rank = 0;
             for (uint32_t i = 0; i < a.sequences; ++i) {
                 const uint32_t other = __builtin_amdgcn_readlane(held, i);
@@ -89,7 +89,7 @@ template <uint32_t ROWS, bool LONGEST, class T> __device__ __forceinline__ bool 
             const uint32_t count = __builtin_amdgcn_readlane(rows.end, sequence) - tile.begin, place = index - __builtin_amdgcn_readlane(upto - own, at);
             tile.rows = count * a.group;
             tile.row = (LONGEST ? __builtin_amdgcn_readlane(own, at) - 1u - place : place) * ROWS;
-            tile.length = paged_length(a, tile.b);
+            tile.length = __builtin_amdgcn_readlane(held, sequence);
             tile.base = int32_t(tile.length) - (a.k_new ? 0 : int32_t(count));
             const uint32_t last = (tile.row + ROWS < tile.rows ? tile.row + ROWS : tile.rows) - 1u;
             tile.first_position = tile.base + int32_t(tile.row / a.group);
@@ -115,6 +115,14 @@ struct ChunkSight {
         head = position < 0 ? 0u : a.first <= uint32_t(position) ? a.first : uint32_t(position) + 1u;
     }
     __device__ __forceinline__ bool operator()(uint32_t j) const { return j - low <= span || j < head; }
+    // Bit r: whether it sees row begin + r, r < 64.
+    __device__ __forceinline__ unsigned long long bits(uint32_t begin) const {
+        const auto below = [&](uint32_t end) {  // rows before ``end``
+            const int32_t n = int32_t(end) - int32_t(begin);
+            return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
+        };
+        return (below(low + span + 1u) & ~below(low)) | below(head);  // (low + span + 1 is 0 where it sees none)
+    }
 };
 
 template <class T> __device__ __forceinline__ bool chunk_not_finite(T v) {
@@ -662,23 +670,17 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                 }
             }
             // rows that some of the wave's tokens do not see (the chunk's own, the window's first), and rows that are not there
-            if (int32_t(begin + KEYS - 1u) > first_position ||
-                (a.window && int64_t(begin) + a.window <= int64_t(last_position) && begin + KEYS > a.first)) {
+            const bool some = int32_t(begin + KEYS - 1u) > first_position ||
+                              (a.window && int64_t(begin) + a.window <= int64_t(last_position) && begin + KEYS > a.first);
+            if (some || here != EVERY) {
+                const unsigned long long visible = some ? here & sight.bits(begin) : here;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
+                    const uint32_t bits = uint32_t(visible >> (32 * t)) >> (4u * half);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        s[t][e] = sight(begin + t * 32u + 8u * (e / 4) + 4u * half + e % 4) ? s[t][e] : neg_inf;
-                    }
-                }
-            }
-            if (here != EVERY) {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    const uint32_t bits = uint32_t(here >> (32 * t)) >> (4u * half);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        s[t][e] = (bits >> (8 * (e / 4) + e % 4)) & 1u ? s[t][e] : neg_inf;
+                    for (int e = 0; e < 16; ++e) {  // a bit spread over a word chooses the score's bits or those of -inf
+                        const uint32_t mask = uint32_t(__builtin_amdgcn_sbfe(int(bits), 8 * (e / 4) + e % 4, 1));
+                        s[t][e] = __uint_as_float((__float_as_uint(s[t][e]) & mask) | (0xff800000u & ~mask));
                     }
                 }
             }
