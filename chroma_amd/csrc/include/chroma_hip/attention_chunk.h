@@ -358,12 +358,22 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
     }
 };
 
+// Four values of a result, rounded by the conversion instruction.
+template <class T> __device__ __forceinline__ void chunk_store4(T* to, f32x4_t v) {
+    if constexpr (sizeof(T) == 2) {
+        const bf16x2_t lo = __builtin_convertvector(f32x2_t{v[0], v[1]}, bf16x2_t), hi = __builtin_convertvector(f32x2_t{v[2], v[3]}, bf16x2_t);
+        *reinterpret_cast<uint2*>(to) = uint2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    } else {
+        *reinterpret_cast<f32x4_t*>(to) = v;
+    }
+}
+
 // A row's result from parts of (maximum, sum, p . v); where a sum is 0 the row saw nothing.
 template <class T>
 __device__ __forceinline__ void chunk_store(const ChunkOperands<T>& a, const ChunkTile& tile, uint32_t kv, uint32_t r, uint32_t d, f32x4_t sum,
                                             float total) {
     const uint32_t row = tile.row + r;
-    paged_store4<T>(a.out + (tile.begin + row / a.group) * a.out_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim + d,
+    chunk_store4<T>(a.out + (tile.begin + row / a.group) * a.out_stride + (uint64_t(kv) * a.group + row % a.group) * a.dim + d,
                     sum * (total == 0.0f ? 0.0f : 1.0f / total));
 }
 
@@ -780,7 +790,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
             for (int e = 0; e < 16; e += 4) {
                 const uint32_t d = dt * 32u + 2u * e + 4u * half;
                 if (FULL || d < a.dim) {
-                    paged_store4<uint16_t>(to + d, f32x4_t{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * scaled);
+                    chunk_store4<uint16_t>(to + d, f32x4_t{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * scaled);
                 }
             }
         }
