@@ -700,6 +700,56 @@ template <class F> __device__ Listed reach_list(const Weights& w, Shared& s, uin
     return Listed{low, before};
 }
 
+// The bin of a key whose bits from ``shift`` + 11 on are those of all others: bin 0 holds the largest ones.
+__device__ __forceinline__ uint32_t bin_of(uint64_t key, uint32_t shift) { return kBuckets - 1u - uint32_t(key >> shift) % kBuckets; }
+
+// The ``n`` > 1 listed keys in bins by their first eleven bits that differ: counts and weights before each bin in s.count and
+// s.before (and of all in s.before[kBuckets]). Returns the bits' shift.
+__device__ uint32_t ordered(const Weights& w, Shared& s, uint32_t n) {
+    uint64_t most = 0, least = 0;  // least: of the inverted keys
+    for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+        s.weight[i] = 0u;
+        s.count[i] = 0u;
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        most = greater(s.list[i], most);
+        least = greater(~s.list[i], least);
+    }
+    most = max_all(s, most);
+    least = ~max_all(s, least);
+    const int bits = 64 - __builtin_clzll(most ^ least);
+    const uint32_t shift = bits > 11 ? uint32_t(bits - 11) : 0u;
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t key = s.list[i];
+        const uint32_t bin = bin_of(key, shift);
+        atomicAdd(&s.count[bin], 1u);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[bin]), static_cast<unsigned long long>(w(value_of(uint32_t(key >> 32)))));
+    }
+    __syncthreads();
+    const uint32_t first = threadIdx.x * kPer;
+    Sums own{0u, 0u};
+#pragma unroll
+    for (uint32_t k = 0; k < kPer; ++k) {
+        own.weight += s.weight[first + k];
+        own.count += s.count[first + k];
+    }
+    const Sums upto = scan_all(s, own);
+    Sums at{upto.weight - own.weight, upto.count - own.count};
+#pragma unroll
+    for (uint32_t k = 0; k < kPer; ++k) {
+        const Sums here{s.weight[first + k], s.count[first + k]};
+        s.before[first + k] = at.weight;
+        s.count[first + k] = at.count;
+        at.weight += here.weight;
+        at.count += here.count;
+    }
+    if (threadIdx.x == kThreads - 1u) {
+        s.before[kBuckets] = upto.weight;
+    }
+    __syncthreads();
+    return shift;
+}
+
 // Lists the tokens of [begin, end): s.listed of them, the first kList to come in s.list.
 template <class T, class S> __device__ void gather(const Settings& set, const Listing& l, const T* x, uint32_t begin, uint32_t end, S& s) {
     if (threadIdx.x == 0u) {
@@ -772,35 +822,38 @@ template <class B> __device__ void choose(const Call& c, uint64_t r, const Setti
             choose_few(c, r, set, w, s.list, n);
             return;
         }
-        // (fewer are listed where the top-k takes tokens that weigh nothing)
-        const uint64_t last = n > uint64_t(set.top_k) ? reach_list(w, s, n, true, 0u, uint64_t(set.top_k), [](uint64_t) { return true; }).key : 0u;
-        if (threadIdx.x == 0u) {
-            s.fews = 0u;
-        }
-        __syncthreads();
-        Sums own{0u, 0u};
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            if (s.list[i] >= last) {
-                own.weight += weight_of(s.list[i]);
-                if (set.top_k <= 64) {
-                    s.few[atomicAdd(&s.fews, 1u)] = s.list[i];
+        // One histogram over the keys' first bits that differ answers every cut but for the keys of a bin (fewer than top_k are
+        // listed where the top-k takes tokens that weigh nothing).
+        const uint32_t shift = ordered(w, s, n);
+        const auto within = [&](uint32_t bin, bool by_count, uint64_t goal) {
+            return reach_list(w, s, n, by_count, by_count ? uint64_t(s.count[bin]) : s.before[bin], goal, [&](uint64_t key) { return bin_of(key, shift) == bin; });
+        };
+        kept = s.before[kBuckets];
+        if (n > uint64_t(set.top_k)) {
+            for (uint32_t i = threadIdx.x; i < kBuckets; i += kThreads) {
+                if (s.count[i] < set.top_k && (i + 1u < kBuckets ? s.count[i + 1u] : n) >= set.top_k) {
+                    s.last = i;
                 }
             }
-        }
-        kept = sum_all(s, own).weight;
-        const auto counted = [&](uint64_t key) { return key >= last; };
-        if (set.top_k <= 64) {
-            choose_few(c, r, set, w, s.few, uint32_t(set.top_k));
-            return;
+            __syncthreads();
+            const uint32_t bin = s.last;
+            const uint64_t last = within(bin, true, uint64_t(set.top_k)).key;
+            Sums own{0u, 0u};
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                own.weight += s.list[i] >= last && bin_of(s.list[i], shift) == bin ? weight_of(s.list[i]) : 0u;
+            }
+            kept = s.before[bin] + sum_all(s, own).weight;
         }
         if (set.top_p < 1.0f) {
-            const Listed cut = reach_list(w, s, n, false, 0u, set.nucleus(kept), counted);
+            const uint64_t goal = set.nucleus(kept);
+            const Listed cut = within(bucket_of(s, goal), false, goal);
             kept = cut.before + weight_of(cut.key);
         }
         if (set.min_p > 0.0f) {
             kept = lesser(kept, greater(at_least(set.least(), 0u, kBuckets), kWhole));
         }
-        drawn = reach_list(w, s, n, false, 0u, set.place(kept), counted);
+        const uint64_t goal = set.place(kept);
+        drawn = within(bucket_of(s, goal), false, goal);
     } else {
         kept = below(kBuckets);
         if (set.top_p < 1.0f) {
