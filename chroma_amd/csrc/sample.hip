@@ -572,6 +572,10 @@ __device__ Listing list_of(const Settings& set, Depths& s) {
     }
     __syncthreads();
     Listing l{0u, 0u, kNone, kNone, 0u, kNone, 0u};
+    if (!(set.rate() < __builtin_inff())) {  // a temperature below 2^-121 has no depths in float
+        l.whole = 1u;
+        return l;
+    }
     if (set.top_k) {
         l.by_count = 1u;
         // (a top-k that takes tokens of the last bucket takes all the others)

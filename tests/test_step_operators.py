@@ -870,6 +870,19 @@ def test_sample_of_settings_at_their_ends(dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("width", [900, 40000])
+def test_sample_at_the_least_temperatures(width, dtype):
+    """Temperatures whose inverse is no float, with logits that differ by as little, and with others."""
+    temperature = torch.tensor([1e-36, 3e-37, 1e-37, 1e-38, 1e-40, 1e-45, 1e-45, 1e-38])
+    x = torch.randn(8, width, generator=torch.Generator().manual_seed(9))
+    x = torch.cat((x[:6] * temperature[:6, None].clamp(min=1e-38), x[6:])).to(dtype)
+    uniform = torch.rand(8, generator=torch.Generator().manual_seed(2))
+    for filters in ({}, {"top_k": torch.full((8,), 50)}, {"top_p": torch.full((8,), 0.9)}, {"min_p": torch.full((8,), 0.1)}):
+        check_sample(x, uniform=uniform, temperature=temperature, **filters)
+
+
+@gpu
+@BOTH
 def test_sample_layouts(dtype):
     """Rows apart and off any alignment, no logprobs."""
     room = torch.full((9, 1333), math.nan, dtype=dtype)
