@@ -3,13 +3,14 @@
 // Every filter keeps a prefix of the row's descending order, and the drawn token is a place in it, so that all of them ask the
 // same question: after which token does a running count, or a running sum of weights, reach a goal. A histogram of weights
 // (of counts where a top-k cuts the row) over the depths below the maximum answers it but for the tokens of a few buckets;
-// those are listed, and the places among them found by descending on their keys. A row is read three times: for its maximum,
-// for the histogram, for the list; the second and third time it lies in the caches.
+// those are listed, and the places among them found by descending on their keys. A row is read three times: for its ends, by which
+// the buckets are spread over the depths that it has, for the histogram, for the list; the second and third time it lies in the
+// caches.
 //
 // Narrow rows have a workgroup each and one launch. Wide ones are cut into spans, and the three readings are launches of their
 // own; the workgroup that comes last with a row's histogram decides what is listed, and a fourth launch draws. Rows of up to kList tokens
-// are listed whole. Where the listed buckets hold more than kList tokens (rows of equal values, temperatures that leave
-// few depths), a workgroup descends on the keys of the whole row.
+// are listed whole. Where the listed buckets hold more than kList tokens (rows of few values), a workgroup descends on the
+// keys of the whole row.
 //
 // What bounds it: one row of 201088 float logits (28 us) the four launches' chains (readings of 3.4, 13, 4.3 and 7 us; of the second
 // 3 are the span's weights and 8 the sum of 24 spans' histograms and the cuts); 256 rows of 100003 (85 us) the weights' vector work:
@@ -38,7 +39,8 @@ constexpr uint64_t kWhole = uint64_t(1) << kOne;
 constexpr uint32_t kThreads = 512, kBuckets = 2048, kPer = kBuckets / kThreads;
 constexpr uint32_t kList = 4096;   // listed tokens of a row
 constexpr int64_t kMostTop = 1024;  // a larger top_k descends on the whole row
-constexpr float kDepths = 44.0f;   // buckets of the histogram for a factor of 2; the last one holds what weighs nothing
+constexpr float kDepths = 44.0f;   // buckets of the histogram for a factor of 2, where not all of a row lies in fewer factors
+constexpr float kFinest = 65536.0f;  // and at most: more would not be exact in float
 constexpr int kDeepest = 64;       // depths (in factors of 2) past which weights are not evaluated; from kOne + 1 on they are 0
 static_assert(float(kBuckets) < kDepths * float(kDeepest - 1) && float(kBuckets - 1u) > kDepths * float(kOne + 2), "buckets");
 
@@ -284,15 +286,36 @@ template <class T, class F> __device__ __forceinline__ void visit(const T* x, ui
     }
 }
 
-// The largest logit's order and the lowest id that has it, as a selection key, of [begin, end).
-template <class T> __device__ uint64_t largest(Waves& s, const T* x, uint32_t begin, uint32_t end) {
-    uint32_t best = 0, id = 0xffffffffu;
+constexpr uint32_t kFinite = 0x00800000u;  // the least finite value's order
+
+// The ends of a row: its largest logit's order and the lowest id that has it, as a selection key, and its least finite logit.
+struct Ends {
+    uint64_t best;
+    uint32_t least;  // its order from kFinite on, inverted; 0: there is none
+    __device__ __forceinline__ float low() const { return value_of(~least + kFinite); }  // (-inf)
+};
+// Of [begin, end).
+template <class T> __device__ Ends ends_of(Waves& s, const T* x, uint32_t begin, uint32_t end) {
+    uint32_t best = 0, id = 0xffffffffu, least = 0xffffffffu;
     visit(x, begin, end, [&](float v, uint32_t i) {
         const uint32_t order = order_of(v);
         id = order > best ? i : id;  // (a thread's ids ascend)
         best = order > best ? order : best;
+        least = min(least, order - kFinite);  // (-inf wraps)
     });
-    return max_all(s, uint64_t(best) << 32 | uint64_t(0xffffffffu - id));
+    const Sums wave{wave_max(uint64_t(best) << 32 | uint64_t(0xffffffffu - id)), wave_max(~least)};
+    if (threadIdx.x % 64u == 0u) {
+        s.waves[threadIdx.x / 64u] = wave;
+    }
+    __syncthreads();
+    Ends ends{0u, 0u};
+#pragma unroll
+    for (uint32_t v = 0; v < kThreads / 64u; ++v) {
+        ends.best = greater(s.waves[v].weight, ends.best);
+        ends.least = max(s.waves[v].count, ends.least);
+    }
+    __syncthreads();
+    return ends;
 }
 
 // A whole row, for descending on its keys.
@@ -408,12 +431,21 @@ struct Settings {
     int64_t top_k;
     uint32_t best;  // id of the largest logit
     bool nan;
+    float depths;  // buckets for a factor of 2: the last one holds what weighs nothing, the others all the rest
+    __device__ __forceinline__ Settings(const Call& c, uint64_t r, const Ends& ends) : Settings(c, r, ends.best) {
+        const float factors = 2.0f * 1.44269504088896341f * (0.5f * top - 0.5f * ends.low()) / temperature;
+        depths = factors * kDepths < float(kBuckets - 2u) ? fminf(float(kBuckets - 2u) / factors, kFinest) : kDepths;
+    }
+
+private:
     __device__ __forceinline__ Settings(const Call& c, uint64_t r, uint64_t key)
         : temperature(c.temperature ? c.temperature[r] : 1.0f), top_p(c.top_p ? c.top_p[r] : 1.0f), min_p(c.min_p ? c.min_p[r] : 0.0f),
           uniform(c.uniform[r]), top_k(c.top_k ? c.top_k[r] : 0), best(0xffffffffu - uint32_t(key)), nan(key >> 32 == 0xffffffffu) {
         top = value_of(uint32_t(key >> 32));
         top_k = top_k >= c.width || top_k < 0 ? 0 : top_k;
     }
+
+public:
     // Whether the largest logit decides alone; ``finish`` then writes the result.
     __device__ __forceinline__ bool greedy() const { return nan || top == -__builtin_inff() || !(temperature > 0.0f); }
     __device__ __forceinline__ void finish(const Call& c, uint64_t r) const {
@@ -431,7 +463,7 @@ struct Settings {
     __device__ __forceinline__ uint32_t bucket_of_finite(float x, float rate) const {
         return uint32_t(fminf((0.5f * top - 0.5f * x) * rate, float(kBuckets - 1u)));
     }
-    __device__ __forceinline__ float rate() const { return 2.0f * kDepths * 1.44269504088896341f / temperature; }
+    __device__ __forceinline__ float rate() const { return 2.0f * depths * 1.44269504088896341f / temperature; }
     // The sum of weights that the kept tokens of ``sum`` must reach under top_p (at least the first one's).
     __device__ __forceinline__ uint64_t nucleus(uint64_t sum) const {
         bool more = false;
@@ -593,7 +625,7 @@ __device__ Listing list_of(const Settings& set, Depths& s) {
     }
     if (set.min_p > 0.0f) {
         // the least weight's bucket, and one on either side for the rounding of a logit's
-        const float t = -__log2f(set.min_p > 1.0f ? 1.0f : set.min_p) * kDepths;
+        const float t = -__log2f(set.min_p > 1.0f ? 1.0f : set.min_p) * set.depths;
         const uint32_t bucket = t < float(kBuckets - 1u) ? uint32_t(t) : kBuckets - 1u;
         l.least_low = bucket ? bucket - 1u : 0u;
         l.least_high = min(bucket + 1u, kBuckets - 2u);
@@ -890,7 +922,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_rows(Call 
     const uint64_t r = blockIdx.x;
     const T* x = static_cast<const T*>(c.x) + r * uint64_t(c.x_stride);
     const uint32_t width = uint32_t(c.width);
-    const Settings set(c, r, largest(s, x, 0u, width));
+    const Settings set(c, r, ends_of(s, x, 0u, width));
     if (set.greedy()) {
         if (threadIdx.x == 0u) {
             set.finish(c, r);
@@ -914,16 +946,16 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_rows(Call 
 
 // Scratch of a row that is cut into spans.
 struct Scratch {
-    uint64_t* best;       // [spans]
+    uint64_t* best;       // [spans], largest key and least order
     uint64_t* histogram;  // [spans, kBuckets]
     uint64_t* before;     // [kBuckets + 1]
     uint64_t* list;       // [kList]
     Listing* listing;
     uint32_t* tickets;  // workgroups that are done with the histogram; listed tokens
-    static __host__ __device__ uint64_t words(uint64_t spans) { return spans * (1u + kBuckets) + kBuckets + 1u + kList + 8u; }
+    static __host__ __device__ uint64_t words(uint64_t spans) { return spans * (2u + kBuckets) + kBuckets + 1u + kList + 8u; }
     __device__ Scratch(uint64_t* base, uint64_t r, uint32_t spans) {
         best = base + r * words(spans);
-        histogram = best + spans;
+        histogram = best + 2u * spans;
         before = histogram + uint64_t(spans) * kBuckets;
         list = before + kBuckets + 1u;
         listing = reinterpret_cast<Listing*>(list + kList);
@@ -947,9 +979,10 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_best(Ca
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
     const Span span(c, gridDim.x, blockIdx.x);
-    const uint64_t best = largest(s, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), span.begin, span.end);
+    const Ends ends = ends_of(s, static_cast<const T*>(c.x) + r * uint64_t(c.x_stride), span.begin, span.end);
     if (threadIdx.x == 0u) {
-        mine.best[blockIdx.x] = best;
+        mine.best[2u * blockIdx.x] = ends.best;
+        mine.best[2u * blockIdx.x + 1u] = ends.least;
         if (blockIdx.x == 0u) {
             mine.tickets[0] = 0u;
             mine.tickets[1] = 0u;
@@ -957,12 +990,13 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_best(Ca
     }
 }
 
-__device__ uint64_t best_of(const Scratch& mine, uint32_t spans) {
-    uint64_t best = 0;
+__device__ Ends ends_of(const Scratch& mine, uint32_t spans) {
+    Ends ends{0u, 0u};
     for (uint32_t i = threadIdx.x % 64u; i < spans; i += 64u) {
-        best = greater(best, mine.best[i]);
+        ends.best = greater(ends.best, mine.best[2u * i]);
+        ends.least = max(ends.least, uint32_t(mine.best[2u * i + 1u]));
     }
-    return wave_max(best);
+    return Ends{wave_max(ends.best), wave_max(ends.least)};
 }
 
 // Whether this workgroup is the last of the row's to come here, after its device-scope stores.
@@ -985,7 +1019,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_depths(
     const uint64_t r = blockIdx.y;
     const uint32_t spans = gridDim.x;
     const Scratch mine(scratch, r, spans);
-    const Settings set(c, r, best_of(mine, spans));
+    const Settings set(c, r, ends_of(mine, spans));
     if (set.greedy()) {
         if (blockIdx.x == 0u && threadIdx.x == 0u) {
             set.finish(c, r);
@@ -1038,7 +1072,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 8) sample_listed(
     __shared__ Gathered s;
     const uint64_t r = blockIdx.y;
     const Scratch mine(scratch, r, gridDim.x);
-    const Settings set(c, r, best_of(mine, gridDim.x));
+    const Settings set(c, r, ends_of(mine, gridDim.x));
     const Listing l = *mine.listing;
     if (set.greedy() || l.whole) {
         return;
@@ -1060,7 +1094,7 @@ template <class T> __global__ void __launch_bounds__(kThreads) sample_token(Call
     __shared__ Shared s;
     const uint64_t r = blockIdx.x;
     const Scratch mine(scratch, r, spans);
-    const Settings set(c, r, best_of(mine, spans));
+    const Settings set(c, r, ends_of(mine, spans));
     if (set.greedy()) {
         return;
     }

@@ -871,6 +871,24 @@ def test_sample_of_settings_at_their_ends(dtype):
 @gpu
 @BOTH
 @pytest.mark.parametrize("width", [900, 40000])
+@pytest.mark.parametrize("spread", [1e-6, 1e-3, 0.05, 1.0])
+def test_sample_of_flat_rows(spread, width, dtype):
+    """Whole rows within a small factor, or nothing: their own depths are what the buckets are spread over."""
+    x = torch.randn(6, width, generator=torch.Generator().manual_seed(3)) * spread
+    x[1, ::7] = -math.inf
+    x[2] = 30 + x[2]
+    x[3, 1:] = -math.inf
+    x[4, 5] = spread * 9
+    x = x.to(dtype)
+    uniform = torch.rand(6, generator=torch.Generator().manual_seed(1))
+    for filters in ({}, {"min_p": torch.tensor([0.999, 0.9, 1.0, 0.5, 1 - 2.0**-20, 1 - 1e-6])}, {"top_p": torch.full((6,), 0.4)}, {"top_k": torch.full((6,), 400)},
+                    {"temperature": torch.full((6,), 40.0), "top_k": torch.tensor([0, 5, 1000, 0, 70, 0]), "top_p": torch.full((6,), 0.9), "min_p": torch.full((6,), 0.97)}):
+        check_sample(x, uniform=uniform, **filters)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("width", [900, 40000])
 def test_sample_at_the_least_temperatures(width, dtype):
     """Temperatures whose inverse is no float, with logits that differ by as little, and with others."""
     temperature = torch.tensor([1e-36, 3e-37, 1e-37, 1e-38, 1e-40, 1e-45, 1e-45, 1e-38])
