@@ -536,15 +536,17 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
     const uint64_t k_pages = uint64_t(a.k + kv * a.head_stride), v_pages = uint64_t(a.v + kv * a.head_stride);  // addresses
     const uint64_t k_new = uint64_t(a.k_new + uint64_t(kv) * a.dim), v_new = uint64_t(a.v_new + uint64_t(kv) * a.dim);
     const int64_t* table = a.table + tile.b * a.table_stride;
-    const uint32_t stop = tile.template blocks<KEYS>(), page_rows = a.page_rows, inverse = 0xffffffffu / page_rows;
+    // (the first rows and the window's follow one another: place v is that of row v, or behind the first rows of row v - head + low)
+    const uint32_t places = tile.head + (tile.end - tile.low), stop = (places + KEYS - 1u) / KEYS, page_rows = a.page_rows, inverse = 0xffffffffu / page_rows;
     // j / page_rows: the rounded reciprocal is right or one too small
     const auto page_index = [&](uint32_t j) {
         const uint32_t q = __umulhi(j, inverse);
         return q + (j - q * page_rows >= page_rows ? 1u : 0u);
     };
+    const auto row_at = [&](uint32_t v) { return v < tile.head ? v : v - tile.head + tile.low; };
     auto page_of = [&](uint32_t x) -> int64_t {  // of this lane's row of block x (-1: none)
-        const uint32_t j = tile.template block_begin<KEYS>(x) + lane;
-        return j < tile.template block_end<KEYS>(x) && j < tile.length ? table[page_index(j)] : -1;
+        const uint32_t v = x * KEYS + lane, j = row_at(v);
+        return lane < KEYS && v < places && j < tile.length ? table[page_index(j)] : -1;
     };
     if constexpr (!FULL) {  // zeros behind the rows' ends
         for (uint32_t c = threadIdx.x; c < 4u * BLOCK / 8u; c += 64u * WAVES) {
@@ -554,9 +556,9 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
     }
     // Copies block x into buffer ``to``; returns which of its rows there are.
     auto copy = [&](uint32_t x, uint32_t to, int64_t page) -> unsigned long long {
-        const uint32_t j = tile.template block_begin<KEYS>(x) + lane;
+        const uint32_t v = x * KEYS + lane, j = row_at(v);
         const bool held = page >= 0 && uint64_t(page) < a.pages;
-        const bool is_new = j >= tile.length && j < tile.template block_end<KEYS>(x);
+        const bool is_new = lane < KEYS && v < places && j >= tile.length;
         const uint64_t place = 2u * (held ? uint64_t(page) * a.page_stride + uint64_t(j - page_index(j) * page_rows) * a.row_stride
                                      : is_new ? uint64_t(tile.begin + (j - tile.length)) * a.new_stride : 0u);
         const unsigned long long here = __ballot(held || is_new), fresh = __ballot(is_new);
@@ -623,7 +625,8 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
             ahead = n + splits < stop ? page_of(n + splits) : -1;
         }
         for (; n < stop; n += splits, buffer ^= 1u) {
-            const uint32_t begin = tile.template block_begin<KEYS>(n), next = n + splits;
+            const uint32_t place = n * KEYS, begin = place - tile.head + tile.low, next = n + splits;
+            const uint32_t firsts = place < tile.head ? tile.head - place : 0u;  // first rows that it begins with
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
             __builtin_amdgcn_s_barrier();  // block n has landed, and every wave is done with the other buffer
@@ -638,7 +641,7 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
             uint16_t* vs = lds + buffer * 2u * BLOCK + BLOCK;
             if (careful) {
                 for (uint32_t r = 0; r < KEYS; ++r) {
-                    const bool sees = ((here >> r) & 1ull) && sight(begin + r);
+                    const bool sees = ((here >> r) & 1ull) && sight(row_at(place + r));
 #pragma unroll
                     for (int dt = 0; dt < DEEP; ++dt) {
 #pragma unroll
@@ -658,8 +661,8 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                 __syncthreads();
             }
             // what none of this wave's rows sees is skipped
-            if (idle || int32_t(begin) > last_position ||
-                (a.window && int64_t(begin) + KEYS - 1 + a.window <= int64_t(first_position) && begin >= a.first)) {
+            if (idle || (!firsts && (int32_t(begin) > last_position ||
+                                     (a.window && int64_t(begin) + KEYS - 1 + a.window <= int64_t(first_position) && begin >= a.first)))) {
                 continue;
             }
             f32x16_t s[TILES];
@@ -680,10 +683,11 @@ __device__ __forceinline__ void attention_chunk_wide(const ChunkOperands<uint16_
                 }
             }
             // rows that some of the wave's tokens do not see (the chunk's own, the window's first), and rows that are not there
-            const bool some = int32_t(begin + KEYS - 1u) > first_position ||
-                              (a.window && int64_t(begin) + a.window <= int64_t(last_position) && begin + KEYS > a.first);
+            const bool some = firsts < KEYS && (int32_t(begin + KEYS - 1u) > first_position ||
+                                                (a.window && int64_t(begin) + a.window <= int64_t(last_position) && begin + KEYS > a.first));
             if (some || here != EVERY) {
-                const unsigned long long visible = some ? here & sight.bits(begin) : here;
+                const unsigned long long others = firsts < 64u ? ~0ull << firsts : 0ull;  // (all see the first rows)
+                const unsigned long long visible = some ? here & (sight.bits(begin) | ~others) : here;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     const uint32_t bits = uint32_t(visible >> (32 * t)) >> (4u * half);

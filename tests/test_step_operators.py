@@ -470,6 +470,21 @@ def test_chunk_window_and_first_rows(window, first, fresh, dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("window,first", [(1, 1), (3, 33), (64, 64), (70, 100), (128, 130), (40, 300), (200, 5)])
+def test_long_chunk_window_and_first_rows(window, first, dim, fresh, dtype):
+    """Blocks of first rows alone, of both, of the window's alone."""
+    counts, lengths = [30, 0, 1, 100], [400, 4, 301, 90]
+    if not fresh:
+        lengths = [n + c for n, c in zip(lengths, counts)]
+    inputs = chunk_inputs(counts, lengths, kv=8, group=8, dim=dim, page=16, dtype=dtype, fresh=fresh, seed=window)
+    inputs["table"][0, 2] = len(inputs["k_pages"])  # (a bad page: 16 rows that are not there)
+    check_chunk(inputs, window=window, first=first)
+
+
+@gpu
+@BOTH
 @pytest.mark.parametrize("counts,lengths", [([1], [4000]), ([3, 1], [2500, 0]), ([40], [1900])])
 def test_chunk_of_few_tokens_over_long_caches(counts, lengths, dtype):
     """Few tiles over many rows: a tile's keys are split over workgroups."""
