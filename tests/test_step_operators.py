@@ -506,6 +506,17 @@ def test_chunk_of_many_sequences(dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("sequences,most,group", [(65, 3, 1), (512, 2, 9), (513, 40, 16), (1300, 2, 3)])
+def test_chunk_of_hundreds_of_sequences(sequences, most, group, dtype):
+    """More than are counted at a time; empty ones at the ends of what a lane and a wave count; 513 fill large tiles."""
+    rng = np.random.default_rng(sequences)
+    counts, lengths = rng.integers(0, most + 1, sequences), rng.integers(0, 20, sequences)
+    counts[[0, 7, 8, 63]], counts[-1] = 0, most
+    check_chunk(chunk_inputs(counts.tolist(), lengths.tolist(), kv=1, group=group, dim=16, page=8, dtype=dtype, seed=sequences))
+
+
+@gpu
+@BOTH
 @pytest.mark.parametrize("fresh", [True, False], ids=["new", "stored"])
 @pytest.mark.parametrize("kv", [2, 80])
 def test_chunk_rows_on_bad_pages_are_not_seen(kv, fresh, dtype):
