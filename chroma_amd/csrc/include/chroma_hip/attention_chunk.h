@@ -3,8 +3,14 @@
 //     o_i = sum_j exp(s_ij - m) v_j / (sum_j exp(s_ij - m) + exp(sink - m)),   s_ij = scale * (q_i . k_j),
 //
 // j over the rows that token i of the sequence sees: j <= p_i (its own row included), and with a window those after
-// p_i - window and the first ones. Scores and sums stay in float and the result is rounded once; a bfloat16 weight meets V
-// rounded to bfloat16.
+// p_i - window and the first ones. Scores and sums stay in float and the result is rounded once.
+//
+// A bfloat16 weight meets V in tiles of 16 rows as two bfloat16 halves (2^-16 of it is lost), as attention_paged.h has it: the
+// copies bound those, and the second product costs nothing (32 sequences of four tokens over 4096 rows 60 us either way, of one
+// 48, 16 tokens over 900 rows 14). In the larger tiles, which the products and the weights themselves bound, it is rounded
+// once (within 2^-8 of it): that adds as much error as the result's own rounding, 0.0023 of a result's size against 64 bits
+// instead of 0.0017, and two halves would take a quarter longer (2 x 2048 tokens over 30000 rows 2241 -> 2871 us, 2048 of heads of
+// 64 over 30000 1465 -> 1844, 4 x 512 over 4096 217 -> 270).
 //
 // A tile is 16 (token, head of the group) rows of a sequence and KV head, token by token: one token of 8 heads fills half of
 // one, 16 tokens 8 of them. The tiles of all sequences are counted from ``starts`` on the device. A wave copies a block of keys
@@ -178,7 +184,8 @@ template <class T> __device__ __forceinline__ bool chunk_not_finite(T v) {
 // row. Lane (quad, col) ends up with values 16 dt + 4 quad .. + 3 of row ``col`` in o[dt], and that row's maximum and sum.
 //
 // Where a row of V is hidden from some rows of the tile and not from others, its weight for the former is 0, and 0 times an
-// infinity or NaN would be NaN: such values join the rows that see them by themselves and leave the product.
+// infinity or NaN would be NaN; so would be an infinity times halves of two signs. Where a sum comes out not finite, a second pass
+// has such values join the rows that see them by themselves and leave the product.
 template <class T, int DP, uint32_t KEYS> struct ChunkWave {
     static constexpr bool BF16 = sizeof(T) == 2;
     static constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
@@ -250,37 +257,32 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                 qf[c] = *reinterpret_cast<const uint4*>(q + (c * 4u + quad) * CHUNK);
             }
         }
-        peak = neg_inf;
-        total = 0.0f;
+        // The pass over the blocks, and a second one where a sum is not finite (``careful``).
+        const uint32_t from = n;
+        for (bool careful = false;; careful = true) {
+            peak = neg_inf;
+            total = 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < DP / 16; ++dt) {
-            o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        while (n < stop) {
-            const uint32_t next = n + step, begin = tile.template block_begin<KEYS>(n);
-            int64_t next_page = -1;
-            if (next < stop) {
-                next_page = page_of(next);
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
-            __builtin_amdgcn_sched_barrier(0);
-            if (seen != (KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull)) {  // what no row sees may hold anything
-                for (uint32_t c = lane; c < KEYS * PER_ROW; c += 64u) {
-                    if (!((seen >> (c / PER_ROW)) & 1ull)) {
-                        *reinterpret_cast<uint4*>(vs + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
+            while (n < stop) {
+                const uint32_t next = n + step, begin = tile.template block_begin<KEYS>(n);
+                int64_t next_page = -1;
+                if (next < stop) {
+                    next_page = page_of(next);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+                __builtin_amdgcn_sched_barrier(0);
+                if (seen != (KEYS == 64u ? ~0ull : (1ull << (KEYS % 64u)) - 1ull)) {  // what no row sees may hold anything
+                    for (uint32_t c = lane; c < KEYS * PER_ROW; c += 64u) {
+                        if (!((seen >> (c / PER_ROW)) & 1ull)) {
+                            *reinterpret_cast<uint4*>(vs + c * CHUNK) = uint4{0u, 0u, 0u, 0u};
+                        }
                     }
                 }
-            }
-            // every row of the tile sees every key of the block (but those that nothing sees)
-            const bool whole = int32_t(begin + KEYS - 1u) <= tile.first_position &&
-                               (!a.window || int64_t(begin) + a.window > int64_t(tile.last_position) || begin + KEYS <= a.first);
-            if (!whole) {
-                bool odd = false;
-                for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
-                    odd |= chunk_not_finite<T>(vs[c]);
-                }
-                if (__ballot(odd) != 0ull) {
+                if (careful) {
                     for (uint32_t r = 0; r < KEYS; ++r) {
                         const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
 #pragma unroll
@@ -299,100 +301,119 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                         }
                     }
                 }
-            }
-            // scores of keys 16 t + 4 quad + r for this lane's row
-            float u[TILES][4], top = neg_inf;
+                // every row of the tile sees every key of the block (but those that nothing sees)
+                const bool whole = int32_t(begin + KEYS - 1u) <= tile.first_position &&
+                                   (!a.window || int64_t(begin) + a.window > int64_t(tile.last_position) || begin + KEYS <= a.first);
+                // scores of keys 16 t + 4 quad + r for this lane's row
+                float u[TILES][4], top = neg_inf;
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int t = 0; t < TILES; ++t) {
+                    f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < PARTS; ++c) {
-                    const uint32_t r = t * 16u + col;
-                    const uint4 kf = *reinterpret_cast<const uint4*>(ks + r * DP + ((c * 4u + quad) ^ ((r / 2u) & SWZ)) * CHUNK);
-                    if constexpr (BF16) {
-                        kwave_mfma<T>(kf, qf[c], s);
-                    } else {
-                        s += kwave_unit(kf, qf[c]);
-                    }
-                }
-                const uint32_t bits = uint32_t(seen >> (t * 16u + quad * 4u)) & 15u;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool sees = ((bits >> r) & 1u) && (whole || sight(begin + t * 16u + quad * 4u + r));
-                    u[t][r] = sees ? s[r] * a.scale : neg_inf;
-                    top = __builtin_fmaxf(top, u[t][r]);
-                }
-            }
-            if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
-                top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
-                top = __builtin_fmaxf(top, __shfl_xor(top, 32, kWave));
-                top = __builtin_fmaxf(top, peak);
-                const float shrink = peak == neg_inf ? 0.0f : fast_exp(peak - top);
-                if (peak != neg_inf) {  // (what has no maximum yet has no sums but values that are not finite)
-                    total *= shrink;
-#pragma unroll
-                    for (int dt = 0; dt < DP / 16; ++dt) {
-                        o[dt] *= shrink;
-                    }
-                }
-                peak = top;
-            }
-            const float base = peak == neg_inf ? 0.0f : peak;
-            float part = 0.0f;
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    u[t][r] = fast_exp(u[t][r] - base);
-                    part += u[t][r];
-                }
-            }
-            total += part;
-            if constexpr (BF16) {
-                // slots 0-3 and 4-7 of lane (d, quad) hold keys 32 h + 4 quad + r and 32 h + 16 + 4 quad + r (attention_flash.h)
-#pragma unroll
-                for (int h = 0; h < TILES / 2; ++h) {
-                    bf16x8_t weights;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        weights[x] = __bf16(u[2 * h + x / 4][x % 4]);
-                    }
-#pragma unroll
-                    for (int dt = 0; dt < DP / 16; ++dt) {
-                        s16x4_t half[2];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t r = h * 32u + x * 16u + quad * 4u + col / 4u;
-                            const uint32_t chunk = (dt * 2u + (col % 4u) / 2u) ^ ((r / 2u) & SWZ);
-                            half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + r * DP + chunk * 8u + (col % 2u) * 4u));
+                    for (int c = 0; c < PARTS; ++c) {
+                        const uint32_t r = t * 16u + col;
+                        const uint4 kf = *reinterpret_cast<const uint4*>(ks + r * DP + ((c * 4u + quad) ^ ((r / 2u) & SWZ)) * CHUNK);
+                        if constexpr (BF16) {
+                            kwave_mfma<T>(kf, qf[c], s);
+                        } else {
+                            s += kwave_unit(kf, qf[c]);
                         }
-                        const uint2 lo = __builtin_bit_cast(uint2, half[0]), hi = __builtin_bit_cast(uint2, half[1]);
-                        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, uint4{lo.x, lo.y, hi.x, hi.y});
-                        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, weights, o[dt], 0, 0, 0);
+                    }
+                    const uint32_t bits = uint32_t(seen >> (t * 16u + quad * 4u)) & 15u;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool sees = ((bits >> r) & 1u) && (whole || sight(begin + t * 16u + quad * 4u + r));
+                        u[t][r] = sees ? s[r] * a.scale : neg_inf;
+                        top = __builtin_fmaxf(top, u[t][r]);
                     }
                 }
-            } else {
-                // product (t, r) takes keys 16 t + 4 quad + r; 16 keys are summed before they join the row's
+                if (__ballot(top > peak + kFlashHeadroom || (peak == neg_inf && top != neg_inf)) != 0ull) {
+                    top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
+                    top = __builtin_fmaxf(top, __shfl_xor(top, 32, kWave));
+                    top = __builtin_fmaxf(top, peak);
+                    const float shrink = peak == neg_inf ? 0.0f : fast_exp(peak - top);
+                    if (peak != neg_inf) {  // (what has no maximum yet has no sums but values that are not finite)
+                        total *= shrink;
+#pragma unroll
+                        for (int dt = 0; dt < DP / 16; ++dt) {
+                            o[dt] *= shrink;
+                        }
+                    }
+                    peak = top;
+                }
+                const float base = peak == neg_inf ? 0.0f : peak;
+                float part = 0.0f;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
 #pragma unroll
-                    for (int dt = 0; dt < DP / 16; ++dt) {
-                        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t key = t * 16u + quad * 4u + r;
-                            const float v = vs[key * DP + ((dt * 4u + col / 4u) ^ ((key / 2u) & SWZ)) * 4u + col % 4u];
-                            sum = __builtin_amdgcn_mfma_f32_16x16x4f32(v, u[t][r], sum, 0, 0, 0);
-                        }
-                        o[dt] += sum;
+                    for (int r = 0; r < 4; ++r) {
+                        u[t][r] = fast_exp(u[t][r] - base);
+                        part += u[t][r];
                     }
                 }
+                total += part;
+                if constexpr (BF16) {
+                    // slots 0-3 and 4-7 of lane (d, quad) hold keys 32 h + 4 quad + r and 32 h + 16 + 4 quad + r (attention_flash.h)
+#pragma unroll
+                    for (int h = 0; h < TILES / 2; ++h) {
+                        bf16x8_t high, low;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const float p = u[2 * h + x / 4][x % 4];
+                            high[x] = __bf16(p);
+                            low[x] = __bf16(p - float(high[x]));
+                        }
+#pragma unroll
+                        for (int dt = 0; dt < DP / 16; ++dt) {
+                            s16x4_t half[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t r = h * 32u + x * 16u + quad * 4u + col / 4u;
+                                const uint32_t chunk = (dt * 2u + (col % 4u) / 2u) ^ ((r / 2u) & SWZ);
+                                half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + r * DP + chunk * 8u + (col % 2u) * 4u));
+                            }
+                            const uint2 lo = __builtin_bit_cast(uint2, half[0]), hi = __builtin_bit_cast(uint2, half[1]);
+                            const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, uint4{lo.x, lo.y, hi.x, hi.y});
+                            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, high, o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, low, o[dt], 0, 0, 0);
+                        }
+                    }
+                } else {
+                    // product (t, r) takes keys 16 t + 4 quad + r; 16 keys are summed before they join the row's
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+                        for (int dt = 0; dt < DP / 16; ++dt) {
+                            f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint32_t key = t * 16u + quad * 4u + r;
+                                const float v = vs[key * DP + ((dt * 4u + col / 4u) ^ ((key / 2u) & SWZ)) * 4u + col % 4u];
+                                sum = __builtin_amdgcn_mfma_f32_16x16x4f32(v, u[t][r], sum, 0, 0, 0);
+                            }
+                            o[dt] += sum;
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (next < stop) {  // both buffers have been read
+                    copy(next, next_page);
+                }
+                n = next;
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (next < stop) {  // both buffers have been read
-                copy(next, next_page);
+            bool odd = false;
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    odd |= !(__builtin_fabsf(o[dt][e]) < __builtin_inff());
+                }
             }
-            n = next;
+            if (careful || __ballot(odd) == 0ull) {
+                break;
+            }
+            n = from;  // (it has blocks: a wave without any has sums of 0)
+            copy(n, page_of(n));
         }
         total += __shfl_xor(total, 16, kWave);
         total += __shfl_xor(total, 32, kWave);

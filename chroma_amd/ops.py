@@ -96,7 +96,8 @@ def paged_chunk_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_new: Op
     rows, token i of a sequence at position lengths[b] + i; or None, where they are the last of the lengths[b] cached rows. A
     token sees the rows up to its position, cached or new, less what ``window`` leaves out. Pages, table [S, N], lengths, sinks,
     window and first are as for ``paged_attention``. A token that sees no row and a row of q that no sequence has get zeros. Scores
-    and sums are float's, the result is rounded once; compiled with bfloat16, a weight meets the values rounded to bfloat16."""
+    and sums are float's, the result is rounded once; compiled with bfloat16, a weight meets the values as two bfloat16 halves
+    (within 2^-16 of it), or, where there are 64 query heads of a KV head or more for each sequence, rounded to bfloat16."""
     _check_chunk(q, k_pages, v_pages, k_new, v_new, table, lengths, starts, sinks, window, first)
     tokens, kv_heads, group, dim = q.shape
     pages, rows = k_pages.shape[:2]

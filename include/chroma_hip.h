@@ -352,8 +352,10 @@ int chroma_hip_cache_store(const chroma_hip_cache_store_call* call, void* stream
  * j <= t, cached or new; ``window`` > 0 leaves out those with j <= t - window except the ``first`` first ones. A token that sees no
  * row gets zeros, and rows of out that belong to no sequence stay as they are.
  *
- * Scores and sums are kept in float and the result is rounded once, at the end; with bfloat16 values each weight exp(s_j - m)
- * meets v_j rounded to bfloat16 (within 2^-8 of it). A value that is not finite reaches only the tokens that see its row.
+ * Scores and sums are kept in float and the result is rounded once, at the end. With bfloat16 values each weight exp(s_j - m)
+ * meets v_j as two bfloat16 halves, which leaves out at most 2^-16 of it, in calls of few query heads (always below 64 of a
+ * KV head for each sequence on average), and rounded to bfloat16 (within 2^-8 of it) in calls of more. A value that is not finite
+ * reaches only the tokens that see its row.
  *
  * ``starts`` must ascend within [0, tokens]; entries outside count as the nearest bound, a range that descends as empty. Lengths,
  * table rows, bad pages, strides and alignments are as for ``chroma_hip_paged_attention``; new_stride and q_stride count from token to
