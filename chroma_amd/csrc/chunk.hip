@@ -56,7 +56,7 @@ const char* mistake(const Call& c) {
     if (c.dim < 8 || c.dim > 256 || c.dim % 8) {
         return "the head dimension must be a multiple of 8 from 8 to 256";
     }
-    if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest + c.tokens >= kMost - 4096) {
+    if (c.pages < 1 || c.pages >= kMost || c.page_rows < 1 || c.page_rows >= kMost || c.longest < 0 || c.longest >= kMost - 4096 - c.tokens) {
         return "pages, page_rows or longest out of range";
     }
     // (a launch holds fewer than 2^32 threads: the most tiles, 2^22 full ones and 2^22 sequences' last ones, have 512 each)

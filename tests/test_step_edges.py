@@ -4,12 +4,12 @@ that only large calls take, and the host's part of a step."""
 from __future__ import annotations
 
 import ctypes
-import math
 
 import pytest
 import torch
 
-from tests.test_step_operators import HALF, chunk_call, chunk_inputs, chunk_reference, on_gpu, queue_in
+from chroma_amd._src import native
+from tests.test_step_operators import HALF, chunk_call, chunk_inputs, chunk_reference, on_gpu, plain_chunk_call, queue_in, refused
 
 gpu = pytest.mark.gpu
 
@@ -37,3 +37,13 @@ def test_few_tokens_meet_the_values_with_two_halves_of_their_weights(shape):
     out = torch.zeros_like(device["q"])
     queue_in("chroma_hip_paged_chunk_attention", chunk_call(**device, out=out))
     assert ((out.cpu().double() - want).abs() <= bound)[taken].all()
+
+
+# ------------------------------------------------------------------------------------------------ extents
+@pytest.mark.parametrize("longest", [2**63 - 1, 2**63 - 5, 2**62, 2**31])
+def test_lengths_near_the_end_of_64_bits_are_refused(longest):
+    """Sums of the extents do not wrap on the way to the refusal (pages and a table row that would hold such a length)."""
+    call = plain_chunk_call(longest=longest, page_rows=2**30, table_stride=2**34)
+    with pytest.raises(RuntimeError, match="paged_chunk_attention: .*longest out of range"):
+        refused("chroma_hip_paged_chunk_attention", call, 1 << 45, 1 << 30)
+    assert native.library().chroma_hip_paged_chunk_attention_workspace(ctypes.byref(call)) == 0
