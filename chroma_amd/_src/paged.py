@@ -260,7 +260,7 @@ class PagedDecoder:
     @staticmethod
     def _tokens_of(tokens: Any) -> np.ndarray:
         """One token or several, as an array of one at least."""
-        ids = np.asarray(tokens)
+        ids = np.asarray(int(tokens) if isinstance(tokens, (int, np.integer)) else tokens)  # (True is one too)
         if ids.ndim > 1 or not ids.size:
             raise ValueError(f"a sequence takes a token or a nonempty 1-D sequence of them, got shape {ids.shape}")
         if not np.issubdtype(ids.dtype, np.integer):

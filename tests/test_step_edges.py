@@ -5,11 +5,14 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
 from chroma_amd._src import native
+from tests.test_paged_decoder import fake_paged_decoder, small_model
 from tests.test_step_operators import HALF, chunk_call, chunk_inputs, chunk_reference, on_gpu, plain_chunk_call, queue_in, refused
+from tests.test_step_paths import fake_chunk_decoder
 
 gpu = pytest.mark.gpu
 
@@ -47,3 +50,19 @@ def test_lengths_near_the_end_of_64_bits_are_refused(longest):
     with pytest.raises(RuntimeError, match="paged_chunk_attention: .*longest out of range"):
         refused("chroma_hip_paged_chunk_attention", call, 1 << 45, 1 << 30)
     assert native.library().chroma_hip_paged_chunk_attention_workspace(ctypes.byref(call)) == 0
+
+
+# ------------------------------------------------------------------------------------------------ the host's part of a step
+def test_a_truth_value_is_a_token():
+    """``True`` is an integer of Python's, and a step of single tokens takes it as such."""
+    model = small_model()
+    with fake_paged_decoder(model) as decoder:
+        a, b = decoder.add([1, 2, 3])[0], decoder.add([1, 2, 3])[0]
+        logits = decoder.step({a: True, b: 1})
+        assert np.array_equal(logits[0], logits[1]) and decoder.position(a) == 4
+        with pytest.raises(TypeError, match="must be integers"):
+            decoder.step({a: 1.0})
+    with fake_chunk_decoder(model) as decoder:
+        a, b = decoder.add([1, 2, 3])[0], decoder.add([1, 2, 3])[0]
+        logits = decoder.step({a: True, b: [1]})
+        assert np.array_equal(logits[0], logits[1]) and decoder.position(a) == 4
