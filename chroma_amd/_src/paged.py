@@ -349,24 +349,30 @@ class PagedDecoder:
             raise RuntimeError("PagedDecoder is closed")
         if not tokens:
             raise ValueError("a step wants a token of at least one sequence")
-        taken_of: Dict[int, np.ndarray] = {}
+        # A token of a sequence stays a number: arrays for each would take as long as the rest of the host's part.
+        counts: Dict[int, int] = {}
+        several: Dict[int, np.ndarray] = {}
         for sequence, token in tokens.items():
             self._known(sequence)
-            if self._decoder is not None and not isinstance(token, (int, np.integer)):
+            if isinstance(token, (int, np.integer)):
+                counts[sequence] = 1
+            elif self._decoder is not None:
                 raise TypeError(f"token ids must be integers, got {token!r}")
-            taken_of[sequence] = self._tokens_of(token)
-            if self._lengths[sequence] + len(taken_of[sequence]) > self._span * self._page_rows:
+            else:
+                several[sequence] = self._tokens_of(token)
+                counts[sequence] = len(several[sequence])
+            if self._lengths[sequence] + counts[sequence] > self._span * self._page_rows:
                 raise ValueError(f"sequence {sequence} holds {self._lengths[sequence]} rows, "
-                                 + ("all that the step program has pages for" if len(taken_of[sequence]) == 1 else
-                                    f"{len(taken_of[sequence])} more are not what the step program has pages for"))
-        if self._decoder is None and sum(map(len, taken_of.values())) > self._room:
-            raise ValueError(f"{sum(map(len, taken_of.values()))} tokens, a step takes {self._room}")
+                                 + ("all that the step program has pages for" if counts[sequence] == 1 else
+                                    f"{counts[sequence]} more are not what the step program has pages for"))
+        if self._decoder is None and sum(counts.values()) > self._room:
+            raise ValueError(f"{sum(counts.values())} tokens, a step takes {self._room}")
         for sequence in rules or ():
             if sequence not in tokens:
                 raise KeyError(f"rules for sequence {sequence}, which has no token in this step")
         # pages for the rows that begin one, and for a copy of a last page that other sequences share
         size = self._page_rows
-        starts = {s: -(-(self._lengths[s] + len(taken_of[s])) // size) - len(self._pages[s]) for s in tokens}
+        starts = {s: more for s, count in counts.items() if (more := -(-(self._lengths[s] + count) // size) - len(self._pages[s]))}
         leaving: Dict[int, int] = {}
         copies = []
         for s in tokens:
@@ -392,15 +398,19 @@ class PagedDecoder:
                 begins[slot] = first
                 if slot in by_place:
                     rows[by_place[slot]] = first
-                    first += len(taken_of[by_place[slot]])
+                    first += counts[by_place[slot]]
                     last[slot] = first - 1
             begins[self._slots] = first
-        for sequence, some in taken_of.items():
+        for sequence, token in tokens.items():
             slot, held = self._slot_of[sequence], self._lengths[sequence]
             row = rows.setdefault(sequence, slot)
-            ids[row : row + len(some)] = some
-            positions[row : row + len(some)] = np.arange(held, held + len(some))
             lengths[slot] = held
+            if sequence in several:
+                stop = row + counts[sequence]
+                ids[row:stop] = several[sequence]
+                positions[row:stop] = np.arange(held, held + counts[sequence])
+            else:
+                ids[row], positions[row] = token, held
         selection = row_rules = None
         if rules:
             plain = TokenRules()
@@ -421,28 +431,31 @@ class PagedDecoder:
         with _interrupts_deferred():
             with self._taking(needed) as taken:
                 left = iter(taken)
-                pages = {s: list(self._pages[s]) for s in tokens}
-                for s in copies:
-                    pages[s][-1] = next(left)
-                self._move(self._cache(), [(self._pages[s][-1] * size, pages[s][-1] * size, self._lengths[s] % size) for s in copies])
-                for s in tokens:
-                    pages[s].extend(next(left) for _ in range(starts[s]))
+                copied = {s: next(left) for s in copies}
+                fresh_pages = {s: [next(left) for _ in range(more)] for s, more in starts.items()}
+                self._move(self._cache(), [(self._pages[s][-1] * size, page * size, self._lengths[s] % size) for s, page in copied.items()])
                 model = self._step.native
                 fresh = native.CacheRows(keys=model.output_pointer(1), values=model.output_pointer(2), rows=self._room,
                                          layer_pitch=self._room * self._row_bytes)
                 moves = []
-                for s in tokens:  # a sequence's rows, page by page
-                    at, stop = self._lengths[s], self._lengths[s] + len(taken_of[s])
-                    while at < stop:
-                        count = min(stop, (at // size + 1) * size) - at
-                        moves.append((rows[s] + at - self._lengths[s], pages[s][at // size] * size + at % size, count))
-                        at += count
+                for s, count in counts.items():  # a sequence's rows: what its last page has room for, then page by page
+                    row, within = rows[s], self._lengths[s] % size
+                    if within:
+                        some = min(count, size - within)
+                        moves.append((row, (copied[s] if s in copied else self._pages[s][-1]) * size + within, some))
+                        row, count = row + some, count - some
+                    for page in fresh_pages.get(s, ()):
+                        moves.append((row, page * size, min(count, size)))
+                        row, count = row + size, count - size
                 self._move(fresh, moves)
-            for sequence in copies:
+            for sequence, page in copied.items():
                 self._pool.release(self._pages[sequence][-1:])
-            for sequence in tokens:
-                self._pages[sequence] = pages[sequence]
-                self._lengths[sequence] += len(taken_of[sequence])
+                self._pages[sequence][-1] = page
+            for sequence, some in fresh_pages.items():
+                self._pages[sequence].extend(some)
+            for sequence, count in counts.items():
+                self._lengths[sequence] += count
+            for sequence in copied.keys() | fresh_pages.keys():
                 self._set_row(sequence)
         return [self._slot_of[s] for s in tokens], selection
 
