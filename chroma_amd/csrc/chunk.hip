@@ -185,11 +185,8 @@ template <class T, int DP> void launch(const Call& c, float* scratch, hipStream_
     const auto combine = [&](auto kernel) { kernel<<<dim3(grid.x, unsigned(cut.rows() / 16)), 256, 0, stream>>>(a, grid.y, scratch); };
     if constexpr (sizeof(T) == 2) {
         if constexpr (DP == 128) {
-            if (cut.waves == 8) {
+            if (cut.waves == 8) {  // (512 workgroups or more: never split)
                 c.dim == DP ? launch_wide<DP, 8, true>(a, grid, scratch, stream) : launch_wide<DP, 8, false>(a, grid, scratch, stream);
-                if (grid.y > 1) {
-                    combine(paged_chunk_combine<T, DP, 256u, true>);
-                }
                 return;
             }
         }
