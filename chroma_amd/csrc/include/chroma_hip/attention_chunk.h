@@ -16,7 +16,8 @@
 // one, 16 tokens 8 of them. The tiles of all sequences are counted from ``starts`` on the device. A wave copies a block of keys
 // and values global -> LDS through the page table and goes over it once, with a running maximum and sum; the waves of a
 // workgroup take blocks in turn and are joined in LDS. Small calls are bound by that chain of dependent requests (starts, lengths,
-// table, rows): 16 tokens over 900 rows, 8 KV heads of 8 heads of 64, 12.4 us; 32 sequences of one over 4096 56 us (4.8 TB/s).
+// table, rows): 16 tokens over 900 rows, 8 KV heads of 8 heads of 64, 12.8 us; 32 sequences of one over 4096 57 us (4.7 TB/s; 48 where
+// they are called again over the same cache, which the last cache then holds in part).
 #pragma once
 
 #include "attention_paged.h"
@@ -557,8 +558,8 @@ __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& 
 //
 // What bounds it is vector work: a score costs a product, a maximum, a power at a quarter of the rate, an addition and half a
 // conversion, 30 cycles a wave's 64 of them against 16 (heads of 64) or 32 (heads of 128) of the matrix cores. 2 x 2048 tokens
-// over 30000 rows with heads of 128 take 2.14-2.24 ms (930-970 TFLOP/s; the matrix cores 37% and the vector units 43% busy, no bank
-// conflicts), 2048 over 30000 with heads of 64 1.49 ms (700 TFLOP/s; 30% and 63%). Without the copies the former would take a quarter
+// over 30000 rows with heads of 128 take 2.12-2.22 ms (940-980 TFLOP/s; the matrix cores 41% and the vector units 45% busy, no bank
+// conflicts), 2048 over 30000 with heads of 64 1.46-1.54 ms (675-710 TFLOP/s; 31% and 64%). Without the copies the former would take a quarter
 // less; copies further ahead, barriers for the scheduler and wave priorities moved it by 4% either way.
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));

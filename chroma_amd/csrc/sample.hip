@@ -12,9 +12,9 @@
 // are listed whole. Where the listed buckets hold more than kList tokens (rows of few values), a workgroup descends on the
 // keys of the whole row.
 //
-// What bounds it: one row of 201088 float logits (28 us) the four launches' chains (readings of 3.4, 13, 4.3 and 7 us; of the second
-// 3 are the span's weights and 8 the sum of 24 spans' histograms and the cuts); 256 rows of 100003 (85 us) the weights' vector work:
-// 31 instructions a token, 35 us, where the first reading takes 18 (5.6 TB/s) and the third 23.
+// What bounds it: one row of 201088 float logits (28 us) the four launches' chains (3.6, 14, 4.1 and 7.1 us; of the second
+// 3 are the span's weights and 8 the sum of 24 spans' histograms and the cuts); 256 rows of 100003 (86 us) the weights' vector work:
+// 31 instructions a token, 36 us, where the first reading takes 19-21 (5 TB/s), the third 22 and the token 10.
 //
 // A weight exp((x - max) / temperature) is evaluated in 64 bits and rounded to units of 2^-44: sums are integers, and the same
 // in whatever order they are taken. In 32 bits the place that a random number names among 200,000 tokens moves by more than

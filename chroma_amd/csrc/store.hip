@@ -2,7 +2,7 @@
 //
 // A row goes in 16-byte units, one to a thread, so that a wave writes whole lines of it; what its length leaves of the last
 // unit goes byte by byte. Row and slot are requested together. What bounds it: a decode step's rows the launch (64 rows of 1 KB
-// 3.0 us), a prompt's the memory, each byte read and written once: 8000 rows of 1 KB in 24 layers 123 us, 6.4 TB/s. Nothing is
+// 2.6 us), a prompt's the memory, each byte read and written once: 8000 rows of 1 KB in 24 layers 124 us, 6.3 TB/s. Nothing is
 // read again here, so loads and stores leave the caches to others.
 #include "../../include/chroma_hip.h"
 
