@@ -6,8 +6,8 @@
 // p_i - window and the first ones. Scores and sums stay in float and the result is rounded once.
 //
 // A bfloat16 weight meets V in tiles of 16 rows as two bfloat16 halves (2^-16 of it is lost), as attention_paged.h has it: the
-// copies bound those, and the second product costs nothing (32 sequences of four tokens over 4096 rows 60 us either way, of one
-// 48, 16 tokens over 900 rows 14). In the larger tiles, which the products and the weights themselves bound, it is rounded
+// copies bound those, and the second product costs up to 4% (16 sequences of four tokens over 2000 rows 22 -> 23 us, 32 over 4096
+// 60 either way, of one token 48, 16 tokens over 900 rows 14). In the larger tiles, which the products and the weights themselves bound, it is rounded
 // once (within 2^-8 of it): that adds as much error as the result's own rounding, 0.0023 of a result's size against 64 bits
 // instead of 0.0017, and two halves would take a quarter longer (2 x 2048 tokens over 30000 rows 2241 -> 2871 us, 2048 of heads of
 // 64 over 30000 1465 -> 1844, 4 x 512 over 4096 217 -> 270).
@@ -185,8 +185,9 @@ template <class T> __device__ __forceinline__ bool chunk_not_finite(T v) {
 // row. Lane (quad, col) ends up with values 16 dt + 4 quad .. + 3 of row ``col`` in o[dt], and that row's maximum and sum.
 //
 // Where a row of V is hidden from some rows of the tile and not from others, its weight for the former is 0, and 0 times an
-// infinity or NaN would be NaN; so would be an infinity times halves of two signs. Where a sum comes out not finite, a second pass
-// has such values join the rows that see them by themselves and leave the product.
+// infinity or NaN would be NaN: such values join the rows that see them by themselves and leave the product. In bfloat16, where an
+// infinity times halves of two signs would be NaN too, in a second pass where a sum comes out not finite; in float in every block
+// that is not seen whole (a second pass takes registers: with heads of 64 a wave less of a SIMD, 2048 tokens over 4096 rows 2.4 -> 3.0 ms).
 template <class T, int DP, uint32_t KEYS> struct ChunkWave {
     static constexpr bool BF16 = sizeof(T) == 2;
     static constexpr uint32_t CHUNK = 16u / sizeof(T), PER_ROW = DP / CHUNK;
@@ -258,7 +259,7 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                 qf[c] = *reinterpret_cast<const uint4*>(q + (c * 4u + quad) * CHUNK);
             }
         }
-        // The pass over the blocks, and a second one where a sum is not finite (``careful``).
+        // The pass over the blocks, and in bfloat16 a second one where a sum is not finite (``careful``).
         const uint32_t from = n;
         for (bool careful = false;; careful = true) {
             peak = neg_inf;
@@ -283,28 +284,34 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                         }
                     }
                 }
-                if (careful) {
-                    for (uint32_t r = 0; r < KEYS; ++r) {
-                        const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
-#pragma unroll
-                        for (int dt = 0; dt < DP / 16; ++dt) {
-#pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e) {
-                                const uint32_t d = dt * 16u + quad * 4u + e;
-                                const T v = vs[r * DP + ((d / CHUNK) ^ ((r / 2u) & SWZ)) * CHUNK + d % CHUNK];
-                                o[dt][e] += sees && chunk_not_finite<T>(v) ? paged_widen<T>(v) : 0.0f;
-                            }
-                        }
-                    }
-                    for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
-                        if (chunk_not_finite<T>(vs[c])) {
-                            vs[c] = T(0);
-                        }
-                    }
-                }
                 // every row of the tile sees every key of the block (but those that nothing sees)
                 const bool whole = int32_t(begin + KEYS - 1u) <= tile.first_position &&
                                    (!a.window || int64_t(begin) + a.window > int64_t(tile.last_position) || begin + KEYS <= a.first);
+                if (BF16 ? careful : !whole) {
+                    bool odd = false;
+                    for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
+                        odd |= chunk_not_finite<T>(vs[c]);
+                    }
+                    if (__ballot(odd) != 0ull) {
+                        for (uint32_t r = 0; r < KEYS; ++r) {
+                            const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
+#pragma unroll
+                            for (int dt = 0; dt < DP / 16; ++dt) {
+#pragma unroll
+                                for (uint32_t e = 0; e < 4; ++e) {
+                                    const uint32_t d = dt * 16u + quad * 4u + e;
+                                    const T v = vs[r * DP + ((d / CHUNK) ^ ((r / 2u) & SWZ)) * CHUNK + d % CHUNK];
+                                    o[dt][e] += sees && chunk_not_finite<T>(v) ? paged_widen<T>(v) : 0.0f;
+                                }
+                            }
+                        }
+                        for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
+                            if (chunk_not_finite<T>(vs[c])) {
+                                vs[c] = T(0);
+                            }
+                        }
+                    }
+                }
                 // scores of keys 16 t + 4 quad + r for this lane's row
                 float u[TILES][4], top = neg_inf;
 #pragma unroll
@@ -410,7 +417,7 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                     odd |= !(__builtin_fabsf(o[dt][e]) < __builtin_inff());
                 }
             }
-            if (careful || __ballot(odd) == 0ull) {
+            if (!BF16 || careful || __ballot(odd) == 0ull) {
                 break;
             }
             n = from;  // (it has blocks: a wave without any has sums of 0)
