@@ -6,17 +6,17 @@
 // p_i - window and the first ones. Scores and sums stay in float and the result is rounded once.
 //
 // A bfloat16 weight meets V in tiles of 16 rows as two bfloat16 halves (2^-16 of it is lost), as attention_paged.h has it: the
-// copies bound those, and the second product costs up to 4% (16 sequences of four tokens over 2000 rows 22 -> 23 us, 32 over 4096
-// 60 either way, of one token 48, 16 tokens over 900 rows 14). In the larger tiles, which the products and the weights themselves bound, it is rounded
-// once (within 2^-8 of it): that adds as much error as the result's own rounding, 0.0023 of a result's size against 64 bits
-// instead of 0.0017, and two halves would take a quarter longer (2 x 2048 tokens over 30000 rows 2241 -> 2871 us, 2048 of heads of
-// 64 over 30000 1465 -> 1844, 4 x 512 over 4096 217 -> 270).
+// copies bound those, and the second product costs little (4 sequences of 16 tokens over 4000 rows, heads of 32, 19.3 -> 20.4 us,
+// 32 of 4 over 4096, heads of 64, 59.5 -> 60.2, 16 tokens over 900 rows 12.5 either way). In the larger tiles, which the products
+// and the weights themselves bound, it is rounded once (within 2^-8 of it): that adds as much error as the result's own rounding,
+// 0.0023 of a result's size against 64 bits instead of 0.0017, and two halves would take a quarter longer (2 x 2048 tokens over
+// 30000 rows 2241 -> 2871 us, 2048 of heads of 64 over 30000 1465 -> 1844, 4 x 512 over 4096 217 -> 270).
 //
 // A tile is 16 (token, head of the group) rows of a sequence and KV head, token by token: one token of 8 heads fills half of
 // one, 16 tokens 8 of them. The tiles of all sequences are counted from ``starts`` on the device. A wave copies a block of keys
 // and values global -> LDS through the page table and goes over it once, with a running maximum and sum; the waves of a
 // workgroup take blocks in turn and are joined in LDS. Small calls are bound by that chain of dependent requests (starts, lengths,
-// table, rows): 16 tokens over 900 rows, 8 KV heads of 8 heads of 64, 12.8 us; 32 sequences of one over 4096 57 us (4.7 TB/s; 48 where
+// table, rows): 16 tokens over 900 rows, 8 KV heads of 8 heads of 64, 12.8 us; 32 sequences of one over 4096 56 us (4.8 TB/s; 48 where
 // they are called again over the same cache, which the last cache then holds in part).
 #pragma once
 
@@ -284,32 +284,38 @@ template <class T, int DP, uint32_t KEYS> struct ChunkWave {
                         }
                     }
                 }
+                const auto join = [&] {  // values that are not finite
+                    for (uint32_t r = 0; r < KEYS; ++r) {
+                        const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
+#pragma unroll
+                        for (int dt = 0; dt < DP / 16; ++dt) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) {
+                                const uint32_t d = dt * 16u + quad * 4u + e;
+                                const T v = vs[r * DP + ((d / CHUNK) ^ ((r / 2u) & SWZ)) * CHUNK + d % CHUNK];
+                                o[dt][e] += sees && chunk_not_finite<T>(v) ? paged_widen<T>(v) : 0.0f;
+                            }
+                        }
+                    }
+                    for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
+                        if (chunk_not_finite<T>(vs[c])) {
+                            vs[c] = T(0);
+                        }
+                    }
+                };
+                if (BF16 && careful) {
+                    join();
+                }
                 // every row of the tile sees every key of the block (but those that nothing sees)
                 const bool whole = int32_t(begin + KEYS - 1u) <= tile.first_position &&
                                    (!a.window || int64_t(begin) + a.window > int64_t(tile.last_position) || begin + KEYS <= a.first);
-                if (BF16 ? careful : !whole) {
+                if (!BF16 && !whole) {
                     bool odd = false;
                     for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
                         odd |= chunk_not_finite<T>(vs[c]);
                     }
                     if (__ballot(odd) != 0ull) {
-                        for (uint32_t r = 0; r < KEYS; ++r) {
-                            const bool sees = ((seen >> r) & 1ull) && sight(begin + r);
-#pragma unroll
-                            for (int dt = 0; dt < DP / 16; ++dt) {
-#pragma unroll
-                                for (uint32_t e = 0; e < 4; ++e) {
-                                    const uint32_t d = dt * 16u + quad * 4u + e;
-                                    const T v = vs[r * DP + ((d / CHUNK) ^ ((r / 2u) & SWZ)) * CHUNK + d % CHUNK];
-                                    o[dt][e] += sees && chunk_not_finite<T>(v) ? paged_widen<T>(v) : 0.0f;
-                                }
-                            }
-                        }
-                        for (uint32_t c = lane; c < KEYS * DP; c += 64u) {
-                            if (chunk_not_finite<T>(vs[c])) {
-                                vs[c] = T(0);
-                            }
-                        }
+                        join();
                     }
                 }
                 // scores of keys 16 t + 4 quad + r for this lane's row
@@ -565,7 +571,7 @@ __device__ __forceinline__ void attention_chunk_combine(const ChunkOperands<T>& 
 //
 // What bounds it is vector work: a score costs a product, a maximum, a power at a quarter of the rate, an addition and half a
 // conversion, 30 cycles a wave's 64 of them against 16 (heads of 64) or 32 (heads of 128) of the matrix cores. 2 x 2048 tokens
-// over 30000 rows with heads of 128 take 2.12-2.22 ms (940-980 TFLOP/s; the matrix cores 41% and the vector units 45% busy, no bank
+// over 30000 rows with heads of 128 take 2.12-2.25 ms (925-980 TFLOP/s; the matrix cores 41% and the vector units 45% busy, no bank
 // conflicts), 2048 over 30000 with heads of 64 1.46-1.54 ms (675-710 TFLOP/s; 31% and 64%). Without the copies the former would take a quarter
 // less; copies further ahead, barriers for the scheduler and wave priorities moved it by 4% either way.
 
